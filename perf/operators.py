@@ -21,6 +21,7 @@ import torch
 own = False
 
 GROUP = 32  # channels that share a scale and a minimum in a 4-bit cache
+LIMIT = 61440.0  # what it clamps to: every value it reads back is then finite in 16 bits
 
 
 def listed():
@@ -282,7 +283,7 @@ def _pack(x):
     """(codes, scales) of f64 rows."""
     *lead, d = x.shape
     n = d // GROUP
-    x = x.clamp(-65504.0, 65504.0).reshape(*lead, n, GROUP)
+    x = x.clamp(-LIMIT, LIMIT).reshape(*lead, n, GROUP)
     low, high = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
     scales = torch.cat([(high - low) / 15.0, low], dim=-1).float().half()
     step, base = scales[..., :1].double(), scales[..., 1:].double()
@@ -471,7 +472,7 @@ def _exact_append(case, s):
             q[b, :n] = new["q"]
         for whole, x in ((k, new["k"]), (v, new["v"])):
             if four:
-                g = x.clamp(-65504, 65504).unflatten(-1, (-1, GROUP))
+                g = x.clamp(-LIMIT, LIMIT).unflatten(-1, (-1, GROUP))
                 low = g.min(-1, keepdim=True).values
                 step = ((g.max(-1, keepdim=True).values - low) / 15).float().half().double()
                 low = low.float().half().double()
