@@ -626,6 +626,76 @@ int mi355x_attn_bwd_noalloc(void* dq, const int64_t* dq_bhs, void* dk,
                             int64_t heads, int64_t sq, int64_t skv, int64_t d,
                             double scale, int causal, int dtype, mi355x_stream_t stream);
 
+/* ---- paged key/value cache --------------------------------------------
+ * Serving keeps the keys and values of earlier tokens in pages.  The
+ * reference has no counterpart: its models recompute the whole prefix for
+ * each token (its Gemma-3 demo runs under torch.compile,
+ * demo_scripts/gemma3.py:11).
+ *
+ * A page holds page_size tokens of every K/V head; token p of sequence b lies
+ * in page table[b * table_stride + p / page_size], slot p % page_size.  Its row
+ * of d channels (unit stride) is d values of `dtype` (bits = 0), or with
+ * bits = 4 d / 2 bytes of codes and d / 32 pairs (scale, minimum) of f16, value
+ * = minimum + scale * code.  32-bit word g * (d / 32) + s of a row of codes
+ * (g < 4) holds channels 32 s + 8 g + e (e < 8), channel e in nibble
+ * e / 2 + 4 (e % 2).  *_phs: (page, head, slot) strides, of k and v in values
+ * (bytes for codes), of the scales in f16 values.  Rows must be 16-byte
+ * aligned; d is a multiple of 8 (bits = 4: of 32) up to 256. */
+typedef struct {
+  void* k;
+  void* v;
+  void* k_scales; /* bits = 4 only */
+  void* v_scales;
+  int64_t k_phs[3];
+  int64_t v_phs[3];
+  int64_t ks_phs[3];
+  int64_t vs_phs[3];
+  int64_t num_pages;
+  int64_t page_size;
+  int64_t kv_heads;
+  int64_t d;
+  int dtype;
+  int bits;
+} mi355x_paged_cache;
+/* In each call, token t of sequence b (t < seq) has position starts[b] + t;
+ * tokens from counts[b] on (null: none) are padding.  A page that the table
+ * does not hold or that does not exist, and a position below zero, set *error
+ * (may be null) to 1 and are left out: nothing out of range is touched.
+ * Sequences may share pages that are only read; two tokens of one call in the
+ * same slot leave either row, or parts of both. */
+
+/* Writes the tokens' keys (turned by the angles of their positions: row p of
+ * the dense [rope_len][d] tables of rope_dtype, as in mi355x_rope; null: as
+ * they are) and values to their pages; q, if given, is turned into q_out,
+ * zero at padding.  *_bht: (batch, head, token) strides in elements.
+ * 4 bits: per 32 channels minimum = f16(min), scale = f16((max - min) / 15),
+ * code = clamp(rint((x - minimum) / scale), 0, 15) in f64, with x clamped to
+ * +-61440; a group with a NaN or an infinity reads back as NaN. */
+int mi355x_paged_append(const mi355x_paged_cache* cache, const int32_t* table, int64_t table_stride,
+                        int64_t table_width, const int32_t* starts, const int32_t* counts, const void* k,
+                        const int64_t* k_bht, const void* v, const int64_t* v_bht, void* q_out,
+                        const int64_t* qo_bht, const void* q, const int64_t* q_bht, const void* cos_table,
+                        const void* sin_table, int rope_dtype, int64_t rope_len, int64_t batch,
+                        int64_t heads, int64_t seq, int dtype, int32_t* error, mi355x_stream_t stream);
+/* The rows of the tokens back as values of dtype, zero at padding. */
+int mi355x_paged_gather(void* k, const int64_t* k_bht, void* v, const int64_t* v_bht,
+                        const mi355x_paged_cache* cache, const int32_t* table, int64_t table_stride,
+                        int64_t table_width, const int32_t* starts, const int32_t* counts, int64_t batch,
+                        int64_t seq, int dtype, int32_t* error, mi355x_stream_t stream);
+/* Attention of the tokens' queries over their sequences: the query at
+ * position p sees key j <= p and, with a window > 0, only p - j < window or
+ * j < sinks.  Query head h reads K/V head h / (heads / kv_heads).  o is zero
+ * at padding and where no key is visible.  q and o are of `dtype`: that of
+ * the pages (bits = 0), or any of f32/bf16/f16.  Long sequences are split over
+ * blocks, whose partial sums the workspace holds. */
+int64_t mi355x_paged_attn_workspace_bytes(const mi355x_paged_cache* cache, int64_t table_width, int64_t batch,
+                                          int64_t heads, int64_t seq, int64_t window, int64_t sinks, int dtype);
+int mi355x_paged_attn(void* o, const int64_t* o_bht, const void* q, const int64_t* q_bht,
+                      const mi355x_paged_cache* cache, const int32_t* table, int64_t table_stride,
+                      int64_t table_width, const int32_t* starts, const int32_t* counts, int64_t batch,
+                      int64_t heads, int64_t seq, double scale, int64_t window, int64_t sinks, int dtype,
+                      void* workspace, int64_t ws_bytes, int32_t* error, mi355x_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

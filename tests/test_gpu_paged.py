@@ -1,0 +1,232 @@
+"""The paged cache on the MI355X against f64: appending, reading back and
+attention, over types, head layouts, page sizes, lengths and masks."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as oracle
+from paged_cases import STEP, Case, check, np64
+from torch_mojo_backend import ops
+from torch_mojo_backend.kv_cache import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _mojo(mojo):
+    return mojo
+
+
+def _tables(n, d, dtype, seed=4):
+    ang = torch.rand(n, d // 2, generator=torch.Generator().manual_seed(seed)).repeat(1, 2) * 6.2
+    return ang.cos().to(dtype), ang.sin().to(dtype)
+
+
+@pytest.mark.parametrize("dtype,bits,d,page,rope", [
+    (BF, None, 256, 16, F32), (BF, None, 64, 24, BF), (HF, None, 128, 8, F32), (F32, None, 80, 1, F32),
+    (BF, 4, 128, 64, F32), (HF, 4, 64, 24, HF), (F32, 4, 96, 16, F32), (BF, 4, 32, 3, BF), (BF, 4, 256, 16, None),
+    (BF, None, 24, 16, None)])
+def test_append_then_gather(dtype, bits, d, page, rope):
+    starts, counts = [0, 5, 1000, 0, 63], [37, 0, 21, 37, 1]
+    t, hk, h = 37, 3, 6
+    c = Case([s + t for s in starts], page=page, bits=bits, device="mojo", d=d, hk=hk, dtype=dtype, slots_first=page == 8)
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(5, t, hk, d, generator=g).to(dtype).transpose(1, 2) for _ in range(2))
+    q = torch.randn(5, t, h, d, generator=g).to(dtype).transpose(1, 2)
+    cos, sin = _tables(1100, d, rope) if rope else (None, None)
+    before = [x.cpu().clone() for x in (c.cache.k, c.cache.v)]
+    up = lambda x: x.to("mojo") if x is not None else None  # noqa: E731
+    rot = ops.paged_append(c.cache, c.dev_table, c.ints(starts), up(k), up(v), up(cos), up(sin),
+                           q=up(q) if rope else None, counts=c.ints(counts))
+    out = F32 if bits == 4 else dtype
+    gk, gv = ops.paged_gather(c.cache, c.dev_table, c.ints(starts), t, counts=c.ints(counts))
+    owned = set()
+    for b in range(5):
+        n = counts[b]
+        pos = np.arange(starts[b], starts[b] + n)
+        owned |= {(int(c.table[b, p // page]), p % page) for p in pos}
+        wq, wk, wv = (np64(x[b, :, :n]) for x in (q, k, v))
+        if rope:
+            wq, wk = (oracle.turn(x, np64(cos)[pos], np64(sin)[pos]) for x in (wq, wk))
+            # a sum of two products in f32, each at most 6 (N(0, 1) rows), rounded once
+            check(rot[b, :, :n], wq, STEP[dtype] * np.abs(wq) + 12 * 2.0 ** -23, "q")
+            assert (np64(rot[b, :, n:]) == 0).all()
+        assert (np64(gk[b, :, n:]) == 0).all() and (np64(gv[b, :, n:]) == 0).all()
+        if bits == 4 and n:
+            # the codes are those of the f64 rows; values leave in f32
+            wk, wv = (oracle.values(*oracle.quantize(x)) for x in (wk, wv))
+            check(gk[b, :, :n], wk, 2.0 ** -23 * 6 + 0 * wk, "k")
+            check(gv[b, :, :n], wv, 2.0 ** -23 * 6 + 0 * wv, "v")
+        elif n:
+            check(gk[b, :, :n], wk, STEP[out] * np.abs(wk) + (12 * 2.0 ** -23 if rope else 0), "k")
+            assert (np64(gv[b, :, :n]) == wv).all()
+    for x, old in zip((c.cache.k, c.cache.v), before):
+        x = x.cpu()
+        for p in range(c.cache.num_pages):
+            for s in range(page):
+                if (p, s) not in owned:
+                    assert torch.equal(x[p, :, s].nan_to_num(7.0), old[p, :, s].nan_to_num(7.0)), (p, s)
+
+
+def _attention(c, h, starts, counts, t, dtype=None, window=0, sinks=0, scale=None):
+    q = c.queries(h, t, dtype)
+    strided = q.transpose(1, 2).contiguous().to("mojo").transpose(1, 2)
+    out = ops.paged_attention(strided, c.cache, c.dev_table, c.ints(starts), counts=c.ints(counts), window=window,
+                              sinks=sinks, scale=scale)
+    check(out, *c.expected(q, starts, counts, window, sinks, scale), f"T{t} window {window} sinks {sinks}")
+
+
+@pytest.mark.parametrize("dtype,bits", [(BF, None), (HF, None), (F32, None), (BF, 4), (HF, 4), (F32, 4)])
+@pytest.mark.parametrize("d,hk,h", [(64, 3, 3), (128, 2, 8), (256, 1, 4), (96, 2, 2), (32, 1, 5)])
+@pytest.mark.parametrize("page", [16, 24, 1])
+def test_attention_of_one_token(dtype, bits, d, hk, h, page):
+    starts = [0, 1, 16, 31, 32, 33, 200, 517, 0]
+    counts = [1] * 8 + [0]
+    c = Case([s + n for s, n in zip(starts, counts)], page=page, bits=bits, device="mojo", d=d, hk=hk, dtype=dtype)
+    _attention(c, h, starts, counts, 1, dtype)
+    _attention(c, h, starts, counts, 1, dtype, window=33, sinks=5, scale=0.3)
+
+
+@pytest.mark.parametrize("dtype,bits", [(BF, None), (HF, None), (F32, None), (BF, 4)])
+@pytest.mark.parametrize("d,hk,h,t", [(64, 2, 2, 5), (128, 2, 8, 4), (256, 1, 4, 9), (128, 1, 16, 3), (64, 1, 1, 70),
+                                      (256, 1, 2, 33), (96, 1, 3, 6)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (16, 0), (40, 70), (1, 1)])
+def test_attention_of_several_tokens(dtype, bits, d, hk, h, t, window, sinks):
+    starts, counts = [0, 3, 90, 250, 0], [t, 1, t, max(t - 2, 1), 0]
+    c = Case([s + n for s, n in zip(starts, counts)], page=16, bits=bits, device="mojo", d=d, hk=hk, dtype=dtype)
+    _attention(c, h, starts, counts, t, dtype, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype,bits", [(BF, None), (F32, None), (BF, 4)])
+@pytest.mark.parametrize("d", [64, 256])
+def test_attention_over_a_long_sequence(dtype, bits, d):
+    c = Case([9001, 130], page=64, bits=bits, device="mojo", d=d, hk=1, dtype=dtype)
+    _attention(c, 4, [9000, 129], [1, 1], 1, dtype)
+    _attention(c, 4, [9000, 129], [1, 1], 1, dtype, window=4096, sinks=100)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.4])
+def test_scale_of_any_sign(scale):
+    c = Case([77], device="mojo", d=128)
+    _attention(c, 2, [70], [7], 7, BF, scale=scale)
+
+
+def test_large_scores_do_not_overflow():
+    for bits in (None, 4):
+        c = Case([300], device="mojo", d=64, hk=1, dtype=HF if bits is None else BF, bits=bits, spread=40.0)
+        _attention(c, 4, [299], [1], 1, HF if bits is None else BF, scale=1.0)
+
+
+def test_hidden_numbers_stay_hidden():
+    """NaN and infinities in keys and values that a query does not see."""
+    for bits in (None, 4):
+        c = Case([100], device="mojo", d=64, hk=1, bits=bits)
+        bad = torch.full((1, 1, 40, 64), float("nan"), dtype=BF)
+        bad[..., ::2] = float("inf")
+        # positions 4 .. 43: neither sinks nor in the window of the queries at 96 .. 99
+        ops.paged_append(c.cache, c.dev_table, c.ints([4]), bad.to("mojo"), bad.to("mojo"))
+        for x in c.values:
+            x[:, :, 4:44] = 0.0
+        _attention(c, 2, [96], [4], 4, BF, window=20, sinks=4)
+        _attention(c, 2, [99], [1], 1, BF, window=56, sinks=4)
+
+
+def test_offsets_past_32_bits():
+    pages, page, hk, d = 70_000, 16, 8, 256  # 2.3e9 values a tensor
+    k, v = (torch.empty(pages, hk, page, d, dtype=BF, device="mojo") for _ in range(2))
+    cache = PagedKVCache(k, v)
+    last = torch.arange(pages - 4, pages, dtype=torch.int32).view(1, 4)
+    g = torch.Generator().manual_seed(5)
+    rows = [torch.randn(1, hk, 50, d, generator=g).to(BF) for _ in range(2)]
+    zero = torch.zeros(1, dtype=torch.int32).to("mojo")
+    ops.paged_append(cache, last.to("mojo"), zero, *(x.to("mojo") for x in rows))
+    got = ops.paged_gather(cache, last.to("mojo"), zero, 50)
+    for a, b in zip(got, rows):
+        assert torch.equal(a.cpu(), b)
+    q = torch.randn(1, 16, 1, d, generator=g).to(BF)
+    out = ops.paged_attention(q.to("mojo"), cache, last.to("mojo"), zero + 49)
+    want = oracle.attend(np64(q)[0], np64(rows[0])[0], np64(rows[1])[0], [49])
+    check(out, want[None], STEP[BF] * np.abs(want[None]) + 1e-4)
+
+
+def test_pages_out_of_range_are_left_out():
+    c = Case([40], device="mojo", d=64, hk=1)
+    x = torch.ones(1, 1, 1, 64, dtype=BF).to("mojo")
+    for table in ([[0, 99, 1]], [[0, -5, 1]], [[0, 2 ** 31 - 1, 1]]):
+        tab = torch.tensor(table, dtype=torch.int32).to("mojo")
+        for call in (lambda: ops.paged_append(c.cache, tab, c.ints([20]), x, x),
+                     lambda: ops.paged_gather(c.cache, tab, c.ints([20]), 3),
+                     lambda: ops.paged_attention(x, c.cache, tab, c.ints([40]))):
+            call()
+            with pytest.raises(IndexError, match="paged cache"):
+                x.cpu()
+    x.cpu()  # the flag is cleared
+
+
+def test_shared_pages_and_repeated_results():
+    """Sequences with a common prefix read the same pages; a call repeated gives the same bits."""
+    c = Case([64, 64], page=16, device="mojo", d=128, hk=2)
+    tab = c.table.clone()
+    tab[1, :2] = tab[0, :2]
+    for x in c.values:
+        x[1][:, :32] = x[0][:, :32]
+    q = c.queries(4, 1)
+    args = (q.to("mojo"), c.cache, tab.to("mojo"), c.ints([63, 60]))
+    first = ops.paged_attention(*args)
+    check(first, *c.expected(q, [63, 60], [1, 1]))
+    assert all(torch.equal(first.cpu(), ops.paged_attention(*args).cpu()) for _ in range(3))
+
+
+def test_captured_and_replayed(kernels):
+    """Append and attention captured into a graph through the C entry points;
+    each replay reads the positions of the moment."""
+    from torch_mojo_backend.eager_kernels import PagedCache, check as ok
+
+    d, hk, h, page, n = 128, 2, 8, 16, 64
+    g = torch.Generator().manual_seed(6)
+    dev = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    kp, vp = torch.zeros(n, hk, page, d, dtype=BF, device="cuda"), torch.zeros(n, hk, page, d, dtype=BF, device="cuda")
+    desc = PagedCache()
+    desc.k, desc.v = kp.data_ptr(), vp.data_ptr()
+    desc.k_phs[:] = desc.v_phs[:] = kp.stride()[:3]
+    desc.num_pages, desc.page_size, desc.kv_heads, desc.d, desc.dtype = n, page, hk, d, 1
+    table = torch.randperm(n, generator=g).int().view(1, n).cuda()
+    starts = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v, q = dev(1, hk, 1, d), dev(1, hk, 1, d), dev(1, h, 1, d)
+    o = torch.empty_like(q)
+    ws = kernels.mi355x_paged_attn_workspace_bytes(desc, n, 1, h, 1, 0, 0, 1)
+    hold = torch.empty(max(ws, 1), dtype=torch.uint8, device="cuda")
+    bht = lambda x: (ctypes.c_int64 * 3)(*x.stride()[:3])  # noqa: E731
+
+    def step(stream):
+        ok("append", kernels.mi355x_paged_append(
+            desc, table.data_ptr(), n, n, starts.data_ptr(), None, k.data_ptr(), bht(k), v.data_ptr(), bht(v),
+            None, None, None, None, None, None, 0, 0, 1, 0, 1, 1, None, stream))
+        ok("attention", kernels.mi355x_paged_attn(
+            o.data_ptr(), bht(o), q.data_ptr(), bht(q), desc, table.data_ptr(), n, n, starts.data_ptr(), None,
+            1, h, 1, d ** -0.5, 0, 0, 1, hold.data_ptr(), ws, None, stream))
+
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step(side.cuda_stream)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            step(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    ks, vs = [], []
+    for i in range(40):
+        k.copy_(dev(1, hk, 1, d)), v.copy_(dev(1, hk, 1, d)), q.copy_(dev(1, h, 1, d))
+        starts.fill_(i)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ks.append(np64(k)[0, :, 0]), vs.append(np64(v)[0, :, 0])
+        want = oracle.attend(np64(q)[0], np.stack(ks, 1), np.stack(vs, 1), [i])
+        check(o, want[None], STEP[BF] * np.abs(want[None]) + 1e-4, f"replay {i}")

@@ -1,0 +1,272 @@
+// Attention of new tokens over a paged key/value cache.
+//
+//   o = softmax(scale q K^T over the visible keys) V,
+// key j visible to the query at position p iff j <= p and, with a window,
+// p - j < window or j < sinks.
+#include <math.h>
+
+#include "paged.h"
+
+namespace mi {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct DecodeArgs {
+  mi355x_paged_cache c;
+  PagedSeqs s;
+  void* o;
+  int64_t o_b, o_h, o_t;
+  const void* q;
+  int64_t q_b, q_h, q_t;
+  int64_t batch;
+  int heads, group, seq;
+  int window, sinks;  // window 0: none
+  int splits;
+  float scale_log2;
+  float* part_o;   // [splits][batch * heads * seq][d]
+  float2* part_ml; // [splits][batch * heads * seq]: maximum (base 2) and sum
+};
+
+// The keys that queries at positions first .. last can see, in tiles of
+// `tile` keys: the sinks' tiles, then from `low` on.
+struct KeySpan {
+  int sink_tiles, low, tiles;  // low: first tile of the window
+  __device__ __forceinline__ KeySpan(int first, int last, int window, int sinks, int tile) {
+    low = window > 0 ? max(first - window + 1, 0) / tile : 0;
+    const int s = window > 0 ? min(sinks, last + 1) : 0;
+    sink_tiles = min((s + tile - 1) / tile, low);
+    tiles = last < 0 ? 0 : sink_tiles + last / tile + 1 - low;
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : low + i - sink_tiles; }
+};
+__device__ __forceinline__ bool visible(int pos, int j, int window, int sinks) {
+  return j <= pos && (window <= 0 || pos - j < window || j < sinks);
+}
+
+// ---------------------------------------------------------------------------
+// any type and head_dim: a block owns one query row and a split of its keys;
+// each 16 lanes of it take every 16th key, a lane eight (or twice eight)
+// channels, and the sixteen partial softmaxes are joined through LDS.
+// ---------------------------------------------------------------------------
+template <typename CT>
+struct Oct8 {
+  CT v[8];
+};
+
+template <typename CT>
+__device__ __forceinline__ void load_oct(float (&x)[8], const void* base, int64_t at, const f16* sc, int oct, int d) {
+  if constexpr (sizeof(CT) == 1) {
+    const int s = oct % (d / kKvGroup);
+    const uint32_t w = ((const uint32_t*)((const uint8_t*)base + at))[oct];
+    const float step = (float)sc[2 * s], low = (float)sc[2 * s + 1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(step, (float)(w >> (4 * (e / 2 + 4 * (e % 2))) & 15), low);
+  } else {
+    const Oct8<CT> o = *(const Oct8<CT>*)((const CT*)base + at + oct * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = to_f32(o.v[e]);
+  }
+}
+// First channel of the eight that a row's piece `oct` holds.
+template <typename CT>
+__device__ __forceinline__ int oct_channel(int oct, int d) {
+  if constexpr (sizeof(CT) == 1) {
+    const int n = d / kKvGroup;
+    return oct % n * kKvGroup + oct / n * 8;
+  }
+  return oct * 8;
+}
+
+template <typename T, typename CT>
+__global__ void __launch_bounds__(kThreads) paged_attn_rows(DecodeArgs a) {
+  __shared__ float so[16][256];
+  __shared__ float sm[16], sl[16];
+  const int d = (int)a.c.d, octs = d / 8;
+  const int lane = threadIdx.x & 15, stream = threadIdx.x >> 4;
+  const uint32_t row = blockIdx.x;  // over batch * heads * seq, token fastest
+  const uint32_t t = row % a.seq, bh = row / a.seq;
+  const int h = bh % a.heads;
+  const int64_t b = bh / a.heads;
+  const int hk = h / a.group;
+  const bool real = (int)t < seq_count(a.s, b, a.seq);
+  const int64_t at = (int64_t)a.s.starts[b] + t;
+  int pos = real && at >= 0 && at <= kMaxPosition ? (int)at : -1;
+  if (real && pos < 0 && a.s.error) *a.s.error = 1;
+  const KeySpan span(pos, pos, a.window, a.sinks, 16);
+  const int per = (span.tiles + a.splits - 1) / a.splits, first = blockIdx.y * per;
+  const int last = min(first + per, span.tiles);
+  float q[2][8], o[2][8], m = -INFINITY, l = 0.f;
+  const T* Q = (const T*)a.q + b * a.q_b + h * a.q_h + t * a.q_t;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int oct = lane + 16 * u;
+      q[u][e] = oct < octs ? to_f32(Q[oct_channel<CT>(oct, d) + e]) : 0.f;
+      o[u][e] = 0.f;
+    }
+  for (int i = first; i < last; ++i) {
+    const int j = span.tile(i) * 16 + stream;
+    if (!visible(pos, j, a.window, a.sinks)) continue;
+    uint32_t slot;
+    const int page = page_of(a.s, b, j, &slot);
+    if (page < 0) continue;
+    const int64_t ka = page * a.c.k_phs[0] + hk * a.c.k_phs[1] + slot * a.c.k_phs[2];
+    const int64_t va = page * a.c.v_phs[0] + hk * a.c.v_phs[1] + slot * a.c.v_phs[2];
+    const f16 *ks = nullptr, *vs = nullptr;
+    if constexpr (sizeof(CT) == 1) {
+      ks = (const f16*)a.c.k_scales + page * a.c.ks_phs[0] + hk * a.c.ks_phs[1] + slot * a.c.ks_phs[2];
+      vs = (const f16*)a.c.v_scales + page * a.c.vs_phs[0] + hk * a.c.vs_phs[1] + slot * a.c.vs_phs[2];
+    }
+    float s = 0.f, x[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 16 * u < octs) {
+        load_oct<CT>(x, a.c.k, ka, ks, lane + 16 * u, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(q[u][e], x[e], s);
+      }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off, 64);
+    s *= a.scale_log2;
+    const float mn = fmaxf(m, s);
+    const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn), p = mn == -INFINITY ? 0.f : exp2f(s - mn);
+    l = l * alpha + p;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 16 * u < octs) {
+        load_oct<CT>(x, a.c.v, va, vs, lane + 16 * u, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[u][e] = fmaf(p, x[e], o[u][e] * alpha);
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (lane + 16 * u < octs) so[stream][oct_channel<CT>(lane + 16 * u, d) + e] = o[u][e];
+  if (lane == 0) sm[stream] = m, sl[stream] = l;
+  __syncthreads();
+  float mx = -INFINITY;
+  for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sm[i]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float total = 0.f, acc = 0.f;
+  for (int i = 0; i < 16; ++i) {
+    const float w = exp2f(sm[i] - base);
+    total += w * sl[i];
+    if ((int)threadIdx.x < d) acc += w * so[i][threadIdx.x];
+  }
+  const int64_t rows = a.batch * a.heads * a.seq;
+  if (a.splits > 1) {
+    if ((int)threadIdx.x < d) a.part_o[(blockIdx.y * rows + row) * d + threadIdx.x] = acc;
+    if (threadIdx.x == 0) a.part_ml[blockIdx.y * rows + row] = make_float2(mx, total);
+  } else if ((int)threadIdx.x < d) {
+    ((T*)a.o)[b * a.o_b + h * a.o_h + t * a.o_t + threadIdx.x] = from_f32<T>(total != 0.f ? acc / total : 0.f);
+  }
+}
+
+// Joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) paged_attn_join(DecodeArgs a) {
+  const int d = (int)a.c.d;
+  const int64_t rows = a.batch * a.heads * a.seq;
+  const uint32_t row = blockIdx.x;
+  const uint32_t t = row % a.seq, bh = row / a.seq;
+  const int h = bh % a.heads;
+  const int64_t b = bh / a.heads;
+  float mx = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_ml[s * rows + row].x);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float total = 0.f, acc = 0.f;
+  if ((int)threadIdx.x >= d) return;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.part_ml[s * rows + row];
+    const float w = exp2f(ml.x - base);
+    total += w * ml.y;
+    acc += w * a.part_o[(s * rows + row) * d + threadIdx.x];
+  }
+  ((T*)a.o)[b * a.o_b + h * a.o_h + t * a.o_t + threadIdx.x] = from_f32<T>(total != 0.f ? acc / total : 0.f);
+}
+
+// Keys that one query can see at most.
+int64_t most_keys(const mi355x_paged_cache& c, int64_t width, int64_t window, int64_t sinks) {
+  int64_t n = width * c.page_size;
+  if (n > kMaxPosition) n = kMaxPosition;
+  return window > 0 && window + sinks < n ? window + sinks : n;
+}
+
+// Blocks that share the keys of a row: enough for two rounds of the 256 CUs
+// where rows alone are fewer, at 128 keys each and more.
+int plan_splits(const mi355x_paged_cache& c, int64_t width, int64_t batch, int64_t heads, int64_t seq, int64_t window,
+                int64_t sinks) {
+  const int64_t rows = batch * heads * seq, keys = most_keys(c, width, window, sinks);
+  int64_t n = rows ? 1024 / rows : 1;
+  if (n > (keys + 127) / 128) n = (keys + 127) / 128;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
+template <typename T>
+int attn_launch(const DecodeArgs& a, hipStream_t s) {
+  const int64_t rows = a.batch * a.heads * a.seq;
+  const dim3 grid((unsigned)rows, (unsigned)a.splits);
+  if (a.c.bits == 4) paged_attn_rows<T, uint8_t><<<grid, kThreads, 0, s>>>(a);
+  else paged_attn_rows<T, T><<<grid, kThreads, 0, s>>>(a);
+  if (a.splits > 1) paged_attn_join<T><<<(unsigned)rows, kThreads, 0, s>>>(a);
+  return check_launch("mi355x_paged_attn");
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" int64_t mi355x_paged_attn_workspace_bytes(const mi355x_paged_cache* cache, int64_t table_width,
+                                                     int64_t batch, int64_t heads, int64_t seq, int64_t window,
+                                                     int64_t sinks, int dtype) {
+  if (!cache || table_width < 0 || batch <= 0 || heads <= 0 || seq <= 0) return 0;
+  const int splits = plan_splits(*cache, table_width, batch, heads, seq, window, sinks);
+  return splits > 1 ? splits * batch * heads * seq * (cache->d + 2) * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int mi355x_paged_attn(void* o, const int64_t* o_bht, const void* q, const int64_t* q_bht,
+                                 const mi355x_paged_cache* cache, const int32_t* table, int64_t table_stride,
+                                 int64_t table_width, const int32_t* starts, const int32_t* counts, int64_t batch,
+                                 int64_t heads, int64_t seq, double scale, int64_t window, int64_t sinks, int dtype,
+                                 void* workspace, int64_t ws_bytes, int32_t* error, mi355x_stream_t stream) {
+  PagedSeqs s;
+  int rc = paged_args("mi355x_paged_attn", cache, table, table_stride, table_width, starts, counts, batch, seq, error,
+                      &s);
+  if (rc) return rc;
+  if (dtype != MI355X_F32 && dtype != MI355X_BF16 && dtype != MI355X_F16)
+    return fail(MI355X_EUNSUPPORTED, "mi355x_paged_attn: dtype %d is not supported (f32/bf16/f16)", dtype);
+  MI_REQUIRE(cache->bits == 4 || cache->dtype == dtype, "mi355x_paged_attn: queries of dtype %d over pages of dtype %d",
+             dtype, cache->dtype);
+  MI_REQUIRE(heads > 0 && heads < 65536 && heads % cache->kv_heads == 0,
+             "mi355x_paged_attn: heads (%lld) must be a multiple of kv_heads (%lld)", (long long)heads,
+             (long long)cache->kv_heads);
+  MI_REQUIRE(window >= 0 && sinks >= 0, "mi355x_paged_attn: bad window or sinks");
+  MI_REQUIRE(isfinite(scale), "mi355x_paged_attn: scale must be finite");
+  if (batch == 0 || seq == 0) return MI355X_OK;
+  MI_REQUIRE(o && q, "mi355x_paged_attn: null pointer");
+  MI_REQUIRE(batch * heads * seq < (1ll << 24), "mi355x_paged_attn: batch x heads x tokens must be below 2^24");
+  const int64_t need = mi355x_paged_attn_workspace_bytes(cache, table_width, batch, heads, seq, window, sinks, dtype);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(MI355X_EWORKSPACE, "mi355x_paged_attn: workspace %lld < %lld", (long long)ws_bytes, (long long)need);
+  DecodeArgs a{};
+  a.c = *cache, a.s = s;
+  a.o = o, a.o_b = o_bht[0], a.o_h = o_bht[1], a.o_t = o_bht[2];
+  a.q = q, a.q_b = q_bht[0], a.q_h = q_bht[1], a.q_t = q_bht[2];
+  a.batch = batch, a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads), a.seq = (int)seq;
+  // a window or sinks past every position are the same as one that ends there
+  a.window = (int)(window < kMaxPosition ? window : 0), a.sinks = (int)(sinks < kMaxPosition ? sinks : kMaxPosition);
+  a.splits = plan_splits(*cache, table_width, batch, heads, seq, window, sinks);
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.part_o = (float*)workspace;
+  a.part_ml = (float2*)(a.part_o + a.splits * batch * heads * seq * cache->d);
+  if (dtype == MI355X_F32) return attn_launch<float>(a, (hipStream_t)stream);
+  if (dtype == MI355X_BF16) return attn_launch<bf16>(a, (hipStream_t)stream);
+  return attn_launch<f16>(a, (hipStream_t)stream);
+}

@@ -65,6 +65,27 @@ class AdamWTensor(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """`mi355x_paged_cache` (layout of include/mi355x_kernels.h)."""
+
+    _fields_ = [
+        ("k", c_vp),
+        ("v", c_vp),
+        ("k_scales", c_vp),
+        ("v_scales", c_vp),
+        ("k_phs", c_i64 * 3),
+        ("v_phs", c_i64 * 3),
+        ("ks_phs", c_i64 * 3),
+        ("vs_phs", c_i64 * 3),
+        ("num_pages", c_i64),
+        ("page_size", c_i64),
+        ("kv_heads", c_i64),
+        ("d", c_i64),
+        ("dtype", c_int),
+        ("bits", c_int),
+    ]
+
+
 # name -> (restype, argtypes).  Kept in the order of the header.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mi355x_abi_version": (c_int, []),
@@ -261,6 +282,30 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp,
             c_i64, c_i64, c_i64, c_i64, c_i64, c_double, c_int, c_int,
             c_vp,
+        ],
+    ),
+    "mi355x_paged_append": (
+        c_int,
+        [
+            ctypes.POINTER(PagedCache), c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, P_i64, c_vp, P_i64,
+            c_vp, P_i64, c_vp, P_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_vp,
+        ],
+    ),
+    "mi355x_paged_gather": (
+        c_int,
+        [
+            c_vp, P_i64, c_vp, P_i64, ctypes.POINTER(PagedCache), c_vp, c_i64, c_i64, c_vp, c_vp,
+            c_i64, c_i64, c_int, c_vp, c_vp,
+        ],
+    ),
+    "mi355x_paged_attn_workspace_bytes": (
+        c_i64, [ctypes.POINTER(PagedCache), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_int],
+    ),
+    "mi355x_paged_attn": (
+        c_int,
+        [
+            c_vp, P_i64, c_vp, P_i64, ctypes.POINTER(PagedCache), c_vp, c_i64, c_i64, c_vp, c_vp,
+            c_i64, c_i64, c_i64, c_double, c_i64, c_i64, c_int, c_vp, c_i64, c_vp, c_vp,
         ],
     ),
 }

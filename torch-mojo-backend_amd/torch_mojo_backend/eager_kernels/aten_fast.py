@@ -1328,8 +1328,9 @@ def fast_aten_index_select(self, dim, index):
 _ERROR_KINDS = (
     (IndexError, "index out of range in self"),
     (IndexError, "Target is out of bounds"),
+    (IndexError, "a position or page of a paged cache is out of range"),
 )
-_INDEX_ERROR, _TARGET_ERROR = 0, 1
+_INDEX_ERROR, _TARGET_ERROR, _PAGE_ERROR = 0, 1, 2
 _error_flags: dict = {}      # device index -> int32 [len(_ERROR_KINDS)] flag tensor
 _errors_pending: set = set()  # devices with a flag launch since the last read
 

@@ -1,19 +1,23 @@
 """Fused ops of the Gemma-3-shaped workload: rotary embedding, GeGLU and
-RMSNorm with a weight offset.
+RMSNorm with a weight offset; and serving's: appending to a paged key/value
+cache and attention over it.
 
 Torch has no single aten op for these (a model writes them as chains of
 slice / neg / cat / mul / add, gelu + mul, and rms_norm with `1 + w`); the
 functions here keep those semantics, run one gfx950 kernel each on the mojo
 device, and fall back to the plain formula elsewhere (the CPU reference),
-so a model written with them runs unchanged on both.  All are
-differentiable.
+so a model written with them runs unchanged on both.  All but those of the
+cache are differentiable.
 """
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
+from . import kv_cache
 from .eager_kernels import aten_fast
 from .mojo_device.torch_mojo_tensor import TorchMojoTensor
 
@@ -94,3 +98,132 @@ def rms_norm(x, weight, eps, weight_offset=0.0):
             return aten_fast.rms_norm_forward(x, shape, weight, float(eps), float(weight_offset))[0]
         return _FusedRMSNorm.apply(x, shape, weight, float(eps), float(weight_offset))
     return F.rms_norm(x, shape, weight.float() + weight_offset, eps)
+
+
+# ---------------------------------------------------------------------------
+# paged key/value cache (torch_mojo_backend.kv_cache)
+# ---------------------------------------------------------------------------
+def _paged_check(what, cache, page_table, starts, counts, batch, **tensors):
+    """The arguments that the cache's operations share."""
+    for name, t, dims in (("page_table", page_table, 2), ("starts", starts, 1), ("counts", counts, 1)):
+        if t is None and name == "counts":
+            continue
+        if t.dtype != torch.int32 or t.dim() != dims or t.shape[0] != batch:
+            raise ValueError(f"{what}: {name} must be int32 with {dims} dimension{'s' * (dims > 1)} and {batch} rows,"
+                             f" got {tuple(t.shape)} of {t.dtype}")
+        if t.numel() and t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{what}: {name} must have unit stride")
+    every = dict(tensors, page_table=page_table, starts=starts, counts=counts)
+    for name, t in every.items():
+        if t is None:
+            continue
+        if t.device != cache.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, the cache on {cache.device}")
+        if cache.on_mojo != isinstance(t, TorchMojoTensor):
+            raise ValueError(f"{what}: {name} and the cache must both be mojo tensors")
+        if _needs_grad(t):
+            raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad(), or detach {name}")
+
+
+def _paged_rows(what, cache, name, t, heads, dtype):
+    if t.dim() != 4 or t.shape[3] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what}: {name} must be [batch, {'heads' if heads is None else heads}, tokens,"
+                         f" {cache.head_dim}], got {tuple(t.shape)}")
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16) or t.dtype != dtype:
+        raise TypeError(f"{what}: {name} is of {t.dtype}, expected {dtype}")
+
+
+def paged_append(cache, page_table, starts, k, v, cos=None, sin=None, *, q=None, counts=None):
+    """Put the keys and values of new tokens into their pages: token t of
+    sequence b (k, v [batch, kv_heads, tokens, head_dim]) goes to position
+    starts[b] + t, page page_table[b, position // page_size]; tokens from
+    counts[b] on are padding and are not written.  With cos and sin
+    [positions, head_dim] (f32 or k's dtype) keys are turned by the angles of
+    their positions, as `rotary_embedding` does, and so is q [batch, heads,
+    tokens, head_dim], which is returned (zero at padding; None without q).
+
+    One kernel.  A position outside the page table, a page that does not exist
+    or a position outside cos raises IndexError (on the mojo device at the next
+    device-to-host read) and is not written.  Two tokens of one call must not
+    name the same slot."""
+    what = "paged_append"
+    if k.dim() != 4:
+        raise ValueError(f"{what}: k must be [batch, kv_heads, tokens, head_dim], got {tuple(k.shape)}")
+    _paged_check(what, cache, page_table, starts, counts, k.shape[0], k=k, v=v, cos=cos, sin=sin, q=q)
+    dtype = k.dtype if cache.bits == 4 else cache.dtype
+    _paged_rows(what, cache, "k", k, cache.kv_heads, dtype)
+    _paged_rows(what, cache, "v", v, cache.kv_heads, dtype)
+    if v.shape != k.shape:
+        raise ValueError(f"{what}: k is {tuple(k.shape)}, v {tuple(v.shape)}")
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: cos and sin come together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape[1] != cache.head_dim or cos.shape != sin.shape:
+            raise ValueError(f"{what}: cos and sin must be [positions, {cache.head_dim}], got {tuple(cos.shape)}"
+                             f" and {tuple(sin.shape)}")
+        if cos.dtype not in (torch.float32, k.dtype) or sin.dtype != cos.dtype:
+            raise TypeError(f"{what}: cos and sin are of {cos.dtype} and {sin.dtype}, expected torch.float32 or {k.dtype}")
+        if cache.head_dim % 16:
+            raise ValueError(f"{what}: the rotation needs a head_dim that is a multiple of 16, not {cache.head_dim}")
+    if q is not None:
+        if cos is None:
+            raise ValueError(f"{what}: q is taken with cos and sin")
+        _paged_rows(what, cache, "q", q, None, dtype)
+        if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] == 0:
+            raise ValueError(f"{what}: q is {tuple(q.shape)}, k {tuple(k.shape)}")
+    if cache.on_mojo:
+        from .eager_kernels import paged
+
+        return paged.append(cache, page_table, starts, k, v, cos, sin, q, counts)
+    return kv_cache.append_plain(cache, page_table, starts, k, v, cos, sin, q, counts)
+
+
+def paged_gather(cache, page_table, starts, length, *, counts=None, dtype=None):
+    """(k, v) [batch, kv_heads, length, head_dim]: the rows at positions
+    starts[b] .. starts[b] + length - 1 back as values of dtype (the cache's,
+    float32 of a 4-bit one), zero from counts[b] on."""
+    what = "paged_gather"
+    _paged_check(what, cache, page_table, starts, counts, page_table.shape[0] if page_table.dim() else 0)
+    dtype = dtype or (torch.float32 if cache.bits == 4 else cache.dtype)
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: values of {dtype} are not supported")
+    length = int(length)
+    if length < 0:
+        raise ValueError(f"{what}: length {length}")
+    if cache.on_mojo:
+        from .eager_kernels import paged
+
+        return paged.gather(cache, page_table, starts, length, counts, dtype)
+    return kv_cache.gather_plain(cache, page_table, starts, length, counts, dtype)
+
+
+def paged_attention(q, cache, page_table, starts, *, counts=None, window=0, sinks=0, scale=None):
+    """Attention of new tokens over their sequences' pages, which hold the
+    tokens' own keys and values already: the query t of sequence b (q [batch,
+    heads, tokens, head_dim]) at position p = starts[b] + t sees key j <= p and,
+    with a window > 0, only p - j < window or j < sinks.  Query head h reads
+    K/V head h // (heads // kv_heads).  Queries from counts[b] on are padding:
+    their rows are zero, as is a row that sees no key.  scale defaults to
+    head_dim ** -0.5.
+
+    A page that does not exist raises IndexError (on the mojo device at the
+    next device-to-host read) and counts as hidden.  What lies in pages behind
+    a sequence's last token is never used."""
+    what = "paged_attention"
+    if q.dim() != 4:
+        raise ValueError(f"{what}: q must be [batch, heads, tokens, head_dim], got {tuple(q.shape)}")
+    _paged_check(what, cache, page_table, starts, counts, q.shape[0], q=q)
+    _paged_rows(what, cache, "q", q, None, q.dtype if cache.bits == 4 else cache.dtype)
+    if q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"{what}: {q.shape[1]} heads over {cache.kv_heads} K/V heads")
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0:
+        raise ValueError(f"{what}: window {window} and sinks {sinks} must not be negative")
+    scale = cache.head_dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: scale {scale} must be finite")
+    if cache.on_mojo:
+        from .eager_kernels import paged
+
+        return paged.attention(q, cache, page_table, starts, counts, window, sinks, scale)
+    return kv_cache.attention_plain(q, cache, page_table, starts, counts, window, sinks, scale)
