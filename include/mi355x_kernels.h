@@ -608,6 +608,31 @@ int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
                         int64_t sq, int64_t skv, int64_t d, double scale, int causal,
                         int64_t window, int dtype, void* workspace, int64_t ws_bytes,
                         mi355x_stream_t stream);
+/* A causal sliding window with sinks: query i sees key j <= i iff i - j <
+ * window or j < sinks (both positive); types, head_dims, strides and grouped
+ * heads as in mi355x_attn_fwd_gen / mi355x_attn_bwd_gen.  Training with the
+ * first tokens left visible, as a model that is served with a window needs;
+ * the reference runs such a mask through its masked-math decomposition
+ * (aten_fast.py:9112-9123). */
+int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, const void* q,
+                         const int64_t* q_bhs, const void* k, const int64_t* k_bhs,
+                         const void* v, const int64_t* v_bhs, int64_t batch, int64_t heads,
+                         int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
+                         int64_t window, int64_t sinks, int dtype, mi355x_stream_t stream);
+/* Workspace: that of mi355x_attn_bwd_gen, and f32 partials of the sinks'
+ * gradients, whose queries are shared by several blocks. */
+int64_t mi355x_attn_bwd_sink_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                             int64_t sq, int64_t skv, int64_t d, int64_t window,
+                                             int64_t sinks);
+int mi355x_attn_bwd_sink(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs,
+                         void* dv, const int64_t* dv_bhs, const void* dout,
+                         const int64_t* do_bhs, const void* q, const int64_t* q_bhs,
+                         const void* k, const int64_t* k_bhs, const void* v,
+                         const int64_t* v_bhs, const void* o, const int64_t* o_bhs,
+                         const float* lse, int64_t batch, int64_t heads, int64_t kv_heads,
+                         int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
+                         int64_t sinks, int dtype, void* workspace, int64_t ws_bytes,
+                         mi355x_stream_t stream);
 /* mi355x_attn_bwd without a workspace argument and without any allocation.
  * No counterpart in the reference: it is for callers that cannot allocate
  * (code under HIP graph capture, tight serving loops, harnesses that forbid

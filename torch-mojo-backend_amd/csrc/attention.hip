@@ -28,6 +28,7 @@
 //          blocks, recomputing S^T and dP^T, and accumulates dQ^T = K^T dS^T.
 #include <math.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "common.h"
@@ -78,6 +79,7 @@ struct AttnArgs {
   int causal;
   int64_t group;   // query heads per K/V head (grouped-query attention), >= 1
   int64_t window;  // > 0: query i sees keys i-window+1 .. i (causal only); 0: none
+  int64_t sinks;   // with a window: first keys that every later query sees
 };
 
 // Stage a 64-row x D tile (rows row0.., row stride rs) into LDS: row-major
@@ -492,7 +494,9 @@ struct KvTileLoad {
 // against P (the same bf16 P that multiplies V).
 constexpr float kSlack = 8.f;
 
-template <typename T, int D, bool POS, int NW, int QPW>
+// SINK: a window with sinks.  The block first walks the 64-key tiles that hold
+// sinks and lie before its window's first tile, then the window's.
+template <typename T, int D, bool POS, int NW, int QPW, bool SINK = false>
 __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 1) attn_fwd_v2(AttnArgs p) {
   constexpr int QT = QPW / 16, QPB = NW * QPW;  // 16-query tiles per wave, queries per block
   typedef typename Mfma<T>::frag frag;
@@ -543,8 +547,10 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
   if (p.causal) kv_end = min(p.Skv, q0 + QPB);
   // first 64-key tile any query of the block can see (sliding window)
   const int64_t j0 = p.window > 0 ? max((int64_t)0, q0 - p.window + 1) / 64 : 0;
-  kl.issue(j0 * 64, p.Skv, lds);
-  vl.issue(j0 * 64, p.Skv, lds + L::TILE);
+  const int64_t ns = SINK ? min(ceil_div64(min(p.sinks, p.Skv), 64), j0) : 0;  // tiles of sinks before j0
+  const int64_t jfirst = SINK && ns > 0 ? 0 : j0;
+  kl.issue(jfirst * 64, p.Skv, lds);
+  vl.issue(jfirst * 64, p.Skv, lds + L::TILE);
   const int sw = L::swz(lr);  // fragment rows kt*16 + lr share the swizzle of lr
   const TrOffsets<D> tro;
   const float c = p.scale_log2;
@@ -558,10 +564,11 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
     const int64_t kb0 = j * 64;
     __builtin_amdgcn_s_waitcnt(0xc07f & 0x3f70);  // vmcnt(0)
     __syncthreads();
-    if (kb0 + 64 < kv_end) {
+    const int64_t kn = SINK && j + 1 == ns ? j0 * 64 : kb0 + 64;
+    if (kn < kv_end) {
       char* nx = lds + (buf ^ 1) * STAGE;
-      kl.issue(kb0 + 64, p.Skv, nx);
-      vl.issue(kb0 + 64, p.Skv, nx + L::TILE);
+      kl.issue(kn, p.Skv, nx);
+      vl.issue(kn, p.Skv, nx + L::TILE);
     }
     const char* Kt = lds + buf * STAGE;
     const char* Vt = Kt + L::TILE;
@@ -572,9 +579,11 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
     if constexpr (MASK) {
       const int64_t qf = q0 + wave * QPW;
       if (p.causal && kb0 > qf + QPW - 1) return;
-      if (p.window > 0 && kb0 + 63 < qf - p.window + 1) return;
+      if (p.window > 0 && kb0 + 63 < qf - p.window + 1 && !(SINK && kb0 < p.sinks)) return;
     }
-      // Per query tile, the keys kb0 + lo..lim are visible to this lane's query.
+      // Per query tile, the keys kb0 + lo..lim are visible to this lane's
+      // query, and those of its sinks, kb0 + 0..ls-1, up to lim.
+      const int ls = SINK ? (int)max((int64_t)0, min((int64_t)64, p.sinks - kb0)) : 0;
       int lo[QT], lim[QT];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
@@ -608,7 +617,8 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float v = POS ? a[e] : a[e] * c;
-            if (MASK && (kt * 16 + lg * 4 + e > lim[qt] || kt * 16 + lg * 4 + e < lo[qt])) v = -INFINITY;
+            const int key = kt * 16 + lg * 4 + e;
+            if (MASK && (key > lim[qt] || (key < lo[qt] && !(SINK && key < ls)))) v = -INFINITY;
             a[e] = v;
             mx[qt] = fmaxf(mx[qt], v);
           }
@@ -673,6 +683,8 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
   if (p.window > 0) jl = min(nkb, max(j0, ceil_div64(q0 + wave * QPW + QPW - p.window, 64)));
   ju = max(ju, jl);
   int64_t j = j0;
+  if constexpr (SINK)
+    for (int64_t i = 0; i < ns; ++i) step(i, BoolTag<true>{});
   for (; j < jl; ++j) step(j, BoolTag<true>{});
   for (; j < ju; ++j) step(j, BoolTag<false>{});
   for (; j < nkb; ++j) step(j, BoolTag<true>{});
@@ -711,6 +723,9 @@ struct AttnBwdArgs {
   float* ndelta;  // [B, H, Sq]: -D, written by attn_bwd_delta
   float* nlse2;   // [B, H, Sq]: -LSE * log2(e), written by attn_bwd_delta
   float* kv_part; // grouped backward: per-query-head dK, dV partials (f32), or null
+  float* sink_part;    // sinks: partials of the sinks' key blocks (attn_bwd_gqa_dkv)
+  int sink_blocks;     // 64-key blocks that hold sinks
+  int sink_chunks;     // blocks that share the queries behind such a block's window
   // (stored negated: the dK/dV and dQ steps add them, which saves a negation
   // per score)
 };
@@ -1351,7 +1366,14 @@ constexpr int kGqaDkvLds = 2 * (2 * KvLayout<D>::TILE + 512);  // 2 stages of Q,
 template <int D>
 constexpr int kGqaDqLds = 2 * (2 * KvLayout<D>::TILE);  // 2 stages of K, V
 
-template <typename T, int D>
+// SINK: sinks are seen by every later query, so a block of keys that holds
+// some would walk the whole sequence while the others walk a window.  The
+// steps behind its window go to sink_chunks further blocks (first in the
+// grid), and all of a sink block's results leave as f32 partials
+// [dK, dV][slot][b][h][sink key][D] that attn_bwd_gqa_sum adds in slot order:
+// slot 0 is the block's own window (with grouped heads that is in kv_part),
+// slot 1 + c chunk c.
+template <typename T, int D, bool SINK = false>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
@@ -1361,7 +1383,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
   const AttnArgs& f = p.f;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int lr = lane & 15, lg = lane >> 4;
-  const int64_t k0 = (int64_t)blockIdx.x * 64;
+  const int nextra = SINK ? p.sink_blocks * p.sink_chunks : 0;
+  const bool extra = SINK && (int)blockIdx.x < nextra;
+  const int64_t k0 = (extra ? (int64_t)blockIdx.x % p.sink_blocks : (int64_t)blockIdx.x - nextra) * 64;
   // with partials, block (x, hk * group + gi) takes query head gi of the
   // group alone; without, it walks the whole group
   const int64_t hsplit = p.kv_part ? f.group : 1;
@@ -1382,8 +1406,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
   // queries that can see keys k0 .. k0 + 63, in 64-query steps from qstart
   int64_t qhi = f.Sq;
   if (f.window > 0) qhi = min(qhi, k0 + 63 + f.window);
-  const int64_t qstart = f.causal ? (k0 / 64) * 64 : 0;
-  const int64_t nqb = qhi > qstart ? (qhi - qstart + 63) / 64 : 0;
+  int64_t qstart = f.causal ? (k0 / 64) * 64 : 0;
+  int64_t nqb = qhi > qstart ? (qhi - qstart + 63) / 64 : 0;
+  if (extra) {  // this chunk's share of the steps behind the window
+    qstart += nqb * 64;
+    const int64_t rest = ceil_div64(f.Sq - qstart, 64), per = ceil_div64(rest, p.sink_chunks);
+    const int64_t first = (int64_t)blockIdx.x / p.sink_blocks * per;
+    qstart += first * 64;
+    nqb = max((int64_t)0, min(per, rest - first));
+  }
   const int64_t nheads = p.kv_part ? 1 : f.group;
   const int64_t total = nqb * nheads;  // steps over (query head, query block)
   const int64_t qs_b = f.q_s * (int64_t)sizeof(T), dos_b = p.do_s * (int64_t)sizeof(T);
@@ -1417,14 +1448,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
     if constexpr (MASK) {
       const int64_t lo64 = f.causal ? max((int64_t)0, kq + lr) : 0;
       int64_t hi = min((int64_t)64, f.Sq - qb0);
-      if (f.window > 0) hi = min(hi, kq + lr + f.window);
+      if (f.window > 0 && !(SINK && kj < f.sinks)) hi = min(hi, kq + lr + f.window);
       lo = (int)min((int64_t)64, lo64);
       span = kj < f.Skv ? (int)max((int64_t)0, hi - lo64) : 0;
     }
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
       if (MASK && f.causal && qs * 32 + 31 < kq) continue;                // every query before every key
-      if (MASK && f.window > 0 && qs * 32 >= kq + 15 + f.window) continue;  // past every key's window
+      if (MASK && f.window > 0 && qs * 32 >= kq + 15 + f.window && !(SINK && kw < f.sinks)) continue;  // past every key's window
       f32x4 pt[2], ds[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -1473,13 +1504,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
     buf ^= 1;
     const int64_t qb0 = qstart + (st % nqb) * 64;
     if (f.causal && kw > qb0 + 63) continue;                     // every query before every key
-    if (f.window > 0 && qb0 >= kw + 15 + f.window) continue;     // past every key's window
+    if (f.window > 0 && qb0 >= kw + 15 + f.window && !(SINK && kw < f.sinks)) continue;  // past every key's window
     const bool inside = (!f.causal || qb0 >= kw + 15) && (f.window <= 0 || qb0 + 63 < kw + f.window) &&
                         qb0 + 64 <= f.Sq && kw + 16 <= f.Skv;
     if (inside) compute(Qt, qb0, BoolTag<false>{});
     else compute(Qt, qb0, BoolTag<true>{});
   }
-  if (kj < f.Skv && p.kv_part) {
+  if (SINK && kj < f.Skv && (extra || (!p.kv_part && k0 / 64 < p.sink_blocks))) {
+    const int64_t slots = p.sink_chunks + 1, keys = (int64_t)p.sink_blocks * 64;
+    const int64_t slot = extra ? 1 + (int64_t)blockIdx.x / p.sink_blocks : 0;
+    float* pk = p.sink_part + (((slot * f.B + b) * f.H + hk * f.group + gfirst) * keys + kj) * D;
+    const int64_t plane = slots * f.B * f.H * keys * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      *(float4*)(pk + dt * 16 + lg * 4) = float4{dka[dt][0], dka[dt][1], dka[dt][2], dka[dt][3]};
+      *(float4*)(pk + plane + dt * 16 + lg * 4) = float4{dva[dt][0], dva[dt][1], dva[dt][2], dva[dt][3]};
+    }
+  } else if (kj < f.Skv && p.kv_part) {
     // f32 partials [gi][b][hk][key][D], dK's then dV's; summed by attn_bwd_gqa_sum
     const int64_t hkn = f.H / f.group, plane = f.group * f.B * hkn * f.Skv * D;
     float* pk = p.kv_part + (((gfirst * f.B + b) * hkn + hk) * f.Skv + kj) * D;
@@ -1507,21 +1548,32 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
 
 // dK = scale * sum over the group's query heads of the dK partials, dV = the
 // sum of the dV partials, in head order (deterministic); four head-dim
-// elements per thread.
-template <typename T, int D>
+// elements per thread.  SINK: a sink block's rows add their slots' partials,
+// head by head; without grouped heads those rows are all there is to do.
+template <typename T, int D, bool SINK = false>
 __global__ void __launch_bounds__(kThreads) attn_bwd_gqa_sum(AttnBwdArgs p) {
   const AttnArgs& f = p.f;
   const int64_t hkn = f.H / f.group, rows = f.B * hkn * f.Skv, plane = f.group * rows * D;
-  const int64_t i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;  // over rows * D / 4
-  if (i4 >= rows * (D / 4)) return;
-  const int64_t row = i4 / (D / 4), d = (i4 - row * (D / 4)) * 4;
-  const int64_t key = row % f.Skv, bh = row / f.Skv, hk = bh % hkn, b = bh / hkn;
+  const int64_t sinks = SINK ? min(f.Skv, (int64_t)p.sink_blocks * 64) : 0;  // keys with slots
+  const int64_t keys = SINK && !p.kv_part ? sinks : f.Skv;                  // keys summed here
+  const int64_t i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;          // over B * hkn * keys * D / 4
+  if (i4 >= f.B * hkn * keys * (D / 4)) return;
+  const int64_t krow = i4 / (D / 4), d = (i4 - krow * (D / 4)) * 4;
+  const int64_t key = krow % keys, bh = krow / keys, hk = bh % hkn, b = bh / hkn;
+  const int64_t row = bh * f.Skv + key;
   float4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
-  for (int64_t g = 0; g < f.group; ++g) {
-    const float4 a = *(const float4*)(p.kv_part + g * rows * D + row * D + d);
-    const float4 c = *(const float4*)(p.kv_part + plane + g * rows * D + row * D + d);
+  auto add = [&](const float* pk, int64_t to_v) {
+    const float4 a = *(const float4*)pk, c = *(const float4*)(pk + to_v);
     sk.x += a.x, sk.y += a.y, sk.z += a.z, sk.w += a.w;
     sv.x += c.x, sv.y += c.y, sv.z += c.z, sv.w += c.w;
+  };
+  for (int64_t g = 0; g < f.group; ++g) {
+    if (!SINK || p.kv_part) add(p.kv_part + g * rows * D + row * D + d, plane);
+    if (SINK && key < sinks) {
+      const int64_t padded = (int64_t)p.sink_blocks * 64, step = f.B * f.H * padded * D;
+      const float* pk = p.sink_part + ((b * f.H + hk * f.group + g) * padded + key) * D + d;
+      for (int c = p.kv_part ? 1 : 0; c <= p.sink_chunks; ++c) add(pk + c * step, (p.sink_chunks + 1) * step);
+    }
   }
   V4<T> k4, v4;
   k4.v[0] = (T)(sk.x * f.scale), k4.v[1] = (T)(sk.y * f.scale), k4.v[2] = (T)(sk.z * f.scale), k4.v[3] = (T)(sk.w * f.scale);
@@ -1530,7 +1582,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_gqa_sum(AttnBwdArgs p) {
   *(V4<T>*)((T*)p.dv + b * p.dv_b + hk * p.dv_h + key * p.dv_s + d) = v4;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SINK = false>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
@@ -1564,7 +1616,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
   if (f.causal) khi = min(khi, q0 + 64);
   const int64_t klo = f.window > 0 ? max((int64_t)0, q0 - f.window + 1) : 0;
   const int64_t kstart = (klo / 64) * 64;
-  const int64_t nkb = khi > kstart ? (khi - kstart + 63) / 64 : 0;
+  // tiles of sinks before the window's come first
+  const int64_t ns = SINK ? min(ceil_div64(min(f.sinks, f.Skv), 64), kstart / 64) : 0;
+  const int64_t nkb = ns + (khi > kstart ? (khi - kstart + 63) / 64 : 0);
+  auto tile_key = [&](int64_t j) { return SINK && j < ns ? j * 64 : kstart + (j - ns) * 64; };
   KvTileLoad<D, 4> kl, vl;
   kl.init((const char*)((const T*)f.k + b * f.k_b + hk * f.k_h), f.k_s * (int64_t)sizeof(T));
   vl.init((const char*)((const T*)f.v + b * f.v_b + hk * f.v_h), f.v_s * (int64_t)sizeof(T));
@@ -1575,19 +1630,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
     constexpr bool MASK = decltype(mask_tag)::value;
     const char* Vt = Kt + L::TILE;
     const int64_t qk = qw - kb0;  // query row 0 minus key row 0
-    // key rows lo <= kr < lo + span are visible to this lane's query
-    int lo = 0, span = 64;
+    // key rows lo <= kr < lo + span are visible to this lane's query, and
+    // those of sinks, kr < ls
+    int lo = 0, span = 64, ls = 0;
     if constexpr (MASK) {
       const int64_t lo64 = f.window > 0 ? max((int64_t)0, qk + lr - f.window + 1) : 0;
       int64_t hi = min((int64_t)64, f.Skv - kb0);
       if (f.causal) hi = min(hi, qk + lr + 1);
       lo = (int)min((int64_t)64, lo64);
       span = qok ? (int)max((int64_t)0, hi - lo64) : 0;
+      if (SINK && qok) ls = (int)max((int64_t)0, min(hi, f.sinks - kb0));
     }
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
       if (MASK && f.causal && ks2 * 32 > qk + 15) continue;                      // after every query
-      if (MASK && f.window > 0 && ks2 * 32 + 31 < qk - f.window + 1) continue;  // before every window
+      if (MASK && f.window > 0 && ks2 * 32 + 31 < qk - f.window + 1 && !(SINK && kb0 + ks2 * 32 < f.sinks))
+        continue;  // before every window
       f32x4 ds[2];
 #pragma unroll
       for (int v2 = 0; v2 < 2; ++v2) {
@@ -1602,7 +1660,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = fmaf(sa[e], c, nl2);
-          if constexpr (MASK) x = (unsigned)(kt * 16 + 4 * lg + e - lo) < (unsigned)span ? x : -INFINITY;
+          if constexpr (MASK) {
+            const int key = kt * 16 + 4 * lg + e;
+            x = (unsigned)(key - lo) < (unsigned)span || (SINK && key < ls) ? x : -INFINITY;
+          }
           ds[v2][e] = fast_exp2(x) * pa[e];
         }
       }
@@ -1619,22 +1680,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
   };
   int buf = 0;
   if (nkb > 0) {
-    kl.issue(kstart, f.Skv, lds);
-    vl.issue(kstart, f.Skv, lds + L::TILE);
+    kl.issue(tile_key(0), f.Skv, lds);
+    vl.issue(tile_key(0), f.Skv, lds + L::TILE);
   }
   for (int64_t j = 0; j < nkb; ++j) {
-    const int64_t kb0 = kstart + j * 64;
+    const int64_t kb0 = tile_key(j);
     __builtin_amdgcn_s_waitcnt(0xc07f & 0x3f70);  // vmcnt(0)
     __syncthreads();
     if (j + 1 < nkb) {
       char* nx = lds + (buf ^ 1) * STAGE;
-      kl.issue(kb0 + 64, f.Skv, nx);
-      vl.issue(kb0 + 64, f.Skv, nx + L::TILE);
+      kl.issue(tile_key(j + 1), f.Skv, nx);
+      vl.issue(tile_key(j + 1), f.Skv, nx + L::TILE);
     }
     const char* Kt = lds + buf * STAGE;
     buf ^= 1;
     if (f.causal && kb0 > qw + 15) continue;                           // every key after every query
-    if (f.window > 0 && kb0 + 63 < qw - f.window + 1) continue;        // before every query's window
+    if (f.window > 0 && kb0 + 63 < qw - f.window + 1 && !(SINK && kb0 < f.sinks)) continue;  // before every query's window
     const bool inside = (!f.causal || kb0 + 63 <= qw) && (f.window <= 0 || kb0 > qw + 15 - f.window) &&
                         kb0 + 64 <= f.Skv && qw + 16 <= f.Sq;
     if (inside) compute(Kt, kb0, BoolTag<false>{});
@@ -1669,15 +1730,15 @@ int check_common(int64_t B, int64_t H, int64_t Sq, int64_t Skv, int64_t D, int d
   return MI355X_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SINK = false>
 int fwd_launch(const AttnArgs& a, hipStream_t s) {
   if constexpr (D == 256) {
     // 64-query blocks of 4 waves x 16 queries; K/V stages need 128 KB of LDS
     constexpr int NW = 4, QPW = 16;
     constexpr size_t kLds = 4 * KvLayout<256>::TILE;
     dim3 grid(ceil_div(a.Sq, NW * QPW), (unsigned)a.H, (unsigned)a.B);
-    auto kp = attn_fwd_v2<T, D, true, NW, QPW>;
-    auto kn = attn_fwd_v2<T, D, false, NW, QPW>;
+    auto kp = attn_fwd_v2<T, D, true, NW, QPW, SINK>;
+    auto kn = attn_fwd_v2<T, D, false, NW, QPW, SINK>;
     static bool attr = false;
     if (!attr) {
       if (hipFuncSetAttribute((const void*)kp, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds) != hipSuccess ||
@@ -1693,8 +1754,8 @@ int fwd_launch(const AttnArgs& a, hipStream_t s) {
   if constexpr (D == 64 || D == 128) {
     constexpr int NW = D == 64 ? ATTN_FWD_WAVES : 4;
     constexpr int QPW = 128 / NW;
-    if (a.scale_log2 > 0.f) attn_fwd_v2<T, D, true, NW, QPW><<<grid, 64 * NW, 0, s>>>(a);
-    else attn_fwd_v2<T, D, false, NW, QPW><<<grid, 64 * NW, 0, s>>>(a);
+    if (a.scale_log2 > 0.f) attn_fwd_v2<T, D, true, NW, QPW, SINK><<<grid, 64 * NW, 0, s>>>(a);
+    else attn_fwd_v2<T, D, false, NW, QPW, SINK><<<grid, 64 * NW, 0, s>>>(a);
   }
   else if (a.scale_log2 > 0.f) attn_fwd_kernel<T, D, true><<<grid, kThreads, 0, s>>>(a);
   else attn_fwd_kernel<T, D, false><<<grid, kThreads, 0, s>>>(a);
@@ -1745,13 +1806,23 @@ int bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
     return FN<f16, 128>(__VA_ARGS__);                                         \
   } while (0)
 
-template <typename T, int D>
+// Blocks that share the steps behind a sink block's window: as many steps
+// each as a block of the window has, and eight at least.
+int sink_chunks(int64_t sq, int64_t window) {
+  const int64_t own = (window + 126) / 64, rest = (sq + 63) / 64 - own;
+  if (rest <= 0) return 0;
+  const int64_t n = (rest + std::max<int64_t>(own, 8) - 1) / std::max<int64_t>(own, 8);
+  return (int)std::min<int64_t>(n, 256);
+}
+int sink_blocks(int64_t skv, int64_t sinks) { return (int)((std::min(skv, sinks) + 63) / 64); }
+
+template <typename T, int D, bool SINK = false>
 int gqa_bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
   const int64_t rows = a.f.B * a.f.H * a.f.Sq;
   MI_REQUIRE(rows < (1ll << 31), "mi355x_attn_bwd: batch x heads x query rows must be below 2^31");
   attn_bwd_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
-  auto kkv = attn_bwd_gqa_dkv<T, D>;
-  auto kq = attn_bwd_gqa_dq<T, D>;
+  auto kkv = attn_bwd_gqa_dkv<T, D, SINK>;
+  auto kq = attn_bwd_gqa_dq<T, D, SINK>;
   constexpr int lkv = kGqaDkvLds<D>, lq = kGqaDqLds<D>;
   static std::once_flag once;
   static hipError_t attr_err = hipSuccess;
@@ -1764,11 +1835,13 @@ int gqa_bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
     return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_gen: cannot raise the LDS limit: %s", hipGetErrorString(attr_err));
   // grouped heads: one dK/dV block per (key block, query head), partials summed after
   const unsigned gy = (unsigned)(a.kv_part ? a.f.H : a.f.H / a.f.group);
-  kkv<<<dim3(ceil_div(a.f.Skv, 64), gy, (unsigned)a.f.B), kThreads, lkv, s>>>(a);
+  const unsigned extra = SINK ? (unsigned)(a.sink_blocks * a.sink_chunks) : 0;
+  kkv<<<dim3(ceil_div(a.f.Skv, 64) + extra, gy, (unsigned)a.f.B), kThreads, lkv, s>>>(a);
   kq<<<dim3(ceil_div(a.f.Sq, 64), (unsigned)a.f.H, (unsigned)a.f.B), kThreads, lq, s>>>(a);
-  if (a.kv_part) {
-    const int64_t n4 = a.f.B * (a.f.H / a.f.group) * a.f.Skv * (D / 4);
-    attn_bwd_gqa_sum<T, D><<<ceil_div(n4, kThreads), kThreads, 0, s>>>(a);
+  if (a.kv_part || SINK) {
+    const int64_t keys = a.kv_part ? a.f.Skv : std::min<int64_t>(a.f.Skv, (int64_t)a.sink_blocks * 64);
+    const int64_t n4 = a.f.B * (a.f.H / a.f.group) * keys * (D / 4);
+    attn_bwd_gqa_sum<T, D, SINK><<<ceil_div(n4, kThreads), kThreads, 0, s>>>(a);
   }
   return check_launch("mi355x_attn_bwd_gen");
 }
@@ -1786,7 +1859,7 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
                           const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                           const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d,
-                          double scale, int causal, int64_t window, int dtype, void* workspace,
+                          double scale, int causal, int64_t window, int64_t sinks, int dtype, void* workspace,
                           hipStream_t stream) {
   if ((dtype != MI355X_BF16 && dtype != MI355X_F16) || (d != 64 && d != 128 && d != 256)) return -1;
   if (kv_heads < 1 || heads % kv_heads != 0 || heads / kv_heads > 65535 || batch >= 65536) return -1;
@@ -1801,7 +1874,7 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
   a.f = AttnArgs{(void*)o, o_bhs[0], o_bhs[1], o_bhs[2], (float*)lse, q, q_bhs[0], q_bhs[1], q_bhs[2],
                  k, k_bhs[0], k_bhs[1], k_bhs[2], v, v_bhs[0], v_bhs[1], v_bhs[2],
                  batch, heads, sq, skv, (float)(scale * 1.4426950408889634), (float)scale, causal,
-                 heads / kv_heads, window};
+                 heads / kv_heads, window, sinks};
   a.dout = dout; a.do_b = do_bhs[0]; a.do_h = do_bhs[1]; a.do_s = do_bhs[2];
   a.dq = dq; a.dq_b = dq_bhs[0]; a.dq_h = dq_bhs[1]; a.dq_s = dq_bhs[2];
   a.dk = dk; a.dk_b = dk_bhs[0]; a.dk_h = dk_bhs[1]; a.dk_s = dk_bhs[2];
@@ -1813,9 +1886,42 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
                   ? (float*)(((uintptr_t)(a.nlse2 + batch * heads * sq) + 255) & ~(uintptr_t)255)
                   : nullptr;
   const bool bf = dtype == MI355X_BF16;
+  if (sinks > 0) {
+    a.sink_blocks = sink_blocks(skv, sinks), a.sink_chunks = sink_chunks(sq, window);
+    float* end = a.kv_part ? a.kv_part + 2 * batch * heads * skv * d : a.nlse2 + batch * heads * sq;
+    a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
+    if (d == 64) return bf ? gqa_bwd_launch<bf16, 64, true>(a, stream) : gqa_bwd_launch<f16, 64, true>(a, stream);
+    if (d == 128) return bf ? gqa_bwd_launch<bf16, 128, true>(a, stream) : gqa_bwd_launch<f16, 128, true>(a, stream);
+    return bf ? gqa_bwd_launch<bf16, 256, true>(a, stream) : gqa_bwd_launch<f16, 256, true>(a, stream);
+  }
   if (d == 64) return bf ? gqa_bwd_launch<bf16, 64>(a, stream) : gqa_bwd_launch<f16, 64>(a, stream);
   if (d == 128) return bf ? gqa_bwd_launch<bf16, 128>(a, stream) : gqa_bwd_launch<f16, 128>(a, stream);
   return bf ? gqa_bwd_launch<bf16, 256>(a, stream) : gqa_bwd_launch<f16, 256>(a, stream);
+}
+
+// Bytes that attn_bwd_grouped_mfma needs for sinks, behind its other parts.
+int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
+                            int64_t sinks) {
+  return 2 * (sink_chunks(sq, window) + 1) * batch * heads * sink_blocks(skv, sinks) * 64 * d * (int64_t)sizeof(float) + 256;
+}
+
+// MFMA forward of a window with sinks, called by mi355x_attn_fwd_sink
+// (attention_generic.hip); -1 for inputs it does not take.
+int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
+                       const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
+                       int64_t window, int64_t sinks, int dtype, hipStream_t stream) {
+  if ((dtype != MI355X_BF16 && dtype != MI355X_F16) || (d != 64 && d != 128 && d != 256)) return -1;
+  if (!(strides_ok(q, q_bhs) && strides_ok(k, k_bhs) && strides_ok(v, v_bhs))) return -1;
+  if ((uintptr_t)o % 8 || o_bhs[0] % 4 || o_bhs[1] % 4 || o_bhs[2] % 4) return -1;
+  AttnArgs a{(void*)o, o_bhs[0], o_bhs[1], o_bhs[2], lse, q, q_bhs[0], q_bhs[1], q_bhs[2],
+             k, k_bhs[0], k_bhs[1], k_bhs[2], v, v_bhs[0], v_bhs[1], v_bhs[2],
+             batch, heads, sq, skv, (float)(scale * 1.4426950408889634), (float)scale, 1,
+             heads / kv_heads, window, sinks};
+  const bool bf = dtype == MI355X_BF16;
+  if (d == 64) return bf ? fwd_launch<bf16, 64, true>(a, stream) : fwd_launch<f16, 64, true>(a, stream);
+  if (d == 128) return bf ? fwd_launch<bf16, 128, true>(a, stream) : fwd_launch<f16, 128, true>(a, stream);
+  return bf ? fwd_launch<bf16, 256, true>(a, stream) : fwd_launch<f16, 256, true>(a, stream);
 }
 
 }  // namespace mi
@@ -1842,7 +1948,7 @@ extern "C" int mi355x_attn_fwd_ex(void* o, const int64_t* o_bhs, float* lse, con
   AttnArgs a{o, o_bhs[0], o_bhs[1], o_bhs[2], lse, q, q_bhs[0], q_bhs[1], q_bhs[2],
              k, k_bhs[0], k_bhs[1], k_bhs[2], v, v_bhs[0], v_bhs[1], v_bhs[2],
              batch, heads, sq, skv, (float)(scale * 1.4426950408889634), (float)scale, causal,
-             heads / kv_heads, window};
+             heads / kv_heads, window, 0};
   MI_ATTN_FWD_DISPATCH(dtype, d, fwd_launch, a, (hipStream_t)stream);
 }
 

@@ -54,14 +54,31 @@ struct GenArgs {
   float scale_log2, scale;
   int causal;
   int64_t window;
+  int64_t sinks;  // with a window: first keys that every later query sees
 };
 
 __device__ __forceinline__ bool visible(const GenArgs& p, int64_t i, int64_t j) {
   if (j >= p.Skv) return false;
   if (p.causal && j > i) return false;
-  if (p.window > 0 && i - j >= p.window) return false;
+  if (p.window > 0 && i - j >= p.window && j >= p.sinks) return false;
   return true;
 }
+
+// First key of the block's `it`-th tile: the tiles of sinks that lie before
+// kbeg, the window's first tile, then those from kbeg on.
+struct GenTiles {
+  int64_t kbeg, ns;
+  __device__ __forceinline__ GenTiles(const GenArgs& p, int64_t kb, int tile) {
+    kbeg = kb / tile * tile;
+    ns = p.window > 0 ? min((min(p.sinks, p.Skv) + tile - 1) / tile, kbeg / tile) : 0;
+  }
+  __device__ __forceinline__ int64_t count(int64_t kend, int tile) const {
+    return ns + (kend > kbeg ? (kend - kbeg + tile - 1) / tile : 0);
+  }
+  __device__ __forceinline__ int64_t key(int64_t it, int tile) const {
+    return it < ns ? it * tile : kbeg + (it - ns) * tile;
+  }
+};
 
 // Sum over the 8 lanes of a row group.
 __device__ __forceinline__ float row_sum8(float x) {
@@ -128,8 +145,10 @@ __global__ void __launch_bounds__(kGT) gen_fwd(GenArgs p) {
   int64_t kbeg = 0, kend = p.Skv;
   if (p.causal) kend = min(kend, qlast + 1);
   if (p.window > 0) kbeg = max((int64_t)0, q0 - p.window + 1);
-  kbeg = kbeg / kTile * kTile;
-  for (int64_t kb0 = kbeg; kb0 < kend; kb0 += kTile) {
+  const GenTiles tiles(p, kbeg, kTile);
+  const int64_t nt = tiles.count(kend, kTile);
+  for (int64_t it = 0; it < nt; ++it) {
+    const int64_t kb0 = tiles.key(it, kTile);
     __syncthreads();
     stage_rows<T, DP, kTile>(Ks, K, p.k_s, kb0, p.Skv, p.D);
     stage_rows<T, DP, kTile>(Vs, V, p.v_s, kb0, p.Skv, p.D);
@@ -214,8 +233,10 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dq(GenArgs p) {
   int64_t kbeg = 0, kend = p.Skv;
   if (p.causal) kend = min(kend, qlast + 1);
   if (p.window > 0) kbeg = max((int64_t)0, q0 - p.window + 1);
-  kbeg = kbeg / kTile * kTile;
-  for (int64_t kb0 = kbeg; kb0 < kend; kb0 += kTile) {
+  const GenTiles tiles(p, kbeg, kTile);
+  const int64_t nt = tiles.count(kend, kTile);
+  for (int64_t it = 0; it < nt; ++it) {
+    const int64_t kb0 = tiles.key(it, kTile);
     __syncthreads();
     stage_rows<T, DP, kTile>(Ks, K, p.k_s, kb0, p.Skv, p.D);
     stage_rows<T, DP, kTile>(Vs, V, p.v_s, kb0, p.Skv, p.D);
@@ -264,7 +285,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dkv(GenArgs p) {
   const int64_t klast = min(p.Skv, k0 + kRows) - 1;
   int64_t qbeg = 0, qend = p.Sq;
   if (p.causal) qbeg = k0;
-  if (p.window > 0) qend = min(qend, klast + p.window);
+  if (p.window > 0 && k0 >= p.sinks) qend = min(qend, klast + p.window);
   qbeg = qbeg / kTile * kTile;
   for (int64_t r = 0; r < g; ++r) {
     const int64_t h = hk * g + r;
@@ -362,7 +383,7 @@ int gen_bwd_launch(const GenArgs& a, hipStream_t s) {
 
 GenArgs gen_args(const void* q, const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                  const int64_t* v_bhs, int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
-                 int64_t d, double scale, int causal, int64_t window) {
+                 int64_t d, double scale, int causal, int64_t window, int64_t sinks = 0) {
   GenArgs a{};
   a.q = q; a.q_b = q_bhs[0]; a.q_h = q_bhs[1]; a.q_s = q_bhs[2];
   a.k = k; a.k_b = k_bhs[0]; a.k_h = k_bhs[1]; a.k_s = k_bhs[2];
@@ -372,6 +393,7 @@ GenArgs gen_args(const void* q, const int64_t* q_bhs, const void* k, const int64
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.causal = causal;
   a.window = window;
+  a.sinks = sinks;
   return a;
 }
 
@@ -420,8 +442,14 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
                           const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                           const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d,
-                          double scale, int causal, int64_t window, int dtype, void* workspace,
+                          double scale, int causal, int64_t window, int64_t sinks, int dtype, void* workspace,
                           hipStream_t stream);
+int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
+                            int64_t sinks);
+int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
+                       const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
+                       int64_t window, int64_t sinks, int dtype, hipStream_t stream);
 }  // namespace mi
 
 // Two floats per query row (the MFMA path keeps -D and -LSE log2(e), the f32
@@ -434,25 +462,24 @@ extern "C" int64_t mi355x_attn_bwd_gen_workspace_bytes(int64_t batch, int64_t he
   return bytes;
 }
 
-extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
+static int attn_bwd_any(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
                                    const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
                                    const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                                    const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
-                                   int64_t d, double scale, int causal, int64_t window, int dtype,
-                                   void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
-  int rc = gen_check(batch, heads, kv_heads, sq, skv, d, dtype, causal, window, "mi355x_attn_bwd_gen");
+                                   int64_t d, double scale, int causal, int64_t window, int64_t sinks, int dtype,
+                                   void* workspace, int64_t ws_bytes, int64_t need, const char* what,
+                                   mi355x_stream_t stream) {
+  int rc = gen_check(batch, heads, kv_heads, sq, skv, d, dtype, causal, window, what);
   if (rc) return rc;
-  MI_REQUIRE(dq && dk && dv && dout && q && k && v && o && lse, "mi355x_attn_bwd_gen: null pointer");
-  const int64_t need = mi355x_attn_bwd_gen_workspace_bytes(batch, heads, kv_heads, sq, skv, d);
+  MI_REQUIRE(dq && dk && dv && dout && q && k && v && o && lse, "%s: null pointer", what);
   if (!workspace || ws_bytes < need)
-    return fail(MI355X_EWORKSPACE, "mi355x_attn_bwd_gen: workspace %lld < %lld", (long long)ws_bytes,
-                (long long)need);
+    return fail(MI355X_EWORKSPACE, "%s: workspace %lld < %lld", what, (long long)ws_bytes, (long long)need);
   const int mrc = attn_bwd_grouped_mfma(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v,
                                         v_bhs, o, o_bhs, lse, batch, heads, kv_heads, sq, skv, d, scale, causal,
-                                        window, dtype, workspace, (hipStream_t)stream);
+                                        window, sinks, dtype, workspace, (hipStream_t)stream);
   if (mrc >= 0) return mrc;  // bf16/f16 at head_dim 64/128/256: MFMA kernels
-  GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, causal, window);
+  GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, causal, window, sinks);
   a.o = (void*)o; a.o_b = o_bhs[0]; a.o_h = o_bhs[1]; a.o_s = o_bhs[2];
   a.lse = (float*)lse;
   a.dout = dout; a.do_b = do_bhs[0]; a.do_h = do_bhs[1]; a.do_s = do_bhs[2];
@@ -466,4 +493,57 @@ extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, co
     if (rc >= 0) return rc;
   }
   MI_GEN_DISPATCH(dtype, d, gen_bwd_launch, a, (hipStream_t)stream);
+}
+
+extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
+                                   const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
+                                   const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
+                                   const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
+                                   int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                                   int64_t d, double scale, int causal, int64_t window, int dtype,
+                                   void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
+  return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
+                      batch, heads, kv_heads, sq, skv, d, scale, causal, window, 0, dtype, workspace, ws_bytes,
+                      mi355x_attn_bwd_gen_workspace_bytes(batch, heads, kv_heads, sq, skv, d), "mi355x_attn_bwd_gen",
+                      stream);
+}
+
+// A window with sinks: causal, query i sees key j iff i - j < window or j <
+// sinks.
+extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
+                                    const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
+                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                                    int64_t d, double scale, int64_t window, int64_t sinks, int dtype,
+                                    mi355x_stream_t stream) {
+  int rc = gen_check(batch, heads, kv_heads, sq, skv, d, dtype, 1, window, "mi355x_attn_fwd_sink");
+  if (rc) return rc;
+  MI_REQUIRE(o && lse && q && k && v, "mi355x_attn_fwd_sink: null pointer");
+  MI_REQUIRE(window > 0 && sinks > 0, "mi355x_attn_fwd_sink: window and sinks must be positive");
+  rc = attn_fwd_sink_mfma(o, o_bhs, lse, q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale,
+                          window, sinks, dtype, (hipStream_t)stream);
+  if (rc >= 0) return rc;
+  GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks);
+  a.o = o; a.o_b = o_bhs[0]; a.o_h = o_bhs[1]; a.o_s = o_bhs[2];
+  a.lse = lse;
+  MI_GEN_DISPATCH(dtype, d, gen_fwd_launch, a, (hipStream_t)stream);
+}
+
+extern "C" int64_t mi355x_attn_bwd_sink_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq,
+                                                        int64_t skv, int64_t d, int64_t window, int64_t sinks) {
+  return mi355x_attn_bwd_gen_workspace_bytes(batch, heads, kv_heads, sq, skv, d) +
+         attn_bwd_sink_bytes(batch, heads, sq, skv, d, window, sinks);
+}
+
+extern "C" int mi355x_attn_bwd_sink(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
+                                    const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
+                                    const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
+                                    const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
+                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                                    int64_t d, double scale, int64_t window, int64_t sinks, int dtype,
+                                    void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
+  MI_REQUIRE(window > 0 && sinks > 0, "mi355x_attn_bwd_sink: window and sinks must be positive");
+  return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
+                      batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks, dtype, workspace, ws_bytes,
+                      mi355x_attn_bwd_sink_workspace_bytes(batch, heads, kv_heads, sq, skv, d, window, sinks),
+                      "mi355x_attn_bwd_sink", stream);
 }

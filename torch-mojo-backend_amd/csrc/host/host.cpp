@@ -185,6 +185,7 @@ struct Call<R (*)(A...), Tag> {
   X(mi355x_rms_norm_fwd) X(mi355x_rms_norm_bwd) X(mi355x_rope) X(mi355x_geglu_fwd) X(mi355x_geglu_bwd)   \
   X(mi355x_attn_fwd_ex) X(mi355x_attn_bwd_workspace_bytes) X(mi355x_attn_bwd) X(mi355x_attn_fwd_gen)     \
   X(mi355x_attn_bwd_gen_workspace_bytes) X(mi355x_attn_bwd_gen) X(mi355x_attn_bwd_noalloc)              \
+  X(mi355x_attn_fwd_sink) X(mi355x_attn_bwd_sink_workspace_bytes) X(mi355x_attn_bwd_sink)                \
   X(mi355x_paged_append) X(mi355x_paged_gather) X(mi355x_paged_attn_workspace_bytes) X(mi355x_paged_attn)
 
 #define TAG(f)                                         \

@@ -2198,17 +2198,26 @@ def _mfma_bwd_ok(q: MT, group, window) -> bool:
     return q._dtype in _MFMA_DTYPES and group == 1 and window == 0 and q._shape[3] in _FUSED_FA_HEAD_DIMS
 
 
-def attention_forward(q: MT, k: MT, v: MT, causal, window, scale):
+def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=0):
     """(out [B,H,Sq,D] over BTHD storage, lse f32 [B,H,Sq]) of causal / full
     attention with optional grouped K/V heads (k, v with H / g heads) and a
-    causal sliding window: MFMA kernels where they apply, else the f32
-    kernels."""
+    causal sliding window, with `sinks` first keys that stay visible: MFMA
+    kernels where they apply, else the f32 kernels."""
     b, h, sq, d = q._shape
     hk, skv = k._shape[1], k._shape[2]
     scale_value = float(scale) if scale is not None else 1.0 / math.sqrt(d)
     out = alloc_bthd(b, h, sq, d, q._dtype, q._device)
     lse = _alloc((b, h, sq), torch.float32, q._device)
-    if _mfma_fwd_ok(q, h // hk, window):
+    if window and sinks:
+        rows = _fa_head_contig if q._dtype in _MFMA_DTYPES and d in _MFMA_EX_HEAD_DIMS else _unit_head_stride
+        q, k, v = rows(q), rows(k), rows(v)
+        check(
+            "mi355x_attn_fwd_sink",
+            lib().mi355x_attn_fwd_sink(out._ptr, _bhs(out), lse._ptr, q._ptr, _bhs(q), k._ptr, _bhs(k),
+                                       v._ptr, _bhs(v), b, h, hk, sq, skv, d, scale_value, int(window), int(sinks),
+                                       _code(q._dtype), _STREAM),
+        )
+    elif _mfma_fwd_ok(q, h // hk, window):
         q, k, v = _fa_head_contig(q), _fa_head_contig(k), _fa_head_contig(v)
         check(
             "mi355x_attn_fwd_ex",
@@ -2227,7 +2236,7 @@ def attention_forward(q: MT, k: MT, v: MT, causal, window, scale):
     return out, lse
 
 
-def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, window, scale):
+def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, window, scale, sinks=0):
     """(dq, dk, dv) of attention_forward: dk/dv have k's heads (the query
     heads of each group summed)."""
     b, h, sq, d = q._shape
@@ -2248,7 +2257,20 @@ def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, 
         dq = alloc_bthd(b, h, sq, d, q._dtype, q._device)
         dk = alloc_bthd(b, hk, skv, d, q._dtype, q._device)
         dv = alloc_bthd(b, hk, skv, d, q._dtype, q._device)
-    if _mfma_bwd_ok(q, h // hk, window):
+    if window and sinks:
+        rows = _fa_head_contig if q._dtype in _MFMA_DTYPES and d in _MFMA_EX_HEAD_DIMS else _unit_head_stride
+        q, k, v, out, dout = rows(q), rows(k), rows(v), rows(out), rows(grad_out)
+        ws = lib().mi355x_attn_bwd_sink_workspace_bytes(b, h, hk, sq, skv, d, int(window), int(sinks))
+        hold, wptr = _workspace(ws, q._device)
+        check(
+            "mi355x_attn_bwd_sink",
+            lib().mi355x_attn_bwd_sink(
+                dq._ptr, _bhs(dq), dk._ptr, _bhs(dk), dv._ptr, _bhs(dv), dout._ptr, _bhs(dout),
+                q._ptr, _bhs(q), k._ptr, _bhs(k), v._ptr, _bhs(v), out._ptr, _bhs(out), lse._ptr,
+                b, h, hk, sq, skv, d, scale_value, int(window), int(sinks), _code(q._dtype), wptr, ws, _STREAM,
+            ),
+        )
+    elif _mfma_bwd_ok(q, h // hk, window):
         q, k, v = _fa_head_contig(q), _fa_head_contig(k), _fa_head_contig(v)
         out, dout = _fa_head_contig(out), _fa_head_contig(grad_out)
         ws = lib().mi355x_attn_bwd_workspace_bytes(b, h, sq, skv, d)
@@ -2352,8 +2374,9 @@ def sdpa_math(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False,
 def fused_fa_ex_inputs(query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gqa):
     """Fused attention beyond the flash-pair gate: grouped K/V heads
     (enable_gqa) and a sliding-window causal mask built by
-    torch_mojo_backend.masks.  Returns (q, k, v, causal, window) or None."""
-    from ..masks import window_of
+    torch_mojo_backend.masks.  Returns (q, k, v, causal, window, sinks) or
+    None."""
+    from ..masks import window_and_sinks_of
 
     q, k, v = _t(query), _t(key), _t(value)
     if (
@@ -2375,13 +2398,13 @@ def fused_fa_ex_inputs(query, key, value, attn_mask, dropout_p, is_causal, scale
         return None
     if scale is not None and not math.isfinite(float(scale)):
         return None
-    causal, window = bool(is_causal), 0
+    causal, window, sinks = bool(is_causal), 0, 0
     if attn_mask is not None:
-        w = window_of(attn_mask)
-        if w is None or is_causal or sq != skv:
+        w = window_and_sinks_of(attn_mask)
+        if w is None or is_causal or sq != skv or attn_mask.shape[-1] != skv:
             return None
-        causal, window = True, w
-    return q, k, v, causal, window
+        causal, (window, sinks) = True, w
+    return q, k, v, causal, window, sinks
 
 
 def fast_aten_scaled_dot_product_attention(
@@ -2392,8 +2415,8 @@ def fast_aten_scaled_dot_product_attention(
     masks from torch_mojo_backend.masks), otherwise the decomposition."""
     ex = fused_fa_ex_inputs(query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gqa)
     if ex is not None:
-        q, k, v, causal, window = ex
-        out, _ = attention_forward(q, k, v, causal, window, scale)
+        q, k, v, causal, window, sinks = ex
+        out, _ = attention_forward(q, k, v, causal, window, scale, sinks)
         return out
     return sdpa_math(query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gqa)
 

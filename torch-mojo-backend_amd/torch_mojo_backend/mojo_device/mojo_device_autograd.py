@@ -71,36 +71,36 @@ def _scaled_dot_product_attention_autograd(
         query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gqa
     )
     if ex is not None:
-        _, _, _, causal, window = ex
-        return _FusedAttention.apply(query, key, value, causal, window, scale)
+        _, _, _, causal, window, sinks = ex
+        return _FusedAttention.apply(query, key, value, causal, window, scale, sinks)
     return aten_fast.sdpa_math(
         query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gqa
     )
 
 
 class _FusedAttention(torch.autograd.Function):
-    """Attention with grouped K/V heads and/or a sliding-window causal mask
-    (the Gemma-3-shaped layers), which the ATen flash pair cannot express:
+    """Attention with grouped K/V heads and/or a sliding-window causal mask,
+    with sinks or without (the Gemma-3-shaped layers), which the ATen flash pair cannot express:
     the fused forward saves (q, k, v, out, lse) like the pair does, and the
     fused backward recomputes P from the LSE, summing dK/dV over each
     group's query heads.  The reference differentiates these through its
     masked-math decomposition (aten_fast.py:9112-9123)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, causal, window, scale):
+    def forward(ctx, q, k, v, causal, window, scale, sinks=0):
         with torch._C._AutoDispatchBelowAutograd():
-            out, lse = aten_fast.attention_forward(q, k, v, causal, window, scale)
+            out, lse = aten_fast.attention_forward(q, k, v, causal, window, scale, sinks)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.args = (causal, window, scale)
+        ctx.args = (causal, window, scale, sinks)
         return out
 
     @staticmethod
     def backward(ctx, grad):
         q, k, v, out, lse = ctx.saved_tensors
-        causal, window, scale = ctx.args
+        causal, window, scale, sinks = ctx.args
         with torch._C._AutoDispatchBelowAutograd():
-            dq, dk, dv = aten_fast.attention_backward(grad, q, k, v, out, lse, causal, window, scale)
-        return dq, dk, dv, None, None, None
+            dq, dk, dv = aten_fast.attention_backward(grad, q, k, v, out, lse, causal, window, scale, sinks)
+        return dq, dk, dv, None, None, None, None
 
 
 def register_autograd_ops() -> None:

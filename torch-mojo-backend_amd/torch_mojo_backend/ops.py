@@ -1,6 +1,6 @@
 """Fused ops of the Gemma-3-shaped workload: rotary embedding, GeGLU and
-RMSNorm with a weight offset; and serving's: appending to a paged key/value
-cache and attention over it.
+RMSNorm with a weight offset, attention over a sliding window with sinks; and
+serving's: appending to a paged key/value cache and attention over it.
 
 Torch has no single aten op for these (a model writes them as chains of
 slice / neg / cat / mul / add, gelu + mul, and rms_norm with `1 + w`); the
@@ -18,7 +18,8 @@ import torch
 import torch.nn.functional as F
 
 from . import kv_cache
-from .eager_kernels import aten_fast
+from .eager_kernels import aten_fast, materialize_touched
+from .masks import sliding_window_causal_mask
 from .mojo_device.torch_mojo_tensor import TorchMojoTensor
 
 
@@ -98,6 +99,50 @@ def rms_norm(x, weight, eps, weight_offset=0.0):
             return aten_fast.rms_norm_forward(x, shape, weight, float(eps), float(weight_offset))[0]
         return _FusedRMSNorm.apply(x, shape, weight, float(eps), float(weight_offset))
     return F.rms_norm(x, shape, weight.float() + weight_offset, eps)
+
+
+def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
+    """Causal attention of q [B, H, T, D] over k, v [B, H_kv, T, D] with a
+    sliding window and `sinks` first tokens that stay visible: query i sees key
+    j <= i with i - j < window or j < sinks.  Query head h reads K/V head
+    h // (H // H_kv); scale defaults to D ** -0.5.  Differentiable in q, k and
+    v.  The scores of what is not visible are not computed, and no mask is
+    held: F.scaled_dot_product_attention with a mask of
+    masks.sliding_window_causal_mask runs the same kernels."""
+    what = "sliding_window_attention"
+    window, sinks = int(window), int(sinks)
+    if window <= 0 or sinks < 0:
+        raise ValueError(f"{what}: window {window} must be positive, sinks {sinks} not negative")
+    if any(x.dim() != 4 for x in (q, k, v)) or k.shape != v.shape or q.shape[0] != k.shape[0] \
+            or q.shape[2:] != k.shape[2:]:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} must be"
+                         " [batch, heads, tokens, head_dim] of the same batch, tokens and head_dim")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{what}: {q.shape[1]} heads over {k.shape[1]} K/V heads")
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+        raise TypeError(f"{what}: q, k and v must be of one dtype on one device")
+    if scale is not None and not math.isfinite(float(scale)):
+        raise ValueError(f"{what}: scale {scale} must be finite")
+    t = q.shape[2]
+    if t <= window:
+        window, sinks = t, 0  # plain causal attention
+    if _on_mojo(q, k, v) and q.numel():
+        if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or q.shape[3] > 256:
+            raise NotImplementedError(f"{what}: {q.dtype} with head_dim {q.shape[3]} is not supported"
+                                      " (float32, bfloat16, float16, head_dim up to 256)")
+        if t <= window:
+            window = 0
+        if not _needs_grad(q, k, v):
+            materialize_touched((q, k, v), None, False)
+            return aten_fast.attention_forward(q, k, v, True, window, scale, sinks)[0]
+        from .mojo_device.mojo_device_autograd import _FusedAttention
+
+        materialize_touched((q, k, v), None, False)
+        return _FusedAttention.apply(q, k, v, True, window, scale, sinks)
+    if not q.numel():
+        return q * 1.0
+    return F.scaled_dot_product_attention(
+        q, k, v, attn_mask=sliding_window_causal_mask(t, window, q.device, sinks=sinks), scale=scale, enable_gqa=True)
 
 
 # ---------------------------------------------------------------------------
