@@ -693,8 +693,8 @@ typedef struct {
  * the dense [rope_len][d] tables of rope_dtype, as in mi355x_rope; null: as
  * they are) and values to their pages; q, if given, is turned into q_out,
  * zero at padding.  *_bht: (batch, head, token) strides in elements.
- * 4 bits: per 32 channels minimum = f16(min), scale = f16((max - min) / 15),
- * code = clamp(rint((x - minimum) / scale), 0, 15) in f64, with x clamped to
+ * 4 bits: per 32 channels minimum = f16(f32(min)), scale = f16(f32((max -
+ * min) / 15)), code = clamp(rint((x - minimum) / scale), 0, 15) in f64, with x clamped to
  * +-61440; a group with a NaN or an infinity reads back as NaN. */
 int mi355x_paged_append(const mi355x_paged_cache* cache, const int32_t* table, int64_t table_stride,
                         int64_t table_width, const int32_t* starts, const int32_t* counts, const void* k,

@@ -73,6 +73,23 @@ def test_append_then_gather(dtype, bits, d, page, rope):
                     assert torch.equal(x[p, :, s].nan_to_num(7.0), old[p, :, s].nan_to_num(7.0)), (p, s)
 
 
+def test_scales_round_by_way_of_f32():
+    """(max - min) / 15 just above the middle of two f16 values, nearer to it
+    than f32 resolves: the f32 value is the middle, which goes to the even one."""
+    x = torch.zeros(1, 1, 2, 32)
+    x[..., 1] = -1.0
+    x[..., 0] = torch.tensor([float.fromhex("0x1.d247fep-1"), float.fromhex("0x1.d8d802p-1")])
+    _, scale, low = oracle.quantize(x.double().numpy())
+    direct = ((x[..., 0].double().numpy() + 1.0) / 15.0).astype(np.float16)
+    assert (direct != scale[..., 0]).all()  # the inputs tell the two apart
+    c = PagedKVCache.zeros(1, 2, 1, 32, bits=4)
+    zero = torch.zeros(1, 1, dtype=torch.int32).to("mojo")
+    ops.paged_append(c, zero, zero.view(1), x.to("mojo"), x.to("mojo"))
+    for scales in (c.k_scales, c.v_scales):
+        got = scales.cpu().numpy()[0, 0, :, 0]
+        assert (got[:, 0] == scale[0, 0, :, 0]).all() and (got[:, 1] == low[0, 0, :, 0]).all()
+
+
 def _attention(c, h, starts, counts, t, dtype=None, window=0, sinks=0, scale=None):
     q = c.queries(h, t, dtype)
     strided = q.transpose(1, 2).contiguous().to("mojo").transpose(1, 2)

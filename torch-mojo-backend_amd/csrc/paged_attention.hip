@@ -5,45 +5,12 @@
 // p - j < window or j < sinks.
 #include <math.h>
 
-#include "paged.h"
+#include "paged_attention.h"
 
 namespace mi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct DecodeArgs {
-  mi355x_paged_cache c;
-  PagedSeqs s;
-  void* o;
-  int64_t o_b, o_h, o_t;
-  const void* q;
-  int64_t q_b, q_h, q_t;
-  int64_t batch;
-  int heads, group, seq;
-  int window, sinks;  // window 0: none
-  int splits;
-  float scale_log2;
-  float* part_o;   // [splits][batch * heads * seq][d]
-  float2* part_ml; // [splits][batch * heads * seq]: maximum (base 2) and sum
-};
-
-// The keys that queries at positions first .. last can see, in tiles of
-// `tile` keys: the sinks' tiles, then from `low` on.
-struct KeySpan {
-  int sink_tiles, low, tiles;  // low: first tile of the window
-  __device__ __forceinline__ KeySpan(int first, int last, int window, int sinks, int tile) {
-    low = window > 0 ? max(first - window + 1, 0) / tile : 0;
-    const int s = window > 0 ? min(sinks, last + 1) : 0;
-    sink_tiles = min((s + tile - 1) / tile, low);
-    tiles = last < 0 ? 0 : sink_tiles + last / tile + 1 - low;
-  }
-  __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : low + i - sink_tiles; }
-};
-__device__ __forceinline__ bool visible(int pos, int j, int window, int sinks) {
-  return j <= pos && (window <= 0 || pos - j < window || j < sinks);
-}
 
 // ---------------------------------------------------------------------------
 // any type and head_dim: a block owns one query row and a split of its keys;
@@ -198,22 +165,32 @@ int64_t most_keys(const mi355x_paged_cache& c, int64_t width, int64_t window, in
   return window > 0 && window + sinks < n ? window + sinks : n;
 }
 
-// Blocks that share the keys of a row: enough for two rounds of the 256 CUs
-// where rows alone are fewer, at 128 keys each and more.
+// Blocks that share the keys of a row, where rows alone are too few to fill
+// the 256 CUs: four blocks a CU in all, of at least 128 keys each.
 int plan_splits(const mi355x_paged_cache& c, int64_t width, int64_t batch, int64_t heads, int64_t seq, int64_t window,
-                int64_t sinks) {
-  const int64_t rows = batch * heads * seq, keys = most_keys(c, width, window, sinks);
-  int64_t n = rows ? 1024 / rows : 1;
+                int64_t sinks, int dtype) {
+  const int64_t keys = most_keys(c, width, window, sinks);
+  int64_t blocks = batch * heads * seq;
+  if (paged_mfma_takes(c, dtype)) {
+    const int64_t rows = heads / c.kv_heads * seq, per = 16 * paged_mfma_row_tiles(rows, c.d);
+    blocks = batch * c.kv_heads * ((rows + per - 1) / per);
+  }
+  int64_t n = blocks > 0 ? (1024 + blocks - 1) / blocks : 1;
   if (n > (keys + 127) / 128) n = (keys + 127) / 128;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
 template <typename T>
-int attn_launch(const DecodeArgs& a, hipStream_t s) {
+int attn_launch(const DecodeArgs& a, int dtype, hipStream_t s) {
   const int64_t rows = a.batch * a.heads * a.seq;
-  const dim3 grid((unsigned)rows, (unsigned)a.splits);
-  if (a.c.bits == 4) paged_attn_rows<T, uint8_t><<<grid, kThreads, 0, s>>>(a);
-  else paged_attn_rows<T, T><<<grid, kThreads, 0, s>>>(a);
+  if (paged_mfma_takes(a.c, dtype)) {
+    const int rc = paged_mfma_launch(a, dtype, s);
+    if (rc) return rc;
+  } else {
+    const dim3 grid((unsigned)rows, (unsigned)a.splits);
+    if (a.c.bits == 4) paged_attn_rows<T, uint8_t><<<grid, kThreads, 0, s>>>(a);
+    else paged_attn_rows<T, T><<<grid, kThreads, 0, s>>>(a);
+  }
   if (a.splits > 1) paged_attn_join<T><<<(unsigned)rows, kThreads, 0, s>>>(a);
   return check_launch("mi355x_paged_attn");
 }
@@ -226,8 +203,8 @@ using namespace mi;
 extern "C" int64_t mi355x_paged_attn_workspace_bytes(const mi355x_paged_cache* cache, int64_t table_width,
                                                      int64_t batch, int64_t heads, int64_t seq, int64_t window,
                                                      int64_t sinks, int dtype) {
-  if (!cache || table_width < 0 || batch <= 0 || heads <= 0 || seq <= 0) return 0;
-  const int splits = plan_splits(*cache, table_width, batch, heads, seq, window, sinks);
+  if (!cache || cache->kv_heads <= 0 || table_width < 0 || batch <= 0 || heads <= 0 || seq <= 0) return 0;
+  const int splits = plan_splits(*cache, table_width, batch, heads, seq, window, sinks, dtype);
   return splits > 1 ? splits * batch * heads * seq * (cache->d + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -262,11 +239,11 @@ extern "C" int mi355x_paged_attn(void* o, const int64_t* o_bht, const void* q, c
   a.batch = batch, a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads), a.seq = (int)seq;
   // a window or sinks past every position are the same as one that ends there
   a.window = (int)(window < kMaxPosition ? window : 0), a.sinks = (int)(sinks < kMaxPosition ? sinks : kMaxPosition);
-  a.splits = plan_splits(*cache, table_width, batch, heads, seq, window, sinks);
+  a.splits = plan_splits(*cache, table_width, batch, heads, seq, window, sinks, dtype);
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.part_o = (float*)workspace;
   a.part_ml = (float2*)(a.part_o + a.splits * batch * heads * seq * cache->d);
-  if (dtype == MI355X_F32) return attn_launch<float>(a, (hipStream_t)stream);
-  if (dtype == MI355X_BF16) return attn_launch<bf16>(a, (hipStream_t)stream);
-  return attn_launch<f16>(a, (hipStream_t)stream);
+  if (dtype == MI355X_F32) return attn_launch<float>(a, dtype, (hipStream_t)stream);
+  if (dtype == MI355X_BF16) return attn_launch<bf16>(a, dtype, (hipStream_t)stream);
+  return attn_launch<f16>(a, dtype, (hipStream_t)stream);
 }

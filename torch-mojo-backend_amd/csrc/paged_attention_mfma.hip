@@ -1,0 +1,642 @@
+// Attention over a paged cache on matrix cores: f32, bf16 and f16 pages, and
+// 4-bit pages, at head_dim 64, 128 and 256.
+//
+// A new token reads every visible row of K and V once and does 4 operations a
+// value and query head with it: memory bounds it, and all that matters is that
+// enough loads are in flight and that nothing else takes longer than they do.
+//
+// A wave owns 16 query rows at a time (QT times) of one K/V head: the heads of
+// its group, token by token, so the keys that they share are read once.  It
+// walks tiles of 32 keys (16 in f32), four waves of a block taking turns, and
+// keeps its own running maximum, sum and output; nothing waits for another
+// wave before the end.  The rows go straight to registers:
+//   S^T = K Q^T: K's operand (a key's channels 8 g .. 8 g + 7 of every 32 in
+//     lane group g) is how a row lies in memory;
+//   O^T += V^T P^T: V's operand has eight keys of one channel in a lane.  Each
+//     lane loads eight channels of its eight keys and exchanges halves of
+//     words in registers (v_perm_b32, half an instruction a value); its O^T
+//     tiles then hold every eighth channel.  No LDS, no transposing loads.
+// The accumulator layout of S^T (keys 4 g .. 4 g + 3 of a query in lane group
+// g) is the operand layout of P^T, for tiles in the order of the keys.
+//
+// P is split in two halves of the pages' type, so its rounding (2^-8 in bf16)
+// does not show beside the result's; the second product costs nothing here.
+//
+// 4-bit rows are turned into f16 in registers, minimum + scale * code in one
+// rounding (2^-11): masked nibbles under f16's exponent of 1024, less 1024,
+// are the codes, two a register.  Queries go to f16 with their row's exponent
+// taken out, which keeps bf16's values as they are.
+//
+// Blocks split the keys of long sequences; paged_attn_join adds the parts.
+#include <math.h>
+
+#include "mfma.h"
+#include "paged_attention.h"
+
+namespace mi {
+namespace {
+
+constexpr int NW = 4;  // waves of a block
+
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float group_max(float x) {  // over the four lane groups
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float group_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// Where the rows of a tile are: lane l looked up key l % TK of it.
+struct Places {
+  int page, slot;
+  uint32_t live;  // keys that some row may see and whose page exists
+};
+
+// Offset of key 16 kt + k of the tile; what is not live goes to page 0.
+template <bool P16>
+__device__ __forceinline__ int64_t row_at(const Places& p, int kt, int k, const int64_t* st, int64_t head) {
+  int page, slot;
+  if constexpr (P16) {  // 16 keys of a tile share a page
+    page = __builtin_amdgcn_readlane(p.page, 16 * kt), slot = __builtin_amdgcn_readlane(p.slot, 16 * kt) + k;
+  } else {
+    page = __shfl(p.page, 16 * kt + k, 64), slot = __shfl(p.slot, 16 * kt + k, 64);
+  }
+  return page * st[0] + head + slot * st[2];
+}
+
+// ---------------------------------------------------------------------------
+// page formats
+// ---------------------------------------------------------------------------
+// 16-bit pages of T.
+template <typename T, int D_>
+struct Pages16 {
+  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW);
+  typedef typename Mfma<T>::frag frag;
+  typedef uint32_t vword __attribute__((ext_vector_type(VW / 2)));
+  struct Keys {
+    frag k[KT][D / 32];
+  };
+  struct Values {
+    vword v[8][NU];
+  };
+  struct Query {
+    frag q[D / 32];
+    float scale;
+  };
+  static __device__ __forceinline__ int channel(int u, int e, int c) { return (u * 16 + c) * VW + e; }
+  template <typename QT_>
+  static __device__ __forceinline__ void load_query(Query& q, const QT_* row, bool real, int g, float scale_log2) {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q.q[s][e] = (T)0.f;
+    if (real)
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) q.q[s] = *(const frag*)(row + s * 32 + g * 8);
+    q.scale = scale_log2;
+  }
+  template <bool P16>
+  static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+    const int64_t kh = hk * a.c.k_phs[1];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const T* row = (const T*)a.c.k + row_at<P16>(p, kt, lr, a.c.k_phs, kh) + g * 8;
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) r.k[kt][s] = *(const frag*)(row + s * 32);
+    }
+  }
+  template <bool P16>
+  static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+    const int64_t vh = hk * a.c.v_phs[1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T* row = (const T*)a.c.v + row_at<P16>(p, i >> 2, 4 * g + (i & 3), a.c.v_phs, vh) + lr * VW;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) r.v[i][u] = *(const vword*)(row + u * 16 * VW);
+    }
+  }
+  static __device__ __forceinline__ void hide_values(Values& r, uint32_t live, int g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(live >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1))
+#pragma unroll
+        for (int u = 0; u < NU; ++u) r.v[i][u] = vword(0);
+  }
+  template <int QT>
+  static __device__ __forceinline__ void scores(f32x4 (&s)[KT][QT], const Keys& r, const Query (&q)[QT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) x = Mfma<T>::mma(r.k[kt][ks], q[qt].q[ks], x);
+        s[kt][qt] = x;
+      }
+  }
+  template <int QT>
+  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], const Values& r, const f32x4 (&p)[KT][QT]) {
+    frag hi[QT], lo[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const T h = (T)p[kt][qt][e];
+          hi[qt][4 * kt + e] = h;
+          lo[qt][4 * kt + e] = (T)(p[kt][qt][e] - (float)h);
+        }
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        union {
+          uint32_t w[4];
+          frag f;
+        } v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v.w[i] = __builtin_amdgcn_perm(r.v[2 * i + 1][u][e / 2], r.v[2 * i][u][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          o[u][e][qt] = Mfma<T>::mma(v.f, hi[qt], o[u][e][qt]);
+          o[u][e][qt] = Mfma<T>::mma(v.f, lo[qt], o[u][e][qt]);
+        }
+      }
+  }
+};
+
+// f32 pages: v_mfma_f32_16x16x4_f32, one key (or channel) a lane group; with
+// the keys of a product step taken as 4 g + step, V's rows need no exchange.
+template <int D_>
+struct Pages32 {
+  static constexpr int D = D_, KT = 1, VW = 4, NU = D / 64;
+  struct Keys {
+    f32x4 k[D / 16];
+  };
+  struct Values {
+    f32x4 v[4][NU];
+  };
+  struct Query {
+    f32x4 q[D / 16];
+    float scale;
+  };
+  static __device__ __forceinline__ int channel(int u, int e, int c) { return u * 64 + c * 4 + e; }
+  static __device__ __forceinline__ void load_query(Query& q, const float* row, bool real, int g, float scale_log2) {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) q.q[s] = real ? *(const f32x4*)(row + s * 16 + g * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
+    q.scale = scale_log2;
+  }
+  template <bool P16>
+  static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+    const float* k = (const float*)a.c.k + row_at<P16>(p, 0, lr, a.c.k_phs, hk * a.c.k_phs[1]) + g * 4;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) r.k[s] = *(const f32x4*)(k + s * 16);
+  }
+  template <bool P16>
+  static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* v = (const float*)a.c.v + row_at<P16>(p, 0, 4 * g + i, a.c.v_phs, hk * a.c.v_phs[1]) + lr * 4;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) r.v[i][u] = *(const f32x4*)(v + u * 64);
+    }
+  }
+  static __device__ __forceinline__ void hide_values(Values& r, uint32_t live, int g) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(live >> (4 * g + i) & 1))
+#pragma unroll
+        for (int u = 0; u < NU; ++u) r.v[i][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  template <int QT>
+  static __device__ __forceinline__ void scores(f32x4 (&s)[KT][QT], const Keys& r, const Query (&q)[QT]) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = __builtin_amdgcn_mfma_f32_16x16x4f32(r.k[ks][e], q[qt].q[ks][e], x, 0, 0, 0);
+      s[0][qt] = x;
+    }
+  }
+  template <int QT>
+  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], const Values& r, const f32x4 (&p)[KT][QT]) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < VW; ++e)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            o[u][e][qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(r.v[i][u][e], p[0][qt][i], o[u][e][qt], 0, 0, 0);
+  }
+};
+
+// 4-bit pages, queries of T.
+template <typename T, int D_>
+struct Pages4 {
+  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), NG = D / kKvGroup;
+  typedef f16x8 frag;
+  typedef uint32_t row_words __attribute__((ext_vector_type(NG)));  // a lane's codes of a K row, or the row's scales
+  struct Keys {
+    row_words k[KT], ks[KT];
+  };
+  struct Values {
+    uint32_t v[8][NU], vs[8][NU];
+  };
+  struct Query {
+    frag q[D / 32];
+    float scale;
+  };
+  // V's lane c holds word c + 16 u of a row; at head_dim 64 two lanes share a
+  // word, c < 8 its even channels and c >= 8 its odd ones.
+  static __device__ __forceinline__ int word(int u, int c) { return D >= 128 ? c + 16 * u : c & 7; }
+  static __device__ __forceinline__ int channel(int u, int e, int c) {
+    const int w = word(u, c);
+    return w % NG * kKvGroup + w / NG * 8 + (D >= 128 ? e : 2 * e + (c >> 3));
+  }
+  static __device__ __forceinline__ void load_query(Query& q, const T* row, bool real, int g, float scale_log2) {
+    float x[D / 32][8], top = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      typename Mfma<T>::frag v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)0.f;
+      if (real) v = *(const typename Mfma<T>::frag*)(row + s * 32 + g * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[s][e] = (float)v[e], top = fmaxf(top, fabsf(x[s][e]));
+    }
+    top = group_max(top);
+    const int ex = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q.q[s][e] = (f16)ldexpf(x[s][e], -ex);
+    q.scale = ldexpf(scale_log2, ex);
+  }
+  template <bool P16>
+  static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      r.k[kt] = *(const row_words*)((const uint8_t*)a.c.k + row_at<P16>(p, kt, lr, a.c.k_phs, hk * a.c.k_phs[1]) + g * (D / 8));
+      r.ks[kt] = *(const row_words*)((const f16*)a.c.k_scales + row_at<P16>(p, kt, lr, a.c.ks_phs, hk * a.c.ks_phs[1]));
+    }
+  }
+  template <bool P16>
+  static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t* v = (const uint32_t*)((const uint8_t*)a.c.v + row_at<P16>(p, i >> 2, 4 * g + (i & 3), a.c.v_phs, hk * a.c.v_phs[1]));
+      const uint32_t* s = (const uint32_t*)((const f16*)a.c.v_scales + row_at<P16>(p, i >> 2, 4 * g + (i & 3), a.c.vs_phs, hk * a.c.vs_phs[1]));
+#pragma unroll
+      for (int u = 0; u < NU; ++u) r.v[i][u] = v[word(u, lr)], r.vs[i][u] = s[word(u, lr) % NG];
+    }
+  }
+  static __device__ __forceinline__ void hide_values(Values& r, uint32_t live, int g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(live >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1))
+#pragma unroll
+        for (int u = 0; u < NU; ++u) r.vs[i][u] = 0;
+  }
+  // Nibble i of both halves of w under the scales and minimums of s and m.
+  static __device__ __forceinline__ f16x2 value(uint32_t w, int i, f16x2 s, f16x2 m) {
+    const f16x2 c = __builtin_bit_cast(f16x2, (w >> (4 * i) & 0x000f000fu) | 0x64006400u) - (f16)1024.f;
+    return __builtin_elementwise_fma(c, s, m);
+  }
+  template <int QT>
+  static __device__ __forceinline__ void scores(f32x4 (&s)[KT][QT], const Keys& r, const Query (&q)[QT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) s[kt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < NG; ++ks) {
+        const f16x2 sm = __builtin_bit_cast(f16x2, (uint32_t)r.ks[kt][ks]);
+        union {
+          f16x2 h[4];
+          frag f;
+        } k;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k.h[i] = value(r.k[kt][ks], i, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]});
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[kt][qt] = Mfma<f16>::mma(k.f, q[qt].q[ks], s[kt][qt]);
+      }
+    }
+  }
+  template <int QT>
+  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], const Values& r, const f32x4 (&p)[KT][QT]) {
+    frag pf[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[qt][4 * kt + e] = (f16)p[kt][qt][e];
+    const bool odd = D < 128 && (threadIdx.x & 8);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      uint32_t even_w[4], odd_w[4];  // words of two keys: their even, their odd channels
+      f16x2 s[4], m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = r.v[2 * i][u], b = r.v[2 * i + 1][u], x = r.vs[2 * i][u], y = r.vs[2 * i + 1][u];
+        even_w[i] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        odd_w[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        if (odd) even_w[i] = odd_w[i];
+        s[i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(y, x, 0x05040100u));
+        m[i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(y, x, 0x07060302u));
+      }
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        union {
+          f16x2 h[4];
+          frag f;
+        } v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v.h[i] = D >= 128 ? value(e % 2 ? odd_w[i] : even_w[i], e / 2, s[i], m[i]) : value(even_w[i], e, s[i], m[i]);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) o[u][e][qt] = Mfma<f16>::mma(v.f, pf[qt], o[u][e][qt]);
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Waves of a SIMD that the registers are shared out to: what keys, values,
+// queries and output take, and 64 more.
+template <typename F, int QT>
+constexpr int waves_of() {
+  const int regs = (int)(sizeof(typename F::Keys) + sizeof(typename F::Values)) / 4 +
+                   QT * ((int)sizeof(typename F::Query) / 4 + F::D / 4) + 64;
+  return regs <= 128 ? 4 : regs <= 168 ? 3 : regs <= 256 ? 2 : 1;
+}
+
+template <typename F, typename T, int QT, bool P16>
+__global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(DecodeArgs a) {
+  constexpr int D = F::D, KT = F::KT, TK = 16 * KT, VW = F::VW, NU = F::NU, W = 16 * VW;
+  __shared__ float so[NW][16][W + 4];
+  __shared__ float sm[NW][16 * QT], sl[NW][16 * QT];
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int lr = lane & 15, g = lane >> 4;
+  // The row groups of a part of a head's keys run on one XCD, whose L2 they share.
+  const uint32_t i0 = blockIdx.x >> 3;
+  const uint32_t unit = i0 / a.row_groups * 8 + (blockIdx.x & 7), rg = i0 % a.row_groups;
+  if (unit >= (uint32_t)a.units) return;
+  const uint32_t hkn = (uint32_t)a.c.kv_heads;
+  const int split = unit % a.splits;
+  const int64_t hk = unit / a.splits % hkn, b = unit / a.splits / hkn;
+  const int rows = a.group * a.seq, r0 = (int)rg * 16 * QT;
+  const int count = seq_count(a.s, b, a.seq);
+  const int64_t start = a.s.starts[b];
+
+  typename F::Query q[QT];
+  int pos[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int r = r0 + qt * 16 + lr, t = r / a.group, h = (int)hk * a.group + r - t * a.group;
+    const int64_t at = start + t;
+    const bool real = r < rows && t < count;
+    const bool ok = real && at >= 0 && at <= kMaxPosition;
+    if (real && !ok && a.s.error) *a.s.error = 1;
+    pos[qt] = ok ? (int)at : -1;
+    F::load_query(q[qt], (const T*)a.q + b * a.q_b + h * a.q_h + t * a.q_t, ok, g, a.scale_log2);
+  }
+  // positions of the block's first and last row (rows are token by token)
+  const int t0 = r0 / a.group, t1 = min(min((r0 + 16 * QT - 1) / a.group, count - 1), a.seq - 1);
+  const int64_t last64 = t1 >= t0 ? start + t1 : -1, first64 = start + t0;
+  const int last = last64 >= 0 && last64 <= kMaxPosition ? (int)last64 : -1;
+  const int first = (int)min(max(first64, (int64_t)-1), kMaxPosition);
+  const KeySpan span(first, last, a.window, a.sinks, TK);
+  const int low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+  const int per = (span.tiles + a.splits - 1) / a.splits;
+  const int end = min((split + 1) * per, span.tiles);
+
+  auto look_up = [&](int i) {
+    Places p{0, 0, 0};
+    const int j = span.tile(i) * TK + (lane & (TK - 1));
+    bool live = j <= last && (j >= low || j < a.sinks);
+    // 16 keys of one page: its number is wanted if any of them is live
+    const int j16 = j & ~15;
+    const bool wanted = P16 ? j16 <= last && (j16 + 15 >= low || j16 < a.sinks) : live;
+    if (wanted) {
+      uint32_t slot;
+      const int page = page_of(a.s, b, (uint32_t)j, &slot);
+      live = live && page >= 0;
+      p.page = max(page, 0), p.slot = page >= 0 ? (int)slot : P16 ? lane & 15 : 0;
+    }
+    p.live = (uint32_t)__builtin_amdgcn_ballot_w64(live) & (uint32_t)((1ull << TK) - 1);
+    return p;
+  };
+  float m[QT], l[QT];
+  f32x4 o[NU][VW][QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m[qt] = -INFINITY, l[qt] = 0.f;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) o[u][e][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // Registers hold one tile: its keys make room for the next ones as soon as
+  // the scores are taken, its values after their product.  The rest of the
+  // time the loads have comes from the other waves of the SIMD, of which
+  // there are more than with two tiles in registers.
+  typename F::Keys keys;
+  typename F::Values values;
+  int i = split * per + wave;
+  Places here{0, 0, 0}, next{0, 0, 0};
+  if (i < end) {
+    here = look_up(i);
+    F::template load_keys<P16>(keys, a, here, hk, lr, g);
+    F::template load_values<P16>(values, a, here, hk, lr, g);
+    if (i + NW < end) next = look_up(i + NW);
+  }
+  for (; i < end; i += NW) {
+    const int j0 = span.tile(i) * TK;
+    const uint32_t live = here.live;
+    const bool more = i + NW < end;
+    // every key of the tile is seen by every row
+    const bool whole = live == (uint32_t)((1ull << TK) - 1) && j0 + TK - 1 <= first &&
+                       (a.window <= 0 || last - j0 < a.window || j0 + TK <= a.sinks);
+    f32x4 s[KT][QT];
+    F::scores(s, keys, q);
+    if (more) F::template load_keys<P16>(keys, a, next, hk, lr, g);
+    bool moved = false;
+    float top[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = s[kt][qt][e] * q[qt].scale;
+          if (!whole) {
+            const int k = 16 * kt + 4 * g + e;
+            if (!(live >> k & 1) || !visible(pos[qt], j0 + k, a.window, a.sinks)) x = -INFINITY;
+          }
+          s[kt][qt][e] = x;
+          mx = fmaxf(mx, x);
+        }
+      top[qt] = fmaxf(m[qt], group_max(mx));
+      moved |= top[qt] > m[qt];
+    }
+    if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const float alpha = top[qt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[qt] - top[qt]);
+        l[qt] *= alpha;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) o[u][e][qt] *= alpha;
+        m[qt] = top[qt];
+      }
+    }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const float base = m[qt] == -INFINITY ? 0.f : m[qt];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = __builtin_amdgcn_exp2f(s[kt][qt][e] - base);
+          s[kt][qt][e] = p;
+          l[qt] += p;
+        }
+    }
+    if (!whole) F::hide_values(values, live, g);
+    F::add_values(o, values, s);
+    if (more) {
+      F::template load_values<P16>(values, a, next, hk, lr, g);
+      here = next;
+      if (i + 2 * NW < end) next = look_up(i + 2 * NW);
+    }
+  }
+
+  // join the waves
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    l[qt] = group_sum(l[qt]);
+    if (g == 0) sm[wave][qt * 16 + lr] = m[qt], sl[wave][qt * 16 + lr] = l[qt];
+  }
+  __syncthreads();
+  const int64_t total_rows = a.batch * a.heads * a.seq;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w][qt * 16 + lr]);
+    const float mine = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[qt] - mx);
+    // the row that this thread stores, and its sum
+    const int sr = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int r = r0 + qt * 16 + sr, t = r / a.group, h = (int)hk * a.group + r - t * a.group;
+    float smx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) smx = fmaxf(smx, sm[w][qt * 16 + sr]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+      sum += smx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[w][qt * 16 + sr] - smx) * sl[w][qt * 16 + sr];
+    // padding took part where tiles were whole: it leaves nothing
+    if (t >= count || start + t < 0 || start + t > kMaxPosition) smx = -INFINITY, sum = 0.f;
+    const bool none = smx == -INFINITY;
+    const int64_t row = (b * a.heads + h) * a.seq + t;
+    if (a.splits > 1 && r < rows && c == 0) a.part_ml[split * total_rows + row] = make_float2(smx, sum);
+    const float inv = a.splits > 1 ? 1.f : (sum != 0.f ? 1.f / sum : 0.f);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      __syncthreads();
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4)
+#pragma unroll
+        for (int e = 0; e < VW; e += 4)
+          *(float4*)&so[wave][lr][(4 * g + e4) * VW + e] =
+              make_float4(o[u][e][qt][e4] * mine, o[u][e + 1][qt][e4] * mine, o[u][e + 2][qt][e4] * mine, o[u][e + 3][qt][e4] * mine);
+      __syncthreads();
+      if (r >= rows) continue;
+      float x[VW];
+#pragma unroll
+      for (int e = 0; e < VW; ++e) x[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) x[e] += none ? 0.f : so[w][sr][c * VW + e];
+      if (a.splits > 1) {
+        float* dst = a.part_o + (split * total_rows + row) * D;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) dst[F::channel(u, e, c)] = x[e];
+      } else {
+        T* dst = (T*)a.o + b * a.o_b + h * a.o_h + t * a.o_t;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) dst[F::channel(u, e, c)] = from_f32<T>(x[e] * inv);
+      }
+    }
+  }
+}
+
+template <typename F, typename T, int QT>
+void launch(const DecodeArgs& a, unsigned blocks, hipStream_t s) {
+  if (a.c.page_size % 16 == 0) paged_attn_mfma<F, T, QT, true><<<blocks, 64 * NW, 0, s>>>(a);
+  else paged_attn_mfma<F, T, QT, false><<<blocks, 64 * NW, 0, s>>>(a);
+}
+
+template <typename F, typename T>
+void launch_rows(const DecodeArgs& a, int qt, unsigned blocks, hipStream_t s) {
+  if constexpr (F::D < 256)
+    if (qt == 2) return launch<F, T, 2>(a, blocks, s);
+  launch<F, T, 1>(a, blocks, s);
+}
+
+template <int D>
+void launch_format(const DecodeArgs& a, int qt, int dtype, unsigned blocks, hipStream_t s) {
+  if (a.c.bits == 4) {
+    if (dtype == MI355X_BF16) launch_rows<Pages4<bf16, D>, bf16>(a, qt, blocks, s);
+    else launch_rows<Pages4<f16, D>, f16>(a, qt, blocks, s);
+  } else if (dtype == MI355X_F32) {
+    launch_rows<Pages32<D>, float>(a, qt, blocks, s);
+  } else if (dtype == MI355X_BF16) {
+    launch_rows<Pages16<bf16, D>, bf16>(a, qt, blocks, s);
+  } else {
+    launch_rows<Pages16<f16, D>, f16>(a, qt, blocks, s);
+  }
+}
+
+}  // namespace
+
+bool paged_mfma_takes(const mi355x_paged_cache& c, int dtype) {
+  if (c.d != 64 && c.d != 128 && c.d != 256) return false;
+  if (c.bits != 4) return true;
+  if (dtype == MI355X_F32) return false;  // queries would lose what f16 does not hold
+  const int64_t align = c.d / 8 < 16 ? c.d / 8 : 16;  // of a row of scales
+  for (const int64_t* st : {c.ks_phs, c.vs_phs})
+    for (int i = 0; i < 3; ++i)
+      if (st[i] * 2 % align) return false;
+  return ((uintptr_t)c.k_scales | (uintptr_t)c.v_scales) % align == 0;
+}
+
+// Query rows of 16 that share a block: two where there are that many and
+// registers hold their output (head_dim 256 would spill).
+int paged_mfma_row_tiles(int64_t rows, int64_t d) { return rows > 16 && d < 256 ? 2 : 1; }
+
+int paged_mfma_launch(DecodeArgs a, int dtype, hipStream_t s) {
+  const int qt = paged_mfma_row_tiles((int64_t)a.group * a.seq, a.c.d);
+  a.row_groups = ((int64_t)a.group * a.seq + 16 * qt - 1) / (16 * qt);
+  a.units = a.batch * a.c.kv_heads * a.splits;
+  const int64_t blocks = (a.units + 7) / 8 * 8 * a.row_groups;
+  MI_REQUIRE(blocks < (1ll << 24), "mi355x_paged_attn: %lld blocks", (long long)blocks);
+  if (a.c.d == 64) launch_format<64>(a, qt, dtype, (unsigned)blocks, s);
+  else if (a.c.d == 128) launch_format<128>(a, qt, dtype, (unsigned)blocks, s);
+  else launch_format<256>(a, qt, dtype, (unsigned)blocks, s);
+  return MI355X_OK;
+}
+
+}  // namespace mi

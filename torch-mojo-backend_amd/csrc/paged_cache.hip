@@ -11,7 +11,8 @@
 // Rotation, half-split: y[i] = x[i] cos[p][i] - x[i + d/2] sin[p][i] and
 // y[i + d/2] = x[i + d/2] cos[p][i + d/2] + x[i] sin[p][i + d/2].
 //
-// 4 bits: m = f16(min), s = f16((max - min) / 15) over 32 channels, code =
+// 4 bits: m = f16(min), s = f16((max - min) / 15) over 32 channels, each rounded to
+// f32 first, code =
 // clamp(rint((x - m) / s), 0, 15).  The rotation and the quotient are taken in
 // f64: products of two values of at most 24 bits are exact there, so which
 // side of a border a value falls on depends neither on the order nor on the
@@ -102,6 +103,16 @@ __device__ __forceinline__ void rotate(W (&y)[8], const T* x, const RT* cos_t, c
   }
 }
 
+// f16 of an f64 value by way of f32, as the cache's format has it (and a host
+// without a conversion in one step).  The compiler would make it one rounding,
+// which differs where the f32 value is halfway between two f16 ones: in one of
+// 15000 scales.
+__device__ __forceinline__ f16 to_f16_by_f32(double x) {
+  float f = (float)x;
+  asm("" : "+v"(f));
+  return (f16)f;
+}
+
 // Packs the eight channels of this lane; four neighbouring lanes hold the 32
 // channels that share a scale.
 __device__ __forceinline__ void pack_row(const double (&x)[8], uint32_t* codes, f16* scales, int ch, int d) {
@@ -120,7 +131,7 @@ __device__ __forceinline__ void pack_row(const double (&x)[8], uint32_t* codes, 
   }
   lo = fmax(lo, -kKvLimit), hi = fmin(hi, kKvLimit);
   lo = fmin(lo, kKvLimit), hi = fmax(hi, -kKvLimit);
-  const f16 step16 = bad ? (f16)NAN : (f16)(float)((hi - lo) / 15.0), base16 = bad ? (f16)NAN : (f16)(float)lo;
+  const f16 step16 = bad ? (f16)NAN : to_f16_by_f32((hi - lo) / 15.0), base16 = bad ? (f16)NAN : to_f16_by_f32(lo);
   const double step = (double)(float)step16, base = (double)(float)base16;
   uint32_t w = 0;
   if (step > 0.0) {
