@@ -135,27 +135,40 @@ __global__ void __launch_bounds__(kThreads) paged_attn_rows(DecodeArgs a) {
   }
 }
 
-// Joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// Joins the (at most 64) splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s
+// 2^(m_s - m) l_s.  A lane of each wave weighs one split; the waves then take
+// turns at the splits' rows, four channels a lane, so that a row costs two
+// trips to memory however many splits it has.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) paged_attn_join(DecodeArgs a) {
-  const int d = (int)a.c.d;
+  __shared__ float4 sum[kThreads / 64][64];
+  const int d = (int)a.c.d, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t rows = a.batch * a.heads * a.seq;
   const uint32_t row = blockIdx.x;
-  const uint32_t t = row % a.seq, bh = row / a.seq;
-  const int h = bh % a.heads;
-  const int64_t b = bh / a.heads;
-  float mx = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_ml[s * rows + row].x);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float total = 0.f, acc = 0.f;
-  if ((int)threadIdx.x >= d) return;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[s * rows + row];
-    const float w = exp2f(ml.x - base);
-    total += w * ml.y;
-    acc += w * a.part_o[(s * rows + row) * d + threadIdx.x];
+  const float2 ml = lane < a.splits ? a.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.f);
+  const float mx = wave_max(ml.x);
+  const float w = mx == -INFINITY ? 0.f : exp2f(ml.x - mx);
+  const float total = wave_sum(w * ml.y);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int ch = min(lane * 4, d - 4);  // every lane stays for the shuffles
+#pragma unroll 4
+  for (int s = wave; s < a.splits; s += kThreads / 64) {
+    const float4 x = *(const float4*)(a.part_o + (s * rows + row) * d + ch);
+    const float ws = __shfl(w, s, 64);
+    acc.x += ws * x.x, acc.y += ws * x.y, acc.z += ws * x.z, acc.w += ws * x.w;
   }
-  ((T*)a.o)[b * a.o_b + h * a.o_h + t * a.o_t + threadIdx.x] = from_f32<T>(total != 0.f ? acc / total : 0.f);
+  sum[wave][lane] = acc;
+  __syncthreads();
+  if ((int)threadIdx.x * 4 >= d) return;
+  for (int i = 1; i < kThreads / 64; ++i) {
+    const float4 x = sum[i][lane];
+    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+  }
+  const uint32_t t = row % a.seq, bh = row / a.seq;
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+  T* o = (T*)a.o + bh / a.heads * a.o_b + bh % a.heads * a.o_h + t * a.o_t + lane * 4;
+  o[0] = from_f32<T>(acc.x * inv), o[1] = from_f32<T>(acc.y * inv);
+  o[2] = from_f32<T>(acc.z * inv), o[3] = from_f32<T>(acc.w * inv);
 }
 
 // Keys that one query can see at most.

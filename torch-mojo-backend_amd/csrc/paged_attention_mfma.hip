@@ -55,16 +55,21 @@ struct Places {
   uint32_t live;  // keys that some row may see and whose page exists
 };
 
-// Offset of key 16 kt + k of the tile; what is not live goes to page 0.
+// Address of the row of key 16 kt + k of the tile, `es` bytes a unit of the
+// strides; what is not live lies in page 0.  16 keys of a tile that share a
+// page (P16) have a base that is the same for all lanes, and of the lane's own
+// address only 32 bits, the same for every tile.
 template <bool P16>
-__device__ __forceinline__ int64_t row_at(const Places& p, int kt, int k, const int64_t* st, int64_t head) {
-  int page, slot;
-  if constexpr (P16) {  // 16 keys of a tile share a page
-    page = __builtin_amdgcn_readlane(p.page, 16 * kt), slot = __builtin_amdgcn_readlane(p.slot, 16 * kt) + k;
+__device__ __forceinline__ const char* row_at(const void* base, int es, const Places& p, int kt, int k,
+                                              const int64_t* st, int64_t hk) {
+  if constexpr (P16) {
+    const int64_t page = __builtin_amdgcn_readlane(p.page, 16 * kt), slot = __builtin_amdgcn_readlane(p.slot, 16 * kt);
+    const char* first = (const char*)base + (page * st[0] + hk * st[1] + slot * st[2]) * es;
+    return first + (uint32_t)(k * ((int)st[2] * es));
   } else {
-    page = __shfl(p.page, 16 * kt + k, 64), slot = __shfl(p.slot, 16 * kt + k, 64);
+    const int64_t page = __shfl(p.page, 16 * kt + k, 64), slot = __shfl(p.slot, 16 * kt + k, 64);
+    return (const char*)base + (page * st[0] + hk * st[1] + slot * st[2]) * es;
   }
-  return page * st[0] + head + slot * st[2];
 }
 
 // ---------------------------------------------------------------------------
@@ -100,20 +105,18 @@ struct Pages16 {
   }
   template <bool P16>
   static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
-    const int64_t kh = hk * a.c.k_phs[1];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const T* row = (const T*)a.c.k + row_at<P16>(p, kt, lr, a.c.k_phs, kh) + g * 8;
+      const T* row = (const T*)row_at<P16>(a.c.k, sizeof(T), p, kt, lr, a.c.k_phs, hk) + g * 8;
 #pragma unroll
       for (int s = 0; s < D / 32; ++s) r.k[kt][s] = *(const frag*)(row + s * 32);
     }
   }
   template <bool P16>
   static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
-    const int64_t vh = hk * a.c.v_phs[1];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const T* row = (const T*)a.c.v + row_at<P16>(p, i >> 2, 4 * g + (i & 3), a.c.v_phs, vh) + lr * VW;
+      const T* row = (const T*)row_at<P16>(a.c.v, sizeof(T), p, i >> 2, 4 * g + (i & 3), a.c.v_phs, hk) + lr * VW;
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = *(const vword*)(row + u * 16 * VW);
     }
@@ -193,7 +196,7 @@ struct Pages32 {
   }
   template <bool P16>
   static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
-    const float* k = (const float*)a.c.k + row_at<P16>(p, 0, lr, a.c.k_phs, hk * a.c.k_phs[1]) + g * 4;
+    const float* k = (const float*)row_at<P16>(a.c.k, 4, p, 0, lr, a.c.k_phs, hk) + g * 4;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) r.k[s] = *(const f32x4*)(k + s * 16);
   }
@@ -201,7 +204,7 @@ struct Pages32 {
   static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* v = (const float*)a.c.v + row_at<P16>(p, 0, 4 * g + i, a.c.v_phs, hk * a.c.v_phs[1]) + lr * 4;
+      const float* v = (const float*)row_at<P16>(a.c.v, 4, p, 0, 4 * g + i, a.c.v_phs, hk) + lr * 4;
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = *(const f32x4*)(v + u * 64);
     }
@@ -285,16 +288,16 @@ struct Pages4 {
   static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      r.k[kt] = *(const row_words*)((const uint8_t*)a.c.k + row_at<P16>(p, kt, lr, a.c.k_phs, hk * a.c.k_phs[1]) + g * (D / 8));
-      r.ks[kt] = *(const row_words*)((const f16*)a.c.k_scales + row_at<P16>(p, kt, lr, a.c.ks_phs, hk * a.c.ks_phs[1]));
+      r.k[kt] = *(const row_words*)(row_at<P16>(a.c.k, 1, p, kt, lr, a.c.k_phs, hk) + g * (D / 8));
+      r.ks[kt] = *(const row_words*)row_at<P16>(a.c.k_scales, 2, p, kt, lr, a.c.ks_phs, hk);
     }
   }
   template <bool P16>
   static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t* v = (const uint32_t*)((const uint8_t*)a.c.v + row_at<P16>(p, i >> 2, 4 * g + (i & 3), a.c.v_phs, hk * a.c.v_phs[1]));
-      const uint32_t* s = (const uint32_t*)((const f16*)a.c.v_scales + row_at<P16>(p, i >> 2, 4 * g + (i & 3), a.c.vs_phs, hk * a.c.vs_phs[1]));
+      const uint32_t* v = (const uint32_t*)row_at<P16>(a.c.v, 1, p, i >> 2, 4 * g + (i & 3), a.c.v_phs, hk);
+      const uint32_t* s = (const uint32_t*)row_at<P16>(a.c.v_scales, 2, p, i >> 2, 4 * g + (i & 3), a.c.vs_phs, hk);
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = v[word(u, lr)], r.vs[i][u] = s[word(u, lr) % NG];
     }
@@ -585,7 +588,9 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
 
 template <typename F, typename T, int QT>
 void launch(const DecodeArgs& a, unsigned blocks, hipStream_t s) {
-  if (a.c.page_size % 16 == 0) paged_attn_mfma<F, T, QT, true><<<blocks, 64 * NW, 0, s>>>(a);
+  bool p16 = a.c.page_size % 16 == 0;  // and 16 rows lie within 2^31 bytes
+  for (const int64_t* st : {a.c.k_phs, a.c.v_phs, a.c.ks_phs, a.c.vs_phs}) p16 &= st[2] < (1ll << 24);
+  if (p16) paged_attn_mfma<F, T, QT, true><<<blocks, 64 * NW, 0, s>>>(a);
   else paged_attn_mfma<F, T, QT, false><<<blocks, 64 * NW, 0, s>>>(a);
 }
 

@@ -13,7 +13,7 @@
 //
 // 4 bits: m = f16(min), s = f16((max - min) / 15) over 32 channels, each rounded to
 // f32 first, code =
-// clamp(rint((x - m) / s), 0, 15).  The rotation and the quotient are taken in
+// clamp(rint((x - m) / s), 0, 15).  The rotation and the quotient are those of
 // f64: products of two values of at most 24 bits are exact there, so which
 // side of a border a value falls on depends neither on the order nor on the
 // contraction of the operations.  A group with a NaN or an infinity reads back
@@ -113,14 +113,31 @@ __device__ __forceinline__ f16 to_f16_by_f32(double x) {
   return (f16)f;
 }
 
+// clamp(rint((x - base) / step), 0, 15) as the quotient in f64 has it.  An f32
+// quotient is within 2^-22 of it and settles all but the one in 50000 that are
+// next to a border; (c + 1/2) * step, of 16 bits, settles those.
+template <typename W>
+__device__ __forceinline__ uint32_t code_of(W x, W base, float inv, double step, double base_d) {
+  const float q = fminf(fmaxf((float)(x - base) * inv, 0.f), 15.f);
+  float c = rintf(q);
+  if (fabsf(fabsf(q - c) - 0.5f) < 1e-5f) {
+    const float k = floorf(q);
+    const double d = (double)x - base_d, border = ((double)k + 0.5) * step;
+    c = d > border || (d == border && ((int)k & 1)) ? k + 1.f : k;
+  }
+  return (uint32_t)c;
+}
+
 // Packs the eight channels of this lane; four neighbouring lanes hold the 32
-// channels that share a scale.
-__device__ __forceinline__ void pack_row(const double (&x)[8], uint32_t* codes, f16* scales, int ch, int d) {
-  double lo = x[0], hi = x[0];
+// channels that share a scale.  W is a type that holds the values exactly.
+template <typename W>
+__device__ __forceinline__ void pack_row(const W (&x)[8], uint32_t* codes, f16* scales, int ch, int d) {
+  const W limit = (W)kKvLimit;
+  W lo = x[0], hi = x[0];
   bool bad = false;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    bad |= !(fabs(x[e]) < INFINITY);
+    bad |= !(fabs(x[e]) < (W)INFINITY);
     lo = fmin(lo, x[e]), hi = fmax(hi, x[e]);
   }
 #pragma unroll
@@ -129,18 +146,15 @@ __device__ __forceinline__ void pack_row(const double (&x)[8], uint32_t* codes, 
     hi = fmax(hi, __shfl_xor(hi, off, 64));
     bad |= (bool)__shfl_xor((int)bad, off, 64);
   }
-  lo = fmax(lo, -kKvLimit), hi = fmin(hi, kKvLimit);
-  lo = fmin(lo, kKvLimit), hi = fmax(hi, -kKvLimit);
-  const f16 step16 = bad ? (f16)NAN : to_f16_by_f32((hi - lo) / 15.0), base16 = bad ? (f16)NAN : to_f16_by_f32(lo);
-  const double step = (double)(float)step16, base = (double)(float)base16;
+  lo = fmin(fmax(lo, -limit), limit), hi = fmin(fmax(hi, -limit), limit);
+  const f16 step16 = bad ? (f16)NAN : to_f16_by_f32(((double)hi - (double)lo) / 15.0), base16 = bad ? (f16)NAN : to_f16_by_f32(lo);
   uint32_t w = 0;
-  if (step > 0.0) {
+  if ((float)step16 > 0.f) {
+    const float inv = 1.f / (float)step16;
+    const double step = (double)(float)step16, base = (double)(float)base16;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double v = fmin(fmax(x[e], -kKvLimit), kKvLimit);
-      const double c = fmin(fmax(rint((v - base) / step), 0.0), 15.0);
-      w |= (uint32_t)(int)c << (4 * (e / 2 + 4 * (e % 2)));
-    }
+    for (int e = 0; e < 8; ++e)
+      w |= code_of<W>(fmin(fmax(x[e], -limit), limit), (W)base, inv, step, base) << (4 * (e / 2 + 4 * (e % 2)));
   }
   const int s = ch / kKvGroup, g = ch % kKvGroup / 8;
   codes[g * (d / kKvGroup) + s] = w;
@@ -191,17 +205,20 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a) {
   const int64_t at = page * st[0] + hk * st[1] + slot * st[2];
   const T* x = row_of<T>(is_k ? a.k : a.v, b, hk, t);
   if constexpr (FOUR) {
-    double y[8];
+    const int64_t* ss = is_k ? a.c.ks_phs : a.c.vs_phs;
+    uint32_t* codes = (uint32_t*)((uint8_t*)(is_k ? a.c.k : a.c.v) + at);
+    f16* scales = (f16*)(is_k ? a.c.k_scales : a.c.v_scales) + page * ss[0] + hk * ss[1] + slot * ss[2];
     if (is_k && a.cos) {
+      double y[8];
       rotate(y, x, (const RT*)a.cos, (const RT*)a.sin, pos, ch, a.d);
+      pack_row(y, codes, scales, ch, a.d);
     } else {
       const Oct<T> o = *(const Oct<T>*)(x + ch);
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (double)to_f32(o.v[e]);
+      for (int e = 0; e < 8; ++e) y[e] = to_f32(o.v[e]);
+      pack_row(y, codes, scales, ch, a.d);
     }
-    const int64_t* ss = is_k ? a.c.ks_phs : a.c.vs_phs;
-    pack_row(y, (uint32_t*)((uint8_t*)(is_k ? a.c.k : a.c.v) + at),
-             (f16*)(is_k ? a.c.k_scales : a.c.v_scales) + page * ss[0] + hk * ss[1] + slot * ss[2], ch, a.d);
   } else {
     Oct<T> o;
     if (is_k && a.cos) {

@@ -10,16 +10,15 @@ allocated here and launches go to the null stream, that of the tensors' device.
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
-from . import PagedCache, check, materialize_touched
+from . import PagedCache, check, lazy_live, materialize_touched
 from . import native_lib as lib
-from .aten_fast import _PAGE_ERROR, _STREAM, _alloc, _code, _error_slot, _workspace, alloc_bthd, materialize_contiguous
+from .aten_fast import _PAGE_ERROR, _STREAM, _code, _error_slot, _workspace, materialize_contiguous
 from ..mojo_device import torch_mojo_tensor as _tensor_mod
 
 MT = _tensor_mod.TorchMojoTensor
+_INT32 = torch.int32
 
 
 def describe(cache) -> PagedCache:
@@ -36,19 +35,53 @@ def describe(cache) -> PagedCache:
     return d
 
 
-def _on(device: int):
-    """A context in which `device` is current: a launch on the null stream
-    goes to the current device."""
+# ---------------------------------------------------------------------------
+# Whether a call is one that needs no further look: a decode step is a few
+# microseconds of kernel, and the checks of torch_mojo_backend.ops, which name
+# what is wrong, take longer than that.
+# ---------------------------------------------------------------------------
+def seqs_ok(cache, table, starts, counts) -> bool:
+    if not cache.on_mojo or type(table) is not MT or type(starts) is not MT:
+        return False
+    dev, shape = cache.k._device, table._shape
+    if not (table._dtype is _INT32 and starts._dtype is _INT32 and len(shape) == 2 and shape[1] and table._strides[1] == 1
+            and table._device == dev and starts._device == dev and starts._shape == shape[:1]
+            and starts._strides == (1,)):
+        return False
+    return counts is None or (type(counts) is MT and counts._dtype is _INT32 and counts._shape == shape[:1]
+                              and counts._strides == (1,) and counts._device == dev)
+
+
+def rows_ok(cache, t, batch) -> bool:
+    """[batch, any heads, any tokens, head_dim] of the pages' type (16 or 32 bits)."""
+    if type(t) is not MT or t.requires_grad:
+        return False
+    shape = t._shape
+    return (len(shape) == 4 and shape[0] == batch and shape[3] == cache.head_dim and t._dtype is cache.dtype
+            and t._device == cache.k._device)
+
+
+def _with_device(device: int, call):
+    """call() with `device` current: a launch on the null stream goes to the
+    current device."""
     if _tensor_mod.storage_kind() == "cuda" and torch.cuda.current_device() != device:
-        return torch.cuda.device(device)
-    return contextlib.nullcontext()
+        with torch.cuda.device(device):
+            return call()
+    return call()
 
 
 def _rows(t: MT) -> MT:
     """t itself when its rows can be read 16 bytes at a time, else a copy."""
-    if t._strides[3] == 1 and t._ptr % 16 == 0 and all(st * t._itemsize % 16 == 0 for st in t._strides[:3]):
+    st, n = t._strides, t._itemsize
+    if st[3] == 1 and not (t._ptr | st[0] * n | st[1] * n | st[2] * n) & 15:
         return t
     return materialize_contiguous(t)
+
+
+def _heads_out(b, h, t, d, dtype, device) -> MT:
+    """A new [b, h, t, d] view of dense [b, t, h, d] storage."""
+    holder = _tensor_mod._alloc_bytes(b * h * t * d * dtype.itemsize, device)
+    return MT._make(holder, holder.data_ptr(), (b, h, t, d), (t * h * d, d, h * d, 1), 0, dtype, device)
 
 
 def _bht(t: MT):
@@ -60,59 +93,68 @@ def _seqs(table: MT, starts: MT, counts):
 
 
 def append(cache, table, starts, k, v, cos, sin, q, counts):
-    b, _, t, d = k._shape
-    written = (cache.k, cache.v) if cache.k_scales is None else (cache.k, cache.v, cache.k_scales, cache.v_scales)
-    materialize_touched((*written, table, starts, k, v, cos, sin, q, counts), None, True)
+    if lazy_live():
+        materialize_touched((*cache.tensors, table, starts, k, v, cos, sin, q, counts), None, True)
     dev = k._device
-    with _on(dev):
-        k, v = _rows(k), _rows(v)
-        out = None
-        if q is not None:
-            q = _rows(q)
-            out = alloc_bthd(b, q._shape[1], t, d, q._dtype, dev)
-        if cos is not None:
-            cos, sin = (x if x._is_contiguous and x._ptr % 16 == 0 else materialize_contiguous(x) for x in (cos, sin))
-        check(
-            "mi355x_paged_append",
-            lib().mi355x_paged_append(
-                cache._desc, *_seqs(table, starts, counts), k._ptr, _bht(k), v._ptr, _bht(v),
-                out._ptr if q is not None else None, _bht(out) if q is not None else None,
-                q._ptr if q is not None else None, _bht(q) if q is not None else None,
-                cos._ptr if cos is not None else None, sin._ptr if cos is not None else None,
-                _code(cos._dtype) if cos is not None else 0, cos._shape[0] if cos is not None else 0,
-                b, q._shape[1] if q is not None else 0, t, _code(k._dtype), _error_slot(dev, _PAGE_ERROR), _STREAM,
-            ),
-        )
-    torch.autograd.graph.increment_version(written)
+    out = _with_device(dev, lambda: _append(cache, table, starts, k, v, cos, sin, q, counts, dev))
+    torch._C._increment_version(cache.tensors)
+    return out
+
+
+def _append(cache, table, starts, k, v, cos, sin, q, counts, dev):
+    b, _, t, d = k._shape
+    k, v = _rows(k), _rows(v)
+    out, q_args, rope = None, (None, None, None, None), (None, None, 0, 0)
+    heads = 0
+    if q is not None:
+        q, heads = _rows(q), q._shape[1]
+        out = _heads_out(b, heads, t, d, q._dtype, dev)
+        q_args = out._ptr, _bht(out), q._ptr, _bht(q)
+    if cos is not None:
+        cos, sin = (x if x._is_contiguous and x._ptr % 16 == 0 else materialize_contiguous(x) for x in (cos, sin))
+        rope = cos._ptr, sin._ptr, _code(cos._dtype), cos._shape[0]
+    check(
+        "mi355x_paged_append",
+        lib().mi355x_paged_append(cache._desc, *_seqs(table, starts, counts), k._ptr, _bht(k), v._ptr, _bht(v), *q_args,
+                                  *rope, b, heads, t, _code(k._dtype), _error_slot(dev, _PAGE_ERROR), _STREAM),
+    )
     return out
 
 
 def gather(cache, table, starts, length, counts, dtype):
-    b, dev = table._shape[0], table._device
-    materialize_touched((cache.k, cache.v, cache.k_scales, cache.v_scales, table, starts, counts), None, False)
-    with _on(dev):
-        k, v = (alloc_bthd(b, cache.kv_heads, length, cache.head_dim, dtype, dev) for _ in range(2))
-        check(
-            "mi355x_paged_gather",
-            lib().mi355x_paged_gather(k._ptr, _bht(k), v._ptr, _bht(v), cache._desc, *_seqs(table, starts, counts),
-                                      b, length, _code(dtype), _error_slot(dev, _PAGE_ERROR), _STREAM),
-        )
+    if lazy_live():
+        materialize_touched((*cache.tensors, table, starts, counts), None, False)
+    return _with_device(table._device, lambda: _gather(cache, table, starts, length, counts, dtype, table._device))
+
+
+def _gather(cache, table, starts, length, counts, dtype, dev):
+    b = table._shape[0]
+    k, v = (_heads_out(b, cache.kv_heads, length, cache.head_dim, dtype, dev) for _ in range(2))
+    check(
+        "mi355x_paged_gather",
+        lib().mi355x_paged_gather(k._ptr, _bht(k), v._ptr, _bht(v), cache._desc, *_seqs(table, starts, counts),
+                                  b, length, _code(dtype), _error_slot(dev, _PAGE_ERROR), _STREAM),
+    )
     return k, v
 
 
 def attention(q, cache, table, starts, counts, window, sinks, scale):
+    if lazy_live():
+        materialize_touched((q, *cache.tensors, table, starts, counts), None, False)
+    return _with_device(q._device, lambda: _attention(q, cache, table, starts, counts, window, sinks, scale, q._device))
+
+
+def _attention(q, cache, table, starts, counts, window, sinks, scale, dev):
     b, h, t, d = q._shape
-    dev, code = q._device, _code(q._dtype)
-    materialize_touched((q, cache.k, cache.v, cache.k_scales, cache.v_scales, table, starts, counts), None, False)
-    with _on(dev):
-        q = _rows(q)
-        out = alloc_bthd(b, h, t, d, q._dtype, dev)
-        ws = lib().mi355x_paged_attn_workspace_bytes(cache._desc, table._shape[1], b, h, t, window, sinks, code)
-        hold, wptr = _workspace(ws, dev)
-        check(
-            "mi355x_paged_attn",
-            lib().mi355x_paged_attn(out._ptr, _bht(out), q._ptr, _bht(q), cache._desc, *_seqs(table, starts, counts),
-                                    b, h, t, scale, window, sinks, code, wptr, ws, _error_slot(dev, _PAGE_ERROR),
-                                    _STREAM),
-        )
+    q = _rows(q)
+    code = _code(q._dtype)
+    out = _heads_out(b, h, t, d, q._dtype, dev)
+    library = lib()
+    ws = library.mi355x_paged_attn_workspace_bytes(cache._desc, table._shape[1], b, h, t, window, sinks, code)
+    hold, wptr = _workspace(ws, dev)
+    check(
+        "mi355x_paged_attn",
+        library.mi355x_paged_attn(out._ptr, _bht(out), q._ptr, _bht(q), cache._desc, *_seqs(table, starts, counts),
+                                  b, h, t, scale, window, sinks, code, wptr, ws, _error_slot(dev, _PAGE_ERROR), _STREAM),
+    )
     return out

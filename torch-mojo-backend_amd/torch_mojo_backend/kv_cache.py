@@ -70,6 +70,9 @@ class PagedKVCache:
             if _overlaps(t):
                 raise ValueError("PagedKVCache: rows of pages must not overlap")
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.tensors = tuple(tensors)
+        self.scale = self.head_dim ** -0.5  # attention's default
+        self.on_mojo = all(isinstance(t, TorchMojoTensor) for t in tensors)
         if self.on_mojo:
             for t in (k, v):
                 if t._ptr % 16 or any(s * t._itemsize % 16 for s in t._strides[:3]):
@@ -84,11 +87,6 @@ class PagedKVCache:
     @property
     def device(self):
         return self.k.device
-
-    @property
-    def on_mojo(self) -> bool:
-        return all(t is None or isinstance(t, TorchMojoTensor)
-                   for t in (self.k, self.v, self.k_scales, self.v_scales))
 
     @classmethod
     def zeros(cls, num_pages, page_size, kv_heads, head_dim, *, dtype=torch.bfloat16, bits=None, device="mojo"):

@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import kv_cache
-from .eager_kernels import aten_fast, materialize_touched
+from .eager_kernels import aten_fast, materialize_touched, paged
 from .masks import sliding_window_causal_mask
 from .mojo_device.torch_mojo_tensor import TorchMojoTensor
 
@@ -191,6 +191,16 @@ def paged_append(cache, page_table, starts, k, v, cos=None, sin=None, *, q=None,
     or a position outside cos raises IndexError (on the mojo device at the next
     device-to-host read) and is not written.  Two tokens of one call must not
     name the same slot."""
+    if (paged.seqs_ok(cache, page_table, starts, counts) and paged.rows_ok(cache, k, page_table._shape[0])
+            and paged.rows_ok(cache, v, page_table._shape[0]) and k._shape[1] == cache.kv_heads and k._shape == v._shape
+            and (cos is None) == (sin is None) == (q is None)
+            and (cos is None or (type(cos) is type(sin) is TorchMojoTensor and cos._dtype is sin._dtype is torch.float32
+                                 and len(cos._shape) == 2 and cos._shape == sin._shape
+                                 and cos._shape[1] == cache.head_dim and cache.head_dim % 16 == 0
+                                 and cos._device == sin._device == k._device and paged.rows_ok(cache, q, k._shape[0])
+                                 and q._shape[2] == k._shape[2] and q._shape[1]))
+            and not _needs_grad(cos, sin)):
+        return paged.append(cache, page_table, starts, k, v, cos, sin, q, counts)
     what = "paged_append"
     if k.dim() != 4:
         raise ValueError(f"{what}: k must be [batch, kv_heads, tokens, head_dim], got {tuple(k.shape)}")
@@ -217,8 +227,6 @@ def paged_append(cache, page_table, starts, k, v, cos=None, sin=None, *, q=None,
         if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] == 0:
             raise ValueError(f"{what}: q is {tuple(q.shape)}, k {tuple(k.shape)}")
     if cache.on_mojo:
-        from .eager_kernels import paged
-
         return paged.append(cache, page_table, starts, k, v, cos, sin, q, counts)
     return kv_cache.append_plain(cache, page_table, starts, k, v, cos, sin, q, counts)
 
@@ -236,8 +244,6 @@ def paged_gather(cache, page_table, starts, length, *, counts=None, dtype=None):
     if length < 0:
         raise ValueError(f"{what}: length {length}")
     if cache.on_mojo:
-        from .eager_kernels import paged
-
         return paged.gather(cache, page_table, starts, length, counts, dtype)
     return kv_cache.gather_plain(cache, page_table, starts, length, counts, dtype)
 
@@ -254,6 +260,10 @@ def paged_attention(q, cache, page_table, starts, *, counts=None, window=0, sink
     A page that does not exist raises IndexError (on the mojo device at the
     next device-to-host read) and counts as hidden.  What lies in pages behind
     a sequence's last token is never used."""
+    if (paged.seqs_ok(cache, page_table, starts, counts) and paged.rows_ok(cache, q, page_table._shape[0])
+            and q._shape[1] and q._shape[1] % cache.kv_heads == 0 and type(window) is type(sinks) is int
+            and window >= 0 and sinks >= 0 and scale is None):
+        return paged.attention(q, cache, page_table, starts, counts, window, sinks, cache.scale)
     what = "paged_attention"
     if q.dim() != 4:
         raise ValueError(f"{what}: q must be [batch, heads, tokens, head_dim], got {tuple(q.shape)}")
@@ -264,11 +274,9 @@ def paged_attention(q, cache, page_table, starts, *, counts=None, window=0, sink
     window, sinks = int(window), int(sinks)
     if window < 0 or sinks < 0:
         raise ValueError(f"{what}: window {window} and sinks {sinks} must not be negative")
-    scale = cache.head_dim ** -0.5 if scale is None else float(scale)
+    scale = cache.scale if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what}: scale {scale} must be finite")
     if cache.on_mojo:
-        from .eager_kernels import paged
-
         return paged.attention(q, cache, page_table, starts, counts, window, sinks, scale)
     return kv_cache.attention_plain(q, cache, page_table, starts, counts, window, sinks, scale)
