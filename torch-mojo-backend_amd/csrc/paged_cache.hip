@@ -3,10 +3,8 @@
 //
 // Every row of new queries, keys and values is read once and written once, so
 // both kernels are bound by memory traffic for a prompt and by latency for a
-// single token: one launch does q, k and v.  A thread owns eight channels of a
-// row (16 bytes of 16-bit values) and, for the rotation, also reads the eight
-// channels half a row away, which another lane of the same wave owns (a hit in
-// the L1), instead of exchanging them.
+// single token: one launch does q, k and v, 16 bytes of 16-bit values at a
+// time.
 //
 // Rotation, half-split: y[i] = x[i] cos[p][i] - x[i + d/2] sin[p][i] and
 // y[i + d/2] = x[i + d/2] cos[p][i + d/2] + x[i] sin[p][i + d/2].
@@ -19,6 +17,8 @@
 // contraction of the operations.  A group with a NaN or an infinity reads back
 // as NaN.
 #include <math.h>
+
+#include <type_traits>
 
 #include "paged.h"
 
@@ -79,6 +79,7 @@ struct AppendArgs {
   const void *cos, *sin;  // null: no rotation
   int64_t rope_len;
   int heads, kv_heads, seq, d;
+  int64_t tokens;      // batch * seq
   uint32_t per_token;  // threads of a token: (heads + 2 kv_heads) * d / 8
 };
 
@@ -113,48 +114,56 @@ __device__ __forceinline__ f16 to_f16_by_f32(double x) {
   return (f16)f;
 }
 
-// clamp(rint((x - base) / step), 0, 15) as the quotient in f64 has it.  An f32
-// quotient is within 2^-22 of it and settles all but the one in 50000 that are
-// next to a border; (c + 1/2) * step, of 16 bits, settles those.
-template <typename W>
-__device__ __forceinline__ uint32_t code_of(W x, W base, float inv, double step, double base_d) {
-  const float q = fminf(fmaxf((float)(x - base) * inv, 0.f), 15.f);
-  float c = rintf(q);
-  if (fabsf(fabsf(q - c) - 0.5f) < 1e-5f) {
-    const float k = floorf(q);
-    const double d = (double)x - base_d, border = ((double)k + 0.5) * step;
-    c = d > border || (d == border && ((int)k & 1)) ? k + 1.f : k;
-  }
-  return (uint32_t)c;
-}
-
 // Packs the eight channels of this lane; four neighbouring lanes hold the 32
 // channels that share a scale.  W is a type that holds the values exactly.
+// A code is clamp(rint((x - base) / step), 0, 15) as the quotient in f64 has
+// it: an f32 quotient is within 2^-22 of it and settles all lanes but the one
+// in 6000 with a value next to a border, (c + 1/2) * step of 16 bits, which
+// settles those.  (The 64-bit quotients took 8 us of 42 for the prompts above
+// paged_append_heads.)
 template <typename W>
 __device__ __forceinline__ void pack_row(const W (&x)[8], uint32_t* codes, f16* scales, int ch, int d) {
   const W limit = (W)kKvLimit;
-  W lo = x[0], hi = x[0];
-  bool bad = false;
+  W lo = x[0], hi = x[0], nan = (W)0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    bad |= !(fabs(x[e]) < (W)INFINITY);
+    nan = fma(x[e], (W)0, nan);  // of an infinity too
     lo = fmin(lo, x[e]), hi = fmax(hi, x[e]);
   }
+  int bad = !(nan == (W)0);
 #pragma unroll
   for (int off = 1; off < 4; off <<= 1) {
     lo = fmin(lo, __shfl_xor(lo, off, 64));
     hi = fmax(hi, __shfl_xor(hi, off, 64));
-    bad |= (bool)__shfl_xor((int)bad, off, 64);
+    bad |= __shfl_xor(bad, off, 64);
   }
   lo = fmin(fmax(lo, -limit), limit), hi = fmin(fmax(hi, -limit), limit);
-  const f16 step16 = bad ? (f16)NAN : to_f16_by_f32(((double)hi - (double)lo) / 15.0), base16 = bad ? (f16)NAN : to_f16_by_f32(lo);
+  // times 1 / 15 is within 2^-53 of the quotient, which f32 does not resolve
+  const f16 step16 = bad ? (f16)NAN : to_f16_by_f32(((double)hi - (double)lo) * (1.0 / 15.0));
+  const f16 base16 = bad ? (f16)NAN : to_f16_by_f32(lo);
   uint32_t w = 0;
   if ((float)step16 > 0.f) {
     const float inv = 1.f / (float)step16;
-    const double step = (double)(float)step16, base = (double)(float)base16;
+    const W base = (W)(float)base16;
+    float far = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      w |= code_of<W>(fmin(fmax(x[e], -limit), limit), (W)base, inv, step, base) << (4 * (e / 2 + 4 * (e % 2)));
+    for (int e = 0; e < 8; ++e) {
+      const float q = fminf(fmaxf((float)(x[e] - base) * inv, 0.f), 15.f), c = rintf(q);
+      far = fmaxf(far, fabsf(q - c));
+      w |= (uint32_t)c << (4 * (e / 2 + 4 * (e % 2)));
+    }
+    if (far > 0.5f - 1e-5f) {
+      const double step = (double)(float)step16;
+      w = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double v = (double)x[e] - (double)base;
+        const float k = floorf(fminf(fmaxf((float)v * inv, 0.f), 15.f));
+        const double border = ((double)k + 0.5) * step;
+        const uint32_t c = (uint32_t)k, up = v > border || (v == border && (c & 1));
+        w |= min(c + up, 15u) << (4 * (e / 2 + 4 * (e % 2)));
+      }
+    }
   }
   const int s = ch / kKvGroup, g = ch % kKvGroup / 8;
   codes[g * (d / kKvGroup) + s] = w;
@@ -164,8 +173,125 @@ __device__ __forceinline__ void pack_row(const W (&x)[8], uint32_t* codes, f16* 
   }
 }
 
-// A block's threads are 256 consecutive (token, row, eight channels) of one
-// sequence; the rows of a token are its query heads, then K, then V.
+// The place of token t of sequence b, or false: padding, or out of range.
+__device__ __forceinline__ bool place_of(const AppendArgs& a, int64_t b, int64_t pos, int* page, uint32_t* slot) {
+  *page = -1;
+  if (pos < 0 || pos > kMaxPosition || (a.cos && pos >= a.rope_len)) {
+    if (a.s.error) *a.s.error = 1;
+  } else {
+    *page = page_of(a.s, b, (uint32_t)pos, slot);
+  }
+  return *page >= 0;
+}
+
+// A thread owns channels ch .. ch + 7 and their partners half a row on, of
+// kHeads rows of one token and of one kind (query, key or value, the same for
+// a block): the angles are read once for all of them, and their loads are all
+// in flight before the first is used.  One row a thread took 42 us for four
+// prompts of 2048 tokens, 16 query and 8 K/V heads of 128, in 4 bits, whose
+// waves are too short to hide the lookup of their page.
+constexpr int kHeads = 4;
+
+template <typename T, typename RT, bool FOUR>
+__global__ void __launch_bounds__(kThreads) paged_append_heads(AppendArgs a) {
+  const int half = a.d / 2;
+  const uint32_t lanes = a.d / 16, id = blockIdx.x * kThreads + threadIdx.x, token = id / lanes;
+  const int ch = (int)(id - token * lanes) * 8;
+  if (token >= (uint32_t)a.tokens) return;
+  const uint32_t bi = token / a.seq, t = token - bi * a.seq;
+  const int64_t b = bi;
+  // blockIdx.y: groups of query heads, then of K heads, then of V heads
+  const int nq = (a.heads + kHeads - 1) / kHeads, nk = (a.kv_heads + kHeads - 1) / kHeads;
+  int group = blockIdx.y;
+  const bool is_q = group < nq, is_k = !is_q && group < nq + nk;
+  if (!is_q) group -= is_k ? nq : nq + nk;
+  const int h0 = group * kHeads, n = min(kHeads, (is_q ? a.heads : a.kv_heads) - h0);
+  const Rows& src = is_q ? a.q : is_k ? a.k : a.v;
+  const T* x = row_of<T>(src, b, h0, t) + ch;
+  Oct<T> lo[kHeads], hi[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i)
+    if (i < n) lo[i] = *(const Oct<T>*)(x + i * src.h), hi[i] = *(const Oct<T>*)(x + i * src.h + half);
+  const bool real = (int)t < seq_count(a.s, b, a.seq);
+  const int64_t pos = (int64_t)a.s.starts[b] + t;
+  const bool turns = (is_q || is_k) && a.cos;
+  Oct<RT> cl, cv, sl, sv;
+  if (turns && real && pos >= 0 && pos < a.rope_len) {
+    const RT *c = (const RT*)a.cos + pos * a.d + ch, *s = (const RT*)a.sin + pos * a.d + ch;
+    cl = *(const Oct<RT>*)c, cv = *(const Oct<RT>*)(c + half);
+    sl = *(const Oct<RT>*)s, sv = *(const Oct<RT>*)(s + half);
+  }
+  auto turn = [&](auto& y, auto& z, int i) {  // the rotated halves, in y's type
+    typedef std::remove_reference_t<decltype(y[0])> W;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const W p = (W)to_f32(lo[i].v[e]), q = (W)to_f32(hi[i].v[e]);
+      y[e] = p * (W)to_f32(cl.v[e]) - q * (W)to_f32(sl.v[e]);
+      z[e] = q * (W)to_f32(cv.v[e]) + p * (W)to_f32(sv.v[e]);
+    }
+  };
+  auto turn_rows = [&](int i) {  // lo and hi rotated and rounded to the rows' type
+    float y[8], z[8];
+    turn(y, z, i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[i].v[e] = from_f32<T>(y[e]), hi[i].v[e] = from_f32<T>(z[e]);
+  };
+  if (is_q) {
+    const bool ok = real && pos >= 0 && pos < a.rope_len;
+    T* o = (T*)a.qo.p + b * a.qo.b + h0 * a.qo.h + t * a.qo.t + ch;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (i >= n) break;
+      if (ok) turn_rows(i);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[i].v[e] = hi[i].v[e] = from_f32<T>(0.f);
+      *(Oct<T>*)(o + i * a.qo.h) = lo[i], *(Oct<T>*)(o + i * a.qo.h + half) = hi[i];
+    }
+    return;
+  }
+  int page;
+  uint32_t slot;
+  if (!real || !place_of(a, b, pos, &page, &slot)) return;
+  const int64_t* st = is_k ? a.c.k_phs : a.c.v_phs;
+  const int64_t at = page * st[0] + h0 * st[1] + slot * st[2];
+  if constexpr (FOUR) {
+    const int64_t* ss = is_k ? a.c.ks_phs : a.c.vs_phs;
+    uint8_t* codes = (uint8_t*)(is_k ? a.c.k : a.c.v) + at;
+    f16* scales = (f16*)(is_k ? a.c.k_scales : a.c.v_scales) + page * ss[0] + h0 * ss[1] + slot * ss[2];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (i >= n) break;
+      uint32_t* c = (uint32_t*)(codes + i * st[1]);
+      if (turns) {
+        double y[8], z[8];
+        turn(y, z, i);
+        pack_row(y, c, scales + i * ss[1], ch, a.d);
+        pack_row(z, c, scales + i * ss[1], ch + half, a.d);
+      } else {
+        float y[8], z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = to_f32(lo[i].v[e]), z[e] = to_f32(hi[i].v[e]);
+        pack_row(y, c, scales + i * ss[1], ch, a.d);
+        pack_row(z, c, scales + i * ss[1], ch + half, a.d);
+      }
+    }
+  } else {
+    T* o = (T*)(is_k ? a.c.k : a.c.v) + at + ch;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (i >= n) break;
+      if (turns) turn_rows(i);
+      *(Oct<T>*)(o + i * st[1]) = lo[i], *(Oct<T>*)(o + i * st[1] + half) = hi[i];
+    }
+  }
+}
+
+// Rows whose halves are no whole pieces of eight channels, or in 4 bits of 32
+// (head_dim 24, or 96 in 4 bits): a thread owns eight channels of one row, and
+// reads their partners for the rotation again.  A block's threads are 256
+// consecutive (token, row, eight channels) of one sequence; the rows of a
+// token are its query heads, then K, then V.
 template <typename T, typename RT, bool FOUR>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a) {
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
@@ -190,17 +316,11 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a) {
     *(Oct<T>*)((T*)a.qo.p + b * a.qo.b + r * a.qo.h + t * a.qo.t + ch) = o;
     return;
   }
-  if (!real) return;
   const bool is_k = h < a.kv_heads;
   const int64_t hk = is_k ? h : h - a.kv_heads;
-  uint32_t slot = 0;
-  int page = -1;
-  if (pos < 0 || pos > kMaxPosition || (a.cos && pos >= a.rope_len)) {
-    if (a.s.error) *a.s.error = 1;
-  } else {
-    page = page_of(a.s, b, (uint32_t)pos, &slot);
-  }
-  if (page < 0) return;  // the same for all rows of the token, and so for all lanes of a group
+  int page;
+  uint32_t slot;
+  if (!real || !place_of(a, b, pos, &page, &slot)) return;  // the same for all lanes of a group
   const int64_t* st = is_k ? a.c.k_phs : a.c.v_phs;
   const int64_t at = page * st[0] + hk * st[1] + slot * st[2];
   const T* x = row_of<T>(is_k ? a.k : a.v, b, hk, t);
@@ -294,16 +414,27 @@ bool rows_ok(const void* p, const int64_t* bht, size_t es) {
          bht[2] * (int64_t)es % 16 == 0;
 }
 
-template <typename T>
-int append_launch(const AppendArgs& a, int rope_dtype, dim3 grid, hipStream_t s) {
-  if (a.c.bits == 4) {
-    if (rope_dtype == MI355X_F32) paged_append_kernel<T, float, true><<<grid, kThreads, 0, s>>>(a);
-    else paged_append_kernel<T, T, true><<<grid, kThreads, 0, s>>>(a);
+template <typename T, typename RT, bool FOUR>
+int append_launch(const AppendArgs& a, hipStream_t s) {
+  if (a.d % (FOUR ? 2 * kKvGroup : 16) == 0) {
+    const int64_t threads = a.tokens * (a.d / 16);
+    MI_REQUIRE(threads < (1ll << 32) - kThreads, "mi355x_paged_append: more than 2^36 values of one head");
+    const unsigned groups = ceil_div(a.heads, kHeads) + 2 * ceil_div(a.kv_heads, kHeads);
+    paged_append_heads<T, RT, FOUR><<<dim3(ceil_div(threads, kThreads), groups), kThreads, 0, s>>>(a);
   } else {
-    if (rope_dtype == MI355X_F32) paged_append_kernel<T, float, false><<<grid, kThreads, 0, s>>>(a);
-    else paged_append_kernel<T, T, false><<<grid, kThreads, 0, s>>>(a);
+    const int64_t per_token = a.per_token;
+    MI_REQUIRE(per_token * a.seq < (1ll << 32) - kThreads, "mi355x_paged_append: more than 2^35 values of one sequence");
+    paged_append_kernel<T, RT, FOUR>
+        <<<dim3(ceil_div(per_token * a.seq, kThreads), (unsigned)(a.tokens / a.seq)), kThreads, 0, s>>>(a);
   }
   return check_launch("mi355x_paged_append");
+}
+
+template <typename T>
+int append_rows(const AppendArgs& a, int rope_dtype, hipStream_t s) {
+  const bool f32 = rope_dtype == MI355X_F32;
+  if (a.c.bits == 4) return f32 ? append_launch<T, float, true>(a, s) : append_launch<T, T, true>(a, s);
+  return f32 ? append_launch<T, float, false>(a, s) : append_launch<T, T, false>(a, s);
 }
 
 template <typename T>
@@ -353,14 +484,13 @@ extern "C" int mi355x_paged_append(const mi355x_paged_cache* cache, const int32_
   if (q) a.q = Rows{(void*)q, q_bht[0], q_bht[1], q_bht[2]}, a.qo = Rows{q_out, qo_bht[0], qo_bht[1], qo_bht[2]};
   a.cos = cos_table, a.sin = sin_table, a.rope_len = rope_len;
   a.heads = (int)heads, a.kv_heads = (int)cache->kv_heads, a.seq = (int)seq, a.d = (int)cache->d;
-  const int64_t per_token = (heads + 2 * cache->kv_heads) * (cache->d / 8);
-  MI_REQUIRE(per_token * seq < (1ll << 32) - kThreads, "mi355x_paged_append: more than 2^35 values of one sequence");
-  a.per_token = (uint32_t)per_token;
-  const dim3 grid(ceil_div(per_token * seq, kThreads), (unsigned)batch);
+  MI_REQUIRE(batch * seq < (1ll << 31), "mi355x_paged_append: batch x tokens must be below 2^31");
+  a.tokens = batch * seq;
+  a.per_token = (uint32_t)((heads + 2 * cache->kv_heads) * (cache->d / 8));
   const int rdt = cos_table ? rope_dtype : MI355X_F32;
-  if (dtype == MI355X_F32) return append_launch<float>(a, rdt, grid, (hipStream_t)stream);
-  if (dtype == MI355X_BF16) return append_launch<bf16>(a, rdt, grid, (hipStream_t)stream);
-  return append_launch<f16>(a, rdt, grid, (hipStream_t)stream);
+  if (dtype == MI355X_F32) return append_rows<float>(a, rdt, (hipStream_t)stream);
+  if (dtype == MI355X_BF16) return append_rows<bf16>(a, rdt, (hipStream_t)stream);
+  return append_rows<f16>(a, rdt, (hipStream_t)stream);
 }
 
 extern "C" int mi355x_paged_gather(void* k, const int64_t* k_bht, void* v, const int64_t* v_bht,
