@@ -55,22 +55,41 @@ struct Places {
   uint32_t live;  // keys that some row may see and whose page exists
 };
 
-// Address of the row of key 16 kt + k of the tile, `es` bytes a unit of the
-// strides; what is not live lies in page 0.  16 keys of a tile that share a
-// page (P16) have a base that is the same for all lanes, and of the lane's own
-// address only 32 bits, the same for every tile.
+// Rows of one tensor of a cache, for one K/V head.
 template <bool P16>
-__device__ __forceinline__ const char* row_at(const void* base, int es, const Places& p, int kt, int k,
-                                              const int64_t* st, int64_t hk) {
-  if constexpr (P16) {
-    const int64_t page = __builtin_amdgcn_readlane(p.page, 16 * kt), slot = __builtin_amdgcn_readlane(p.slot, 16 * kt);
-    const char* first = (const char*)base + (page * st[0] + hk * st[1] + slot * st[2]) * es;
-    return first + (uint32_t)(k * ((int)st[2] * es));
-  } else {
-    const int64_t page = __shfl(p.page, 16 * kt + k, 64), slot = __shfl(p.slot, 16 * kt + k, 64);
-    return (const char*)base + (page * st[0] + hk * st[1] + slot * st[2]) * es;
+struct RowsOf {
+  const char* base;
+  int64_t page_bytes, slot_bytes;
+  __device__ __forceinline__ RowsOf(const void* p, int es, const int64_t* st, int64_t hk)
+      : base((const char*)p + hk * st[1] * es), page_bytes(st[0] * es), slot_bytes(st[2] * es) {}
+  // Byte `at` of the row of key 16 kt + k of the tile; what is not live lies in
+  // page 0.  16 keys of a tile that share a page (P16) have a base that is the
+  // same for all lanes, and of the lane's own address only 32 bits, the same
+  // for every tile.
+  __device__ __forceinline__ const char* row(const Places& p, int kt, int k, int at) const {
+    if constexpr (P16) {
+      const uint32_t page = __builtin_amdgcn_readlane(p.page, 16 * kt), slot = __builtin_amdgcn_readlane(p.slot, 16 * kt);
+      const char* first = base + (uint64_t)page * (uint32_t)page_bytes + slot * (uint32_t)slot_bytes;
+      return first + (uint32_t)(k * (int)slot_bytes + at);
+    } else {
+      const int64_t page = __shfl(p.page, 16 * kt + k, 64), slot = __shfl(p.slot, 16 * kt + k, 64);
+      return base + page * page_bytes + slot * slot_bytes + at;
+    }
   }
+};
+// Whether P16 takes such rows: 32-bit offsets within a page, page strides
+// below 2^32 bytes.
+bool short_strides(const int64_t* st, int64_t es, int64_t page_size) {
+  return st[0] * es < (1ll << 32) && st[2] * es * (page_size + 16) < (1ll << 31);
 }
+
+// What a block reads from its cache.
+template <bool P16>
+struct CacheRows {
+  RowsOf<P16> k, v, ks, vs;
+  __device__ __forceinline__ CacheRows(const mi355x_paged_cache& c, int es, int64_t hk)
+      : k(c.k, es, c.k_phs, hk), v(c.v, es, c.v_phs, hk), ks(c.k_scales, 2, c.ks_phs, hk), vs(c.v_scales, 2, c.vs_phs, hk) {}
+};
 
 // ---------------------------------------------------------------------------
 // page formats
@@ -78,7 +97,7 @@ __device__ __forceinline__ const char* row_at(const void* base, int es, const Pl
 // 16-bit pages of T.
 template <typename T, int D_>
 struct Pages16 {
-  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW);
+  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), kBytes = 2;
   typedef typename Mfma<T>::frag frag;
   typedef uint32_t vword __attribute__((ext_vector_type(VW / 2)));
   struct Keys {
@@ -104,19 +123,19 @@ struct Pages16 {
     q.scale = scale_log2;
   }
   template <bool P16>
-  static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+  static __device__ __forceinline__ void load_keys(Keys& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const T* row = (const T*)row_at<P16>(a.c.k, sizeof(T), p, kt, lr, a.c.k_phs, hk) + g * 8;
+      const T* row = (const T*)c.k.row(p, kt, lr, g * 16);
 #pragma unroll
       for (int s = 0; s < D / 32; ++s) r.k[kt][s] = *(const frag*)(row + s * 32);
     }
   }
   template <bool P16>
-  static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+  static __device__ __forceinline__ void load_values(Values& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const T* row = (const T*)row_at<P16>(a.c.v, sizeof(T), p, i >> 2, 4 * g + (i & 3), a.c.v_phs, hk) + lr * VW;
+      const T* row = (const T*)c.v.row(p, i >> 2, 4 * g + (i & 3), lr * VW * 2);
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = *(const vword*)(row + u * 16 * VW);
     }
@@ -177,7 +196,7 @@ struct Pages16 {
 // the keys of a product step taken as 4 g + step, V's rows need no exchange.
 template <int D_>
 struct Pages32 {
-  static constexpr int D = D_, KT = 1, VW = 4, NU = D / 64;
+  static constexpr int D = D_, KT = 1, VW = 4, NU = D / 64, kBytes = 4;
   struct Keys {
     f32x4 k[D / 16];
   };
@@ -195,16 +214,16 @@ struct Pages32 {
     q.scale = scale_log2;
   }
   template <bool P16>
-  static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
-    const float* k = (const float*)row_at<P16>(a.c.k, 4, p, 0, lr, a.c.k_phs, hk) + g * 4;
+  static __device__ __forceinline__ void load_keys(Keys& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
+    const float* k = (const float*)c.k.row(p, 0, lr, g * 16);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) r.k[s] = *(const f32x4*)(k + s * 16);
   }
   template <bool P16>
-  static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+  static __device__ __forceinline__ void load_values(Values& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* v = (const float*)row_at<P16>(a.c.v, 4, p, 0, 4 * g + i, a.c.v_phs, hk) + lr * 4;
+      const float* v = (const float*)c.v.row(p, 0, 4 * g + i, lr * 16);
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = *(const f32x4*)(v + u * 64);
     }
@@ -245,7 +264,7 @@ struct Pages32 {
 // 4-bit pages, queries of T.
 template <typename T, int D_>
 struct Pages4 {
-  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), NG = D / kKvGroup;
+  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), NG = D / kKvGroup, kBytes = 1;
   typedef f16x8 frag;
   typedef uint32_t row_words __attribute__((ext_vector_type(NG)));  // a lane's codes of a K row, or the row's scales
   struct Keys {
@@ -285,21 +304,22 @@ struct Pages4 {
     q.scale = ldexpf(scale_log2, ex);
   }
   template <bool P16>
-  static __device__ __forceinline__ void load_keys(Keys& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+  static __device__ __forceinline__ void load_keys(Keys& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      r.k[kt] = *(const row_words*)(row_at<P16>(a.c.k, 1, p, kt, lr, a.c.k_phs, hk) + g * (D / 8));
-      r.ks[kt] = *(const row_words*)row_at<P16>(a.c.k_scales, 2, p, kt, lr, a.c.ks_phs, hk);
+      r.k[kt] = *(const row_words*)c.k.row(p, kt, lr, g * (D / 8));
+      r.ks[kt] = *(const row_words*)c.ks.row(p, kt, lr, 0);
     }
   }
   template <bool P16>
-  static __device__ __forceinline__ void load_values(Values& r, const DecodeArgs& a, const Places& p, int64_t hk, int lr, int g) {
+  static __device__ __forceinline__ void load_values(Values& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t* v = (const uint32_t*)row_at<P16>(a.c.v, 1, p, i >> 2, 4 * g + (i & 3), a.c.v_phs, hk);
-      const uint32_t* s = (const uint32_t*)row_at<P16>(a.c.v_scales, 2, p, i >> 2, 4 * g + (i & 3), a.c.vs_phs, hk);
 #pragma unroll
-      for (int u = 0; u < NU; ++u) r.v[i][u] = v[word(u, lr)], r.vs[i][u] = s[word(u, lr) % NG];
+      for (int u = 0; u < NU; ++u) {
+        r.v[i][u] = *(const uint32_t*)c.v.row(p, i >> 2, 4 * g + (i & 3), word(u, lr) * 4);
+        r.vs[i][u] = *(const uint32_t*)c.vs.row(p, i >> 2, 4 * g + (i & 3), word(u, lr) % NG * 4);
+      }
     }
   }
   static __device__ __forceinline__ void hide_values(Values& r, uint32_t live, int g) {
@@ -310,12 +330,20 @@ struct Pages4 {
         for (int u = 0; u < NU; ++u) r.vs[i][u] = 0;
   }
   // Nibble i of both halves of w under the scales and minimums of s and m.
-  static __device__ __forceinline__ f16x2 value(uint32_t w, int i, f16x2 s, f16x2 m) {
-    const f16x2 c = __builtin_bit_cast(f16x2, (w >> (4 * i) & 0x000f000fu) | 0x64006400u) - (f16)1024.f;
+  // `mask` is 0x000f000f in a vector register: an instruction takes one
+  // constant from elsewhere, and two make it an AND and an OR.
+  static __device__ __forceinline__ f16x2 value(uint32_t w, int i, uint32_t mask, f16x2 s, f16x2 m) {
+    const f16x2 c = __builtin_bit_cast(f16x2, (w >> (4 * i) & mask) | 0x64006400u) - (f16)1024.f;
     return __builtin_elementwise_fma(c, s, m);
+  }
+  static __device__ __forceinline__ uint32_t nibbles() {
+    uint32_t mask;
+    asm("v_mov_b32 %0, 0x000f000f" : "=v"(mask));
+    return mask;
   }
   template <int QT>
   static __device__ __forceinline__ void scores(f32x4 (&s)[KT][QT], const Keys& r, const Query (&q)[QT]) {
+    const uint32_t mask = nibbles();
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
@@ -328,7 +356,7 @@ struct Pages4 {
           frag f;
         } k;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k.h[i] = value(r.k[kt][ks], i, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]});
+        for (int i = 0; i < 4; ++i) k.h[i] = value(r.k[kt][ks], i, mask, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]});
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) s[kt][qt] = Mfma<f16>::mma(k.f, q[qt].q[ks], s[kt][qt]);
       }
@@ -343,6 +371,7 @@ struct Pages4 {
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) pf[qt][4 * kt + e] = (f16)p[kt][qt][e];
+    const uint32_t mask = nibbles();
     const bool odd = D < 128 && (threadIdx.x & 8);
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -365,7 +394,7 @@ struct Pages4 {
         } v;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          v.h[i] = D >= 128 ? value(e % 2 ? odd_w[i] : even_w[i], e / 2, s[i], m[i]) : value(even_w[i], e, s[i], m[i]);
+          v.h[i] = D >= 128 ? value(e % 2 ? odd_w[i] : even_w[i], e / 2, mask, s[i], m[i]) : value(even_w[i], e, mask, s[i], m[i]);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) o[u][e][qt] = Mfma<f16>::mma(v.f, pf[qt], o[u][e][qt]);
       }
@@ -455,12 +484,13 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
   // there are more than with two tiles in registers.
   typename F::Keys keys;
   typename F::Values values;
+  const CacheRows<P16> rows_of(a.c, F::kBytes, hk);
   int i = split * per + wave;
   Places here{0, 0, 0}, next{0, 0, 0};
   if (i < end) {
     here = look_up(i);
-    F::template load_keys<P16>(keys, a, here, hk, lr, g);
-    F::template load_values<P16>(values, a, here, hk, lr, g);
+    F::template load_keys<P16>(keys, rows_of, here, lr, g);
+    F::template load_values<P16>(values, rows_of, here, lr, g);
     if (i + NW < end) next = look_up(i + NW);
   }
   for (; i < end; i += NW) {
@@ -472,7 +502,7 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
                        (a.window <= 0 || last - j0 < a.window || j0 + TK <= a.sinks);
     f32x4 s[KT][QT];
     F::scores(s, keys, q);
-    if (more) F::template load_keys<P16>(keys, a, next, hk, lr, g);
+    if (more) F::template load_keys<P16>(keys, rows_of, next, lr, g);
     bool moved = false;
     float top[QT];
 #pragma unroll
@@ -520,7 +550,7 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
     if (!whole) F::hide_values(values, live, g);
     F::add_values(o, values, s);
     if (more) {
-      F::template load_values<P16>(values, a, next, hk, lr, g);
+      F::template load_values<P16>(values, rows_of, next, lr, g);
       here = next;
       if (i + 2 * NW < end) next = look_up(i + 2 * NW);
     }
@@ -588,8 +618,9 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
 
 template <typename F, typename T, int QT>
 void launch(const DecodeArgs& a, unsigned blocks, hipStream_t s) {
-  bool p16 = a.c.page_size % 16 == 0;  // and 16 rows lie within 2^31 bytes
-  for (const int64_t* st : {a.c.k_phs, a.c.v_phs, a.c.ks_phs, a.c.vs_phs}) p16 &= st[2] < (1ll << 24);
+  bool p16 = a.c.page_size % 16 == 0;
+  for (const int64_t* st : {a.c.k_phs, a.c.v_phs}) p16 &= short_strides(st, F::kBytes, a.c.page_size);
+  for (const int64_t* st : {a.c.ks_phs, a.c.vs_phs}) p16 &= short_strides(st, 2, a.c.page_size);
   if (p16) paged_attn_mfma<F, T, QT, true><<<blocks, 64 * NW, 0, s>>>(a);
   else paged_attn_mfma<F, T, QT, false><<<blocks, 64 * NW, 0, s>>>(a);
 }
