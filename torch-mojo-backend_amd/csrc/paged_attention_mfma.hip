@@ -40,13 +40,19 @@ constexpr int NW = 4;  // waves of a block
 
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float group_max(float x) {  // over the four lane groups
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+// Over the four lane groups: v_permlane{16,32}_swap of a value with itself
+// leaves the lane 16 (32) further on in the second result.
+__device__ __forceinline__ float group_max(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float group_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // Where the rows of a tile are: lane l looked up key l % TK of it.
@@ -55,41 +61,45 @@ struct Places {
   uint32_t live;  // keys that some row may see and whose page exists
 };
 
-// Rows of one tensor of a cache, for one K/V head.
+// Rows of a cache, for one K/V head.  row(tensor, ...) is byte `at` of the row
+// of key 16 kt + k of the tile in k, v, ks or vs; what is not live lies in
+// page 0.  Rows close together (P16): 16 keys share a page, K and V are laid
+// out alike and scales like their rows a quarter as far apart, so that the 16
+// keys have one offset, the same for all lanes and, shifted, for all tensors,
+// and the lane's own part of an address is 32 bits that no tile changes.
+enum Tensor { kKeys, kValues, kKeyScales, kValueScales };
 template <bool P16>
-struct RowsOf {
-  const char* base;
-  int64_t page_bytes, slot_bytes;
-  __device__ __forceinline__ RowsOf(const void* p, int es, const int64_t* st, int64_t hk)
-      : base((const char*)p + hk * st[1] * es), page_bytes(st[0] * es), slot_bytes(st[2] * es) {}
-  // Byte `at` of the row of key 16 kt + k of the tile; what is not live lies in
-  // page 0.  16 keys of a tile that share a page (P16) have a base that is the
-  // same for all lanes, and of the lane's own address only 32 bits, the same
-  // for every tile.
-  __device__ __forceinline__ const char* row(const Places& p, int kt, int k, int at) const {
+struct CacheRows {
+  const char* base[4];
+  int64_t page_bytes[4], slot_bytes[4];
+  __device__ __forceinline__ CacheRows(const mi355x_paged_cache& c, int es, int64_t hk) {
+    const void* p[4] = {c.k, c.v, c.k_scales, c.v_scales};
+    const int64_t* st[4] = {c.k_phs, c.v_phs, c.ks_phs, c.vs_phs};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int n = t < 2 ? es : 2;
+      base[t] = (const char*)p[t] + hk * st[t][1] * n, page_bytes[t] = st[t][0] * n, slot_bytes[t] = st[t][2] * n;
+    }
+  }
+  __device__ __forceinline__ const char* row(int t, const Places& p, int kt, int k, int at) const {
     if constexpr (P16) {
       const uint32_t page = __builtin_amdgcn_readlane(p.page, 16 * kt), slot = __builtin_amdgcn_readlane(p.slot, 16 * kt);
-      const char* first = base + (uint64_t)page * (uint32_t)page_bytes + slot * (uint32_t)slot_bytes;
-      return first + (uint32_t)(k * (int)slot_bytes + at);
+      const uint64_t off = (uint64_t)page * (uint32_t)page_bytes[0] + slot * (uint32_t)slot_bytes[0];
+      return base[t] + (t < 2 ? off : off >> 2) + (uint32_t)((t < 2 ? k * (int)slot_bytes[0] : k * (int)slot_bytes[0] / 4) + at);
     } else {
       const int64_t page = __shfl(p.page, 16 * kt + k, 64), slot = __shfl(p.slot, 16 * kt + k, 64);
-      return base + page * page_bytes + slot * slot_bytes + at;
+      return base[t] + page * page_bytes[t] + slot * slot_bytes[t] + at;
     }
   }
 };
-// Whether P16 takes such rows: 32-bit offsets within a page, page strides
-// below 2^32 bytes.
-bool short_strides(const int64_t* st, int64_t es, int64_t page_size) {
-  return st[0] * es < (1ll << 32) && st[2] * es * (page_size + 16) < (1ll << 31);
+bool rows_close(const mi355x_paged_cache& c, int64_t es) {
+  const int64_t page = c.k_phs[0] * es, slot = c.k_phs[2] * es;
+  bool ok = c.page_size % 16 == 0 && page < (1ll << 32) && slot * (c.page_size + 16) < (1ll << 31) &&
+            c.v_phs[0] == c.k_phs[0] && c.v_phs[2] == c.k_phs[2];
+  if (c.bits == 4)
+    for (const int64_t* st : {c.ks_phs, c.vs_phs}) ok &= st[0] * 8 == page && st[2] * 8 == slot;
+  return ok;
 }
-
-// What a block reads from its cache.
-template <bool P16>
-struct CacheRows {
-  RowsOf<P16> k, v, ks, vs;
-  __device__ __forceinline__ CacheRows(const mi355x_paged_cache& c, int es, int64_t hk)
-      : k(c.k, es, c.k_phs, hk), v(c.v, es, c.v_phs, hk), ks(c.k_scales, 2, c.ks_phs, hk), vs(c.v_scales, 2, c.vs_phs, hk) {}
-};
 
 // ---------------------------------------------------------------------------
 // page formats
@@ -119,14 +129,19 @@ struct Pages16 {
       for (int e = 0; e < 8; ++e) q.q[s][e] = (T)0.f;
     if (real)
 #pragma unroll
-      for (int s = 0; s < D / 32; ++s) q.q[s] = *(const frag*)(row + s * 32 + g * 8);
-    q.scale = scale_log2;
+      for (int s = 0; s < D / 32; ++s) {
+        q.q[s] = *(const frag*)(row + s * 32 + g * 8);
+        if (scale_log2 < 0.f)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q.q[s][e] = -q.q[s][e];
+      }
+    q.scale = fabsf(scale_log2);
   }
   template <bool P16>
   static __device__ __forceinline__ void load_keys(Keys& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const T* row = (const T*)c.k.row(p, kt, lr, g * 16);
+      const T* row = (const T*)c.row(kKeys, p, kt, lr, g * 16);
 #pragma unroll
       for (int s = 0; s < D / 32; ++s) r.k[kt][s] = *(const frag*)(row + s * 32);
     }
@@ -135,7 +150,7 @@ struct Pages16 {
   static __device__ __forceinline__ void load_values(Values& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const T* row = (const T*)c.v.row(p, i >> 2, 4 * g + (i & 3), lr * VW * 2);
+      const T* row = (const T*)c.row(kValues, p, i >> 2, 4 * g + (i & 3), lr * VW * 2);
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = *(const vword*)(row + u * 16 * VW);
     }
@@ -211,11 +226,14 @@ struct Pages32 {
   static __device__ __forceinline__ void load_query(Query& q, const float* row, bool real, int g, float scale_log2) {
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) q.q[s] = real ? *(const f32x4*)(row + s * 16 + g * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
-    q.scale = scale_log2;
+    if (scale_log2 < 0.f)
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) q.q[s] = -q.q[s];
+    q.scale = fabsf(scale_log2);
   }
   template <bool P16>
   static __device__ __forceinline__ void load_keys(Keys& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
-    const float* k = (const float*)c.k.row(p, 0, lr, g * 16);
+    const float* k = (const float*)c.row(kKeys, p, 0, lr, g * 16);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) r.k[s] = *(const f32x4*)(k + s * 16);
   }
@@ -223,7 +241,7 @@ struct Pages32 {
   static __device__ __forceinline__ void load_values(Values& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* v = (const float*)c.v.row(p, 0, 4 * g + i, lr * 16);
+      const float* v = (const float*)c.row(kValues, p, 0, 4 * g + i, lr * 16);
 #pragma unroll
       for (int u = 0; u < NU; ++u) r.v[i][u] = *(const f32x4*)(v + u * 64);
     }
@@ -297,18 +315,19 @@ struct Pages4 {
     }
     top = group_max(top);
     const int ex = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
+    const float sign = scale_log2 < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q.q[s][e] = (f16)ldexpf(x[s][e], -ex);
-    q.scale = ldexpf(scale_log2, ex);
+      for (int e = 0; e < 8; ++e) q.q[s][e] = (f16)ldexpf(sign * x[s][e], -ex);
+    q.scale = ldexpf(fabsf(scale_log2), ex);
   }
   template <bool P16>
   static __device__ __forceinline__ void load_keys(Keys& r, const CacheRows<P16>& c, const Places& p, int lr, int g) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      r.k[kt] = *(const row_words*)c.k.row(p, kt, lr, g * (D / 8));
-      r.ks[kt] = *(const row_words*)c.ks.row(p, kt, lr, 0);
+      r.k[kt] = *(const row_words*)c.row(kKeys, p, kt, lr, g * (D / 8));
+      r.ks[kt] = *(const row_words*)c.row(kKeyScales, p, kt, lr, 0);
     }
   }
   template <bool P16>
@@ -317,8 +336,8 @@ struct Pages4 {
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        r.v[i][u] = *(const uint32_t*)c.v.row(p, i >> 2, 4 * g + (i & 3), word(u, lr) * 4);
-        r.vs[i][u] = *(const uint32_t*)c.vs.row(p, i >> 2, 4 * g + (i & 3), word(u, lr) % NG * 4);
+        r.v[i][u] = *(const uint32_t*)c.row(kValues, p, i >> 2, 4 * g + (i & 3), word(u, lr) * 4);
+        r.vs[i][u] = *(const uint32_t*)c.row(kValueScales, p, i >> 2, 4 * g + (i & 3), word(u, lr) % NG * 4);
       }
     }
   }
@@ -503,6 +522,8 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
     f32x4 s[KT][QT];
     F::scores(s, keys, q);
     if (more) F::template load_keys<P16>(keys, rows_of, next, lr, g);
+    // the scale is not negative (its sign went into q), so the maximum can be
+    // taken before it
     bool moved = false;
     float top[QT];
 #pragma unroll
@@ -512,15 +533,14 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = s[kt][qt][e] * q[qt].scale;
           if (!whole) {
             const int k = 16 * kt + 4 * g + e;
-            if (!(live >> k & 1) || !visible(pos[qt], j0 + k, a.window, a.sinks)) x = -INFINITY;
+            if (!(live >> k & 1) || !visible(pos[qt], j0 + k, a.window, a.sinks)) s[kt][qt][e] = -INFINITY;
           }
-          s[kt][qt][e] = x;
-          mx = fmaxf(mx, x);
+          mx = fmaxf(mx, s[kt][qt][e]);
         }
-      top[qt] = fmaxf(m[qt], group_max(mx));
+      mx = group_max(mx);
+      top[qt] = fmaxf(m[qt], mx == -INFINITY ? mx : mx * q[qt].scale);
       moved |= top[qt] > m[qt];
     }
     if (__builtin_amdgcn_ballot_w64(moved)) {
@@ -542,7 +562,9 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(s[kt][qt][e] - base);
+          float x = fmaf(s[kt][qt][e], q[qt].scale, -base);
+          if (!whole && s[kt][qt][e] == -INFINITY) x = -INFINITY;  // a scale of zero would make it NaN
+          const float p = __builtin_amdgcn_exp2f(x);
           s[kt][qt][e] = p;
           l[qt] += p;
         }
@@ -618,10 +640,7 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
 
 template <typename F, typename T, int QT>
 void launch(const DecodeArgs& a, unsigned blocks, hipStream_t s) {
-  bool p16 = a.c.page_size % 16 == 0;
-  for (const int64_t* st : {a.c.k_phs, a.c.v_phs}) p16 &= short_strides(st, F::kBytes, a.c.page_size);
-  for (const int64_t* st : {a.c.ks_phs, a.c.vs_phs}) p16 &= short_strides(st, 2, a.c.page_size);
-  if (p16) paged_attn_mfma<F, T, QT, true><<<blocks, 64 * NW, 0, s>>>(a);
+  if (rows_close(a.c, F::kBytes)) paged_attn_mfma<F, T, QT, true><<<blocks, 64 * NW, 0, s>>>(a);
   else paged_attn_mfma<F, T, QT, false><<<blocks, 64 * NW, 0, s>>>(a);
 }
 
