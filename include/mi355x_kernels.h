@@ -609,7 +609,7 @@ int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
                         int64_t window, int dtype, void* workspace, int64_t ws_bytes,
                         mi355x_stream_t stream);
 /* A causal sliding window with sinks: query i sees key j <= i iff i - j <
- * window or j < sinks (both positive); types, head_dims, strides and grouped
+ * window or j < sinks (window > 0, sinks >= 0); types, head_dims, strides and grouped
  * heads as in mi355x_attn_fwd_gen / mi355x_attn_bwd_gen.  Training with the
  * first tokens left visible, as a model that is served with a window needs;
  * the reference runs such a mask through its masked-math decomposition

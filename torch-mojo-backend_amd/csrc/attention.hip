@@ -723,9 +723,10 @@ struct AttnBwdArgs {
   float* ndelta;  // [B, H, Sq]: -D, written by attn_bwd_delta
   float* nlse2;   // [B, H, Sq]: -LSE * log2(e), written by attn_bwd_delta
   float* kv_part; // grouped backward: per-query-head dK, dV partials (f32), or null
-  float* sink_part;    // sinks: partials of the sinks' key blocks (attn_bwd_gqa_dkv)
-  int sink_blocks;     // 64-key blocks that hold sinks
-  int sink_chunks;     // blocks that share the queries behind such a block's window
+  float* sink_part;    // sinks: f32 partials of their dK, dV (dkv_body)
+  int sink_blocks;     // blocks of keys that hold sinks
+  int sink_chunks;     // further blocks for each, which share the queries behind its window
+  int sink_keys;       // rows of a slot of sink_part
   // (stored negated: the dK/dV and dQ steps add them, which saves a negation
   // per score)
 };
@@ -967,31 +968,61 @@ constexpr int kDkvLds = 2 * (2 * KvLayout<D>::TILE + 512);  // 2 stages of Q, dO
 template <int D>
 constexpr int kDqLds = 2 * (2 * KvLayout<D>::TILE);  // 2 stages of K, V
 
-template <typename T, int D>
-__device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char* lds) {
+// Where a block of a windowed backward stands: its tile, and the chunk of the
+// queries behind the window of a block of sinks (-1: the block's own window).
+struct WindowPos {
+  BlockCoord bc;
+  int chunk;
+};
+// Slots of sink_part: 0 for the window of a block of sinks (grouped heads have
+// that in kv_part), then four (one a wave) for each chunk.
+__device__ __forceinline__ float* sink_slot(const AttnBwdArgs& p, int64_t slot, int64_t b, int64_t h, int64_t key, int D) {
+  return p.sink_part + (((slot * p.f.B + b) * p.f.H + h) * p.sink_keys + key) * D;
+}
+__host__ __device__ inline int64_t sink_plane(const AttnBwdArgs& p, int D) {  // from dK's slots to dV's
+  return (4 * (int64_t)p.sink_chunks + 1) * p.f.B * p.f.H * p.sink_keys * D;
+}
+
+// WIN: a causal window, with sinks or without, and grouped K/V heads.  A block
+// takes one query head; with grouped heads it leaves f32 partials that
+// attn_bwd_window_sum adds in head order.  Sinks are seen by every later
+// query, so a block of keys that holds some would walk the whole sequence
+// while the others walk a window: the steps behind its window go to
+// sink_chunks further blocks.  There a wave takes 32 sinks and, where there are
+// fewer than four such waves, every second or fourth pair of query tiles.
+template <typename T, int D, bool WIN = false, int RT = 2>
+__device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, WindowPos at, char* lds) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
   constexpr int KS = D / 32, DT = D / 16;
   constexpr int STAGE = 2 * L::TILE + 512;  // Q tile, dO tile, LSE[64], D[64]
+  constexpr int KW = 16 * RT;  // keys of a wave
 
   const AttnArgs& f = p.f;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int lr = lane & 15, lg = lane >> 4;
-  const BlockCoord bc = block_coord(gp);
-  const int64_t k0 = bc.x * 128;
-  const int64_t b = bc.b, h = bc.h;
+  const BlockCoord bc = at.bc;
+  const int64_t k0 = bc.x * (4 * KW);
+  const int64_t b = bc.b, h = bc.h, hk = WIN ? h / f.group : h;
   const char* Q = (const char*)((const T*)f.q + b * f.q_b + h * f.q_h);
-  const T* K = (const T*)f.k + b * f.k_b + h * f.k_h;
-  const T* V = (const T*)f.v + b * f.v_b + h * f.v_h;
+  const T* K = (const T*)f.k + b * f.k_b + hk * f.k_h;
+  const T* V = (const T*)f.v + b * f.v_b + hk * f.v_h;
   const char* dO = (const char*)((const T*)p.dout + b * p.do_b + h * p.do_h);
   const float* LSE = p.nlse2 + (b * f.H + h) * f.Sq;   // -LSE * log2(e)
   const float* DEL = p.ndelta + (b * f.H + h) * f.Sq;  // -D
   const int64_t qs_b = f.q_s * (int64_t)sizeof(T), dos_b = p.do_s * (int64_t)sizeof(T);
 
-  const int64_t kw = k0 + wave * 32;
-  frag kf[2][KS], vf[2][KS];
+  const bool extra = WIN && at.chunk >= 0;
+  int wave_key = wave, part = 0, parts = 1;  // of a chunk: the wave's 32 keys, and its share of the query tiles
+  if (extra) {
+    const int waves = (int)min((int64_t)4, (f.sinks - k0 + KW - 1) / KW);
+    parts = waves == 1 ? 4 : waves == 2 ? 2 : 1;
+    wave_key = parts == 1 ? wave : wave % waves, part = parts == 1 ? 0 : wave / waves;
+  }
+  const int64_t kw = k0 + wave_key * KW;
+  frag kf[RT][KS], vf[RT][KS];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < RT; ++t) {
     const int64_t kj = kw + t * 16 + lr;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -999,10 +1030,11 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
       vf[t][ks] = kj < f.Skv ? *(const frag*)(V + kj * f.v_s + ks * 32 + lg * 8) : zero_frag<T>();
     }
   }
-  f32x4 dva[DT][2], dka[DT][2];
+  f32x4 dva[DT][RT], dka[DT][RT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
-    dva[dt][0] = dva[dt][1] = dka[dt][0] = dka[dt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < RT; ++t) dva[dt][t] = dka[dt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   KvTileLoad<D, 4> ql, dl;
   ql.init(Q, qs_b);
@@ -1018,11 +1050,22 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
     }
   };
 
-  const int64_t qstart = f.causal ? (k0 / 64) * 64 : 0;
+  int64_t qstart = f.causal ? (k0 / 64) * 64 : 0;
+  int64_t qend = f.Sq;  // of this block's steps
+  if constexpr (WIN) {
+    const int64_t near = min(f.Sq, qstart + ceil_div64(k0 + 4 * KW - 1 + f.window - qstart, 64) * 64);
+    if (extra) {
+      const int64_t per = ceil_div64(ceil_div64(f.Sq - near, 64), p.sink_chunks) * 64;
+      qstart = min(f.Sq, near + at.chunk * per);
+      qend = min(f.Sq, qstart + per);
+    } else {
+      qend = near;
+    }
+  }
   const int sw = L::swz(lr);
   const TrOffsets<D> tro;
   int buf = 0;
-  if (qstart < f.Sq) issue(qstart, lds);
+  if (qstart < qend) issue(qstart, lds);
   // One step per 64 queries.  Masks are needed only where the tile crosses
   // this wave's causal diagonal (the first steps), the query end (the last
   // step) or the key end (every step); the steps are split into three loops
@@ -1033,34 +1076,39 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
     const int64_t qb0 = qstart + j * 64;
     __builtin_amdgcn_s_waitcnt(0xc07f & 0x3f70);  // vmcnt(0)
     __syncthreads();
-    if (qb0 + 64 < f.Sq) issue(qb0 + 64, lds + (buf ^ 1) * STAGE);
+    if (qb0 + 64 < qend) issue(qb0 + 64, lds + (buf ^ 1) * STAGE);
     const char* Qt = lds + buf * STAGE;
     const char* dOt = Qt + L::TILE;
     const float* lse_s = (const float*)(Qt + 2 * L::TILE);
     const float* del_s = lse_s + 64;
     buf ^= 1;
     if (f.causal && kw > qb0 + 63) return;  // every key of this wave is after every query
+    if (WIN && kw >= f.sinks && (extra || qb0 >= kw + KW - 1 + f.window)) return;  // past every key's window
       const int q_lim = (int)min((int64_t)64, f.Sq - qb0);   // query rows < q_lim exist
-      const int k_lim = (int)min((int64_t)32, f.Skv - kw);   // key rows < k_lim exist
-      const int kq = (int)max((int64_t)-128, min((int64_t)128, kw - qb0));  // key row 0 minus query row 0
+      const int k_lim = (int)min((int64_t)KW, f.Skv - kw);   // key rows < k_lim exist
+      const int kq = (int)max(WIN ? (int64_t)-(1 << 30) : (int64_t)-128, min((int64_t)128, kw - qb0));  // key row 0 minus query row 0
       const float c = f.scale_log2;
       // Masked steps keep query row qr of key row kr iff lo[t] <= qr <
       // q_lim (lo = the causal diagonal), tested as one unsigned compare
       // (qr - lo[t]) < span[t]; a dropped score's exponent is -inf, so the
       // exp2 runs unconditionally and gives 0 (no branch per element).
-      int lo[2], span[2];
+      int lo[RT], span[RT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < RT; ++t) {
         const int kr = t * 16 + lr;
         lo[t] = f.causal ? max(0, kq + kr) : 0;
-        span[t] = kr < k_lim ? max(0, q_lim - lo[t]) : 0;
+        int hi = q_lim;
+        if (WIN && kw + kr >= f.sinks) hi = (int)min((int64_t)hi, kq + kr + f.window);
+        span[t] = kr < k_lim ? max(0, hi - lo[t]) : 0;
       }
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         // on the causal diagonal, a pair of query tiles that lies wholly
         // before this wave's first key contributes nothing
         if (MASK && f.causal && qs * 32 + 31 < kq) continue;
-        f32x4 pt[2][2], ds[2][2];  // [query tile in pair][key tile]
+        if (WIN && MASK && kw >= f.sinks && qs * 32 >= kq + KW - 1 + f.window) continue;  // past every key's window
+        if (WIN && ((2 * (int)j + qs) & (parts - 1)) != part) continue;                // another wave's
+        f32x4 pt[2][RT], ds[2][RT];  // [query tile in pair][key tile]
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int qt = 2 * qs + u;
@@ -1075,7 +1123,7 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
           const float4 d4 = *(const float4*)(del_s + qt * 16 + 4 * lg);
           const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < RT; ++t) {
             // dP - D: the accumulator of dO V^T starts at -D
             f32x4 sa = {0.f, 0.f, 0.f, 0.f}, pa = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
@@ -1096,9 +1144,9 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
             }
           }
         }
-        frag pb[2], sb[2];
+        frag pb[RT], sb[RT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             pb[t][e] = (T)pt[0][t][e];
@@ -1111,19 +1159,23 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
           const frag dof = tr_frag_at<T, D>(dOt, tro, dt, 2 * qs, 2 * qs + 1);
           const frag qtf = tr_frag_at<T, D>(Qt, tro, dt, 2 * qs, 2 * qs + 1);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < RT; ++t) {
             dva[dt][t] = Mfma<T>::mma(dof, pb[t], dva[dt][t]);
             dka[dt][t] = Mfma<T>::mma(qtf, sb[t], dka[dt][t]);
           }
         }
       }
   };
-  const int64_t nqb = qstart < f.Sq ? (f.Sq - qstart + 63) / 64 : 0;
+  const int64_t nqb = qstart < qend ? (qend - qstart + 63) / 64 : 0;
   int64_t j1 = 0, j2 = nqb;  // masked [0, j1), unmasked [j1, j2), masked [j2, nqb)
-  if (kw + 32 > f.Skv) {
+  if (kw + KW > f.Skv || extra) {
     j1 = nqb;
+  } else if constexpr (WIN) {  // queries from the last key on, up to the end of the first key's window
+    j1 = min(nqb, max((int64_t)0, ceil_div64(kw + KW - 1 - qstart, 64)));
+    const int64_t inside = min(f.Sq, kw + f.window) - qstart;
+    j2 = max(j1, min(nqb, inside < 0 ? 0 : inside / 64));
   } else {
-    if (f.causal) j1 = min(nqb, max((int64_t)0, ceil_div64(kw + 31 - qstart, 64)));
+    if (f.causal) j1 = min(nqb, max((int64_t)0, ceil_div64(kw + KW - 1 - qstart, 64)));
     j2 = max(j1, min(nqb, (f.Sq - qstart) / 64));
   }
   int64_t j = 0;
@@ -1131,11 +1183,30 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
   for (; j < j2; ++j) step(j, BoolTag<false>{});
   for (; j < nqb; ++j) step(j, BoolTag<true>{});
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < RT; ++t) {
     const int64_t kj = kw + t * 16 + lr;
     if (kj >= f.Skv) continue;
-    T* dK = (T*)p.dk + b * p.dk_b + h * p.dk_h + kj * p.dk_s;
-    T* dV = (T*)p.dv + b * p.dv_b + h * p.dv_h + kj * p.dv_s;
+    if constexpr (WIN) {  // f32 partials: of sinks, and of a head of a group
+      float* pk = nullptr;
+      int64_t plane = 0;
+      if (extra || (!p.kv_part && kj < f.sinks)) {
+        if (kj >= f.sinks) continue;
+        pk = sink_slot(p, extra ? 1 + 4 * at.chunk + part : 0, b, h, kj, D), plane = sink_plane(p, D);
+      } else if (p.kv_part) {
+        const int64_t hkn = f.H / f.group, gi = h - hk * f.group;
+        pk = p.kv_part + (((gi * f.B + b) * hkn + hk) * f.Skv + kj) * D, plane = f.B * f.H * f.Skv * D;
+      }
+      if (pk) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          *(f32x4*)(pk + dt * 16 + lg * 4) = dka[dt][t];
+          *(f32x4*)(pk + plane + dt * 16 + lg * 4) = dva[dt][t];
+        }
+        continue;
+      }
+    }
+    T* dK = (T*)p.dk + b * p.dk_b + hk * p.dk_h + kj * p.dk_s;
+    T* dV = (T*)p.dv + b * p.dv_b + hk * p.dv_h + kj * p.dv_s;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       V4<T> k4, v4;
@@ -1150,31 +1221,30 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, GridPos gp, char*
   }
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* lds) {
+template <typename T, int D, bool WIN = false, int RT = 2>
+__device__ __forceinline__ void dq_body(const AttnBwdArgs& p, BlockCoord bc, int64_t qblock, char* lds) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
   constexpr int KS = D / 32, DT = D / 16;
   constexpr int STAGE = 2 * L::TILE;  // K tile, V tile
+  constexpr int QW = 16 * RT;  // queries of a wave
 
   const AttnArgs& f = p.f;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int lr = lane & 15, lg = lane >> 4;
-  const BlockCoord bc = block_coord(gp);
-  const int64_t qblock = f.causal ? (int64_t)gp.nx - 1 - bc.x : bc.x;
-  const int64_t q0 = qblock * 128;
-  const int64_t b = bc.b, h = bc.h;
+  const int64_t q0 = qblock * (4 * QW);
+  const int64_t b = bc.b, h = bc.h, hk = WIN ? h / f.group : h;
   const T* Q = (const T*)f.q + b * f.q_b + h * f.q_h;
-  const char* K = (const char*)((const T*)f.k + b * f.k_b + h * f.k_h);
-  const char* V = (const char*)((const T*)f.v + b * f.v_b + h * f.v_h);
+  const char* K = (const char*)((const T*)f.k + b * f.k_b + hk * f.k_h);
+  const char* V = (const char*)((const T*)f.v + b * f.v_b + hk * f.v_h);
   const T* dO = (const T*)p.dout + b * p.do_b + h * p.do_h;
   const int64_t ks_b = f.k_s * (int64_t)sizeof(T), vs_b = f.v_s * (int64_t)sizeof(T);
 
-  const int64_t qw = q0 + wave * 32;
-  frag qf[2][KS], df[2][KS];
-  float lse2[2], dlt[2];
+  const int64_t qw = q0 + wave * QW;
+  frag qf[RT][KS], df[RT][KS];
+  float lse2[RT], dlt[RT];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < RT; ++u) {
     const int64_t qi = qw + u * 16 + lr;
     const bool ok = qi < f.Sq;
 #pragma unroll
@@ -1185,20 +1255,28 @@ __device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* 
     lse2[u] = ok ? p.nlse2[(b * f.H + h) * f.Sq + qi] : 0.f;  // -LSE * log2(e)
     dlt[u] = ok ? p.ndelta[(b * f.H + h) * f.Sq + qi] : 0.f;  // -D, the start of dP - D
   }
-  f32x4 dqa[DT][2];
+  f32x4 dqa[DT][RT];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) dqa[dt][0] = dqa[dt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int u = 0; u < RT; ++u) dqa[dt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   int64_t kv_end = f.Skv;
-  if (f.causal) kv_end = min(f.Skv, q0 + 128);
+  if (f.causal) kv_end = min(f.Skv, q0 + 4 * QW);
   const int sw = L::swz(lr);
   const TrOffsets<D> tro;
   int buf = 0;
   KvTileLoad<D, 4> kl, vl;
   kl.init(K, ks_b);
   vl.init(V, vs_b);
-  kl.issue(0, f.Skv, lds);
-  vl.issue(0, f.Skv, lds + L::TILE);
+  // WIN: the tiles of sinks before the window's first tile jw, then the window's
+  const int64_t jw = WIN ? max((int64_t)0, q0 - f.window + 1) / 64 : 0;
+  const int64_t ns = WIN ? min(ceil_div64(min(f.sinks, f.Skv), 64), jw) : 0;
+  const int64_t jfirst = ns > 0 ? 0 : jw;
+  if (!WIN || jfirst * 64 < kv_end) {
+    kl.issue(jfirst * 64, f.Skv, lds);
+    vl.issue(jfirst * 64, f.Skv, lds + L::TILE);
+  }
   // One step per 64 keys: unmasked steps first, then the ones that cross
   // this wave's causal diagonal or the key end (or all of them when the
   // wave's queries cross the query end); same step count on every wave.
@@ -1207,34 +1285,40 @@ __device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* 
     const int64_t kb0 = j * 64;
     __builtin_amdgcn_s_waitcnt(0xc07f & 0x3f70);  // vmcnt(0)
     __syncthreads();
-    if (kb0 + 64 < kv_end) {
+    const int64_t kn = WIN && j + 1 == ns ? jw * 64 : kb0 + 64;
+    if (kn < kv_end) {
       char* nx = lds + (buf ^ 1) * STAGE;
-      kl.issue(kb0 + 64, f.Skv, nx);
-      vl.issue(kb0 + 64, f.Skv, nx + L::TILE);
+      kl.issue(kn, f.Skv, nx);
+      vl.issue(kn, f.Skv, nx + L::TILE);
     }
     const char* Kt = lds + buf * STAGE;
     const char* Vt = Kt + L::TILE;
     buf ^= 1;
-    if (f.causal && kb0 > qw + 31) return;  // every key after every query of this wave
-      const int q_lim = (int)min((int64_t)32, f.Sq - qw);    // query rows < q_lim exist
+    if (f.causal && kb0 > qw + QW - 1) return;  // every key after every query of this wave
+    if (WIN && kb0 >= f.sinks && kb0 + 63 < qw - f.window + 1) return;  // before every query's window
+      const int q_lim = (int)min((int64_t)QW, f.Sq - qw);    // query rows < q_lim exist
       const int k_lim = (int)min((int64_t)64, f.Skv - kb0);  // key rows < k_lim exist
-      const int qk = (int)max((int64_t)-128, min((int64_t)128, qw - kb0));  // query row 0 minus key row 0
+      const int qk = (int)max((int64_t)-128, min(WIN ? (int64_t)(1 << 30) : (int64_t)128, qw - kb0));  // query row 0 minus key row 0
       const float c = f.scale_log2;
       // Masked steps keep key row kr of query row qr iff kr < lim[u]
       // (the key end, the causal diagonal, nothing past the query end); a
       // dropped score's exponent is -inf (no branch per element).
-      int lim[2];
+      // WIN: of them, those from lo[u] on or below ls, the sinks.
+      int lim[RT], lo[RT] = {};
+      const int ls = WIN ? (int)max((int64_t)0, min((int64_t)64, f.sinks - kb0)) : 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < RT; ++u) {
         const int qr = u * 16 + lr;
         lim[u] = qr < q_lim ? (f.causal ? min(k_lim, qk + qr + 1) : k_lim) : 0;
+        if (WIN) lo[u] = (int)max((int64_t)0, min((int64_t)64, qk + qr - f.window + 1));
       }
 #pragma unroll
       for (int ks2 = 0; ks2 < 2; ++ks2) {
         // on the causal diagonal, a pair of key tiles that lies wholly after
         // this wave's last query contributes nothing
-        if (MASK && f.causal && ks2 * 32 > qk + 31) continue;
-        f32x4 ds[2][2];  // [key tile in pair][query tile]
+        if (MASK && f.causal && ks2 * 32 > qk + QW - 1) continue;
+        if (WIN && MASK && ks2 * 32 >= ls && ks2 * 32 + 31 < qk - f.window + 1) continue;  // before every query's window
+        f32x4 ds[2][RT];  // [key tile in pair][query tile]
 #pragma unroll
         for (int v2 = 0; v2 < 2; ++v2) {
           const int kt = 2 * ks2 + v2;
@@ -1246,7 +1330,7 @@ __device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* 
             va[ks] = *(const frag*)(Vt + off);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < RT; ++u) {
             f32x4 sa = {0.f, 0.f, 0.f, 0.f}, pa = {dlt[u], dlt[u], dlt[u], dlt[u]};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -1256,14 +1340,17 @@ __device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float x = fmaf(sa[e], c, lse2[u]);
-              if constexpr (MASK) x = kt * 16 + 4 * lg + e < lim[u] ? x : -INFINITY;
+              if constexpr (MASK) {
+                const int key = kt * 16 + 4 * lg + e;
+                x = key < lim[u] && (!WIN || key >= lo[u] || key < ls) ? x : -INFINITY;
+              }
               ds[v2][u][e] = fast_exp2(x) * pa[e];
             }
           }
         }
-        frag sb[2];
+        frag sb[RT];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < RT; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             sb[u][e] = (T)ds[0][u][e];
@@ -1273,21 +1360,26 @@ __device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* 
         for (int dt = 0; dt < DT; ++dt) {
           const frag ktf = tr_frag_at<T, D>(Kt, tro, dt, 2 * ks2, 2 * ks2 + 1);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) dqa[dt][u] = Mfma<T>::mma(ktf, sb[u], dqa[dt][u]);
+          for (int u = 0; u < RT; ++u) dqa[dt][u] = Mfma<T>::mma(ktf, sb[u], dqa[dt][u]);
         }
       }
   };
   const int64_t nkb = (kv_end + 63) / 64;
   int64_t ju = 0;  // unmasked [0, ju), masked [ju, nkb)
-  if (qw + 32 <= f.Sq) {
+  if (qw + QW <= f.Sq) {
     ju = min(nkb, f.Skv / 64);
     if (f.causal) ju = min(ju, qw < 63 ? (int64_t)0 : (qw - 63) / 64 + 1);
   }
   int64_t j = 0;
+  if constexpr (WIN) {  // masked: the sinks, and the window's lower edge
+    for (; j < ns; ++j) step(j, BoolTag<true>{});
+    const int64_t jl = min(nkb, max(jw, ceil_div64(qw + QW - f.window, 64)));
+    for (j = jw; j < jl; ++j) step(j, BoolTag<true>{});
+  }
   for (; j < ju; ++j) step(j, BoolTag<false>{});
   for (; j < nkb; ++j) step(j, BoolTag<true>{});
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < RT; ++u) {
     const int64_t qi = qw + u * 16 + lr;
     if (qi >= f.Sq) continue;
     T* dQ = (T*)p.dq + b * p.dq_b + h * p.dq_h + qi * p.dq_s;
@@ -1304,13 +1396,14 @@ __device__ __forceinline__ void dq_body(const AttnBwdArgs& p, GridPos gp, char* 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_bwd_dkv_v2(AttnBwdArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[kDkvLds<D>];
-  dkv_body<T, D>(p, hw_grid(), lds);
+  dkv_body<T, D>(p, WindowPos{block_coord(), -1}, lds);
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_bwd_dq_v2(AttnBwdArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[kDqLds<D>];
-  dq_body<T, D>(p, hw_grid(), lds);
+  const BlockCoord bc = block_coord();
+  dq_body<T, D>(p, bc, p.f.causal ? (int64_t)gridDim.x - 1 - bc.x : bc.x, lds);
 }
 
 // dK/dV and dQ blocks from one launch over a 1-D grid of 2 x (tiles x H x B)
@@ -1340,8 +1433,89 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_b
   const uint32_t kind = hi ? (i >> KB) & 1 : i & 1;
   const uint32_t w = hi ? ((i >> (KB + 1)) << KB) | (i & ((1u << KB) - 1)) : i >> 1;
   const uint32_t v = w * 8 + (l & 7);
-  if (kind) dq_body<T, D>(p, GridPos{nqx, (uint32_t)p.f.H, (uint32_t)p.f.B, v}, lds);
-  else dkv_body<T, D>(p, GridPos{nkx, (uint32_t)p.f.H, (uint32_t)p.f.B, v}, lds);
+  const BlockCoord bc = block_coord(GridPos{kind ? nqx : nkx, (uint32_t)p.f.H, (uint32_t)p.f.B, v});
+  if (kind) dq_body<T, D>(p, bc, p.f.causal ? (int64_t)nqx - 1 - bc.x : bc.x, lds);
+  else dkv_body<T, D>(p, WindowPos{bc, -1}, lds);
+}
+
+// The windowed backward in one launch: dK/dV blocks, the blocks that share the
+// queries behind the sinks' windows, dQ blocks.  All but the second kind walk
+// a window, so they are nearly alike and the kinds fill each other's last
+// rounds.  Blocks of one head stand side by side on an XCD (they read the same
+// rows): the hardware deals blocks to the 8 in turn, and each takes a
+// contiguous run of a kind.
+// 16-row tiles of a wave: two, or one of keys at head_dim 256, where the dK and
+// dV of two would take all of its registers.
+template <int D>
+constexpr int kKeyTiles = D == 256 ? 1 : 2;
+constexpr int kQueryTiles = 2;
+template <int D>
+constexpr int kWindowLds = kDkvLds<D> > kDqLds<D> ? kDkvLds<D> : kDqLds<D>;
+__device__ __forceinline__ BlockCoord run_of(uint32_t l, uint32_t total, uint32_t nx, uint32_t heads) {
+  const uint32_t xcd = l & 7, q = total >> 3, r = total & 7, i = xcd * q + min(xcd, r) + (l >> 3);
+  const uint32_t bh = i / nx;
+  return BlockCoord{i - bh * nx, bh % heads, bh / heads};
+}
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_bwd_window(AttnBwdArgs p, uint32_t nkx, uint32_t nqx) {
+  char* const lds = attn_dyn_lds;
+  const uint32_t heads = (uint32_t)p.f.H, bh = heads * (uint32_t)p.f.B;
+  const uint32_t ndkv = nkx * bh, chunks = (uint32_t)(p.sink_blocks * p.sink_chunks), nextra = chunks * bh;
+  uint32_t l = blockIdx.x;
+  if (l < ndkv) return dkv_body<T, D, true, kKeyTiles<D>>(p, WindowPos{run_of(l, ndkv, nkx, heads), -1}, lds);
+  l -= ndkv;
+  if (l < nextra) {
+    BlockCoord bc = run_of(l, nextra, chunks, heads);
+    const int chunk = (int)bc.x / p.sink_blocks;
+    bc.x -= (int64_t)chunk * p.sink_blocks;
+    return dkv_body<T, D, true, kKeyTiles<D>>(p, WindowPos{bc, chunk}, lds);
+  }
+  l -= nextra;
+  const BlockCoord bc = run_of(l, nqx * bh, nqx, heads);
+  dq_body<T, D, true, kQueryTiles>(p, bc, bc.x, lds);
+}
+
+// dK = scale * the sum of its f32 partials, dV likewise, four head-dim elements
+// per thread: of every key over its group's query heads, in head order
+// (kv_part), of a sink besides over the slots of the blocks that shared its
+// queries (without grouped heads sinks are all there is to do).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attn_bwd_window_sum(AttnBwdArgs p) {
+  const AttnArgs& f = p.f;
+  const int64_t hkn = f.H / f.group, plane = f.B * f.H * f.Skv * D;
+  const int64_t sinks = min(f.Skv, f.sinks), keys = p.kv_part ? f.Skv : sinks;
+  const int64_t i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i4 >= f.B * hkn * keys * (D / 4)) return;
+  const int64_t row = i4 / (D / 4), d = (i4 - row * (D / 4)) * 4;
+  const int64_t key = row % keys, bhk = row / keys, hk = bhk % hkn, b = bhk / hkn;
+  f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
+  const int64_t splane = sink_plane(p, D);
+  // of a chunk's four slots, those that waves of the sink's block wrote
+  constexpr int KW = 16 * kKeyTiles<D>;
+  const int64_t waves = min((int64_t)4, (sinks - key / (4 * KW) * (4 * KW) + KW - 1) / KW);
+  const int parts = waves == 1 ? 4 : waves == 2 ? 2 : 1;
+  for (int64_t g = 0; g < f.group; ++g) {
+    const int64_t h = hk * f.group + g;
+    if (p.kv_part) {
+      const float* pk = p.kv_part + (((g * f.B + b) * hkn + hk) * f.Skv + key) * D + d;
+      sk += *(const f32x4*)pk, sv += *(const f32x4*)(pk + plane);
+    }
+    if (key >= sinks) continue;
+    if (!p.kv_part) {
+      const float* pk = sink_slot(p, 0, b, h, key, D) + d;
+      sk += *(const f32x4*)pk, sv += *(const f32x4*)(pk + splane);
+    }
+    for (int c = 0; c < p.sink_chunks; ++c)
+      for (int i = 0; i < parts; ++i) {
+        const float* pk = sink_slot(p, 1 + 4 * c + i, b, h, key, D) + d;
+        sk += *(const f32x4*)pk, sv += *(const f32x4*)(pk + splane);
+      }
+  }
+  V4<T> k4, v4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) k4.v[e] = (T)(sk[e] * f.scale), v4.v[e] = (T)sv[e];
+  *(V4<T>*)((T*)p.dk + b * p.dk_b + hk * p.dk_h + key * p.dk_s + d) = k4;
+  *(V4<T>*)((T*)p.dv + b * p.dv_b + hk * p.dv_h + key * p.dv_s + d) = v4;
 }
 
 // ---------------------------------------------------------------------------
@@ -1366,14 +1540,7 @@ constexpr int kGqaDkvLds = 2 * (2 * KvLayout<D>::TILE + 512);  // 2 stages of Q,
 template <int D>
 constexpr int kGqaDqLds = 2 * (2 * KvLayout<D>::TILE);  // 2 stages of K, V
 
-// SINK: sinks are seen by every later query, so a block of keys that holds
-// some would walk the whole sequence while the others walk a window.  The
-// steps behind its window go to sink_chunks further blocks (first in the
-// grid), and all of a sink block's results leave as f32 partials
-// [dK, dV][slot][b][h][sink key][D] that attn_bwd_gqa_sum adds in slot order:
-// slot 0 is the block's own window (with grouped heads that is in kv_part),
-// slot 1 + c chunk c.
-template <typename T, int D, bool SINK = false>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
@@ -1383,9 +1550,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
   const AttnArgs& f = p.f;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int lr = lane & 15, lg = lane >> 4;
-  const int nextra = SINK ? p.sink_blocks * p.sink_chunks : 0;
-  const bool extra = SINK && (int)blockIdx.x < nextra;
-  const int64_t k0 = (extra ? (int64_t)blockIdx.x % p.sink_blocks : (int64_t)blockIdx.x - nextra) * 64;
+  const int64_t k0 = (int64_t)blockIdx.x * 64;
   // with partials, block (x, hk * group + gi) takes query head gi of the
   // group alone; without, it walks the whole group
   const int64_t hsplit = p.kv_part ? f.group : 1;
@@ -1406,15 +1571,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
   // queries that can see keys k0 .. k0 + 63, in 64-query steps from qstart
   int64_t qhi = f.Sq;
   if (f.window > 0) qhi = min(qhi, k0 + 63 + f.window);
-  int64_t qstart = f.causal ? (k0 / 64) * 64 : 0;
-  int64_t nqb = qhi > qstart ? (qhi - qstart + 63) / 64 : 0;
-  if (extra) {  // this chunk's share of the steps behind the window
-    qstart += nqb * 64;
-    const int64_t rest = ceil_div64(f.Sq - qstart, 64), per = ceil_div64(rest, p.sink_chunks);
-    const int64_t first = (int64_t)blockIdx.x / p.sink_blocks * per;
-    qstart += first * 64;
-    nqb = max((int64_t)0, min(per, rest - first));
-  }
+  const int64_t qstart = f.causal ? (k0 / 64) * 64 : 0;
+  const int64_t nqb = qhi > qstart ? (qhi - qstart + 63) / 64 : 0;
   const int64_t nheads = p.kv_part ? 1 : f.group;
   const int64_t total = nqb * nheads;  // steps over (query head, query block)
   const int64_t qs_b = f.q_s * (int64_t)sizeof(T), dos_b = p.do_s * (int64_t)sizeof(T);
@@ -1448,14 +1606,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
     if constexpr (MASK) {
       const int64_t lo64 = f.causal ? max((int64_t)0, kq + lr) : 0;
       int64_t hi = min((int64_t)64, f.Sq - qb0);
-      if (f.window > 0 && !(SINK && kj < f.sinks)) hi = min(hi, kq + lr + f.window);
+      if (f.window > 0) hi = min(hi, kq + lr + f.window);
       lo = (int)min((int64_t)64, lo64);
       span = kj < f.Skv ? (int)max((int64_t)0, hi - lo64) : 0;
     }
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
       if (MASK && f.causal && qs * 32 + 31 < kq) continue;                // every query before every key
-      if (MASK && f.window > 0 && qs * 32 >= kq + 15 + f.window && !(SINK && kw < f.sinks)) continue;  // past every key's window
+      if (MASK && f.window > 0 && qs * 32 >= kq + 15 + f.window) continue;  // past every key's window
       f32x4 pt[2], ds[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -1504,23 +1662,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
     buf ^= 1;
     const int64_t qb0 = qstart + (st % nqb) * 64;
     if (f.causal && kw > qb0 + 63) continue;                     // every query before every key
-    if (f.window > 0 && qb0 >= kw + 15 + f.window && !(SINK && kw < f.sinks)) continue;  // past every key's window
+    if (f.window > 0 && qb0 >= kw + 15 + f.window) continue;     // past every key's window
     const bool inside = (!f.causal || qb0 >= kw + 15) && (f.window <= 0 || qb0 + 63 < kw + f.window) &&
                         qb0 + 64 <= f.Sq && kw + 16 <= f.Skv;
     if (inside) compute(Qt, qb0, BoolTag<false>{});
     else compute(Qt, qb0, BoolTag<true>{});
   }
-  if (SINK && kj < f.Skv && (extra || (!p.kv_part && k0 / 64 < p.sink_blocks))) {
-    const int64_t slots = p.sink_chunks + 1, keys = (int64_t)p.sink_blocks * 64;
-    const int64_t slot = extra ? 1 + (int64_t)blockIdx.x / p.sink_blocks : 0;
-    float* pk = p.sink_part + (((slot * f.B + b) * f.H + hk * f.group + gfirst) * keys + kj) * D;
-    const int64_t plane = slots * f.B * f.H * keys * D;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      *(float4*)(pk + dt * 16 + lg * 4) = float4{dka[dt][0], dka[dt][1], dka[dt][2], dka[dt][3]};
-      *(float4*)(pk + plane + dt * 16 + lg * 4) = float4{dva[dt][0], dva[dt][1], dva[dt][2], dva[dt][3]};
-    }
-  } else if (kj < f.Skv && p.kv_part) {
+  if (kj < f.Skv && p.kv_part) {
     // f32 partials [gi][b][hk][key][D], dK's then dV's; summed by attn_bwd_gqa_sum
     const int64_t hkn = f.H / f.group, plane = f.group * f.B * hkn * f.Skv * D;
     float* pk = p.kv_part + (((gfirst * f.B + b) * hkn + hk) * f.Skv + kj) * D;
@@ -1548,32 +1696,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dkv(AttnBwdArgs p) {
 
 // dK = scale * sum over the group's query heads of the dK partials, dV = the
 // sum of the dV partials, in head order (deterministic); four head-dim
-// elements per thread.  SINK: a sink block's rows add their slots' partials,
-// head by head; without grouped heads those rows are all there is to do.
-template <typename T, int D, bool SINK = false>
+// elements per thread.
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) attn_bwd_gqa_sum(AttnBwdArgs p) {
   const AttnArgs& f = p.f;
   const int64_t hkn = f.H / f.group, rows = f.B * hkn * f.Skv, plane = f.group * rows * D;
-  const int64_t sinks = SINK ? min(f.Skv, (int64_t)p.sink_blocks * 64) : 0;  // keys with slots
-  const int64_t keys = SINK && !p.kv_part ? sinks : f.Skv;                  // keys summed here
-  const int64_t i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;          // over B * hkn * keys * D / 4
-  if (i4 >= f.B * hkn * keys * (D / 4)) return;
-  const int64_t krow = i4 / (D / 4), d = (i4 - krow * (D / 4)) * 4;
-  const int64_t key = krow % keys, bh = krow / keys, hk = bh % hkn, b = bh / hkn;
-  const int64_t row = bh * f.Skv + key;
+  const int64_t i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;  // over rows * D / 4
+  if (i4 >= rows * (D / 4)) return;
+  const int64_t row = i4 / (D / 4), d = (i4 - row * (D / 4)) * 4;
+  const int64_t key = row % f.Skv, bh = row / f.Skv, hk = bh % hkn, b = bh / hkn;
   float4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
-  auto add = [&](const float* pk, int64_t to_v) {
-    const float4 a = *(const float4*)pk, c = *(const float4*)(pk + to_v);
+  for (int64_t g = 0; g < f.group; ++g) {
+    const float4 a = *(const float4*)(p.kv_part + g * rows * D + row * D + d);
+    const float4 c = *(const float4*)(p.kv_part + plane + g * rows * D + row * D + d);
     sk.x += a.x, sk.y += a.y, sk.z += a.z, sk.w += a.w;
     sv.x += c.x, sv.y += c.y, sv.z += c.z, sv.w += c.w;
-  };
-  for (int64_t g = 0; g < f.group; ++g) {
-    if (!SINK || p.kv_part) add(p.kv_part + g * rows * D + row * D + d, plane);
-    if (SINK && key < sinks) {
-      const int64_t padded = (int64_t)p.sink_blocks * 64, step = f.B * f.H * padded * D;
-      const float* pk = p.sink_part + ((b * f.H + hk * f.group + g) * padded + key) * D + d;
-      for (int c = p.kv_part ? 1 : 0; c <= p.sink_chunks; ++c) add(pk + c * step, (p.sink_chunks + 1) * step);
-    }
   }
   V4<T> k4, v4;
   k4.v[0] = (T)(sk.x * f.scale), k4.v[1] = (T)(sk.y * f.scale), k4.v[2] = (T)(sk.z * f.scale), k4.v[3] = (T)(sk.w * f.scale);
@@ -1582,7 +1719,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_gqa_sum(AttnBwdArgs p) {
   *(V4<T>*)((T*)p.dv + b * p.dv_b + hk * p.dv_h + key * p.dv_s + d) = v4;
 }
 
-template <typename T, int D, bool SINK = false>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
@@ -1616,10 +1753,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
   if (f.causal) khi = min(khi, q0 + 64);
   const int64_t klo = f.window > 0 ? max((int64_t)0, q0 - f.window + 1) : 0;
   const int64_t kstart = (klo / 64) * 64;
-  // tiles of sinks before the window's come first
-  const int64_t ns = SINK ? min(ceil_div64(min(f.sinks, f.Skv), 64), kstart / 64) : 0;
-  const int64_t nkb = ns + (khi > kstart ? (khi - kstart + 63) / 64 : 0);
-  auto tile_key = [&](int64_t j) { return SINK && j < ns ? j * 64 : kstart + (j - ns) * 64; };
+  const int64_t nkb = khi > kstart ? (khi - kstart + 63) / 64 : 0;
   KvTileLoad<D, 4> kl, vl;
   kl.init((const char*)((const T*)f.k + b * f.k_b + hk * f.k_h), f.k_s * (int64_t)sizeof(T));
   vl.init((const char*)((const T*)f.v + b * f.v_b + hk * f.v_h), f.v_s * (int64_t)sizeof(T));
@@ -1630,22 +1764,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
     constexpr bool MASK = decltype(mask_tag)::value;
     const char* Vt = Kt + L::TILE;
     const int64_t qk = qw - kb0;  // query row 0 minus key row 0
-    // key rows lo <= kr < lo + span are visible to this lane's query, and
-    // those of sinks, kr < ls
-    int lo = 0, span = 64, ls = 0;
+    // key rows lo <= kr < lo + span are visible to this lane's query
+    int lo = 0, span = 64;
     if constexpr (MASK) {
       const int64_t lo64 = f.window > 0 ? max((int64_t)0, qk + lr - f.window + 1) : 0;
       int64_t hi = min((int64_t)64, f.Skv - kb0);
       if (f.causal) hi = min(hi, qk + lr + 1);
       lo = (int)min((int64_t)64, lo64);
       span = qok ? (int)max((int64_t)0, hi - lo64) : 0;
-      if (SINK && qok) ls = (int)max((int64_t)0, min(hi, f.sinks - kb0));
     }
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
       if (MASK && f.causal && ks2 * 32 > qk + 15) continue;                      // after every query
-      if (MASK && f.window > 0 && ks2 * 32 + 31 < qk - f.window + 1 && !(SINK && kb0 + ks2 * 32 < f.sinks))
-        continue;  // before every window
+      if (MASK && f.window > 0 && ks2 * 32 + 31 < qk - f.window + 1) continue;  // before every window
       f32x4 ds[2];
 #pragma unroll
       for (int v2 = 0; v2 < 2; ++v2) {
@@ -1660,10 +1791,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = fmaf(sa[e], c, nl2);
-          if constexpr (MASK) {
-            const int key = kt * 16 + 4 * lg + e;
-            x = (unsigned)(key - lo) < (unsigned)span || (SINK && key < ls) ? x : -INFINITY;
-          }
+          if constexpr (MASK) x = (unsigned)(kt * 16 + 4 * lg + e - lo) < (unsigned)span ? x : -INFINITY;
           ds[v2][e] = fast_exp2(x) * pa[e];
         }
       }
@@ -1680,22 +1808,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_gqa_dq(AttnBwdArgs p) {
   };
   int buf = 0;
   if (nkb > 0) {
-    kl.issue(tile_key(0), f.Skv, lds);
-    vl.issue(tile_key(0), f.Skv, lds + L::TILE);
+    kl.issue(kstart, f.Skv, lds);
+    vl.issue(kstart, f.Skv, lds + L::TILE);
   }
   for (int64_t j = 0; j < nkb; ++j) {
-    const int64_t kb0 = tile_key(j);
+    const int64_t kb0 = kstart + j * 64;
     __builtin_amdgcn_s_waitcnt(0xc07f & 0x3f70);  // vmcnt(0)
     __syncthreads();
     if (j + 1 < nkb) {
       char* nx = lds + (buf ^ 1) * STAGE;
-      kl.issue(tile_key(j + 1), f.Skv, nx);
-      vl.issue(tile_key(j + 1), f.Skv, nx + L::TILE);
+      kl.issue(kb0 + 64, f.Skv, nx);
+      vl.issue(kb0 + 64, f.Skv, nx + L::TILE);
     }
     const char* Kt = lds + buf * STAGE;
     buf ^= 1;
     if (f.causal && kb0 > qw + 15) continue;                           // every key after every query
-    if (f.window > 0 && kb0 + 63 < qw - f.window + 1 && !(SINK && kb0 < f.sinks)) continue;  // before every query's window
+    if (f.window > 0 && kb0 + 63 < qw - f.window + 1) continue;        // before every query's window
     const bool inside = (!f.causal || kb0 + 63 <= qw) && (f.window <= 0 || kb0 > qw + 15 - f.window) &&
                         kb0 + 64 <= f.Skv && qw + 16 <= f.Sq;
     if (inside) compute(Kt, kb0, BoolTag<false>{});
@@ -1806,23 +1934,13 @@ int bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
     return FN<f16, 128>(__VA_ARGS__);                                         \
   } while (0)
 
-// Blocks that share the steps behind a sink block's window: as many steps
-// each as a block of the window has, and eight at least.
-int sink_chunks(int64_t sq, int64_t window) {
-  const int64_t own = (window + 126) / 64, rest = (sq + 63) / 64 - own;
-  if (rest <= 0) return 0;
-  const int64_t n = (rest + std::max<int64_t>(own, 8) - 1) / std::max<int64_t>(own, 8);
-  return (int)std::min<int64_t>(n, 256);
-}
-int sink_blocks(int64_t skv, int64_t sinks) { return (int)((std::min(skv, sinks) + 63) / 64); }
-
-template <typename T, int D, bool SINK = false>
+template <typename T, int D>
 int gqa_bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
   const int64_t rows = a.f.B * a.f.H * a.f.Sq;
   MI_REQUIRE(rows < (1ll << 31), "mi355x_attn_bwd: batch x heads x query rows must be below 2^31");
   attn_bwd_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
-  auto kkv = attn_bwd_gqa_dkv<T, D, SINK>;
-  auto kq = attn_bwd_gqa_dq<T, D, SINK>;
+  auto kkv = attn_bwd_gqa_dkv<T, D>;
+  auto kq = attn_bwd_gqa_dq<T, D>;
   constexpr int lkv = kGqaDkvLds<D>, lq = kGqaDqLds<D>;
   static std::once_flag once;
   static hipError_t attr_err = hipSuccess;
@@ -1835,15 +1953,84 @@ int gqa_bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
     return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_gen: cannot raise the LDS limit: %s", hipGetErrorString(attr_err));
   // grouped heads: one dK/dV block per (key block, query head), partials summed after
   const unsigned gy = (unsigned)(a.kv_part ? a.f.H : a.f.H / a.f.group);
-  const unsigned extra = SINK ? (unsigned)(a.sink_blocks * a.sink_chunks) : 0;
-  kkv<<<dim3(ceil_div(a.f.Skv, 64) + extra, gy, (unsigned)a.f.B), kThreads, lkv, s>>>(a);
+  kkv<<<dim3(ceil_div(a.f.Skv, 64), gy, (unsigned)a.f.B), kThreads, lkv, s>>>(a);
   kq<<<dim3(ceil_div(a.f.Sq, 64), (unsigned)a.f.H, (unsigned)a.f.B), kThreads, lq, s>>>(a);
-  if (a.kv_part || SINK) {
-    const int64_t keys = a.kv_part ? a.f.Skv : std::min<int64_t>(a.f.Skv, (int64_t)a.sink_blocks * 64);
-    const int64_t n4 = a.f.B * (a.f.H / a.f.group) * keys * (D / 4);
-    attn_bwd_gqa_sum<T, D, SINK><<<ceil_div(n4, kThreads), kThreads, 0, s>>>(a);
+  if (a.kv_part) {
+    const int64_t n4 = a.f.B * (a.f.H / a.f.group) * a.f.Skv * (D / 4);
+    attn_bwd_gqa_sum<T, D><<<ceil_div(n4, kThreads), kThreads, 0, s>>>(a);
   }
   return check_launch("mi355x_attn_bwd_gen");
+}
+
+// Blocks that share the steps behind the window of a block of sinks: eight
+// steps each, which their four waves share where there are few sinks, so that
+// one is shorter than a block of a window of 512 and more.
+int sink_chunks(int64_t sq, int64_t window, int64_t sinks) {
+  const int64_t rest = (sq + 63) / 64 - window / 64;
+  return sinks <= 0 || rest <= 0 ? 0 : (int)std::min<int64_t>((rest + 7) / 8, 1024);
+}
+int64_t sink_keys(int64_t skv, int64_t sinks) { return std::min(skv, sinks); }
+
+template <typename T, int D>
+int window_bwd_launch(AttnBwdArgs a, hipStream_t s) {
+  const int64_t rows = a.f.B * a.f.H * a.f.Sq;
+  MI_REQUIRE(rows < (1ll << 31), "mi355x_attn_bwd_sink: batch x heads x query rows must be below 2^31");
+  attn_bwd_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
+  auto k = attn_bwd_window<T, D>;
+  static std::once_flag once;
+  static hipError_t attr_err = hipSuccess;
+  std::call_once(once, [&] {
+    attr_err = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kWindowLds<D>);
+  });
+  if (attr_err != hipSuccess)
+    return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_sink: cannot raise the LDS limit: %s", hipGetErrorString(attr_err));
+  constexpr int KB = 64 * kKeyTiles<D>, QB = 64 * kQueryTiles;
+  a.sink_blocks = (a.sink_keys + KB - 1) / KB;
+  const int64_t nkx = (a.f.Skv + KB - 1) / KB, nqx = (a.f.Sq + QB - 1) / QB, bh = a.f.H * a.f.B;
+  const int64_t blocks = bh * (nkx + nqx + (int64_t)a.sink_blocks * a.sink_chunks);
+  MI_REQUIRE(blocks < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)blocks);
+  k<<<(unsigned)blocks, kThreads, kWindowLds<D>, s>>>(a, (uint32_t)nkx, (uint32_t)nqx);
+  if (a.kv_part || a.sink_keys) {
+    const int64_t n4 = a.f.B * (a.f.H / a.f.group) * (a.kv_part ? a.f.Skv : a.sink_keys) * (D / 4);
+    attn_bwd_window_sum<T, D><<<ceil_div(n4, kThreads), kThreads, 0, s>>>(a);
+  }
+  return check_launch("mi355x_attn_bwd_sink");
+}
+
+bool bwd_operands_ok(const void* dq, const int64_t* dq_bhs, const void* dk, const int64_t* dk_bhs, const void* dv,
+                     const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
+                     const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
+                     const void* o, const int64_t* o_bhs) {
+  if (!(strides_ok(q, q_bhs) && strides_ok(k, k_bhs) && strides_ok(v, v_bhs) && strides_ok(dout, do_bhs) &&
+        strides_ok(o, o_bhs)))
+    return false;
+  for (const int64_t* st : {dq_bhs, dk_bhs, dv_bhs})
+    if (st[0] % 4 || st[1] % 4 || st[2] % 4) return false;
+  return ((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 8 == 0;
+}
+
+// The kernels' arguments; the workspace holds 2 floats per query row and, with
+// grouped heads, the per-query-head dK/dV partials, 256-byte aligned.
+AttnBwdArgs bwd_args(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv, const int64_t* dv_bhs,
+                     const void* dout, const int64_t* do_bhs, const void* q, const int64_t* q_bhs, const void* k,
+                     const int64_t* k_bhs, const void* v, const int64_t* v_bhs, const void* o, const int64_t* o_bhs,
+                     const float* lse, int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                     double scale, int causal, int64_t window, int64_t sinks, void* workspace) {
+  AttnBwdArgs a{};
+  a.f = AttnArgs{(void*)o, o_bhs[0], o_bhs[1], o_bhs[2], (float*)lse, q, q_bhs[0], q_bhs[1], q_bhs[2],
+                 k, k_bhs[0], k_bhs[1], k_bhs[2], v, v_bhs[0], v_bhs[1], v_bhs[2],
+                 batch, heads, sq, skv, (float)(scale * 1.4426950408889634), (float)scale, causal,
+                 heads / kv_heads, window, sinks};
+  a.dout = dout; a.do_b = do_bhs[0]; a.do_h = do_bhs[1]; a.do_s = do_bhs[2];
+  a.dq = dq; a.dq_b = dq_bhs[0]; a.dq_h = dq_bhs[1]; a.dq_s = dq_bhs[2];
+  a.dk = dk; a.dk_b = dk_bhs[0]; a.dk_h = dk_bhs[1]; a.dk_s = dk_bhs[2];
+  a.dv = dv; a.dv_b = dv_bhs[0]; a.dv_h = dv_bhs[1]; a.dv_s = dv_bhs[2];
+  a.ndelta = (float*)workspace;
+  a.nlse2 = a.ndelta + batch * heads * sq;
+  a.kv_part = heads > kv_heads
+                  ? (float*)(((uintptr_t)(a.nlse2 + batch * heads * sq) + 255) & ~(uintptr_t)255)
+                  : nullptr;
+  return a;
 }
 
 }  // namespace
@@ -1859,54 +2046,24 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
                           const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                           const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d,
-                          double scale, int causal, int64_t window, int64_t sinks, int dtype, void* workspace,
+                          double scale, int causal, int64_t window, int dtype, void* workspace,
                           hipStream_t stream) {
   if ((dtype != MI355X_BF16 && dtype != MI355X_F16) || (d != 64 && d != 128 && d != 256)) return -1;
   if (kv_heads < 1 || heads % kv_heads != 0 || heads / kv_heads > 65535 || batch >= 65536) return -1;
   if (window > 0 && !causal) return -1;
-  if (!(strides_ok(q, q_bhs) && strides_ok(k, k_bhs) && strides_ok(v, v_bhs) && strides_ok(dout, do_bhs) &&
-        strides_ok(o, o_bhs)))
+  if (!bwd_operands_ok(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs))
     return -1;
-  for (const int64_t* st : {dq_bhs, dk_bhs, dv_bhs})
-    if (st[0] % 4 || st[1] % 4 || st[2] % 4) return -1;
-  if (((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 8) return -1;
-  AttnBwdArgs a;
-  a.f = AttnArgs{(void*)o, o_bhs[0], o_bhs[1], o_bhs[2], (float*)lse, q, q_bhs[0], q_bhs[1], q_bhs[2],
-                 k, k_bhs[0], k_bhs[1], k_bhs[2], v, v_bhs[0], v_bhs[1], v_bhs[2],
-                 batch, heads, sq, skv, (float)(scale * 1.4426950408889634), (float)scale, causal,
-                 heads / kv_heads, window, sinks};
-  a.dout = dout; a.do_b = do_bhs[0]; a.do_h = do_bhs[1]; a.do_s = do_bhs[2];
-  a.dq = dq; a.dq_b = dq_bhs[0]; a.dq_h = dq_bhs[1]; a.dq_s = dq_bhs[2];
-  a.dk = dk; a.dk_b = dk_bhs[0]; a.dk_h = dk_bhs[1]; a.dk_s = dk_bhs[2];
-  a.dv = dv; a.dv_b = dv_bhs[0]; a.dv_h = dv_bhs[1]; a.dv_s = dv_bhs[2];
-  a.ndelta = (float*)workspace;
-  a.nlse2 = a.ndelta + batch * heads * sq;
-  // partials after the row terms, 256-byte aligned (grouped heads only)
-  a.kv_part = heads > kv_heads
-                  ? (float*)(((uintptr_t)(a.nlse2 + batch * heads * sq) + 255) & ~(uintptr_t)255)
-                  : nullptr;
+  AttnBwdArgs a = bwd_args(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
+                           batch, heads, kv_heads, sq, skv, scale, causal, window, 0, workspace);
   const bool bf = dtype == MI355X_BF16;
-  if (sinks > 0) {
-    a.sink_blocks = sink_blocks(skv, sinks), a.sink_chunks = sink_chunks(sq, window);
-    float* end = a.kv_part ? a.kv_part + 2 * batch * heads * skv * d : a.nlse2 + batch * heads * sq;
-    a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
-    if (d == 64) return bf ? gqa_bwd_launch<bf16, 64, true>(a, stream) : gqa_bwd_launch<f16, 64, true>(a, stream);
-    if (d == 128) return bf ? gqa_bwd_launch<bf16, 128, true>(a, stream) : gqa_bwd_launch<f16, 128, true>(a, stream);
-    return bf ? gqa_bwd_launch<bf16, 256, true>(a, stream) : gqa_bwd_launch<f16, 256, true>(a, stream);
-  }
   if (d == 64) return bf ? gqa_bwd_launch<bf16, 64>(a, stream) : gqa_bwd_launch<f16, 64>(a, stream);
   if (d == 128) return bf ? gqa_bwd_launch<bf16, 128>(a, stream) : gqa_bwd_launch<f16, 128>(a, stream);
   return bf ? gqa_bwd_launch<bf16, 256>(a, stream) : gqa_bwd_launch<f16, 256>(a, stream);
 }
 
-// Bytes that attn_bwd_grouped_mfma needs for sinks, behind its other parts.
-int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
-                            int64_t sinks) {
-  return 2 * (sink_chunks(sq, window) + 1) * batch * heads * sink_blocks(skv, sinks) * 64 * d * (int64_t)sizeof(float) + 256;
-}
-
-// MFMA forward of a window with sinks, called by mi355x_attn_fwd_sink
-// (attention_generic.hip); -1 for inputs it does not take.
+// MFMA forward and backward of a window with sinks, called by
+// mi355x_attn_fwd_sink and mi355x_attn_bwd_sink (attention_generic.hip); -1
+// for inputs they do not take.
 int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
                        const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs, int64_t batch,
                        int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
@@ -1922,6 +2079,32 @@ int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const vo
   if (d == 64) return bf ? fwd_launch<bf16, 64, true>(a, stream) : fwd_launch<f16, 64, true>(a, stream);
   if (d == 128) return bf ? fwd_launch<bf16, 128, true>(a, stream) : fwd_launch<f16, 128, true>(a, stream);
   return bf ? fwd_launch<bf16, 256, true>(a, stream) : fwd_launch<f16, 256, true>(a, stream);
+}
+
+// Bytes of the sinks' partials, behind the workspace's other parts.
+int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
+                            int64_t sinks) {
+  return 2 * (4 * (int64_t)sink_chunks(sq, window, sinks) + 1) * batch * heads * sink_keys(skv, sinks) * d * (int64_t)sizeof(float) + 256;
+}
+
+int attn_bwd_sink_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
+                       const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
+                       const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
+                       const void* o, const int64_t* o_bhs, const float* lse, int64_t batch, int64_t heads,
+                       int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
+                       int64_t sinks, int dtype, void* workspace, hipStream_t stream) {
+  if ((dtype != MI355X_BF16 && dtype != MI355X_F16) || (d != 64 && d != 128 && d != 256)) return -1;
+  if (!bwd_operands_ok(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs))
+    return -1;
+  AttnBwdArgs a = bwd_args(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
+                           batch, heads, kv_heads, sq, skv, scale, 1, window, sinks, workspace);
+  a.sink_chunks = sink_chunks(sq, window, sinks), a.sink_keys = (int)sink_keys(skv, sinks);
+  float* end = a.kv_part ? a.kv_part + 2 * batch * heads * skv * d : a.nlse2 + batch * heads * sq;
+  a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
+  const bool bf = dtype == MI355X_BF16;
+  if (d == 64) return bf ? window_bwd_launch<bf16, 64>(a, stream) : window_bwd_launch<f16, 64>(a, stream);
+  if (d == 128) return bf ? window_bwd_launch<bf16, 128>(a, stream) : window_bwd_launch<f16, 128>(a, stream);
+  return bf ? window_bwd_launch<bf16, 256>(a, stream) : window_bwd_launch<f16, 256>(a, stream);
 }
 
 }  // namespace mi

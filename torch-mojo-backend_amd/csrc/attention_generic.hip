@@ -442,7 +442,7 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
                           const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                           const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d,
-                          double scale, int causal, int64_t window, int64_t sinks, int dtype, void* workspace,
+                          double scale, int causal, int64_t window, int dtype, void* workspace,
                           hipStream_t stream);
 int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
                             int64_t sinks);
@@ -450,6 +450,12 @@ int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const vo
                        const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs, int64_t batch,
                        int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
                        int64_t window, int64_t sinks, int dtype, hipStream_t stream);
+int attn_bwd_sink_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
+                       const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
+                       const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
+                       const void* o, const int64_t* o_bhs, const float* lse, int64_t batch, int64_t heads,
+                       int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
+                       int64_t sinks, int dtype, void* workspace, hipStream_t stream);
 }  // namespace mi
 
 // Two floats per query row (the MFMA path keeps -D and -LSE log2(e), the f32
@@ -467,19 +473,23 @@ static int attn_bwd_any(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
                                    const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
                                    const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
-                                   int64_t d, double scale, int causal, int64_t window, int64_t sinks, int dtype,
-                                   void* workspace, int64_t ws_bytes, int64_t need, const char* what,
+                                   int64_t d, double scale, int causal, int64_t window, int64_t sinks /* -1: not asked for */,
+                                   int dtype, void* workspace, int64_t ws_bytes, int64_t need, const char* what,
                                    mi355x_stream_t stream) {
   int rc = gen_check(batch, heads, kv_heads, sq, skv, d, dtype, causal, window, what);
   if (rc) return rc;
   MI_REQUIRE(dq && dk && dv && dout && q && k && v && o && lse, "%s: null pointer", what);
   if (!workspace || ws_bytes < need)
     return fail(MI355X_EWORKSPACE, "%s: workspace %lld < %lld", what, (long long)ws_bytes, (long long)need);
-  const int mrc = attn_bwd_grouped_mfma(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v,
-                                        v_bhs, o, o_bhs, lse, batch, heads, kv_heads, sq, skv, d, scale, causal,
-                                        window, sinks, dtype, workspace, (hipStream_t)stream);
+  const int mrc =
+      sinks >= 0 ? attn_bwd_sink_mfma(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o,
+                                      o_bhs, lse, batch, heads, kv_heads, sq, skv, d, scale, window, sinks, dtype,
+                                      workspace, (hipStream_t)stream)
+                 : attn_bwd_grouped_mfma(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs,
+                                         o, o_bhs, lse, batch, heads, kv_heads, sq, skv, d, scale, causal, window, dtype,
+                                         workspace, (hipStream_t)stream);
   if (mrc >= 0) return mrc;  // bf16/f16 at head_dim 64/128/256: MFMA kernels
-  GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, causal, window, sinks);
+  GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, causal, window, sinks > 0 ? sinks : 0);
   a.o = (void*)o; a.o_b = o_bhs[0]; a.o_h = o_bhs[1]; a.o_s = o_bhs[2];
   a.lse = (float*)lse;
   a.dout = dout; a.do_b = do_bhs[0]; a.do_h = do_bhs[1]; a.do_s = do_bhs[2];
@@ -503,7 +513,7 @@ extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, co
                                    int64_t d, double scale, int causal, int64_t window, int dtype,
                                    void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
   return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
-                      batch, heads, kv_heads, sq, skv, d, scale, causal, window, 0, dtype, workspace, ws_bytes,
+                      batch, heads, kv_heads, sq, skv, d, scale, causal, window, -1, dtype, workspace, ws_bytes,
                       mi355x_attn_bwd_gen_workspace_bytes(batch, heads, kv_heads, sq, skv, d), "mi355x_attn_bwd_gen",
                       stream);
 }
@@ -518,7 +528,7 @@ extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, c
   int rc = gen_check(batch, heads, kv_heads, sq, skv, d, dtype, 1, window, "mi355x_attn_fwd_sink");
   if (rc) return rc;
   MI_REQUIRE(o && lse && q && k && v, "mi355x_attn_fwd_sink: null pointer");
-  MI_REQUIRE(window > 0 && sinks > 0, "mi355x_attn_fwd_sink: window and sinks must be positive");
+  MI_REQUIRE(window > 0 && sinks >= 0, "mi355x_attn_fwd_sink: window must be positive, sinks not negative");
   rc = attn_fwd_sink_mfma(o, o_bhs, lse, q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale,
                           window, sinks, dtype, (hipStream_t)stream);
   if (rc >= 0) return rc;
@@ -541,7 +551,7 @@ extern "C" int mi355x_attn_bwd_sink(void* dq, const int64_t* dq_bhs, void* dk, c
                                     int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
                                     int64_t d, double scale, int64_t window, int64_t sinks, int dtype,
                                     void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
-  MI_REQUIRE(window > 0 && sinks > 0, "mi355x_attn_bwd_sink: window and sinks must be positive");
+  MI_REQUIRE(window > 0 && sinks >= 0, "mi355x_attn_bwd_sink: window must be positive, sinks not negative");
   return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
                       batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks, dtype, workspace, ws_bytes,
                       mi355x_attn_bwd_sink_workspace_bytes(batch, heads, kv_heads, sq, skv, d, window, sinks),

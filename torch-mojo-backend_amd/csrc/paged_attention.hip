@@ -150,12 +150,21 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join(DecodeArgs a) {
   const float w = mx == -INFINITY ? 0.f : exp2f(ml.x - mx);
   const float total = wave_sum(w * ml.y);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int ch = min(lane * 4, d - 4);  // every lane stays for the shuffles
-#pragma unroll 4
-  for (int s = wave; s < a.splits; s += kThreads / 64) {
-    const float4 x = *(const float4*)(a.part_o + (s * rows + row) * d + ch);
-    const float ws = __shfl(w, s, 64);
-    acc.x += ws * x.x, acc.y += ws * x.y, acc.z += ws * x.z, acc.w += ws * x.w;
+  constexpr int kEach = 16;  // of 64 splits to a wave; all of their loads in flight
+  const int ch = min(lane * 4, d - 4);
+  float4 x[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int s = wave + i * (kThreads / 64);
+    if (s < a.splits) x[i] = *(const float4*)(a.part_o + (s * rows + row) * d + ch);
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int s = wave + i * (kThreads / 64);
+    if (s < a.splits) {
+      const float ws = __shfl(w, s, 64);
+      acc.x += ws * x[i].x, acc.y += ws * x[i].y, acc.z += ws * x[i].z, acc.w += ws * x[i].w;
+    }
   }
   sum[wave][lane] = acc;
   __syncthreads();

@@ -2198,17 +2198,18 @@ def _mfma_bwd_ok(q: MT, group, window) -> bool:
     return q._dtype in _MFMA_DTYPES and group == 1 and window == 0 and q._shape[3] in _FUSED_FA_HEAD_DIMS
 
 
-def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=0):
+def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=None):
     """(out [B,H,Sq,D] over BTHD storage, lse f32 [B,H,Sq]) of causal / full
     attention with optional grouped K/V heads (k, v with H / g heads) and a
-    causal sliding window, with `sinks` first keys that stay visible: MFMA
-    kernels where they apply, else the f32 kernels."""
+    causal sliding window: MFMA kernels where they apply, else the f32
+    kernels.  With `sinks` (0 too) the window's own kernels, which leave that
+    many first keys visible."""
     b, h, sq, d = q._shape
     hk, skv = k._shape[1], k._shape[2]
     scale_value = float(scale) if scale is not None else 1.0 / math.sqrt(d)
     out = alloc_bthd(b, h, sq, d, q._dtype, q._device)
     lse = _alloc((b, h, sq), torch.float32, q._device)
-    if window and sinks:
+    if window and sinks is not None:
         rows = _fa_head_contig if q._dtype in _MFMA_DTYPES and d in _MFMA_EX_HEAD_DIMS else _unit_head_stride
         q, k, v = rows(q), rows(k), rows(v)
         check(
@@ -2236,7 +2237,7 @@ def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=0):
     return out, lse
 
 
-def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, window, scale, sinks=0):
+def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, window, scale, sinks=None):
     """(dq, dk, dv) of attention_forward: dk/dv have k's heads (the query
     heads of each group summed)."""
     b, h, sq, d = q._shape
@@ -2245,7 +2246,7 @@ def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, 
     if grad_out._dtype != q._dtype:
         grad_out = materialize_contiguous(grad_out, q._dtype)
     lse = _contig(lse)
-    if hk == h and skv == sq:
+    if hk == h and skv == sq and (sinks is None or q._holder is k._holder is v._holder):
         # dQ, dK, dV side by side in one [B, S, 3, H, D] buffer: the backward of
         # the fused qkv projection's split is then a cat of adjacent slices,
         # which fast_aten_cat returns as a view of this buffer (no copies)
@@ -2257,7 +2258,7 @@ def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, 
         dq = alloc_bthd(b, h, sq, d, q._dtype, q._device)
         dk = alloc_bthd(b, hk, skv, d, q._dtype, q._device)
         dv = alloc_bthd(b, hk, skv, d, q._dtype, q._device)
-    if window and sinks:
+    if window and sinks is not None:
         rows = _fa_head_contig if q._dtype in _MFMA_DTYPES and d in _MFMA_EX_HEAD_DIMS else _unit_head_stride
         q, k, v, out, dout = rows(q), rows(k), rows(v), rows(out), rows(grad_out)
         ws = lib().mi355x_attn_bwd_sink_workspace_bytes(b, h, hk, sq, skv, d, int(window), int(sinks))
@@ -2398,12 +2399,12 @@ def fused_fa_ex_inputs(query, key, value, attn_mask, dropout_p, is_causal, scale
         return None
     if scale is not None and not math.isfinite(float(scale)):
         return None
-    causal, window, sinks = bool(is_causal), 0, 0
+    causal, window, sinks = bool(is_causal), 0, None
     if attn_mask is not None:
         w = window_and_sinks_of(attn_mask)
         if w is None or is_causal or sq != skv or attn_mask.shape[-1] != skv:
             return None
-        causal, (window, sinks) = True, w
+        causal, window, sinks = True, w[0], w[1] or None
     return q, k, v, causal, window, sinks
 
 

@@ -87,7 +87,7 @@ class _FusedAttention(torch.autograd.Function):
     masked-math decomposition (aten_fast.py:9112-9123)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, causal, window, scale, sinks=0):
+    def forward(ctx, q, k, v, causal, window, scale, sinks=None):
         with torch._C._AutoDispatchBelowAutograd():
             out, lse = aten_fast.attention_forward(q, k, v, causal, window, scale, sinks)
         ctx.save_for_backward(q, k, v, out, lse)

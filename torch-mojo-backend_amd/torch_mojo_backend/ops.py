@@ -124,14 +124,12 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
     if scale is not None and not math.isfinite(float(scale)):
         raise ValueError(f"{what}: scale {scale} must be finite")
     t = q.shape[2]
-    if t <= window:
-        window, sinks = t, 0  # plain causal attention
     if _on_mojo(q, k, v) and q.numel():
         if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or q.shape[3] > 256:
             raise NotImplementedError(f"{what}: {q.dtype} with head_dim {q.shape[3]} is not supported"
                                       " (float32, bfloat16, float16, head_dim up to 256)")
         if t <= window:
-            window = 0
+            window, sinks = 0, None  # plain causal attention
         if not _needs_grad(q, k, v):
             materialize_touched((q, k, v), None, False)
             return aten_fast.attention_forward(q, k, v, True, window, scale, sinks)[0]
@@ -142,7 +140,7 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
     if not q.numel():
         return q * 1.0
     return F.scaled_dot_product_attention(
-        q, k, v, attn_mask=sliding_window_causal_mask(t, window, q.device, sinks=sinks), scale=scale, enable_gqa=True)
+        q, k, v, attn_mask=sliding_window_causal_mask(t, min(window, t), q.device, sinks=sinks), scale=scale, enable_gqa=True)
 
 
 # ---------------------------------------------------------------------------
