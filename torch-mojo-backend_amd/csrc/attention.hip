@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <mutex>
 
+#include "attention_window.h"
 #include "common.h"
 #include "mfma.h"
 
@@ -54,33 +55,8 @@
 namespace mi {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-template <typename T>
-struct alignas(16) V8 {
-  T v[8];
-};
-template <typename T>
-struct alignas(8) V4 {
-  T v[4];
-};
-
-struct AttnArgs {
-  void* o; int64_t o_b, o_h, o_s;
-  float* lse;
-  const void* q; int64_t q_b, q_h, q_s;
-  const void* k; int64_t k_b, k_h, k_s;
-  const void* v; int64_t v_b, v_h, v_s;
-  int64_t B, H, Sq, Skv;
-  float scale_log2;  // scale * log2(e)
-  float scale;
-  int causal;
-  int64_t group;   // query heads per K/V head (grouped-query attention), >= 1
-  int64_t window;  // > 0: query i sees keys i-window+1 .. i (causal only); 0: none
-  int64_t sinks;   // with a window: first keys that every later query sees
-};
 
 // Stage a 64-row x D tile (rows row0.., row stride rs) into LDS: row-major
 // [64][D+8] and/or transposed [D][64+8].  Rows past nrows read as zero.
@@ -714,23 +690,6 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
-struct AttnBwdArgs {
-  AttnArgs f;  // o = forward output (read), q/k/v inputs, lse
-  const void* dout; int64_t do_b, do_h, do_s;
-  void* dq; int64_t dq_b, dq_h, dq_s;
-  void* dk; int64_t dk_b, dk_h, dk_s;
-  void* dv; int64_t dv_b, dv_h, dv_s;
-  float* ndelta;  // [B, H, Sq]: -D, written by attn_bwd_delta
-  float* nlse2;   // [B, H, Sq]: -LSE * log2(e), written by attn_bwd_delta
-  float* kv_part; // grouped backward: per-query-head dK, dV partials (f32), or null
-  float* sink_part;    // sinks: f32 partials of their dK, dV (dkv_body)
-  int sink_blocks;     // blocks of keys that hold sinks
-  int sink_chunks;     // further blocks for each, which share the queries behind its window
-  int sink_keys;       // rows of a slot of sink_part
-  // (stored negated: the dK/dV and dQ steps add them, which saves a negation
-  // per score)
-};
-
 // D_i = sum_d dO[i, d] * O[i, d]: D/8 lanes per row, one 16-byte load of
 // each operand per lane, reduced across the row's lanes.
 template <typename T, int D>
@@ -974,15 +933,6 @@ struct WindowPos {
   BlockCoord bc;
   int chunk;
 };
-// Slots of sink_part: 0 for the window of a block of sinks (grouped heads have
-// that in kv_part), then four (one a wave) for each chunk.
-__device__ __forceinline__ float* sink_slot(const AttnBwdArgs& p, int64_t slot, int64_t b, int64_t h, int64_t key, int D) {
-  return p.sink_part + (((slot * p.f.B + b) * p.f.H + h) * p.sink_keys + key) * D;
-}
-__host__ __device__ inline int64_t sink_plane(const AttnBwdArgs& p, int D) {  // from dK's slots to dV's
-  return (4 * (int64_t)p.sink_chunks + 1) * p.f.B * p.f.H * p.sink_keys * D;
-}
-
 // WIN: a causal window, with sinks or without, and grouped K/V heads.  A block
 // takes one query head; with grouped heads it leaves f32 partials that
 // attn_bwd_window_sum adds in head order.  Sinks are seen by every later
@@ -1475,62 +1425,6 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_b
   dq_body<T, D, true, kQueryTiles>(p, bc, bc.x, lds);
 }
 
-// dK = scale * the sum of its f32 partials, dV likewise.  The first `plain`
-// blocks take the keys that are no sinks of grouped heads, four head-dim
-// elements per thread: the sum over the group's query heads, in head order.
-// Each further block takes one sink, whose partials are many (a slot a wave of
-// the blocks that shared its queries, and each head): its threads sum every
-// kSlices-th of them, and the slices are added in order.  (One thread for all
-// of them waited for 112 loads in turn: 36 us against 15 for Gemma's local
-// layer at 4096 tokens.)
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attn_bwd_window_sum(AttnBwdArgs p, uint32_t plain) {
-  const AttnArgs& f = p.f;
-  const int64_t hkn = f.H / f.group, plane = f.B * f.H * f.Skv * D;
-  auto store = [&](f32x4 sk, f32x4 sv, int64_t b, int64_t hk, int64_t key, int64_t d) {
-    V4<T> k4, v4;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) k4.v[e] = (T)(sk[e] * f.scale), v4.v[e] = (T)sv[e];
-    *(V4<T>*)((T*)p.dk + b * p.dk_b + hk * p.dk_h + key * p.dk_s + d) = k4;
-    *(V4<T>*)((T*)p.dv + b * p.dv_b + hk * p.dv_h + key * p.dv_s + d) = v4;
-  };
-  f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
-  if (blockIdx.x < plain) {
-    const int64_t keys = f.Skv - p.sink_keys, i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i4 >= f.B * hkn * keys * (D / 4)) return;
-    const int64_t row = i4 / (D / 4), d = (i4 - row * (D / 4)) * 4, bhk = row / keys, hk = bhk % hkn, b = bhk / hkn;
-    const int64_t key = row - bhk * keys + p.sink_keys;
-#pragma unroll 4
-    for (int64_t g = 0; g < f.group; ++g) {
-      const float* pk = p.kv_part + (((g * f.B + b) * hkn + hk) * f.Skv + key) * D + d;
-      sk += *(const f32x4*)pk, sv += *(const f32x4*)(pk + plane);
-    }
-    return store(sk, sv, b, hk, key, d);
-  }
-  constexpr int kSlices = kThreads / (D / 4), KW = 16 * kKeyTiles<D>;
-  __shared__ f32x4 part[2][kThreads];
-  const int64_t row = blockIdx.x - plain, key = row % p.sink_keys, bhk = row / p.sink_keys, hk = bhk % hkn, b = bhk / hkn;
-  const int slice = threadIdx.x / (D / 4), d = (int)(threadIdx.x % (D / 4)) * 4;
-  const int64_t splane = sink_plane(p, D);
-  // of a chunk's four slots, those that waves of the sink's block wrote
-  const int waves = (int)min((int64_t)4, (p.sink_keys - key / (4 * KW) * (4 * KW) + KW - 1) / KW);
-  const int parts = waves == 1 ? 4 : waves == 2 ? 2 : 1;
-  const int each = 1 + p.sink_chunks * parts, total = (int)f.group * each;  // partials of a head, of all
-#pragma unroll 4
-  for (int i = slice; i < total; i += kSlices) {
-    const int g = i / each, n = i - g * each, c = (n - 1) / parts;
-    const int64_t h = hk * f.group + g;
-    const float* pk = n == 0 && p.kv_part ? p.kv_part + (((g * f.B + b) * hkn + hk) * f.Skv + key) * D
-                                          : sink_slot(p, n == 0 ? 0 : 1 + 4 * c + (n - 1 - c * parts), b, h, key, D);
-    sk += *(const f32x4*)(pk + d), sv += *(const f32x4*)(pk + d + (n == 0 && p.kv_part ? plane : splane));
-  }
-  part[0][threadIdx.x] = sk, part[1][threadIdx.x] = sv;
-  __syncthreads();
-  if (slice) return;
-  for (int i = 1; i < kSlices; ++i) sk += part[0][threadIdx.x + i * (D / 4)], sv += part[1][threadIdx.x + i * (D / 4)];
-  store(sk, sv, b, hk, key, d);
-}
-
 // ---------------------------------------------------------------------------
 // backward with grouped K/V heads and sliding windows (MFMA), head_dim
 // 64/128/256
@@ -1975,15 +1869,6 @@ int gqa_bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
   return check_launch("mi355x_attn_bwd_gen");
 }
 
-// Blocks that share the steps behind the window of a block of sinks: eight
-// steps each, which their four waves share where there are few sinks, so that
-// one is shorter than a block of a window of 512 and more.
-int sink_chunks(int64_t sq, int64_t window, int64_t sinks) {
-  const int64_t rest = (sq + 63) / 64 - window / 64;
-  return sinks <= 0 || rest <= 0 ? 0 : (int)std::min<int64_t>((rest + 7) / 8, 1024);
-}
-int64_t sink_keys(int64_t skv, int64_t sinks) { return std::min(skv, sinks); }
-
 template <typename T, int D>
 int window_bwd_launch(AttnBwdArgs a, hipStream_t s) {
   const int64_t rows = a.f.B * a.f.H * a.f.Sq;
@@ -2003,11 +1888,8 @@ int window_bwd_launch(AttnBwdArgs a, hipStream_t s) {
   const int64_t blocks = bh * (nkx + nqx + (int64_t)a.sink_blocks * a.sink_chunks);
   MI_REQUIRE(blocks < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)blocks);
   k<<<(unsigned)blocks, kThreads, kWindowLds<D>, s>>>(a, (uint32_t)nkx, (uint32_t)nqx);
-  const int64_t kvh = a.f.B * (a.f.H / a.f.group);
-  const unsigned plain = a.kv_part ? ceil_div(kvh * (a.f.Skv - a.sink_keys) * (D / 4), kThreads) : 0;
-  const int64_t sums = plain + kvh * a.sink_keys;
-  MI_REQUIRE(sums < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)sums);
-  if (sums) attn_bwd_window_sum<T, D><<<(unsigned)sums, kThreads, 0, s>>>(a, plain);
+  const int rc = window_sum_launch<T, D, 16 * kKeyTiles<D>>(a, s);
+  if (rc) return rc;
   return check_launch("mi355x_attn_bwd_sink");
 }
 
@@ -2112,9 +1994,7 @@ int attn_bwd_sink_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64_t*
     return -1;
   AttnBwdArgs a = bwd_args(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
                            batch, heads, kv_heads, sq, skv, scale, 1, window, sinks, workspace);
-  a.sink_chunks = sink_chunks(sq, window, sinks), a.sink_keys = (int)sink_keys(skv, sinks);
-  float* end = a.kv_part ? a.kv_part + 2 * batch * heads * skv * d : a.nlse2 + batch * heads * sq;
-  a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
+  window_parts(a, d);
   const bool bf = dtype == MI355X_BF16;
   if (d == 64) return bf ? window_bwd_launch<bf16, 64>(a, stream) : window_bwd_launch<f16, 64>(a, stream);
   if (d == 128) return bf ? window_bwd_launch<bf16, 128>(a, stream) : window_bwd_launch<f16, 128>(a, stream);

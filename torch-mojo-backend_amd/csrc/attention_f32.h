@@ -20,10 +20,19 @@ struct AttnF32 {
   int64_t B, H, Sq, Skv;
   float scale_log2, scale;  // scale * log2(e), scale
   int causal;
+  // A causal window: query i sees key j <= i iff i - j < window or j < sinks;
+  // query head h reads K/V head h / group.  attn_f32_window_* alone read these.
+  int64_t group, window, sinks;
+  float *kv_part, *sink_part;  // the backward's partials (attention_window.h)
+  int sink_blocks, sink_chunks, sink_keys;
 };
 
 // -1 when the inputs are not taken (other head dims, unaligned rows).
 int attn_f32_fwd(const AttnF32& p, int64_t d, hipStream_t s);
 int attn_f32_bwd(const AttnF32& p, int64_t d, hipStream_t s);
+// The same of a window, head_dim 256 and grouped K/V heads as well.  The
+// backward's workspace: D and one more float per query row, then the partials.
+int attn_f32_window_fwd(const AttnF32& p, int64_t d, hipStream_t s);
+int attn_f32_window_bwd(const AttnF32& p, int64_t d, hipStream_t s);
 
 }  // namespace mi

@@ -23,9 +23,17 @@
 // [4, 12, 255, 64] forward 105 -> 18.1 us, backward 243 -> 43.2 us; [8, 12, 512,
 // 64] 424 -> 70.4 us and 1033 -> 183 us (46 and 44 TFLOP/s, counting the causal
 // half).
+//
+// A window with sinks has the same kernels (WIN), head_dim 256 too, grouped
+// K/V heads and 16-key partials of the sinks' gradients.  [2, 12, 255, 64],
+// window 64, 1 sink: forward 15.6 us, backward 18.8 (dK, dV, dQ) + 5.2 (D) +
+// 4.0 (sums), against 47 and 153 us in the element-per-lane kernels.  96 blocks
+// of 4 to 5 tiles leave most of the chip idle: a wave's chain of loads and
+// MFMAs bounds it, about 3 us a tile.
 #include <math.h>
 
 #include "attention_f32.h"
+#include "attention_window.h"
 #include "common.h"
 #include "mfma.h"
 
@@ -188,8 +196,37 @@ __device__ __forceinline__ void load_frags(const float* row, int lg, float f, f3
   for (int ks = 0; ks < D / 16; ++ks) x[ks] = *(const f32x4*)(row + ks * 16 + lg * 4) * f;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kNT, 2) fwd_f32(AttnF32 p, uint32_t nblk) {
+// WIN, a causal window (with sinks or without) and grouped K/V heads: the
+// tiles that the 64 queries from q0 on can see, those of sinks that lie before
+// the window's first tile, then the window's.
+struct WinTiles {
+  int64_t ns, jw, count;
+  __device__ __forceinline__ WinTiles(const AttnF32& p, int64_t q0) {
+    jw = max((int64_t)0, q0 - p.window + 1) / kRow;
+    ns = min((min(p.sinks, p.Skv) + kRow - 1) / kRow, jw);
+    count = ns + max((int64_t)0, (min(p.Skv, q0 + kBlk) + kRow - 1) / kRow - jw);
+  }
+  __device__ __forceinline__ int64_t key(int64_t i) const { return (i < ns ? i : jw + i - ns) * kRow; }
+};
+// Of a tile's rows c = 0 .. 31, those in [lo, hi) and those below sk are seen.
+// In 32 bits, against bounds of the tile: with each element's position tested
+// the backward took 252 registers at head_dim 64 and spilled 82 at 128; 179 and
+// 235 so, and 22 spilled at 256.
+struct WinRows {
+  int lo, hi, sk;
+  __device__ __forceinline__ bool sees(int c) const { return c < hi && (c >= lo || c < sk); }
+};
+__device__ __forceinline__ int clamp32(int64_t x) { return (int)min(max(x, (int64_t)-(1 << 30)), (int64_t)(1 << 30)); }
+// Whether no, or not every, query w0 .. w0 + 15 sees the tile's keys.
+__device__ __forceinline__ bool win_none(const AttnF32& p, int64_t w0, int64_t k0) {
+  return k0 >= p.sinks && k0 + kRow - 1 < w0 - p.window + 1;
+}
+__device__ __forceinline__ bool win_some(const AttnF32& p, int64_t w0, int64_t k0) {
+  return k0 < w0 + 15 - p.window + 1;
+}
+
+template <int D, bool WIN = false>
+__global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint32_t nblk) {
   typedef Tile<D> T;
   char* const lds = attn_f32_smem;  // 2 stages of a K and a V tile
   uint32_t bh, x;
@@ -198,8 +235,9 @@ __global__ void __launch_bounds__(kNT, 2) fwd_f32(AttnF32 p, uint32_t nblk) {
   const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, q0 = (int64_t)x * kBlk;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int64_t w0 = q0 + wave_id() * 16, qi = w0 + lr;
-  const float* K = p.k + b * p.k_b + h * p.k_h;
-  const float* V = p.v + b * p.v_b + h * p.v_h;
+  const int64_t hk = WIN ? h / p.group : h;
+  const float* K = p.k + b * p.k_b + hk * p.k_h;
+  const float* V = p.v + b * p.v_b + hk * p.v_h;
   f32x4 q[T::NF], o[T::NF];
   load_frags<D>(p.q + b * p.q_b + h * p.q_h + min(qi, p.Sq - 1) * p.q_s, lg, p.scale_log2, q);
 #pragma unroll
@@ -208,27 +246,35 @@ __global__ void __launch_bounds__(kNT, 2) fwd_f32(AttnF32 p, uint32_t nblk) {
 
   const int64_t kend = p.causal ? min(p.Skv, q0 + kBlk) : p.Skv;
   const int64_t wend = p.causal ? min(p.Skv, w0 + 16) : p.Skv;  // keys this wave can see
-  T::load(K, p.k_s, 0, p.Skv, lds);
-  T::load(V, p.v_s, 0, p.Skv, lds + T::BYTES);
+  const WinTiles tiles(p, q0);  // WIN
+  const int64_t nt = WIN ? tiles.count : (kend + kRow - 1) / kRow;
+  auto key = [&](int64_t i) { return WIN ? tiles.key(i) : i * kRow; };
+  if (!WIN || nt > 0) {
+    T::load(K, p.k_s, key(0), p.Skv, lds);
+    T::load(V, p.v_s, key(0), p.Skv, lds + T::BYTES);
+  }
   int cur = 0;
-  for (int64_t k0 = 0; k0 < kend; k0 += kRow, cur ^= 1) {
+  for (int64_t i = 0; i < nt; ++i, cur ^= 1) {
+    const int64_t k0 = key(i);
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
-    if (k0 + kRow < kend) {
-      T::load(K, p.k_s, k0 + kRow, p.Skv, lds + (cur ^ 1) * 2 * T::BYTES);
-      T::load(V, p.v_s, k0 + kRow, p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES);
+    if (i + 1 < nt) {
+      T::load(K, p.k_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES);
+      T::load(V, p.v_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES);
     }
-    if (k0 >= wend) continue;
+    if (k0 >= wend || (WIN && win_none(p, w0, k0))) continue;
     const char* kt = lds + cur * 2 * T::BYTES;
     f32x4 s[2];
     scores<D>(kt, q, lr, lg, s);
-    if (k0 + kRow > p.Skv || (p.causal && k0 + kRow - 1 > w0)) {
+    if (k0 + kRow > p.Skv || (p.causal && k0 + kRow - 1 > w0) || (WIN && win_some(p, w0, k0))) {
+      const WinRows seen{clamp32(qi - k0 - p.window + 1), clamp32(min(p.Skv, qi + 1) - k0), clamp32(p.sinks - k0)};
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int64_t j = k0 + sub * 16 + 4 * lg + e;
-          if (j >= p.Skv || (p.causal && j > qi)) s[sub][e] = -INFINITY;
+          const int c = sub * 16 + 4 * lg + e;
+          const int64_t j = k0 + c;
+          if (WIN ? !seen.sees(c) : j >= p.Skv || (p.causal && j > qi)) s[sub][e] = -INFINITY;
         }
     }
     float mx = -INFINITY;
@@ -289,7 +335,7 @@ __global__ void __launch_bounds__(kNT) delta_f32(AttnF32 p, int64_t rows) {
 }
 
 // dQ of 64 queries: dS^T = P^T (dP^T - D), dQ^T = scale K^T dS^T.
-template <int D>
+template <int D, bool WIN = false>
 __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk) {
   typedef Tile<D> T;
   char* const lds = attn_f32_smem;
@@ -299,8 +345,9 @@ __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t to
   const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, q0 = (int64_t)x * kBlk;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int64_t w0 = q0 + wave_id() * 16, qi = w0 + lr, qc = min(qi, p.Sq - 1);
-  const float* K = p.k + b * p.k_b + h * p.k_h;
-  const float* V = p.v + b * p.v_b + h * p.v_h;
+  const int64_t hk = WIN ? h / p.group : h;
+  const float* K = p.k + b * p.k_b + hk * p.k_h;
+  const float* V = p.v + b * p.v_b + hk * p.v_h;
   f32x4 q[T::NF], dO[T::NF], dq[T::NF];
   load_frags<D>(p.q + b * p.q_b + h * p.q_h + qc * p.q_s, lg, p.scale_log2, q);
   load_frags<D>(p.dout + b * p.do_b + h * p.do_h + qc * p.do_s, lg, 1.f, dO);
@@ -311,29 +358,38 @@ __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t to
 
   const int64_t kend = p.causal ? min(p.Skv, q0 + kBlk) : p.Skv;
   const int64_t wend = p.causal ? min(p.Skv, w0 + 16) : p.Skv;
-  T::load(K, p.k_s, 0, p.Skv, lds);
-  T::load(V, p.v_s, 0, p.Skv, lds + T::BYTES);
+  const WinTiles tiles(p, q0);  // WIN
+  const int64_t nt = WIN ? tiles.count : (kend + kRow - 1) / kRow;
+  auto key = [&](int64_t i) { return WIN ? tiles.key(i) : i * kRow; };
+  if (!WIN || nt > 0) {
+    T::load(K, p.k_s, key(0), p.Skv, lds);
+    T::load(V, p.v_s, key(0), p.Skv, lds + T::BYTES);
+  }
   int cur = 0;
-  for (int64_t k0 = 0; k0 < kend; k0 += kRow, cur ^= 1) {
+  for (int64_t i = 0; i < nt; ++i, cur ^= 1) {
+    const int64_t k0 = key(i);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (k0 + kRow < kend) {
-      T::load(K, p.k_s, k0 + kRow, p.Skv, lds + (cur ^ 1) * 2 * T::BYTES);
-      T::load(V, p.v_s, k0 + kRow, p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES);
+    if (i + 1 < nt) {
+      T::load(K, p.k_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES);
+      T::load(V, p.v_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES);
     }
-    if (k0 >= wend) continue;
+    if (k0 >= wend || (WIN && win_none(p, w0, k0))) continue;
     const char* kt = lds + cur * 2 * T::BYTES;
     f32x4 s[2], dp[2];
     scores<D>(kt, q, lr, lg, s);
     scores<D>(kt + T::BYTES, dO, lr, lg, dp);
-    const bool masked = k0 + kRow > p.Skv || (p.causal && k0 + kRow - 1 > w0);
+    const WinRows seen{clamp32(qi - k0 - p.window + 1), clamp32(min(p.Skv, qi + 1) - k0), clamp32(p.sinks - k0)};  // WIN
+    const bool masked = k0 + kRow > p.Skv || (p.causal && k0 + kRow - 1 > w0) || (WIN && win_some(p, w0, k0));
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t j = k0 + sub * 16 + 4 * lg + e;
+        const int c = sub * 16 + 4 * lg + e;
+        const int64_t j = k0 + c;
         float pr = exp2f(s[sub][e] - lse2);
-        if (masked && (j >= p.Skv || (p.causal && j > qi))) pr = 0.f;
+        if (masked && (WIN ? !seen.sees(c) : j >= p.Skv || (p.causal && j > qi)))
+          pr = 0.f;
         s[sub][e] = pr * (dp[sub][e] - di);
       }
     accumulate<D>(kt, s, lr, lg, dq);
@@ -341,53 +397,77 @@ __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t to
   if (qi < p.Sq) T::store(p.dq + b * p.dq_b + h * p.dq_h + qi * p.dq_s, dq, lg, p.scale);
 }
 
-// dK, dV of 64 keys: dV^T = dO^T P, dK^T = scale Q^T dS.
-template <int D>
-__device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk) {
+// dK, dV of 64 keys: dV^T = dO^T P, dK^T = scale Q^T dS.  WIN: of one query
+// head, and (extra) of one chunk of the queries behind the window of a block of
+// sinks, as attention.hip's dkv_body.
+template <int D, bool WIN = false>
+__device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk, bool extra = false) {
   typedef Tile<D> T;
   char* const lds = attn_f32_smem;                    // 2 stages of a Q and a dO tile
   float* const terms = (float*)(lds + 4 * T::BYTES);  // 2 stages of 32 LSE, 32 D
   uint32_t bh, x;
   block_of(L, total, nblk, &bh, &x);
-  const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, k0 = (int64_t)x * kBlk;
+  int chunk = 0;
+  if (WIN && extra) chunk = x / p.sink_blocks, x -= chunk * p.sink_blocks;
+  const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, hk = WIN ? h / p.group : h, k0 = (int64_t)x * kBlk;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-  const int64_t w0 = k0 + wave_id() * 16, kj = w0 + lr, kc = min(kj, p.Skv - 1);
+  int wave_key = wave_id(), part = 0, parts = 1;  // of a chunk: the wave's keys, and its share of the steps
+  if (WIN && extra) {
+    const int waves = (int)min((int64_t)4, (p.sinks - k0 + 15) / 16);
+    parts = waves == 1 ? 4 : waves == 2 ? 2 : 1;
+    wave_key = parts == 1 ? wave_id() : wave_id() % waves, part = parts == 1 ? 0 : wave_id() / waves;
+  }
+  const int64_t w0 = k0 + wave_key * 16, kj = w0 + lr, kc = min(kj, p.Skv - 1);
   const float* Q = p.q + b * p.q_b + h * p.q_h;
   const float* dO = p.dout + b * p.do_b + h * p.do_h;
   const float* rt = (lane < 32 ? p.lse : p.delta) + (b * p.H + h) * p.Sq;  // this lane's row term
   f32x4 k[T::NF], v[T::NF], dk[T::NF], dv[T::NF];
-  load_frags<D>(p.k + b * p.k_b + h * p.k_h + kc * p.k_s, lg, p.scale_log2, k);
-  load_frags<D>(p.v + b * p.v_b + h * p.v_h + kc * p.v_s, lg, 1.f, v);
+  load_frags<D>(p.k + b * p.k_b + hk * p.k_h + kc * p.k_s, lg, p.scale_log2, k);
+  load_frags<D>(p.v + b * p.v_b + hk * p.v_h + kc * p.v_s, lg, 1.f, v);
 #pragma unroll
   for (int n = 0; n < T::NF; ++n) dk[n] = dv[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int64_t qbeg = p.causal ? k0 : 0;  // a multiple of 32; may lie past the last query
+  int64_t qbeg = p.causal ? k0 : 0;  // a multiple of 32; may lie past the last query
+  int64_t qend = p.Sq;
+  if constexpr (WIN) {
+    const int64_t near = min(p.Sq, qbeg + (kBlk - 1 + p.window + 63) / 64 * 64);  // end of the window's steps
+    qend = near;
+    if (extra) {
+      const int64_t per = ((p.Sq - near + 63) / 64 + p.sink_chunks - 1) / p.sink_chunks * 64;
+      qbeg = min(p.Sq, near + chunk * per), qend = min(p.Sq, qbeg + per);
+    }
+  }
   auto issue = [&](int64_t r0, int st) {
     T::load(Q, p.q_s, r0, p.Sq, lds + st * 2 * T::BYTES);
     T::load(dO, p.do_s, r0, p.Sq, lds + st * 2 * T::BYTES + T::BYTES);
     if (wave_id() == 0) dma_b32(rt + min(r0 + (lane & 31), p.Sq - 1), lds_base_of(terms + st * 64));
   };
-  if (qbeg < p.Sq) issue(qbeg, 0);
+  if (qbeg < qend) issue(qbeg, 0);
   int cur = 0;
-  for (int64_t r0 = qbeg; r0 < p.Sq; r0 += kRow, cur ^= 1) {
+  for (int64_t r0 = qbeg; r0 < qend; r0 += kRow, cur ^= 1) {
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (r0 + kRow < p.Sq) issue(r0 + kRow, cur ^ 1);
+    if (r0 + kRow < qend) issue(r0 + kRow, cur ^ 1);
     if (p.causal && r0 + kRow - 1 < w0) continue;  // no query of the tile sees this wave's keys
+    if (WIN && w0 >= p.sinks && (extra || r0 >= w0 + 15 + p.window)) continue;
+    if (WIN && ((int)((r0 - qbeg) / kRow) & (parts - 1)) != part) continue;  // another wave's
     const char* qt = lds + cur * 2 * T::BYTES;
     f32x4 s[2], dp[2];
     scores<D>(qt, k, lr, lg, s);
     scores<D>(qt + T::BYTES, v, lr, lg, dp);
-    const bool masked = r0 + kRow > p.Sq || (p.causal && r0 < w0 + 15);
+    const WinRows seen{clamp32(kj - r0), clamp32((kj < p.sinks ? p.Sq : min(p.Sq, kj + p.window)) - r0), 0};  // WIN
+    const bool masked = r0 + kRow > p.Sq || (p.causal && r0 < w0 + 15) || (WIN && r0 + kRow - 1 >= w0 + p.window);
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       const f32x4 lse = *(const f32x4*)(terms + cur * 64 + sub * 16 + 4 * lg);
       const f32x4 di = *(const f32x4*)(terms + cur * 64 + 32 + sub * 16 + 4 * lg);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t i = r0 + sub * 16 + 4 * lg + e;
+        const int c = sub * 16 + 4 * lg + e;
+        const int64_t i = r0 + c;
         float pr = exp2f(s[sub][e] - lse[e] * kLog2e);
-        if (masked && (i >= p.Sq || (p.causal && i < kj))) pr = 0.f;
+        if (masked && (WIN ? c < seen.lo || c >= seen.hi : i >= p.Sq || (p.causal && i < kj)))
+          pr = 0.f;
         s[sub][e] = pr;
         dp[sub][e] = pr * (dp[sub][e] - di[e]);
       }
@@ -396,8 +476,24 @@ __device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t t
     accumulate<D>(qt, dp, lr, lg, dk);
   }
   if (kj >= p.Skv) return;
-  T::store(p.dk + b * p.dk_b + h * p.dk_h + kj * p.dk_s, dk, lg, p.scale);
-  T::store(p.dv + b * p.dv_b + h * p.dv_h + kj * p.dv_s, dv, lg, 1.f);
+  if constexpr (WIN) {  // partials: of sinks, and of a head of a group
+    const int64_t keys = p.sink_keys, slots = 4 * (int64_t)p.sink_chunks + 1;
+    if (extra || (!p.kv_part && kj < p.sinks)) {
+      if (kj >= p.sinks) return;
+      const int64_t slot = extra ? 1 + 4 * chunk + part : 0;
+      float* pk = p.sink_part + (((slot * p.B + b) * p.H + h) * keys + kj) * D;
+      T::store(pk, dk, lg, 1.f);
+      return T::store(pk + slots * p.B * p.H * keys * D, dv, lg, 1.f);
+    }
+    if (p.kv_part) {
+      const int64_t hkn = p.H / p.group, gi = h - hk * p.group;
+      float* pk = p.kv_part + (((gi * p.B + b) * hkn + hk) * p.Skv + kj) * D;
+      T::store(pk, dk, lg, 1.f);
+      return T::store(pk + p.B * p.H * p.Skv * D, dv, lg, 1.f);
+    }
+  }
+  T::store(p.dk + b * p.dk_b + hk * p.dk_h + kj * p.dk_s, dk, lg, p.scale);
+  T::store(p.dv + b * p.dv_b + hk * p.dv_h + kj * p.dv_s, dv, lg, 1.f);
 }
 
 // Both in one launch: the first `ndkv` blocks do dK and dV, the rest dQ, so
@@ -406,6 +502,16 @@ template <int D>
 __global__ void __launch_bounds__(kNT, 2) bwd_f32(AttnF32 p, uint32_t ndkv, uint32_t kblk, uint32_t qblk) {
   if (blockIdx.x < ndkv) dkv_f32<D>(p, blockIdx.x, ndkv, kblk);
   else dq_f32<D>(p, blockIdx.x - ndkv, gridDim.x - ndkv, qblk);
+}
+
+// A window's: dK/dV blocks, the blocks that share the queries behind the
+// windows of blocks of sinks, dQ blocks.
+template <int D>
+__global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) bwd_window_f32(AttnF32 p, uint32_t ndkv, uint32_t nextra, uint32_t kblk, uint32_t qblk) {
+  const uint32_t l = blockIdx.x, first = ndkv + nextra;
+  if (l >= first) return dq_f32<D, true>(p, l - first, gridDim.x - first, qblk);
+  const bool extra = l >= ndkv;  // one call: two copies of the body spill registers
+  dkv_f32<D, true>(p, extra ? l - ndkv : l, extra ? nextra : ndkv, extra ? p.sink_blocks * p.sink_chunks : kblk, extra);
 }
 
 // Dynamic LDS of a launch; the first launch of a kernel that needs more than
@@ -437,6 +543,40 @@ int run_bwd(const AttnF32& p, hipStream_t s) {
   return check_launch("mi355x_attn_bwd_gen");
 }
 
+template <int D>
+int run_window_fwd(const AttnF32& p, hipStream_t s) {
+  static const bool ok = opt_in((const void*)fwd_f32<D, true>, lds_bytes<D>(false));
+  if (!ok) return fail(MI355X_ELAUNCH, "mi355x_attn_fwd_sink: cannot reserve %zu bytes of LDS", lds_bytes<D>(false));
+  const uint32_t nblk = ceil_div(p.Sq, kBlk);
+  fwd_f32<D, true><<<(unsigned)(nblk * p.B * p.H), kNT, lds_bytes<D>(false), s>>>(p, nblk);
+  return check_launch("mi355x_attn_fwd_sink");
+}
+
+template <int D>
+int run_window_bwd(AttnF32 p, hipStream_t s) {
+  static const bool ok = opt_in((const void*)bwd_window_f32<D>, lds_bytes<D>(true));
+  if (!ok) return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_sink: cannot reserve %zu bytes of LDS", lds_bytes<D>(true));
+  const int64_t rows = p.B * p.H * p.Sq;
+  delta_f32<D><<<ceil_div(rows * kChains<D>, kNT), kNT, 0, s>>>(p, rows);
+  AttnBwdArgs a{};
+  a.f.B = p.B, a.f.H = p.H, a.f.Sq = p.Sq, a.f.Skv = p.Skv, a.f.scale = p.scale, a.f.group = p.group;
+  a.f.window = p.window, a.f.sinks = p.sinks;
+  a.dk = p.dk, a.dk_b = p.dk_b, a.dk_h = p.dk_h, a.dk_s = p.dk_s;
+  a.dv = p.dv, a.dv_b = p.dv_b, a.dv_h = p.dv_h, a.dv_s = p.dv_s;
+  a.ndelta = p.delta;
+  if (p.group > 1) a.kv_part = (float*)(((uintptr_t)(p.delta + 2 * rows) + 255) & ~(uintptr_t)255);
+  window_parts(a, D);
+  p.kv_part = a.kv_part, p.sink_part = a.sink_part;
+  p.sink_chunks = a.sink_chunks, p.sink_keys = a.sink_keys, p.sink_blocks = (a.sink_keys + kBlk - 1) / kBlk;
+  const int64_t kblk = (p.Skv + kBlk - 1) / kBlk, qblk = (p.Sq + kBlk - 1) / kBlk, heads = p.B * p.H;
+  const int64_t extra = (int64_t)p.sink_blocks * p.sink_chunks;
+  MI_REQUIRE((kblk + qblk + extra) * heads < (1ll << 24), "mi355x_attn_bwd_sink: too many blocks");
+  bwd_window_f32<D><<<(unsigned)((kblk + qblk + extra) * heads), kNT, lds_bytes<D>(true), s>>>(
+      p, (uint32_t)(kblk * heads), (uint32_t)(extra * heads), (uint32_t)kblk, (uint32_t)qblk);
+  const int rc = window_sum_launch<float, D, 16>(a, s);
+  return rc ? rc : check_launch("mi355x_attn_bwd_sink");
+}
+
 // Tiles are loaded and rows stored 16 bytes at a time.
 bool wide(const void* p, int64_t b, int64_t h, int64_t s) {
   return ((uintptr_t)p & 15) == 0 && b % 4 == 0 && h % 4 == 0 && s % 4 == 0;
@@ -450,7 +590,28 @@ bool takes(const AttnF32& p) {
          wide(p.o, p.o_b, p.o_h, p.o_s);
 }
 
+bool takes_grads(const AttnF32& p) {
+  return wide(p.dout, p.do_b, p.do_h, p.do_s) && wide(p.dq, p.dq_b, p.dq_h, p.dq_s) &&
+         wide(p.dk, p.dk_b, p.dk_h, p.dk_s) && wide(p.dv, p.dv_b, p.dv_h, p.dv_s);
+}
+
 }  // namespace
+
+int attn_f32_window_fwd(const AttnF32& p, int64_t d, hipStream_t s) {
+  if (!takes(p)) return -1;
+  if (d == 64) return run_window_fwd<64>(p, s);
+  if (d == 128) return run_window_fwd<128>(p, s);
+  if (d == 256) return run_window_fwd<256>(p, s);
+  return d == 32 ? run_window_fwd<32>(p, s) : -1;
+}
+
+int attn_f32_window_bwd(const AttnF32& p, int64_t d, hipStream_t s) {
+  if (!takes(p) || !takes_grads(p)) return -1;
+  if (d == 64) return run_window_bwd<64>(p, s);
+  if (d == 128) return run_window_bwd<128>(p, s);
+  if (d == 256) return run_window_bwd<256>(p, s);
+  return d == 32 ? run_window_bwd<32>(p, s) : -1;
+}
 
 int attn_f32_fwd(const AttnF32& p, int64_t d, hipStream_t s) {
   if (!takes(p)) return -1;
@@ -460,9 +621,7 @@ int attn_f32_fwd(const AttnF32& p, int64_t d, hipStream_t s) {
 }
 
 int attn_f32_bwd(const AttnF32& p, int64_t d, hipStream_t s) {
-  if (!takes(p) || !wide(p.dout, p.do_b, p.do_h, p.do_s) || !wide(p.dq, p.dq_b, p.dq_h, p.dq_s) ||
-      !wide(p.dk, p.dk_b, p.dk_h, p.dk_s) || !wide(p.dv, p.dv_b, p.dv_h, p.dv_s))
-    return -1;
+  if (!takes(p) || !takes_grads(p)) return -1;
   if (d == 64) return run_bwd<64>(p, s);
   if (d == 128) return run_bwd<128>(p, s);
   return d == 32 ? run_bwd<32>(p, s) : -1;

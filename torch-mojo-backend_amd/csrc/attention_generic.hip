@@ -1,8 +1,9 @@
 // Fused attention for the inputs the MFMA kernels do not take: any head_dim
 // up to 256, f32 with grouped K/V heads or a window, and the backward of
 // grouped-K/V-head and sliding-window attention.  Everything is computed in
-// f32.  Plain f32 attention at head_dim 32, 64 and 128 goes on from these
-// entry points to the matrix cores (attention_f32.hip).
+// f32.  Plain f32 attention at head_dim 32, 64 and 128, and a window with sinks
+// at 256 as well, goes on from these entry points to the matrix cores
+// (attention_f32.hip).
 //
 // Semantics are those of attention.hip: S = scale Q K^T over the visible keys
 // (top-left causal: key j visible to query i iff j <= i; with a window w > 0
@@ -21,6 +22,8 @@
 // through LDS as f32 (the 8 lanes of a row read 8 consecutive floats; every
 // row group of a wave reads the same address, a broadcast).
 #include <math.h>
+
+#include <algorithm>
 
 #include "attention_f32.h"
 #include "common.h"
@@ -399,14 +402,15 @@ GenArgs gen_args(const void* q, const int64_t* q_bhs, const void* k, const int64
 
 // The operands for attention_f32.hip, where the call is one it can take: f32,
 // a K/V head for each query head, no window.
-bool f32_args(const GenArgs& a, int dtype, AttnF32* f) {
-  if (dtype != MI355X_F32 || a.H != a.HK || a.window != 0) return false;
+// (Those of a window with sinks it takes too, with grouped heads.)
+bool f32_args(const GenArgs& a, int dtype, AttnF32* f, bool sink = false) {
+  if (dtype != MI355X_F32 || (!sink && (a.H != a.HK || a.window != 0))) return false;
   *f = AttnF32{(float*)a.o, a.o_b, a.o_h, a.o_s, a.lse,
                (const float*)a.q, a.q_b, a.q_h, a.q_s, (const float*)a.k, a.k_b, a.k_h, a.k_s,
                (const float*)a.v, a.v_b, a.v_h, a.v_s, (const float*)a.dout, a.do_b, a.do_h, a.do_s,
                (float*)a.dq, a.dq_b, a.dq_h, a.dq_s, (float*)a.dk, a.dk_b, a.dk_h, a.dk_s,
                (float*)a.dv, a.dv_b, a.dv_h, a.dv_s, a.delta, a.B, a.H, a.Sq, a.Skv,
-               a.scale_log2, a.scale, a.causal};
+               a.scale_log2, a.scale, a.causal, a.H / a.HK, a.window, a.sinks};
   return true;
 }
 
@@ -498,8 +502,8 @@ static int attn_bwd_any(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
   a.dv = dv; a.dv_b = dv_bhs[0]; a.dv_h = dv_bhs[1]; a.dv_s = dv_bhs[2];
   a.delta = (float*)workspace;
   AttnF32 f;
-  if (f32_args(a, dtype, &f)) {
-    rc = attn_f32_bwd(f, d, (hipStream_t)stream);
+  if (f32_args(a, dtype, &f, sinks >= 0)) {
+    rc = sinks >= 0 ? attn_f32_window_bwd(f, d, (hipStream_t)stream) : attn_f32_bwd(f, d, (hipStream_t)stream);
     if (rc >= 0) return rc;
   }
   MI_GEN_DISPATCH(dtype, d, gen_bwd_launch, a, (hipStream_t)stream);
@@ -518,6 +522,12 @@ extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, co
                       stream);
 }
 
+// A window past the queries and sinks past the keys mask what the clipped ones
+// do, and sums of positions with them stay in range.
+static void clip_window(int64_t& window, int64_t& sinks, int64_t sq, int64_t skv) {
+  window = std::min(window, std::max(sq, (int64_t)1)), sinks = std::min(sinks, skv);
+}
+
 // A window with sinks: causal, query i sees key j iff i - j < window or j <
 // sinks.
 extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
@@ -529,17 +539,24 @@ extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, c
   if (rc) return rc;
   MI_REQUIRE(o && lse && q && k && v, "mi355x_attn_fwd_sink: null pointer");
   MI_REQUIRE(window > 0 && sinks >= 0, "mi355x_attn_fwd_sink: window must be positive, sinks not negative");
+  clip_window(window, sinks, sq, skv);
   rc = attn_fwd_sink_mfma(o, o_bhs, lse, q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale,
                           window, sinks, dtype, (hipStream_t)stream);
   if (rc >= 0) return rc;
   GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks);
   a.o = o; a.o_b = o_bhs[0]; a.o_h = o_bhs[1]; a.o_s = o_bhs[2];
   a.lse = lse;
+  AttnF32 f;
+  if (f32_args(a, dtype, &f, true)) {
+    rc = attn_f32_window_fwd(f, d, (hipStream_t)stream);
+    if (rc >= 0) return rc;
+  }
   MI_GEN_DISPATCH(dtype, d, gen_fwd_launch, a, (hipStream_t)stream);
 }
 
 extern "C" int64_t mi355x_attn_bwd_sink_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq,
                                                         int64_t skv, int64_t d, int64_t window, int64_t sinks) {
+  clip_window(window, sinks, sq, skv);
   return mi355x_attn_bwd_gen_workspace_bytes(batch, heads, kv_heads, sq, skv, d) +
          attn_bwd_sink_bytes(batch, heads, sq, skv, d, window, sinks);
 }
@@ -552,6 +569,7 @@ extern "C" int mi355x_attn_bwd_sink(void* dq, const int64_t* dq_bhs, void* dk, c
                                     int64_t d, double scale, int64_t window, int64_t sinks, int dtype,
                                     void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
   MI_REQUIRE(window > 0 && sinks >= 0, "mi355x_attn_bwd_sink: window must be positive, sinks not negative");
+  clip_window(window, sinks, sq, skv);
   return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
                       batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks, dtype, workspace, ws_bytes,
                       mi355x_attn_bwd_sink_workspace_bytes(batch, heads, kv_heads, sq, skv, d, window, sinks),

@@ -1,0 +1,150 @@
+// What the attention kernels share: their arguments, and the partial sums of a
+// windowed backward (attention.hip for 16-bit types, attention_f32.hip).
+#pragma once
+#include <algorithm>
+
+#include "common.h"
+
+namespace mi {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+struct alignas(16) V8 {
+  T v[8];
+};
+template <typename T>
+struct alignas(8) V4 {
+  T v[4];
+};
+
+struct AttnArgs {
+  void* o; int64_t o_b, o_h, o_s;
+  float* lse;
+  const void* q; int64_t q_b, q_h, q_s;
+  const void* k; int64_t k_b, k_h, k_s;
+  const void* v; int64_t v_b, v_h, v_s;
+  int64_t B, H, Sq, Skv;
+  float scale_log2;  // scale * log2(e)
+  float scale;
+  int causal;
+  int64_t group;   // query heads per K/V head (grouped-query attention), >= 1
+  int64_t window;  // > 0: query i sees keys i-window+1 .. i (causal only); 0: none
+  int64_t sinks;   // with a window: first keys that every later query sees
+};
+
+struct AttnBwdArgs {
+  AttnArgs f;  // o = forward output (read), q/k/v inputs, lse
+  const void* dout; int64_t do_b, do_h, do_s;
+  void* dq; int64_t dq_b, dq_h, dq_s;
+  void* dk; int64_t dk_b, dk_h, dk_s;
+  void* dv; int64_t dv_b, dv_h, dv_s;
+  float* ndelta;  // [B, H, Sq]: -D, written by attn_bwd_delta
+  float* nlse2;   // [B, H, Sq]: -LSE * log2(e), written by attn_bwd_delta
+  float* kv_part; // grouped backward: per-query-head dK, dV partials (f32), or null
+  float* sink_part;    // sinks: f32 partials of their dK, dV (dkv_body)
+  int sink_blocks;     // blocks of keys that hold sinks
+  int sink_chunks;     // further blocks for each, which share the queries behind its window
+  int sink_keys;       // rows of a slot of sink_part
+  // (stored negated: the dK/dV and dQ steps add them, which saves a negation
+  // per score)
+};
+
+// Slots of sink_part: 0 for the window of a block of sinks (grouped heads have
+// that in kv_part), then four (one a wave) for each chunk.
+__device__ __forceinline__ float* sink_slot(const AttnBwdArgs& p, int64_t slot, int64_t b, int64_t h, int64_t key, int D) {
+  return p.sink_part + (((slot * p.f.B + b) * p.f.H + h) * p.sink_keys + key) * D;
+}
+__host__ __device__ inline int64_t sink_plane(const AttnBwdArgs& p, int D) {  // from dK's slots to dV's
+  return (4 * (int64_t)p.sink_chunks + 1) * p.f.B * p.f.H * p.sink_keys * D;
+}
+
+// KW: keys of a wave of the kernel that left the partials, which has four.
+//
+// dK = scale * the sum of its f32 partials, dV likewise.  The first `plain`
+// blocks take the keys that are no sinks of grouped heads, four head-dim
+// elements per thread: the sum over the group's query heads, in head order.
+// Each further block takes one sink, whose partials are many (a slot a wave of
+// the blocks that shared its queries, and each head): its threads sum every
+// kSlices-th of them, and the slices are added in order.  (One thread for all
+// of them waited for 112 loads in turn: 36 us against 15 for Gemma's local
+// layer at 4096 tokens.)
+template <typename T, int D, int KW>
+__global__ void __launch_bounds__(kThreads) attn_bwd_window_sum(AttnBwdArgs p, uint32_t plain) {
+  const AttnArgs& f = p.f;
+  const int64_t hkn = f.H / f.group, plane = f.B * f.H * f.Skv * D;
+  auto store = [&](f32x4 sk, f32x4 sv, int64_t b, int64_t hk, int64_t key, int64_t d) {
+    V4<T> k4, v4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k4.v[e] = (T)(sk[e] * f.scale), v4.v[e] = (T)sv[e];
+    *(V4<T>*)((T*)p.dk + b * p.dk_b + hk * p.dk_h + key * p.dk_s + d) = k4;
+    *(V4<T>*)((T*)p.dv + b * p.dv_b + hk * p.dv_h + key * p.dv_s + d) = v4;
+  };
+  f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
+  if (blockIdx.x < plain) {
+    const int64_t keys = f.Skv - p.sink_keys, i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i4 >= f.B * hkn * keys * (D / 4)) return;
+    const int64_t row = i4 / (D / 4), d = (i4 - row * (D / 4)) * 4, bhk = row / keys, hk = bhk % hkn, b = bhk / hkn;
+    const int64_t key = row - bhk * keys + p.sink_keys;
+#pragma unroll 4
+    for (int64_t g = 0; g < f.group; ++g) {
+      const float* pk = p.kv_part + (((g * f.B + b) * hkn + hk) * f.Skv + key) * D + d;
+      sk += *(const f32x4*)pk, sv += *(const f32x4*)(pk + plane);
+    }
+    return store(sk, sv, b, hk, key, d);
+  }
+  constexpr int kSlices = kThreads / (D / 4);
+  __shared__ f32x4 part[2][kThreads];
+  const int64_t row = blockIdx.x - plain, key = row % p.sink_keys, bhk = row / p.sink_keys, hk = bhk % hkn, b = bhk / hkn;
+  const int slice = threadIdx.x / (D / 4), d = (int)(threadIdx.x % (D / 4)) * 4;
+  const int64_t splane = sink_plane(p, D);
+  // of a chunk's four slots, those that waves of the sink's block wrote
+  const int waves = (int)min((int64_t)4, (p.sink_keys - key / (4 * KW) * (4 * KW) + KW - 1) / KW);
+  const int parts = waves == 1 ? 4 : waves == 2 ? 2 : 1;
+  const int each = 1 + p.sink_chunks * parts, total = (int)f.group * each;  // partials of a head, of all
+#pragma unroll 4
+  for (int i = slice; i < total; i += kSlices) {
+    const int g = i / each, n = i - g * each, c = (n - 1) / parts;
+    const int64_t h = hk * f.group + g;
+    const float* pk = n == 0 && p.kv_part ? p.kv_part + (((g * f.B + b) * hkn + hk) * f.Skv + key) * D
+                                          : sink_slot(p, n == 0 ? 0 : 1 + 4 * c + (n - 1 - c * parts), b, h, key, D);
+    sk += *(const f32x4*)(pk + d), sv += *(const f32x4*)(pk + d + (n == 0 && p.kv_part ? plane : splane));
+  }
+  part[0][threadIdx.x] = sk, part[1][threadIdx.x] = sv;
+  __syncthreads();
+  if (slice) return;
+  for (int i = 1; i < kSlices; ++i) sk += part[0][threadIdx.x + i * (D / 4)], sv += part[1][threadIdx.x + i * (D / 4)];
+  store(sk, sv, b, hk, key, d);
+}
+
+// Blocks that share the steps behind the window of a block of sinks: eight
+// steps each, which their four waves share where there are few sinks, so that
+// one is shorter than a block of a window of 512 and more.
+inline int sink_chunks(int64_t sq, int64_t window, int64_t sinks) {
+  const int64_t rest = (sq + 63) / 64 - window / 64;
+  return sinks <= 0 || rest <= 0 ? 0 : (int)std::min<int64_t>((rest + 7) / 8, 1024);
+}
+inline int64_t sink_keys(int64_t skv, int64_t sinks) { return std::min(skv, sinks); }
+
+// The sinks' part of the arguments; their partials lie behind the workspace's
+// other parts.
+inline void window_parts(AttnBwdArgs& a, int64_t d) {
+  const int64_t rows = a.f.B * a.f.H * a.f.Sq;
+  a.sink_chunks = sink_chunks(a.f.Sq, a.f.window, a.f.sinks), a.sink_keys = (int)sink_keys(a.f.Skv, a.f.sinks);
+  float* end = a.kv_part ? a.kv_part + 2 * a.f.B * a.f.H * a.f.Skv * d : a.ndelta + 2 * rows;
+  a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
+}
+
+template <typename T, int D, int KW>
+inline int window_sum_launch(const AttnBwdArgs& a, hipStream_t s) {
+  const int64_t kvh = a.f.B * (a.f.H / a.f.group);
+  const unsigned plain = a.kv_part ? ceil_div(kvh * (a.f.Skv - a.sink_keys) * (D / 4), kThreads) : 0;
+  const int64_t sums = plain + kvh * a.sink_keys;
+  MI_REQUIRE(sums < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)sums);
+  if (sums) attn_bwd_window_sum<T, D, KW><<<(unsigned)sums, kThreads, 0, s>>>(a, plain);
+  return MI355X_OK;
+}
+
+}  // namespace
+}  // namespace mi
