@@ -153,6 +153,17 @@ def test_hidden_numbers_stay_hidden():
         _attention(c, 2, [99], [1], 1, BF, window=56, sinks=4)
 
 
+@pytest.mark.parametrize("dtype,bits", [(BF, None), (F32, None), (BF, 4)])
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 4), (256, 48), (96, 16)])
+def test_pages_that_no_query_sees_are_not_looked_up(dtype, bits, d, page):
+    c = Case([600, 400], page=page, bits=bits, device="mojo", d=d, hk=1, dtype=dtype)
+    # windows begin at 597 - 100 + 1 and 397 - 100 + 1, sinks end at 7
+    c.table[0, -(-7 // page):498 // page], c.table[1, -(-7 // page):298 // page], c.table[1, -(-400 // page):] = -1, 10 ** 6, -7
+    q = c.queries(2, 3, dtype)
+    out = ops.paged_attention(q.to("mojo"), c.cache, c.table.to("mojo"), c.ints([597, 397]), window=100, sinks=7)
+    check(out, *c.expected(q, [597, 397], [3, 3], 100, 7))  # reads the flag as well
+
+
 def test_offsets_past_32_bits():
     pages, page, hk, d = 70_000, 16, 8, 256  # 2.3e9 values a tensor
     k, v = (torch.empty(pages, hk, page, d, dtype=BF, device="mojo") for _ in range(2))

@@ -132,6 +132,16 @@ def test_attention_matches_the_oracle(device, bits, window, sinks):
     check(out, *c.expected(q, starts, counts, window, sinks))
 
 
+def test_pages_that_no_query_sees_are_not_looked_up(device):
+    """Between the sinks' pages and the window's, and behind the last token."""
+    c = Case([60, 40], page=4, device=device, dtype=torch.float32)
+    c.table[0, 1:9], c.table[1, 1:4], c.table[1, 10:] = -1, 10 ** 6, -7  # windows begin at 57 - 20 + 1 and 18
+    q = c.queries(2, 3)
+    out = ops.paged_attention(q.to(device), c.cache, c.table.to(device), c.ints([57, 37]), window=20, sinks=4)
+    check(out, *c.expected(q, [57, 37], [3, 3], 20, 4))
+    c.cache.k.cpu()
+
+
 def test_lengths_of_zero_and_one(device):
     c = Case([1, 1], page=4, device=device, dtype=torch.float32)
     q = c.queries(2, 1)

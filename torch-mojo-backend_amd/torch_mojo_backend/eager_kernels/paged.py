@@ -19,6 +19,7 @@ from ..mojo_device import torch_mojo_tensor as _tensor_mod
 
 MT = _tensor_mod.TorchMojoTensor
 _INT32 = torch.int32
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def describe(cache) -> PagedCache:
@@ -52,13 +53,14 @@ def seqs_ok(cache, table, starts, counts) -> bool:
                               and counts._strides == (1,) and counts._device == dev)
 
 
-def rows_ok(cache, t, batch) -> bool:
-    """[batch, any heads, any tokens, head_dim] of the pages' type (16 or 32 bits)."""
+def rows_ok(cache, t, batch, like=None) -> bool:
+    """[batch, any heads, any tokens, head_dim] of the pages' type, or for 4-bit
+    pages of a float type, that of `like` where given."""
     if type(t) is not MT or t.requires_grad:
         return False
-    shape = t._shape
-    return (len(shape) == 4 and shape[0] == batch and shape[3] == cache.head_dim and t._dtype is cache.dtype
-            and t._device == cache.k._device)
+    shape, dtype = t._shape, t._dtype
+    return (len(shape) == 4 and shape[0] == batch and shape[3] == cache.head_dim and t._device == cache.k._device
+            and (dtype is cache.dtype if cache.bits != 4 else dtype in _FLOATS if like is None else dtype is like._dtype))
 
 
 def _with_device(device: int, call):

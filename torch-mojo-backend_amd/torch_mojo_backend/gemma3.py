@@ -1,4 +1,5 @@
-"""A Gemma-3-1B-shaped decoder for the prefill workload (forward only).
+"""A Gemma-3-1B-shaped decoder (forward only): prefill of whole sequences, and
+new tokens against a paged key/value cache.
 
 The shapes are those of Gemma 3 1B: 26 layers, d_model 1152, 4 query heads
 sharing 1 K/V head (grouped-query attention), head_dim 256, GeGLU MLP with
@@ -14,7 +15,10 @@ gfx950 kernels: linear -> GEMM, RMSNorm (1 + w) -> the fused RMSNorm, SDPA
 with enable_gqa / a sliding-window mask from torch_mojo_backend.masks -> the
 grouped-query windowed flash forward, RoPE and GeGLU -> their fused kernels
 (torch_mojo_backend.ops, which falls back to the plain formulas off the
-device).
+device).  `Gemma3.forward_cached` takes the tokens of each call, one or many a
+sequence, into a paged cache (ops.paged_append, which also turns q and k) and
+attends over its pages (ops.paged_attention).  With `sinks` the local layers
+keep a sequence's first tokens visible beside the window.
 """
 
 from __future__ import annotations
@@ -27,6 +31,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
+from .kv_cache import PagedKVCache
 from .masks import sliding_window_causal_mask
 
 
@@ -40,6 +45,7 @@ class Gemma3Config:
     head_dim: int = 256
     d_ff: int = 6912
     window: int = 512
+    sinks: int = 0  # first tokens that local layers see beside the window
     global_every: int = 6  # layers 5, 11, 17, 23 are global: five local to one global
     rope_local_base: float = 10000.0
     rope_global_base: float = 1000000.0
@@ -84,7 +90,7 @@ class Attention(nn.Module):
         self.q_norm = RMSNorm(d, cfg.eps)
         self.k_norm = RMSNorm(d, cfg.eps)
 
-    def forward(self, x, rope, mask):
+    def _qkv(self, x):
         b, t, _ = x.shape
         c = self.cfg
         # the per-head norms run on the projections' dense [B, T, H, D] rows,
@@ -92,6 +98,12 @@ class Attention(nn.Module):
         q = self.q_norm(self.q_proj(x).view(b, t, c.heads, c.head_dim)).transpose(1, 2)
         k = self.k_norm(self.k_proj(x).view(b, t, c.kv_heads, c.head_dim)).transpose(1, 2)
         v = self.v_proj(x).view(b, t, c.kv_heads, c.head_dim).transpose(1, 2)
+        return q, k, v
+
+    def forward(self, x, rope, mask):
+        b, t, _ = x.shape
+        c = self.cfg
+        q, k, v = self._qkv(x)
         cos, sin = rope
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         scale = 1.0 / math.sqrt(c.head_dim)
@@ -99,6 +111,15 @@ class Attention(nn.Module):
             y = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=scale, enable_gqa=True)
         else:
             y = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale, enable_gqa=True)
+        return self.o_proj(y.transpose(1, 2).reshape(b, t, c.heads * c.head_dim))
+
+    def forward_cached(self, x, rope, cache, page_table, starts, counts):
+        b, t, _ = x.shape
+        c = self.cfg
+        q, k, v = self._qkv(x)
+        q = ops.paged_append(cache, page_table, starts, k, v, *rope, q=q, counts=counts)
+        window, sinks = (c.window, c.sinks) if self.local else (0, 0)
+        y = ops.paged_attention(q, cache, page_table, starts, counts=counts, window=window, sinks=sinks)
         return self.o_proj(y.transpose(1, 2).reshape(b, t, c.heads * c.head_dim))
 
 
@@ -129,6 +150,11 @@ class Block(nn.Module):
         x = x + self.post_attn_norm(self.attn(self.input_norm(x), rope, mask))
         return x + self.post_ffw_norm(self.mlp(self.pre_ffw_norm(x)))
 
+    def forward_cached(self, x, rope_local, rope_global, *cached):
+        rope = rope_local if self.local else rope_global
+        x = x + self.post_attn_norm(self.attn.forward_cached(self.input_norm(x), rope, *cached))
+        return x + self.post_ffw_norm(self.mlp(self.pre_ffw_norm(x)))
+
 
 class Gemma3(nn.Module):
     def __init__(self, cfg: Gemma3Config):
@@ -146,6 +172,7 @@ class Gemma3(nn.Module):
         # device, dtype) seen: built on the host and copied over, they cost
         # more than a third of a prefill's host time when rebuilt per call
         self._tables = {}
+        self._cached_tables = {}  # the same for forward_cached: of the most positions seen
 
     def _rope_and_mask(self, t, dev, dt):
         key = (t, str(dev), dt)
@@ -154,7 +181,7 @@ class Gemma3(nn.Module):
             c = self.cfg
             hit = (rope_tables(t, c.head_dim, c.rope_local_base, dev, dt),
                    rope_tables(t, c.head_dim, c.rope_global_base, dev, dt),
-                   sliding_window_causal_mask(t, c.window, dev))
+                   sliding_window_causal_mask(t, c.window, dev, c.sinks))
             self._tables = {key: hit}
         return hit
 
@@ -169,3 +196,27 @@ class Gemma3(nn.Module):
             x = blk(x, rope_local, rope_global, mask)
         x = self.norm(x)
         return F.linear(x, self.embed.weight)
+
+    def caches(self, num_pages, page_size, *, bits=None):
+        """Empty pages for each layer: of the weights' type, or of 4 bits."""
+        c, w = self.cfg, self.embed.weight
+        return [PagedKVCache.zeros(num_pages, page_size, c.kv_heads, c.head_dim, dtype=w.dtype, bits=bits, device=w.device)
+                for _ in self.blocks]
+
+    @torch.no_grad()
+    def forward_cached(self, idx, caches, page_table, starts, counts=None):
+        """Logits [B, T, vocab] of new tokens idx [B, T] at positions starts[b]
+        .. starts[b] + T - 1 of their sequences, whose earlier tokens earlier
+        calls have put into `caches` (one a layer, all under page_table [B,
+        pages]); these are put there too.  Tokens from counts[b] on are padding."""
+        c = self.cfg
+        dev, dt = idx.device, self.embed.weight.dtype
+        need, key = page_table.shape[1] * caches[0].page_size, (str(dev), dt)
+        rope = self._cached_tables.get(key)
+        if rope is None or rope[0][0].shape[0] < need:
+            rope = tuple(rope_tables(need, c.head_dim, base, dev, dt) for base in (c.rope_local_base, c.rope_global_base))
+            self._cached_tables = {key: rope}
+        x = self.embed(idx) * torch.tensor(c.hidden ** 0.5, dtype=dt, device=dev)
+        for blk, cache in zip(self.blocks, caches, strict=True):
+            x = blk.forward_cached(x, *rope, cache, page_table, starts, counts)
+        return F.linear(self.norm(x), self.embed.weight)

@@ -145,11 +145,13 @@ def unpack(codes, scales):
     return (scales[..., 1:] + scales[..., :1] * x).flatten(-2)
 
 
-def _places(cache, table, starts, tokens, counts):
-    """(real, page, slot) [batch, tokens] of each token."""
+def _places(cache, table, starts, tokens, counts, wanted=None):
+    """(real, page, slot) [batch, tokens] of each token, or of the wanted ones."""
     t = torch.arange(tokens)
     pos = starts.long()[:, None] + t
     real = (t < counts[:, None]) if counts is not None else torch.ones_like(pos, dtype=torch.bool)
+    if wanted is not None:
+        real = wanted
     place = pos // cache.page_size
     bad = real & ((pos < 0) | (place >= table.shape[1]))
     if bad.any():
@@ -190,8 +192,8 @@ def append_plain(cache, table, starts, k, v, cos, sin, q, counts):
     return out
 
 
-def gather_plain(cache, table, starts, length, counts, dtype):
-    real, page, slot = _places(cache, table, starts, length, counts)
+def gather_plain(cache, table, starts, length, counts, dtype, wanted=None):
+    real, page, slot = _places(cache, table, starts, length, counts, wanted)
 
     def rows(pages, scales):
         x = pages[page, :, slot] if scales is None else unpack(pages[page, :, slot], scales[page, :, slot])
@@ -207,14 +209,15 @@ def attention_plain(q, cache, table, starts, counts, window, sinks, scale):
     ends = torch.where(n > 0, starts + n, 0)
     _places(cache, table, torch.where(n > 0, starts, 0), t, n)  # the queries' own places exist
     length = int(ends.max()) if b else 0
-    k, v = gather_plain(cache, table, torch.zeros_like(starts), length, ends, torch.float32)
-    g = h // cache.kv_heads
-    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
     i = torch.where(torch.arange(t) < n[:, None], starts[:, None] + torch.arange(t), -1)[:, None, :, None]
     j = torch.arange(length)
     keep = j <= i
     if window:
         keep = keep & ((i - j < window) | (j < sinks))
+    wanted = keep.any(2)[:, 0]
+    k, v = gather_plain(cache, table, torch.zeros_like(starts), length, ends, torch.float32, wanted)
+    g = h // cache.kv_heads
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
     s = (q.float() @ k.transpose(-1, -2) * scale).masked_fill(~keep, float("-inf"))
     p = torch.where(keep.any(-1, keepdim=True), torch.softmax(s, dim=-1), 0.0)
     return (p @ v).to(q.dtype)

@@ -190,12 +190,13 @@ def paged_append(cache, page_table, starts, k, v, cos=None, sin=None, *, q=None,
     device-to-host read) and is not written.  Two tokens of one call must not
     name the same slot."""
     if (paged.seqs_ok(cache, page_table, starts, counts) and paged.rows_ok(cache, k, page_table._shape[0])
-            and paged.rows_ok(cache, v, page_table._shape[0]) and k._shape[1] == cache.kv_heads and k._shape == v._shape
+            and paged.rows_ok(cache, v, page_table._shape[0], k) and k._shape[1] == cache.kv_heads and k._shape == v._shape
             and (cos is None) == (sin is None) == (q is None)
-            and (cos is None or (type(cos) is type(sin) is TorchMojoTensor and cos._dtype is sin._dtype is torch.float32
+            and (cos is None or (type(cos) is type(sin) is TorchMojoTensor and cos._dtype is sin._dtype
+                                 and (cos._dtype is torch.float32 or cos._dtype is k._dtype)
                                  and len(cos._shape) == 2 and cos._shape == sin._shape
                                  and cos._shape[1] == cache.head_dim and cache.head_dim % 16 == 0
-                                 and cos._device == sin._device == k._device and paged.rows_ok(cache, q, k._shape[0])
+                                 and cos._device == sin._device == k._device and paged.rows_ok(cache, q, k._shape[0], k)
                                  and q._shape[2] == k._shape[2] and q._shape[1]))
             and not _needs_grad(cos, sin)):
         return paged.append(cache, page_table, starts, k, v, cos, sin, q, counts)
@@ -256,8 +257,12 @@ def paged_attention(q, cache, page_table, starts, *, counts=None, window=0, sink
     head_dim ** -0.5.
 
     A page that does not exist raises IndexError (on the mojo device at the
-    next device-to-host read) and counts as hidden.  What lies in pages behind
-    a sequence's last token is never used."""
+    next device-to-host read) and counts as hidden.  Pages that no query sees
+    are not looked up: the table may say anything of pages that lie behind a
+    sequence's last token, or between its sinks and its window.  What lies in
+    rows that no query sees is never used; a NaN or an infinity in the value of
+    a row that some query of the sequence sees may reach the call's others, as
+    0 * NaN does in the plain formula."""
     if (paged.seqs_ok(cache, page_table, starts, counts) and paged.rows_ok(cache, q, page_table._shape[0])
             and q._shape[1] and q._shape[1] % cache.kv_heads == 0 and type(window) is type(sinks) is int
             and window >= 0 and sinks >= 0 and scale is None):
