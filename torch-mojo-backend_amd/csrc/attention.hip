@@ -472,8 +472,11 @@ constexpr float kSlack = 8.f;
 
 // SINK: a window with sinks.  The block first walks the 64-key tiles that hold
 // sinks and lie before its window's first tile, then the window's.
+// At head_dim 128 it is held to 256 registers, two waves a SIMD: a window's few
+// tiles a block leave one wave's waits bare ([2, 16 over 4, 2000, 128], window
+// 512: 52 -> 36 us; 16 queries a wave in twice the blocks 39).
 template <typename T, int D, bool POS, int NW, int QPW, bool SINK = false>
-__global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 1) attn_fwd_v2(AttnArgs p) {
+__global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : SINK && D == 128 && POS ? 2 : 1) attn_fwd_v2(AttnArgs p) {
   constexpr int QT = QPW / 16, QPB = NW * QPW;  // 16-query tiles per wave, queries per block
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;

@@ -190,7 +190,10 @@ int64_t most_keys(const mi355x_paged_cache& c, int64_t width, int64_t window, in
 // Blocks that share the keys of a row, where rows alone are too few to fill
 // the 256 CUs: eight blocks a CU in all (lengths differ, and the last round is
 // shorter than with four: 282 against 276 us for the batch above
-// paged_attn_mfma), of at least 128 keys each.
+// paged_attn_mfma), of at least 128 keys each.  Up to 384 keys one block does
+// it: the second launch takes 3.5 us and as long again to reach the GPU, which
+// is what the three tiles of 32 keys (six of 16) that a wave then has take
+// ([3 x 4, 12, 64] f32 over 333 keys: 7.8 + 3.6 us and a launch between, or 12.4).
 int plan_splits(const mi355x_paged_cache& c, int64_t width, int64_t batch, int64_t heads, int64_t seq, int64_t window,
                 int64_t sinks, int dtype) {
   const int64_t keys = most_keys(c, width, window, sinks);
@@ -199,6 +202,7 @@ int plan_splits(const mi355x_paged_cache& c, int64_t width, int64_t batch, int64
     const int64_t rows = heads / c.kv_heads * seq, per = 16 * paged_mfma_row_tiles(rows, c.d);
     blocks = batch * c.kv_heads * ((rows + per - 1) / per);
   }
+  if (keys <= 384) return 1;
   int64_t n = blocks > 0 ? (2048 + blocks - 1) / blocks : 1;
   if (n > (keys + 127) / 128) n = (keys + 127) / 128;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);

@@ -63,13 +63,13 @@ def rows_ok(cache, t, batch, like=None) -> bool:
             and (dtype is cache.dtype if cache.bits != 4 else dtype in _FLOATS if like is None else dtype is like._dtype))
 
 
-def _with_device(device: int, call):
-    """call() with `device` current: a launch on the null stream goes to the
-    current device."""
-    if _tensor_mod.storage_kind() == "cuda" and torch.cuda.current_device() != device:
+def _on_device(device: int, call, *args):
+    """call(*args) with `device` current: a launch on the null stream goes to
+    the current device."""
+    if _tensor_mod.storage_kind() == "cuda" and torch._C._cuda_getDevice() != device:
         with torch.cuda.device(device):
-            return call()
-    return call()
+            return call(*args)
+    return call(*args)
 
 
 def _rows(t: MT) -> MT:
@@ -98,7 +98,7 @@ def append(cache, table, starts, k, v, cos, sin, q, counts):
     if lazy_live():
         materialize_touched((*cache.tensors, table, starts, k, v, cos, sin, q, counts), None, True)
     dev = k._device
-    out = _with_device(dev, lambda: _append(cache, table, starts, k, v, cos, sin, q, counts, dev))
+    out = _on_device(dev, _append, cache, table, starts, k, v, cos, sin, q, counts, dev)
     torch._C._increment_version(cache.tensors)
     return out
 
@@ -126,7 +126,7 @@ def _append(cache, table, starts, k, v, cos, sin, q, counts, dev):
 def gather(cache, table, starts, length, counts, dtype):
     if lazy_live():
         materialize_touched((*cache.tensors, table, starts, counts), None, False)
-    return _with_device(table._device, lambda: _gather(cache, table, starts, length, counts, dtype, table._device))
+    return _on_device(table._device, _gather, cache, table, starts, length, counts, dtype, table._device)
 
 
 def _gather(cache, table, starts, length, counts, dtype, dev):
@@ -143,7 +143,7 @@ def _gather(cache, table, starts, length, counts, dtype, dev):
 def attention(q, cache, table, starts, counts, window, sinks, scale):
     if lazy_live():
         materialize_touched((q, *cache.tensors, table, starts, counts), None, False)
-    return _with_device(q._device, lambda: _attention(q, cache, table, starts, counts, window, sinks, scale, q._device))
+    return _on_device(q._device, _attention, q, cache, table, starts, counts, window, sinks, scale, q._device)
 
 
 def _attention(q, cache, table, starts, counts, window, sinks, scale, dev):
