@@ -475,13 +475,17 @@ constexpr float kSlack = 8.f;
 // At head_dim 128 it is held to 256 registers, two waves a SIMD: a window's few
 // tiles a block leave one wave's waits bare ([2, 16 over 4, 2000, 128], window
 // 512: 52 -> 36 us; 16 queries a wave in twice the blocks 39).
-template <typename T, int D, bool POS, int NW, int QPW, bool SINK = false>
+// At 256, where two stages of K and V leave room for one block a CU, KH = 2 has
+// the same from eight waves: each half of them takes half of a tile's keys, and
+// they join at the end ([1, 4 over 1, 4096, 256], window 512: 31 -> 25 us).
+template <typename T, int D, bool POS, int NW, int QPW, bool SINK = false, int KH = 1>
 __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : SINK && D == 128 && POS ? 2 : 1) attn_fwd_v2(AttnArgs p) {
-  constexpr int QT = QPW / 16, QPB = NW * QPW;  // 16-query tiles per wave, queries per block
+  constexpr int QT = QPW / 16, QPB = NW / KH * QPW;  // 16-query tiles per wave, queries per block
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
   constexpr int KS = D / 32, DT = D / 16;
   constexpr int STAGE = 2 * L::TILE;  // K tile + V tile
+  constexpr int KN = 64 / KH;         // keys of a tile that a wave takes
   char* lds;
   if constexpr (D == 256) {
     lds = attn_dyn_lds;  // 2 x 64 KB, launched with dynamic LDS
@@ -490,7 +494,9 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
     lds = lds_static;
   }
 
-  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int lane = threadIdx.x & 63;
+  const int wave = KH == 1 ? wave_id() : wave_id() % (NW / KH);  // its queries,
+  const int wk = KH == 1 ? 0 : wave_id() / (NW / KH);            // and its share of a tile's keys
   const int lr = lane & 15, lg = lane >> 4;
   const BlockCoord bc = block_coord(/*zigzag=*/true);
   const int64_t qblock = p.causal ? (int64_t)gridDim.x - 1 - bc.x : bc.x;
@@ -549,20 +555,21 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
       kl.issue(kn, p.Skv, nx);
       vl.issue(kn, p.Skv, nx + L::TILE);
     }
-    const char* Kt = lds + buf * STAGE;
+    const char* Kt = lds + buf * STAGE + wk * (L::TILE / KH);
     const char* Vt = Kt + L::TILE;
+    const int64_t kb = kb0 + wk * KN;  // the wave's first key
     buf ^= 1;
     // a tile none of this wave's queries can see (past the causal diagonal
     // of its last query, or before the window of its first) adds nothing:
     // the wave keeps the block's loads and barriers and skips the math
     if constexpr (MASK) {
       const int64_t qf = q0 + wave * QPW;
-      if (p.causal && kb0 > qf + QPW - 1) return;
-      if (p.window > 0 && kb0 + 63 < qf - p.window + 1 && !(SINK && kb0 < p.sinks)) return;
+      if (p.causal && kb > qf + QPW - 1) return;
+      if (p.window > 0 && kb + KN - 1 < qf - p.window + 1 && !(SINK && kb < p.sinks)) return;
     }
-      // Per query tile, the keys kb0 + lo..lim are visible to this lane's
-      // query, and those of its sinks, kb0 + 0..ls-1, up to lim.
-      const int ls = SINK ? (int)max((int64_t)0, min((int64_t)64, p.sinks - kb0)) : 0;
+      // Per query tile, the keys kb + lo..lim are visible to this lane's
+      // query, and those of its sinks, kb + 0..ls-1, up to lim.
+      const int ls = SINK ? (int)max((int64_t)0, min((int64_t)64, p.sinks - kb)) : 0;
       int lo[QT], lim[QT];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
@@ -570,20 +577,20 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
         lim[qt] = 63;
         if constexpr (MASK) {
           const int64_t qi = q0 + wave * QPW + qt * 16 + lr;
-          int64_t lm = p.Skv - 1 - kb0;
-          if (p.causal && qi - kb0 < lm) lm = qi - kb0;
+          int64_t lm = p.Skv - 1 - kb;
+          if (p.causal && qi - kb < lm) lm = qi - kb;
           lim[qt] = (int)max((int64_t)-1, min((int64_t)63, lm));
-          if (p.window > 0) lo[qt] = (int)max((int64_t)0, min((int64_t)64, qi - p.window + 1 - kb0));
+          if (p.window > 0) lo[qt] = (int)max((int64_t)0, min((int64_t)64, qi - p.window + 1 - kb));
         }
       }
       // S^T tiles, each masked and folded into the row maxima right after
       // its MFMAs, so that work can issue beside the next tile's MFMAs.
-      f32x4 s[4][QT];
+      f32x4 s[4 / KH][QT];
       float mx[QT];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) mx[qt] = -INFINITY;
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
+      for (int kt = 0; kt < 4 / KH; ++kt) {
         frag kf[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) m_use[qt] = m[qt] == -INFINITY ? 0.f : m[qt];
 #pragma unroll
-      for (int ks2 = 0; ks2 < 2; ++ks2) {
+      for (int ks2 = 0; ks2 < 2 / KH; ++ks2) {
         frag pf[QT];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
@@ -672,6 +679,33 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
   float l[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) l[qt] = lacc[qt][0];
+  if constexpr (KH == 2) {  // the second half of the keys joins the first
+    static_assert(NW / 2 * QT * (DT * 1024 + 512) <= 2 * STAGE, "");
+    __builtin_amdgcn_s_waitcnt(0xc07f & 0x3f70);  // no load is still on its way to LDS
+    __syncthreads();
+    f32x4* const ox = (f32x4*)lds + wave * QT * DT * 64 + lane;
+    float2* const mx = (float2*)(lds + NW / 2 * QT * DT * 1024) + wave * QT * 64 + lane;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+      if (wk) {
+        mx[qt * 64] = make_float2(m[qt], l[qt]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) ox[(qt * DT + dt) * 64] = oacc[dt][qt];
+      }
+    __syncthreads();
+    if (wk) return;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const float2 other = mx[qt * 64];
+      const float top = fmaxf(m[qt], other.x);
+      const float a0 = m[qt] == -INFINITY ? 0.f : fast_exp2(m[qt] - top);
+      const float a1 = other.x == -INFINITY ? 0.f : fast_exp2(other.x - top);
+      l[qt] = l[qt] * a0 + other.y * a1;
+      m[qt] = top;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) oacc[dt][qt] = oacc[dt][qt] * a0 + ox[(qt * DT + dt) * 64] * a1;
+    }
+  }
   T* O = (T*)p.o + b * p.o_b + h * p.o_h;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -1772,11 +1806,12 @@ template <typename T, int D, bool SINK = false>
 int fwd_launch(const AttnArgs& a, hipStream_t s) {
   if constexpr (D == 256) {
     // 64-query blocks of 4 waves x 16 queries; K/V stages need 128 KB of LDS
-    constexpr int NW = 4, QPW = 16;
+    // (a window's with sinks: 8, in pairs that share queries)
+    constexpr int KH = SINK ? 2 : 1, NW = 4 * KH, QPW = 16;
     constexpr size_t kLds = 4 * KvLayout<256>::TILE;
-    dim3 grid(ceil_div(a.Sq, NW * QPW), (unsigned)a.H, (unsigned)a.B);
-    auto kp = attn_fwd_v2<T, D, true, NW, QPW, SINK>;
-    auto kn = attn_fwd_v2<T, D, false, NW, QPW, SINK>;
+    dim3 grid(ceil_div(a.Sq, NW / KH * QPW), (unsigned)a.H, (unsigned)a.B);
+    auto kp = attn_fwd_v2<T, D, true, NW, QPW, SINK, KH>;
+    auto kn = attn_fwd_v2<T, D, false, NW, QPW, SINK, KH>;
     static bool attr = false;
     if (!attr) {
       if (hipFuncSetAttribute((const void*)kp, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds) != hipSuccess ||

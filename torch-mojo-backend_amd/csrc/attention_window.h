@@ -68,10 +68,11 @@ __host__ __device__ inline int64_t sink_plane(const AttnBwdArgs& p, int D) {  //
 // Each further block takes one sink, whose partials are many (a slot a wave of
 // the blocks that shared its queries, and each head): its threads sum every
 // kSlices-th of them, and the slices are added in order.  (One thread for all
-// of them waited for 112 loads in turn: 36 us against 15 for Gemma's local
-// layer at 4096 tokens.)
+// of them waited for 112 loads in turn: 36 us for Gemma's local layer at 4096
+// tokens, 15 with four slices of 64 threads each, 12.7 with sixteen.)
+constexpr int kSumThreads = 1024;
 template <typename T, int D, int KW>
-__global__ void __launch_bounds__(kThreads) attn_bwd_window_sum(AttnBwdArgs p, uint32_t plain) {
+__global__ void __launch_bounds__(kSumThreads) attn_bwd_window_sum(AttnBwdArgs p, uint32_t plain) {
   const AttnArgs& f = p.f;
   const int64_t hkn = f.H / f.group, plane = f.B * f.H * f.Skv * D;
   auto store = [&](f32x4 sk, f32x4 sv, int64_t b, int64_t hk, int64_t key, int64_t d) {
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_window_sum(AttnBwdArgs p, u
   };
   f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sv = sk;
   if (blockIdx.x < plain) {
-    const int64_t keys = f.Skv - p.sink_keys, i4 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t keys = f.Skv - p.sink_keys, i4 = (int64_t)blockIdx.x * kSumThreads + threadIdx.x;
     if (i4 >= f.B * hkn * keys * (D / 4)) return;
     const int64_t row = i4 / (D / 4), d = (i4 - row * (D / 4)) * 4, bhk = row / keys, hk = bhk % hkn, b = bhk / hkn;
     const int64_t key = row - bhk * keys + p.sink_keys;
@@ -94,8 +95,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_window_sum(AttnBwdArgs p, u
     }
     return store(sk, sv, b, hk, key, d);
   }
-  constexpr int kSlices = kThreads / (D / 4);
-  __shared__ f32x4 part[2][kThreads];
+  constexpr int kSlices = kSumThreads / (D / 4);
+  __shared__ f32x4 part[2][kSumThreads];
   const int64_t row = blockIdx.x - plain, key = row % p.sink_keys, bhk = row / p.sink_keys, hk = bhk % hkn, b = bhk / hkn;
   const int slice = threadIdx.x / (D / 4), d = (int)(threadIdx.x % (D / 4)) * 4;
   const int64_t splane = sink_plane(p, D);
@@ -139,10 +140,10 @@ inline void window_parts(AttnBwdArgs& a, int64_t d) {
 template <typename T, int D, int KW>
 inline int window_sum_launch(const AttnBwdArgs& a, hipStream_t s) {
   const int64_t kvh = a.f.B * (a.f.H / a.f.group);
-  const unsigned plain = a.kv_part ? ceil_div(kvh * (a.f.Skv - a.sink_keys) * (D / 4), kThreads) : 0;
+  const unsigned plain = a.kv_part ? ceil_div(kvh * (a.f.Skv - a.sink_keys) * (D / 4), kSumThreads) : 0;
   const int64_t sums = plain + kvh * a.sink_keys;
   MI_REQUIRE(sums < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)sums);
-  if (sums) attn_bwd_window_sum<T, D, KW><<<(unsigned)sums, kThreads, 0, s>>>(a, plain);
+  if (sums) attn_bwd_window_sum<T, D, KW><<<(unsigned)sums, kSumThreads, 0, s>>>(a, plain);
   return MI355X_OK;
 }
 
