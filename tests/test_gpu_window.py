@@ -85,3 +85,108 @@ def test_broadcast_gradient_and_shared_leaf():
     want = window_cases.expected(x, x, x, torch.ones_like(x), 20, 2)
     check(leaf.grad, sum(want[n][0] for n in ("dq", "dk", "dv")),
           sum(want[n][1] for n in ("dq", "dk", "dv")) + 2.0 ** -22 * 4)
+
+
+@pytest.mark.parametrize("d,h,hk", [(32, 2, 2), (32, 3, 1), (128, 4, 2), (256, 6, 3)])
+@pytest.mark.parametrize("t,window,sinks", [(64, 1, 1), (129, 31, 17), (300, 64, 40), (777, 100, 4)])
+def test_f32_heads(d, h, hk, t, window, sinks):
+    x = window_cases.inputs(1, h, hk, t, d, F32)
+    compare(run(x, window, sinks), window_cases.expected(*x, window, sinks))
+
+
+@pytest.mark.parametrize("dtype,d,hk", [(BF, 64, 2), (BF, 128, 1), (HF, 256, 2), (F32, 64, 1), (F32, 256, 2), (F32, 80, 1)])
+def test_many_sinks(dtype, d, hk):
+    """More sinks than one block of keys has, a last block with a few of them, and all of them."""
+    for t, window, sinks in ((600, 70, 300), (450, 33, 129), (300, 20, 2 ** 40)):
+        x = window_cases.inputs(1, 2, hk, t, d, dtype)
+        compare(run(x, window, sinks), window_cases.expected(*x, window, min(sinks, t)))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128), (F32, 64), (BF, 256)])
+def test_strides_and_alignment(dtype, d):
+    """Rows of one packed projection, at odd offsets, heads first, and an expanded gradient."""
+    h, t = 2, 150
+    x = window_cases.inputs(2, h, h, t, d, dtype)
+    want = window_cases.expected(*x, 40, 3)
+    packed = torch.cat([y.transpose(1, 2).reshape(2, t, h * d) for y in x[:3]], dim=-1).to("mojo").requires_grad_()
+    q, k, v = (y.view(2, t, h, d).transpose(1, 2) for y in packed.split(h * d, dim=-1))
+    out = ops.sliding_window_attention(q, k, v, 40, sinks=3)
+    out.backward(x[3].to("mojo"))
+    got = [y.view(2, t, h, d).transpose(1, 2) for y in packed.grad.cpu().split(h * d, dim=-1)]
+    compare(dict(zip(("out", "dq", "dk", "dv"), (out, *got))), want)
+
+    def odd(y):  # one element past an aligned address, rows of d + 1
+        wide = torch.zeros(2, h, t, d + 1, dtype=dtype)
+        wide[..., 1:] = y
+        return wide.to("mojo")[..., 1:]
+
+    leaves = [odd(y).detach().requires_grad_() for y in x[:3]]
+    out = ops.sliding_window_attention(*leaves, 40, sinks=3)
+    out.backward(odd(x[3]))
+    compare(dict(zip(("out", "dq", "dk", "dv"), (out, *(y.grad for y in leaves)))), want)
+
+    ones = torch.ones(1, dtype=dtype)
+    leaves = [y.contiguous().to("mojo").requires_grad_() for y in x[:3]]
+    out = ops.sliding_window_attention(*leaves, 40, sinks=3)
+    out.backward(ones.to("mojo").expand(2, h, t, d))
+    want = window_cases.expected(*x[:3], torch.ones(2, h, t, d, dtype=dtype), 40, 3)
+    compare(dict(zip(("out", "dq", "dk", "dv"), (out, *(y.grad for y in leaves)))), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_hidden_numbers_stay_hidden(dtype):
+    """NaN in a row of keys and values reaches no query whose tiles lie elsewhere."""
+    x = window_cases.inputs(1, 2, 2, 400, 64, dtype)
+    want = window_cases.expected(*x, 30, 2)["out"]
+    k, v = x[1].clone(), x[2].clone()
+    k[:, :, 200] = float("nan")
+    v[:, :, 200] = float("nan")
+    out = ops.sliding_window_attention(x[0].to("mojo"), k.to("mojo"), v.to("mojo"), 30, sinks=2)
+    keep = torch.ones(400, dtype=torch.bool)
+    keep[128:320] = False  # rows that share a 64-key tile with key 200: 192 .. 255 + 30, in blocks of 128 queries
+    check(out.cpu()[:, :, keep], want[0][:, :, keep.numpy()], want[1][:, :, keep.numpy()])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (BF, 256), (HF, 128), (F32, 64), (F32, 96)])
+def test_captured_and_replayed(kernels, dtype, d):
+    """Forward and backward through the C entry points, in a graph whose inputs
+    change between the replays."""
+    import ctypes
+
+    from torch_mojo_backend.eager_kernels import check as ok
+
+    b, h, hk, t, window, sinks = 1, 4, 2, 700, 100, 4
+    code = {F32: 0, BF: 1, HF: 2}[dtype]
+    make = lambda n: torch.empty(b, t, n, d, dtype=dtype, device="cuda").transpose(1, 2)  # noqa: E731
+    q, k, v, do, o, dq, dk, dv = make(h), make(hk), make(hk), make(h), make(h), make(h), make(hk), make(hk)
+    lse = torch.empty(b, h, t, device="cuda")
+    ws = kernels.mi355x_attn_bwd_sink_workspace_bytes(b, h, hk, t, t, d, window, sinks)
+    hold = torch.empty(ws, dtype=torch.uint8, device="cuda")
+    st = lambda x: (ctypes.c_int64 * 3)(*x.stride()[:3])  # noqa: E731
+    at = lambda *xs: [y for x in xs for y in (x.data_ptr(), st(x))]  # noqa: E731
+
+    def step(stream):
+        ok("forward", kernels.mi355x_attn_fwd_sink(o.data_ptr(), st(o), lse.data_ptr(), *at(q, k, v), b, h, hk, t, t, d,
+                                                   d ** -0.5, window, sinks, code, stream))
+        ok("backward", kernels.mi355x_attn_bwd_sink(*at(dq, dk, dv, do, q, k, v, o), lse.data_ptr(), b, h, hk, t, t, d,
+                                                    d ** -0.5, window, sinks, code, hold.data_ptr(), ws, stream))
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    for x in (q, k, v, do):
+        x.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step(side.cuda_stream)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            step(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for seed in range(3):
+        x = window_cases.inputs(b, h, hk, t, d, dtype, seed=seed)
+        for dst, src in zip((q, k, v, do), x):
+            dst.copy_(src.cuda())
+        hold.fill_(255)  # what is left there is not used
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        compare({"out": o, "dq": dq, "dk": dk, "dv": dv}, window_cases.expected(*x, window, sinks))

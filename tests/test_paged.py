@@ -1,6 +1,8 @@
 """The paged cache off the GPU: the oracle, the plain formulas, the refusals,
 and the mojo path's argument packing over the stand-in of the library."""
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -221,3 +223,24 @@ def test_append_counts_as_a_write(device):
     before = c.k._version
     ops.paged_append(c, torch.zeros(1, 1, dtype=torch.int32).to(device), torch.zeros(1, dtype=torch.int32).to(device), x, x)
     assert c.k._version > before and float(c.k.cpu()[0, 0, 0].sum()) == 64
+
+
+def test_no_sequences(device):
+    c = Case([1], page=4, device=device, dtype=torch.float32)
+    table, none = torch.zeros(0, 3, dtype=torch.int32).to(device), c.ints([])
+    x = torch.zeros(0, 2, 5, 64).to(device)
+    assert ops.paged_append(c.cache, table, none, x, x) is None
+    assert ops.paged_attention(x, c.cache, table, none).shape == (0, 2, 5, 64)
+    assert ops.paged_gather(c.cache, table, none, 3)[1].shape == (0, 2, 3, 64)
+
+
+@pytest.mark.parametrize("bits", [None, 4])
+def test_a_copy_of_a_cache_is_its_own(device, bits):
+    c = PagedKVCache.zeros(2, 4, 1, 64, dtype=torch.float32, bits=bits, device=device)
+    other = type(c)(*(t.clone() for t in c.tensors)) if device == "mojo" else copy.deepcopy(c)
+    assert copy.copy(c).k is c.k
+    x = torch.ones(1, 1, 1, 64).to(device)
+    zero = torch.zeros(1, dtype=torch.int32).to(device)
+    ops.paged_append(other, zero.view(1, 1), zero, x, x)
+    assert (ops.paged_gather(c, zero.view(1, 1), zero, 1)[0].cpu() == 0).all()
+    assert (ops.paged_gather(other, zero.view(1, 1), zero, 1)[0].cpu() == 1).all()

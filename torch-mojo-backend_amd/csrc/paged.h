@@ -72,6 +72,12 @@ __device__ __forceinline__ int page_of(const PagedSeqs& s, int64_t b, uint32_t p
   return page;
 }
 
+// Rows [batch, heads, tokens, d] that can be read 16 bytes at a time.
+inline bool rows_ok(const void* p, const int64_t* bht, size_t es) {
+  return (uintptr_t)p % 16 == 0 && bht[0] * (int64_t)es % 16 == 0 && bht[1] * (int64_t)es % 16 == 0 &&
+         bht[2] * (int64_t)es % 16 == 0;
+}
+
 // Checks of the arguments that every entry point shares; fills `s`.
 int paged_args(const char* what, const mi355x_paged_cache* c, const int32_t* table, int64_t table_stride,
                int64_t table_width, const int32_t* starts, const int32_t* counts, int64_t batch, int64_t seq,

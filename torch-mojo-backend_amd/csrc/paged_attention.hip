@@ -256,7 +256,10 @@ extern "C" int mi355x_paged_attn(void* o, const int64_t* o_bht, const void* q, c
   MI_REQUIRE(isfinite(scale), "mi355x_paged_attn: scale must be finite");
   if (batch == 0 || seq == 0) return MI355X_OK;
   MI_REQUIRE(o && q, "mi355x_paged_attn: null pointer");
-  MI_REQUIRE(batch * heads * seq < (1ll << 24), "mi355x_paged_attn: batch x heads x tokens must be below 2^24");
+  MI_REQUIRE(rows_ok(q, q_bht, dtype_size(dtype)), "mi355x_paged_attn: rows of queries must be 16-byte aligned");
+  // (a launch has below 2^32 threads: a block a row below, 16 rows and more a block on matrix cores)
+  const int64_t most = paged_mfma_takes(*cache, dtype) ? 1ll << 31 : 1ll << 24;
+  MI_REQUIRE(batch * heads * seq < most, "mi355x_paged_attn: batch x heads x tokens must be below %lld", (long long)most);
   const int64_t need = mi355x_paged_attn_workspace_bytes(cache, table_width, batch, heads, seq, window, sinks, dtype);
   if (need && (!workspace || ws_bytes < need))
     return fail(MI355X_EWORKSPACE, "mi355x_paged_attn: workspace %lld < %lld", (long long)ws_bytes, (long long)need);

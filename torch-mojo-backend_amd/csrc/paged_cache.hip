@@ -408,12 +408,6 @@ __global__ void __launch_bounds__(kThreads) paged_gather_kernel(GatherArgs a) {
   *(Oct<T>*)((T*)w.p + b * w.b + hk * w.h + t * w.t + ch) = o;
 }
 
-// Rows of eight-channel pieces at 16-byte steps.
-bool rows_ok(const void* p, const int64_t* bht, size_t es) {
-  return (uintptr_t)p % 16 == 0 && bht[0] * (int64_t)es % 16 == 0 && bht[1] * (int64_t)es % 16 == 0 &&
-         bht[2] * (int64_t)es % 16 == 0;
-}
-
 template <typename T, typename RT, bool FOUR>
 int append_launch(const AppendArgs& a, hipStream_t s) {
   if (a.d % (FOUR ? 2 * kKvGroup : 16) == 0) {

@@ -30,7 +30,8 @@ class PagedKVCache:
     """Pages of keys and values: k, v [num_pages, kv_heads, page_size,
     head_dim] of a float dtype, or, with k_scales and v_scales [num_pages,
     kv_heads, page_size, head_dim / 32, 2] in float16, uint8 codes
-    [num_pages, kv_heads, page_size, head_dim / 2]."""
+    [num_pages, kv_heads, page_size, head_dim / 2].  The tensors are those it
+    was made with; a copy of the cache is made from copies of them."""
 
     def __init__(self, k, v, k_scales=None, v_scales=None):
         for name, t in (("k", k), ("v", v)):
@@ -83,6 +84,9 @@ class PagedKVCache:
             from .eager_kernels import paged
 
             self._desc = paged.describe(self)
+
+    def __reduce__(self):  # the kernels' description holds addresses
+        return type(self), (self.k, self.v, self.k_scales, self.v_scales)
 
     @property
     def device(self):
