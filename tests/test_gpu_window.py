@@ -190,3 +190,56 @@ def test_captured_and_replayed(kernels, dtype, d):
         graph.replay()
         torch.cuda.synchronize()
         compare({"out": o, "dq": dq, "dk": dk, "dv": dv}, window_cases.expected(*x, window, sinks))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128), (BF, 256), (F32, 64), (F32, 256), (F32, 40)])
+@pytest.mark.parametrize("sq,skv,window,sinks", [(300, 100, 50, 3), (300, 100, 50, 0), (90, 400, 30, 2), (1, 70, 5, 1)])
+def test_more_queries_or_more_keys(kernels, dtype, d, sq, skv, window, sinks):
+    """The C entry points take lengths that differ: queries that see nothing give
+    zeros, and so do the gradients of keys that nothing sees."""
+    import ctypes
+
+    import numpy as np
+
+    from paged_cases import np64
+    from torch_mojo_backend.eager_kernels import check as ok
+
+    n = max(sq, skv)
+    x = window_cases.inputs(1, 2, 1, n, d, dtype)
+    q, do = (y[:, :, :sq] for y in (x[0], x[3]))
+    k, v = (y[:, :, :skv] for y in x[1:3])
+    dev = [y.contiguous().cuda() for y in (q, k, v, do)]
+    o, dq, dk, dv = (torch.full_like(dev[i], float("nan")) for i in (0, 0, 1, 2))
+    lse = torch.empty(1, 2, sq, device="cuda")
+    st = lambda y: (ctypes.c_int64 * 3)(*y.stride()[:3])  # noqa: E731
+    at = lambda *ys: [z for y in ys for z in (y.data_ptr(), st(y))]  # noqa: E731
+    code = {F32: 0, BF: 1, HF: 2}[dtype]
+    ws = kernels.mi355x_attn_bwd_sink_workspace_bytes(1, 2, 1, sq, skv, d, window, sinks)
+    hold = torch.full((ws,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ok("forward", kernels.mi355x_attn_fwd_sink(o.data_ptr(), st(o), lse.data_ptr(), *at(*dev[:3]), 1, 2, 1, sq, skv, d,
+                                               d ** -0.5, window, sinks, code, None))
+    ok("backward", kernels.mi355x_attn_bwd_sink(*at(dq, dk, dv, dev[3], *dev[:3], o), lse.data_ptr(), 1, 2, 1, sq, skv, d,
+                                                d ** -0.5, window, sinks, code, hold.data_ptr(), ws, None))
+    torch.cuda.synchronize()
+    # the same with n queries and n keys, those that are not there without weight or gradient
+    qn, kn, vn, dn = (np64(y) for y in x)
+    dn[:, :, sq:] = 0
+    i, j = np.arange(n)[:, None], np.arange(n)[None]
+    seen = (j <= i) & ((i - j < window) | (j < sinks)) & (j < skv)
+    s = np.where(seen, d ** -0.5 * (qn @ kn.swapaxes(-1, -2)), -np.inf)
+    top = np.where(seen.any(-1), s.max(-1), 0.0)[..., None]
+    p = np.where(seen, np.exp(s - top), 0.0)
+    p = p / np.maximum(p.sum(-1, keepdims=True), 1e-300)
+    on = p @ vn
+    ds = p * (dn @ vn.swapaxes(-1, -2) - (dn * on).sum(-1, keepdims=True))
+    want = {"out": on[:, :, :sq], "dq": (d ** -0.5 * ds @ kn)[:, :, :sq],
+            "dk": (d ** -0.5 * ds.swapaxes(-1, -2) @ qn).sum(1, keepdims=True)[:, :, :skv],
+            "dv": (p.swapaxes(-1, -2) @ dn).sum(1, keepdims=True)[:, :, :skv]}
+    bound = window_cases.expected(*x, window, max(sinks, 1))
+    for name, got in (("out", o), ("dq", dq), ("dk", dk), ("dv", dv)):
+        assert torch.isfinite(got).all(), name
+        # at most the largest bound of the square case, whose sums have no fewer terms
+        check(got, want[name], np.full(want[name].shape, bound[name][1].max()), name)
+    empty = ~seen.any(-1)[:sq]
+    assert (np64(o)[:, :, empty] == 0).all() and (np64(dq)[:, :, empty] == 0).all()
