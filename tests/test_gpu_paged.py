@@ -127,6 +127,15 @@ def test_attention_over_a_long_sequence(dtype, bits, d):
     _attention(c, 4, [9000, 129], [1, 1], 1, dtype, window=4096, sinks=100)
 
 
+@pytest.mark.parametrize("d,h", [(64, 2), (128, 4), (256, 4), (64, 20), (128, 20)])
+@pytest.mark.parametrize("page", [16, 24])
+def test_f16_queries_over_4_bits_round_nothing_but_the_result(d, h, page):
+    c = Case([700, 90], page=page, bits=4, device="mojo", d=d, hk=1, dtype=HF)
+    c.bits = None  # the bound without a row's and a weight's rounding to f16
+    _attention(c, h, [697, 88], [3, 2], 3, HF)
+    _attention(c, h, [699, 89], [1, 1], 1, HF, window=100, sinks=3)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.4])
 def test_scale_of_any_sign(scale):
     c = Case([77], device="mojo", d=128)

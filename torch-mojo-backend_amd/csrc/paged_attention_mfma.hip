@@ -22,13 +22,20 @@
 // P is split in two halves of the pages' type, so its rounding (2^-8 in bf16)
 // does not show beside the result's; the second product costs nothing here.
 //
-// 4-bit rows are turned into f16 in registers, minimum + scale * code in one
-// rounding (2^-11): masked nibbles under f16's exponent of 1024, less 1024,
-// are the codes, two a register.  Queries go to f16 with their row's exponent
+// 4-bit rows are turned into f16 in registers: masked nibbles under f16's
+// exponent of 512, less 512, are half the codes, two a register.  For bf16
+// queries a value is minimum + 2 * scale * (code / 2) in one rounding and P one
+// f16 value: 2^-11 each, an eighth of the result's own step.  For f16 queries
+// these would be as large as that, so nothing is rounded: the scale is taken as
+// a sum of two numbers of 7 and 4 bits, whose products with a code fit f16, the
+// minimums have a product of their own (they are the same for the 8 channels
+// of a word), and P is split.  Queries go to f16 with their row's exponent
 // taken out, which keeps bf16's values as they are.
 //
 // Blocks split the keys of long sequences; paged_attn_join adds the parts.
 #include <math.h>
+
+#include <type_traits>
 
 #include "mfma.h"
 #include "paged_attention.h"
@@ -104,12 +111,22 @@ bool rows_close(const mi355x_paged_cache& c, int64_t es) {
 // ---------------------------------------------------------------------------
 // page formats
 // ---------------------------------------------------------------------------
+// What a format adds up beside o: nothing.
+struct NoRest {
+  template <int N>
+  __device__ __forceinline__ void scale(float (&)[N]) {}
+  template <typename O>
+  __device__ __forceinline__ void finish(O&) {}
+};
+
 // 16-bit pages of T.
 template <typename T, int D_>
 struct Pages16 {
-  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), kBytes = 2;
+  static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), kBytes = 2, kMore = 64;
   typedef typename Mfma<T>::frag frag;
   typedef uint32_t vword __attribute__((ext_vector_type(VW / 2)));
+  template <int QT>
+  using Rest = NoRest;
   struct Keys {
     frag k[KT][D / 32];
   };
@@ -175,7 +192,7 @@ struct Pages16 {
       }
   }
   template <int QT>
-  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], const Values& r, const f32x4 (&p)[KT][QT]) {
+  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], NoRest&, const Values& r, const f32x4 (&p)[KT][QT]) {
     frag hi[QT], lo[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
@@ -211,7 +228,9 @@ struct Pages16 {
 // the keys of a product step taken as 4 g + step, V's rows need no exchange.
 template <int D_>
 struct Pages32 {
-  static constexpr int D = D_, KT = 1, VW = 4, NU = D / 64, kBytes = 4;
+  static constexpr int D = D_, KT = 1, VW = 4, NU = D / 64, kBytes = 4, kMore = 64;
+  template <int QT>
+  using Rest = NoRest;
   struct Keys {
     f32x4 k[D / 16];
   };
@@ -266,7 +285,7 @@ struct Pages32 {
     }
   }
   template <int QT>
-  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], const Values& r, const f32x4 (&p)[KT][QT]) {
+  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], NoRest&, const Values& r, const f32x4 (&p)[KT][QT]) {
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -283,6 +302,8 @@ struct Pages32 {
 template <typename T, int D_>
 struct Pages4 {
   static constexpr int D = D_, KT = 2, VW = D >= 128 ? 8 : 4, NU = D / (16 * VW), NG = D / kKvGroup, kBytes = 1;
+  static constexpr bool EXACT = std::is_same_v<T, f16>;
+  static constexpr int kMore = EXACT ? 96 : 64;
   typedef f16x8 frag;
   typedef uint32_t row_words __attribute__((ext_vector_type(NG)));  // a lane's codes of a K row, or the row's scales
   struct Keys {
@@ -291,6 +312,27 @@ struct Pages4 {
   struct Values {
     uint32_t v[8][NU], vs[8][NU];
   };
+  // The minimums' share of O, by word; o has that of half the codes.
+  template <int QT>
+  struct Minimums {
+    f32x4 m[NU][QT] = {};
+    __device__ __forceinline__ void scale(float (&alpha)[QT]) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) m[u][qt] *= alpha[qt];
+    }
+    __device__ __forceinline__ void finish(f32x4 (&o)[NU][VW][QT]) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < VW; ++e)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) o[u][e][qt] = 2.f * o[u][e][qt] + m[u][qt];
+    }
+  };
+  template <int QT>
+  using Rest = std::conditional_t<EXACT, Minimums<QT>, NoRest>;
   struct Query {
     frag q[D / 32];
     float scale;
@@ -348,12 +390,15 @@ struct Pages4 {
 #pragma unroll
         for (int u = 0; u < NU; ++u) r.vs[i][u] = 0;
   }
-  // Nibble i of both halves of w under the scales and minimums of s and m.
-  // `mask` is 0x000f000f in a vector register: an instruction takes one
-  // constant from elsewhere, and two make it an AND and an OR.
-  static __device__ __forceinline__ f16x2 value(uint32_t w, int i, uint32_t mask, f16x2 s, f16x2 m) {
-    const f16x2 c = __builtin_bit_cast(f16x2, (w >> (4 * i) & mask) | 0x64006400u) - (f16)1024.f;
-    return __builtin_elementwise_fma(c, s, m);
+  // Half the codes of nibble i of both halves of w.  `mask` is 0x000f000f in a
+  // vector register: an instruction takes one constant from elsewhere, and two
+  // make it an AND and an OR.
+  static __device__ __forceinline__ f16x2 half_codes(uint32_t w, int i, uint32_t mask) {
+    return __builtin_bit_cast(f16x2, (w >> (4 * i) & mask) | 0x60006000u) - (f16)512.f;
+  }
+  // s as a number of 7 bits, whose product with half a code is exact, and the rest
+  static __device__ __forceinline__ f16x2 upper(f16x2 s) {
+    return __builtin_bit_cast(f16x2, __builtin_bit_cast(uint32_t, s) & 0xfff0fff0u);
   }
   static __device__ __forceinline__ uint32_t nibbles() {
     uint32_t mask;
@@ -365,37 +410,70 @@ struct Pages4 {
     const uint32_t mask = nibbles();
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
+      f32x4 low[QT];  // EXACT: the minimums' share
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) s[kt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int qt = 0; qt < QT; ++qt) s[kt][qt] = low[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < NG; ++ks) {
         const f16x2 sm = __builtin_bit_cast(f16x2, (uint32_t)r.ks[kt][ks]);
+        const f16x2 sc = f16x2{sm[0], sm[0]}, mn = f16x2{sm[1], sm[1]};
         union {
           f16x2 h[4];
           frag f;
-        } k;
+        } k, rest, m;
+        if constexpr (EXACT) {
+          const f16x2 up = upper(sc), down = sc - up;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k.h[i] = value(r.k[kt][ks], i, mask, f16x2{sm[0], sm[0]}, f16x2{sm[1], sm[1]});
+          for (int i = 0; i < 4; ++i) {
+            const f16x2 c = half_codes(r.k[kt][ks], i, mask);
+            k.h[i] = c * up, rest.h[i] = c * down, m.h[i] = mn;
+          }
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) s[kt][qt] = Mfma<f16>::mma(k.f, q[qt].q[ks], s[kt][qt]);
+          for (int qt = 0; qt < QT; ++qt) {
+            s[kt][qt] = Mfma<f16>::mma(k.f, q[qt].q[ks], s[kt][qt]);
+            s[kt][qt] = Mfma<f16>::mma(rest.f, q[qt].q[ks], s[kt][qt]);
+            low[qt] = Mfma<f16>::mma(m.f, q[qt].q[ks], low[qt]);
+          }
+        } else {
+          const f16x2 sc2 = sc + sc;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k.h[i] = __builtin_elementwise_fma(half_codes(r.k[kt][ks], i, mask), sc2, mn);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[kt][qt] = Mfma<f16>::mma(k.f, q[qt].q[ks], s[kt][qt]);
+        }
       }
+      if constexpr (EXACT)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[kt][qt] = 2.f * s[kt][qt] + low[qt];
     }
   }
   template <int QT>
-  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], const Values& r, const f32x4 (&p)[KT][QT]) {
-    frag pf[QT];
+  static __device__ __forceinline__ void add_values(f32x4 (&o)[NU][VW][QT], Rest<QT>& rest, const Values& r, const f32x4 (&p)[KT][QT]) {
+    frag hi[QT], lo[QT];  // lo: EXACT alone
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pf[qt][4 * kt + e] = (f16)p[kt][qt][e];
+        for (int e = 0; e < 4; ++e) {
+          const f16 h = (f16)p[kt][qt][e];
+          hi[qt][4 * kt + e] = h;
+          if (EXACT) lo[qt][4 * kt + e] = (f16)(p[kt][qt][e] - (float)h);
+        }
     const uint32_t mask = nibbles();
     const bool odd = D < 128 && (threadIdx.x & 8);
+    auto add = [&](f32x4& x, frag v, int qt) {
+      x = Mfma<f16>::mma(v, hi[qt], x);
+      if (EXACT) x = Mfma<f16>::mma(v, lo[qt], x);
+    };
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       uint32_t even_w[4], odd_w[4];  // words of two keys: their even, their odd channels
-      f16x2 s[4], m[4];
+      f16x2 s[4], down[4];
+      union {
+        f16x2 h[4];
+        frag f;
+      } m;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a = r.v[2 * i][u], b = r.v[2 * i + 1][u], x = r.vs[2 * i][u], y = r.vs[2 * i + 1][u];
@@ -403,19 +481,30 @@ struct Pages4 {
         odd_w[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         if (odd) even_w[i] = odd_w[i];
         s[i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(y, x, 0x05040100u));
-        m[i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(y, x, 0x07060302u));
+        m.h[i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(y, x, 0x07060302u));
+        if constexpr (EXACT) down[i] = s[i] - upper(s[i]), s[i] = upper(s[i]);
+        else s[i] = s[i] + s[i];
       }
+      if constexpr (EXACT)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) add(rest.m[u][qt], m.f, qt);
 #pragma unroll
       for (int e = 0; e < VW; ++e) {
         union {
           f16x2 h[4];
           frag f;
-        } v;
+        } v, w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v.h[i] = D >= 128 ? value(e % 2 ? odd_w[i] : even_w[i], e / 2, mask, s[i], m[i]) : value(even_w[i], e, mask, s[i], m[i]);
+        for (int i = 0; i < 4; ++i) {
+          const f16x2 c = D >= 128 ? half_codes(e % 2 ? odd_w[i] : even_w[i], e / 2, mask) : half_codes(even_w[i], e, mask);
+          if constexpr (EXACT) v.h[i] = c * s[i], w.h[i] = c * down[i];
+          else v.h[i] = __builtin_elementwise_fma(c, s[i], m.h[i]);
+        }
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[u][e][qt] = Mfma<f16>::mma(v.f, pf[qt], o[u][e][qt]);
+        for (int qt = 0; qt < QT; ++qt) {
+          add(o[u][e][qt], v.f, qt);
+          if constexpr (EXACT) add(o[u][e][qt], w.f, qt);
+        }
       }
     }
   }
@@ -423,11 +512,11 @@ struct Pages4 {
 
 // ---------------------------------------------------------------------------
 // Waves of a SIMD that the registers are shared out to: what keys, values,
-// queries and output take, and 64 more.
+// queries and output take, and some more.
 template <typename F, int QT>
 constexpr int waves_of() {
   const int regs = (int)(sizeof(typename F::Keys) + sizeof(typename F::Values)) / 4 +
-                   QT * ((int)sizeof(typename F::Query) / 4 + F::D / 4) + 64;
+                   QT * ((int)sizeof(typename F::Query) / 4 + F::D / 4) + F::kMore;
   return regs <= 128 ? 4 : regs <= 168 ? 3 : regs <= 256 ? 2 : 1;
 }
 
@@ -489,6 +578,7 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
   };
   float m[QT], l[QT];
   f32x4 o[NU][VW][QT];
+  typename F::template Rest<QT> rest;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     m[qt] = -INFINITY, l[qt] = 0.f;
@@ -544,16 +634,18 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
       moved |= top[qt] > m[qt];
     }
     if (__builtin_amdgcn_ballot_w64(moved)) {
+      float alpha[QT];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        const float alpha = top[qt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[qt] - top[qt]);
-        l[qt] *= alpha;
+        alpha[qt] = top[qt] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[qt] - top[qt]);
+        l[qt] *= alpha[qt];
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int e = 0; e < VW; ++e) o[u][e][qt] *= alpha;
+          for (int e = 0; e < VW; ++e) o[u][e][qt] *= alpha[qt];
         m[qt] = top[qt];
       }
+      rest.scale(alpha);
     }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -570,13 +662,15 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
         }
     }
     if (!whole) F::hide_values(values, live, g);
-    F::add_values(o, values, s);
+    F::add_values(o, rest, values, s);
     if (more) {
       F::template load_values<P16>(values, rows_of, next, lr, g);
       here = next;
       if (i + 2 * NW < end) next = look_up(i + 2 * NW);
     }
   }
+
+  rest.finish(o);
 
   // join the waves
 #pragma unroll
