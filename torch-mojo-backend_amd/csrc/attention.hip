@@ -1431,6 +1431,11 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_b
 // rounds.  Blocks of one head stand side by side on an XCD (they read the same
 // rows): the hardware deals blocks to the 8 in turn, and each takes a
 // contiguous run of a kind.
+// bf16, [1, 12, 8192, 64], window 1024, 4 sinks: 136 us and 8 for D, 5.5 for the
+// sums, 430 TFLOP/s of the pairs seen.  [1, 4 over 1, 4096, 256], window 512: 85,
+// 6 and 12.7 us, 200 TFLOP/s; there a block takes a CU and a wave a SIMD, whose
+// waits for LDS are bare (the matrix units are busy a seventh of the time).
+// Eight waves that split a step's channels or its queries' tiles took 80 to 95.
 // 16-row tiles of a wave: two, or one of keys at head_dim 256, where the dK and
 // dV of two would take all of its registers.
 template <int D>

@@ -33,6 +33,13 @@
 // taken out, which keeps bf16's values as they are.
 //
 // Blocks split the keys of long sequences; paged_attn_join adds the parts.
+//
+// 32 sequences of up to 16384 keys, 32 query heads over 8 of 128: 275 us in
+// bf16, 5.6 TB/s, as fast as memory is read here by anything.  In 4 bits 139 us,
+// 3.8 TB/s: turning the codes takes 57% of the issue slots and the waits on the
+// lookups and loads of a tile most of the rest (164 us with f16 queries).  One
+// token over 516 keys of 4 heads over 1 of 256, bf16: 9.9 us, of which a tile of
+// 32 keys is 2; over 8191 in 4 bits 9.7.
 #include <math.h>
 
 #include <type_traits>
