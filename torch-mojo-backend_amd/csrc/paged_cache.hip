@@ -188,10 +188,10 @@ __device__ __forceinline__ bool place_of(const AppendArgs& a, int64_t b, int64_t
 // kHeads rows of one token and of one kind (query, key or value, the same for
 // a block): the angles are read once for all of them, and their loads are all
 // in flight before the first is used.  Four prompts of 2048 tokens, 16 query
-// and 8 K/V heads of 128, into 4 bits (111 MB): one row a thread 38.7 us, whose
-// waves are too short to hide the lookup of their page, two 42.4, four 36.8;
-// the f64 rotation of the keys and the packing bound it, the copy alone would
-// take 23.  Five of 333 into f32 pages (41 MB) 6.2 us, one token 3.0, a launch.
+// and 8 K/V heads of 128 at most, into 4 bits (89 MB): one row a thread 38.7 us,
+// whose waves are too short to hide the lookup of their page, two 42.4, four
+// 36.8; the f64 rotation of the keys and the packing bound it, a copy would take
+// 17.  Five of 333 at most into f32 pages (13 MB) 6.2 us, one token 3.0, a launch.
 constexpr int kHeads = 4;
 
 template <typename T, typename RT, bool FOUR>
@@ -364,7 +364,7 @@ struct GatherArgs {
 };
 
 // Eight channels a thread, bound by the bytes written: the rows of the prompts
-// above from 4 bits to f32, 77 MB, in 17.5 us.
+// above from 4 bits to f32, 61 MB, in 17.5 us.
 // T: the type of the values written; CT: of the pages (uint8_t: 4 bits).
 template <typename T, typename CT>
 __global__ void __launch_bounds__(kThreads) paged_gather_kernel(GatherArgs a) {
