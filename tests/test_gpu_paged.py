@@ -205,6 +205,30 @@ def test_pages_out_of_range_are_left_out():
     x.cpu()  # the flag is cleared
 
 
+@pytest.mark.parametrize("dtype,bits,d,n", [(BF, None, 64, 1), (F32, None, 128, 40), (HF, 4, 256, 1), (BF, None, 96, 1),
+                                            (BF, 4, 64, 700), (BF, None, 96, 700)])
+def test_visible_nan_is_seen(dtype, bits, d, n):
+    """A sequence whose keys are NaN answers NaN, and its neighbour does not."""
+    c = Case([n, n], page=16, bits=bits, device="mojo", d=d, hk=1, dtype=dtype)
+    nan = torch.full((1, 1, n, d), float("nan"), dtype=dtype).to("mojo")
+    tab = c.dev_table[:1]
+    _, v = ops.paged_gather(c.cache, tab, c.ints([0]), n, dtype=dtype)
+    ops.paged_append(c.cache, tab, c.ints([0]), nan, v)
+    q = c.queries(2, 1, dtype)
+    out = ops.paged_attention(q.to("mojo"), c.cache, c.dev_table, c.ints([n - 1, n - 1])).cpu()
+    assert torch.isnan(out[0]).all()
+    want, bound = c.expected(q, [0, n - 1], [0, 1])
+    check(out[1:], want[1:], bound[1:])
+
+
+def test_windows_past_every_position():
+    c = Case([77], device="mojo", d=64)
+    q = c.queries(4, 2)
+    want = c.expected(q, [75], [2])
+    for window, sinks in ((2 ** 31, 0), (2 ** 70, 2 ** 70), (3, 2 ** 40)):
+        check(ops.paged_attention(q.to("mojo"), c.cache, c.dev_table, c.ints([75]), window=window, sinks=sinks), *want)
+
+
 def test_shared_pages_and_repeated_results():
     """Sequences with a common prefix read the same pages; a call repeated gives the same bits."""
     c = Case([64, 64], page=16, device="mojo", d=128, hk=2)

@@ -548,6 +548,7 @@ int run_window_fwd(const AttnF32& p, hipStream_t s) {
   static const bool ok = opt_in((const void*)fwd_f32<D, true>, lds_bytes<D>(false));
   if (!ok) return fail(MI355X_ELAUNCH, "mi355x_attn_fwd_sink: cannot reserve %zu bytes of LDS", lds_bytes<D>(false));
   const uint32_t nblk = ceil_div(p.Sq, kBlk);
+  MI_REQUIRE(nblk * p.B * p.H < (1ll << 24), "mi355x_attn_fwd_sink: too many blocks");
   fwd_f32<D, true><<<(unsigned)(nblk * p.B * p.H), kNT, lds_bytes<D>(false), s>>>(p, nblk);
   return check_launch("mi355x_attn_fwd_sink");
 }

@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_rows(DecodeArgs a) {
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off, 64);
     s *= a.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn), p = mn == -INFINITY ? 0.f : exp2f(s - mn);
+    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;  // of a NaN score: m, and p is NaN
+    const float alpha = exp2f(m - ref), p = exp2f(s - ref);
     l = l * alpha + p;
     m = mn;
 #pragma unroll
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join(DecodeArgs a) {
   const uint32_t row = blockIdx.x;
   const float2 ml = lane < a.splits ? a.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.f);
   const float mx = wave_max(ml.x);
-  const float w = mx == -INFINITY ? 0.f : exp2f(ml.x - mx);
+  const float w = mx == -INFINITY ? 1.f : exp2f(ml.x - mx);  // sums of 0, or of NaN
   const float total = wave_sum(w * ml.y);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kEach = 16;  // of 64 splits to a wave; all of their loads in flight

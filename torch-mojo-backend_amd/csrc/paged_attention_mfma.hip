@@ -692,7 +692,8 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
     float mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w][qt * 16 + lr]);
-    const float mine = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[qt] - mx);
+    // (rows without a maximum have sums of 0, or of NaN)
+    const float mine = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[qt] - mx);
     // the row that this thread stores, and its sum
     const int sr = threadIdx.x >> 4, c = threadIdx.x & 15;
     const int r = r0 + qt * 16 + sr, t = r / a.group, h = (int)hk * a.group + r - t * a.group;
@@ -701,10 +702,10 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
     for (int w = 0; w < NW; ++w) smx = fmaxf(smx, sm[w][qt * 16 + sr]);
 #pragma unroll
     for (int w = 0; w < NW; ++w)
-      sum += smx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[w][qt * 16 + sr] - smx) * sl[w][qt * 16 + sr];
+      sum += smx == -INFINITY ? sl[w][qt * 16 + sr] : __builtin_amdgcn_exp2f(sm[w][qt * 16 + sr] - smx) * sl[w][qt * 16 + sr];
     // padding took part where tiles were whole: it leaves nothing
-    if (t >= count || start + t < 0 || start + t > kMaxPosition) smx = -INFINITY, sum = 0.f;
-    const bool none = smx == -INFINITY;
+    const bool none = t >= count || start + t < 0 || start + t > kMaxPosition;
+    if (none) smx = -INFINITY, sum = 0.f;
     const int64_t row = (b * a.heads + h) * a.seq + t;
     if (a.splits > 1 && r < rows && c == 0) a.part_ml[split * total_rows + row] = make_float2(smx, sum);
     const float inv = a.splits > 1 ? 1.f : (sum != 0.f ? 1.f / sum : 0.f);

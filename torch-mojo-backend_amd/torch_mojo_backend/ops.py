@@ -130,6 +130,8 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
                                       " (float32, bfloat16, float16, head_dim up to 256)")
         if t <= window:
             window, sinks = 0, None  # plain causal attention
+        else:
+            sinks = min(sinks, t)
         if not _needs_grad(q, k, v):
             materialize_touched((q, k, v), None, False)
             return aten_fast.attention_forward(q, k, v, True, window, scale, sinks)[0]
@@ -265,7 +267,7 @@ def paged_attention(q, cache, page_table, starts, *, counts=None, window=0, sink
     0 * NaN does in the plain formula."""
     if (paged.seqs_ok(cache, page_table, starts, counts) and paged.rows_ok(cache, q, page_table._shape[0])
             and q._shape[1] and q._shape[1] % cache.kv_heads == 0 and type(window) is type(sinks) is int
-            and window >= 0 and sinks >= 0 and scale is None):
+            and 0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31 and scale is None):
         return paged.attention(q, cache, page_table, starts, counts, window, sinks, cache.scale)
     what = "paged_attention"
     if q.dim() != 4:
@@ -277,6 +279,7 @@ def paged_attention(q, cache, page_table, starts, *, counts=None, window=0, sink
     window, sinks = int(window), int(sinks)
     if window < 0 or sinks < 0:
         raise ValueError(f"{what}: window {window} and sinks {sinks} must not be negative")
+    window, sinks = min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)  # past every position
     scale = cache.scale if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what}: scale {scale} must be finite")
