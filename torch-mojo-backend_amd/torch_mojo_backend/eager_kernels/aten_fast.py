@@ -2181,8 +2181,8 @@ def _unit_head_stride(t: MT) -> MT:
 def alloc_bthd(b, h, s, d, dtype, device) -> MT:
     """[B,H,S,D] view over dense [B,S,H,D] storage (aten_fast.py:7433-7459):
     `out.transpose(1, 2)` is then a free contiguous [B,S,H,D]."""
-    dense = _alloc((b, s, h, d), dtype, device)
-    return MT._view_of(dense, (b, h, s, d), (s * h * d, d, h * d, 1), 0)
+    holder = _alloc_bytes(b * h * s * d * dtype.itemsize, device)
+    return MT._make(holder, holder.data_ptr(), (b, h, s, d), (s * h * d, d, h * d, 1), 0, dtype, device)
 
 
 def _mfma_fwd_ok(q: MT, group, window) -> bool:

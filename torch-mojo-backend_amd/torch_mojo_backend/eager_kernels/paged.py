@@ -14,7 +14,7 @@ import torch
 
 from . import PagedCache, check, lazy_live, materialize_touched
 from . import native_lib as lib
-from .aten_fast import _PAGE_ERROR, _STREAM, _code, _error_slot, _workspace, materialize_contiguous
+from .aten_fast import _PAGE_ERROR, _STREAM, _code, _error_slot, _workspace, alloc_bthd, materialize_contiguous
 from ..mojo_device import torch_mojo_tensor as _tensor_mod
 
 MT = _tensor_mod.TorchMojoTensor
@@ -80,12 +80,6 @@ def _rows(t: MT) -> MT:
     return materialize_contiguous(t)
 
 
-def _heads_out(b, h, t, d, dtype, device) -> MT:
-    """A new [b, h, t, d] view of dense [b, t, h, d] storage."""
-    holder = _tensor_mod._alloc_bytes(b * h * t * d * dtype.itemsize, device)
-    return MT._make(holder, holder.data_ptr(), (b, h, t, d), (t * h * d, d, h * d, 1), 0, dtype, device)
-
-
 def _bht(t: MT):
     return t._strides[:3]
 
@@ -110,7 +104,7 @@ def _append(cache, table, starts, k, v, cos, sin, q, counts, dev):
     heads = 0
     if q is not None:
         q, heads = _rows(q), q._shape[1]
-        out = _heads_out(b, heads, t, d, q._dtype, dev)
+        out = alloc_bthd(b, heads, t, d, q._dtype, dev)
         q_args = out._ptr, _bht(out), q._ptr, _bht(q)
     if cos is not None:
         cos, sin = (x if x._is_contiguous and x._ptr % 16 == 0 else materialize_contiguous(x) for x in (cos, sin))
@@ -131,7 +125,7 @@ def gather(cache, table, starts, length, counts, dtype):
 
 def _gather(cache, table, starts, length, counts, dtype, dev):
     b = table._shape[0]
-    k, v = (_heads_out(b, cache.kv_heads, length, cache.head_dim, dtype, dev) for _ in range(2))
+    k, v = (alloc_bthd(b, cache.kv_heads, length, cache.head_dim, dtype, dev) for _ in range(2))
     check(
         "mi355x_paged_gather",
         lib().mi355x_paged_gather(k._ptr, _bht(k), v._ptr, _bht(v), cache._desc, *_seqs(table, starts, counts),
@@ -150,7 +144,7 @@ def _attention(q, cache, table, starts, counts, window, sinks, scale, dev):
     b, h, t, d = q._shape
     q = _rows(q)
     code = _code(q._dtype)
-    out = _heads_out(b, h, t, d, q._dtype, dev)
+    out = alloc_bthd(b, h, t, d, q._dtype, dev)
     library = lib()
     ws = library.mi355x_paged_attn_workspace_bytes(cache._desc, table._shape[1], b, h, t, window, sinks, code)
     hold, wptr = _workspace(ws, dev)
