@@ -613,8 +613,10 @@ int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
  * heads as in mi355x_attn_fwd_gen / mi355x_attn_bwd_gen.  Training with the
  * first tokens left visible, as a model that is served with a window needs;
  * the reference runs such a mask through its masked-math decomposition
- * (aten_fast.py:9112-9123). */
-int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, const void* q,
+ * (aten_fast.py:9112-9123).  o_low may be null, or of o's type and strides: the
+ * forward leaves there what rounding took from o, and the backward takes the
+ * row terms dO . O from both (in f32 it is left alone). */
+int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, void* o_low, float* lse, const void* q,
                          const int64_t* q_bhs, const void* k, const int64_t* k_bhs,
                          const void* v, const int64_t* v_bhs, int64_t batch, int64_t heads,
                          int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
@@ -629,7 +631,7 @@ int mi355x_attn_bwd_sink(void* dq, const int64_t* dq_bhs, void* dk, const int64_
                          const int64_t* do_bhs, const void* q, const int64_t* q_bhs,
                          const void* k, const int64_t* k_bhs, const void* v,
                          const int64_t* v_bhs, const void* o, const int64_t* o_bhs,
-                         const float* lse, int64_t batch, int64_t heads, int64_t kv_heads,
+                         const void* o_low, const float* lse, int64_t batch, int64_t heads, int64_t kv_heads,
                          int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
                          int64_t sinks, int dtype, void* workspace, int64_t ws_bytes,
                          mi355x_stream_t stream);

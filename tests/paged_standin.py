@@ -88,7 +88,7 @@ HostStandIn.mi355x_paged_attn = _attn
 HostStandIn.mi355x_paged_attn_workspace_bytes = lambda self, *a: 64
 
 
-def _attn_fwd_sink(self, o, o_bhs, lse, q, q_bhs, k, k_bhs, v, v_bhs, b, h, hk, sq, skv, d, scale, window, sinks, dt,
+def _attn_fwd_sink(self, o, o_bhs, o_low, lse, q, q_bhs, k, k_bhs, v, v_bhs, b, h, hk, sq, skv, d, scale, window, sinks, dt,
                    stream):
     qq = _rows(q, DT[dt], (b, h, sq, d), q_bhs).float()
     kk, vv = (_rows(p, DT[dt], (b, hk, skv, d), s).float().repeat_interleave(h // hk, 1)
@@ -96,20 +96,24 @@ def _attn_fwd_sink(self, o, o_bhs, lse, q, q_bhs, k, k_bhs, v, v_bhs, b, h, hk, 
     i, j = torch.arange(sq)[:, None], torch.arange(skv)[None, :]
     s = (qq @ kk.mT * scale).masked_fill((j > i) | ((i - j >= window) & (j >= sinks)), float("-inf"))
     view(_val(lse), torch.float32, (b, h, sq), (h * sq, sq, 1)).copy_(torch.logsumexp(s, -1))
-    _rows(o, DT[dt], (b, h, sq, d), o_bhs).copy_(torch.softmax(s, -1) @ vv)
+    x, oo = torch.softmax(s, -1) @ vv, _rows(o, DT[dt], (b, h, sq, d), o_bhs)
+    oo.copy_(x)
+    if _val(o_low):
+        _rows(o_low, DT[dt], (b, h, sq, d), o_bhs).copy_(x - oo.float())
     return 0
 
 
-def _attn_bwd_sink(self, dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, do, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
-                   b, h, hk, sq, skv, d, scale, window, sinks, dt, ws, nws, stream):
+def _attn_bwd_sink(self, dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, do, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, o_low,
+                   lse, b, h, hk, sq, skv, d, scale, window, sinks, dt, ws, nws, stream):
     assert ws and nws >= 64
+    low = _rows(o_low, DT[dt], (b, h, sq, d), o_bhs).float() if _val(o_low) else 0.0
     qq, gg, oo = (_rows(p, DT[dt], (b, h, sq, d), s).float() for p, s in ((q, q_bhs), (do, do_bhs), (o, o_bhs)))
     kk, vv = (_rows(p, DT[dt], (b, hk, skv, d), s).float().repeat_interleave(h // hk, 1)
               for p, s in ((k, k_bhs), (v, v_bhs)))
     i, j = torch.arange(sq)[:, None], torch.arange(skv)[None, :]
     s = (qq @ kk.mT * scale).masked_fill((j > i) | ((i - j >= window) & (j >= sinks)), float("-inf"))
     p = torch.exp(s - view(_val(lse), torch.float32, (b, h, sq, 1), (h * sq, sq, 1, 1)))
-    ds = p * (gg @ vv.mT - (gg * oo).sum(-1, keepdim=True)) * scale
+    ds = p * (gg @ vv.mT - (gg * (oo + low)).sum(-1, keepdim=True)) * scale
     grads = (ds @ kk, *(x.reshape(b, hk, h // hk, skv, d).sum(2) for x in (ds.mT @ qq, p.mT @ gg)))
     for p, s, x in zip((dq, dk, dv), (dq_bhs, dk_bhs, dv_bhs), grads):
         _rows(p, DT[dt], tuple(x.shape), s).copy_(x)

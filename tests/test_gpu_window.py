@@ -159,6 +159,7 @@ def test_captured_and_replayed(kernels, dtype, d):
     code = {F32: 0, BF: 1, HF: 2}[dtype]
     make = lambda n: torch.empty(b, t, n, d, dtype=dtype, device="cuda").transpose(1, 2)  # noqa: E731
     q, k, v, do, o, dq, dk, dv = make(h), make(hk), make(hk), make(h), make(h), make(h), make(hk), make(hk)
+    low = torch.full_like(o, float("nan"))
     lse = torch.empty(b, h, t, device="cuda")
     ws = kernels.mi355x_attn_bwd_sink_workspace_bytes(b, h, hk, t, t, d, window, sinks)
     hold = torch.empty(ws, dtype=torch.uint8, device="cuda")
@@ -166,9 +167,9 @@ def test_captured_and_replayed(kernels, dtype, d):
     at = lambda *xs: [y for x in xs for y in (x.data_ptr(), st(x))]  # noqa: E731
 
     def step(stream):
-        ok("forward", kernels.mi355x_attn_fwd_sink(o.data_ptr(), st(o), lse.data_ptr(), *at(q, k, v), b, h, hk, t, t, d,
+        ok("forward", kernels.mi355x_attn_fwd_sink(o.data_ptr(), st(o), low.data_ptr(), lse.data_ptr(), *at(q, k, v), b, h, hk, t, t, d,
                                                    d ** -0.5, window, sinks, code, stream))
-        ok("backward", kernels.mi355x_attn_bwd_sink(*at(dq, dk, dv, do, q, k, v, o), lse.data_ptr(), b, h, hk, t, t, d,
+        ok("backward", kernels.mi355x_attn_bwd_sink(*at(dq, dk, dv, do, q, k, v, o), low.data_ptr(), lse.data_ptr(), b, h, hk, t, t, d,
                                                     d ** -0.5, window, sinks, code, hold.data_ptr(), ws, stream))
 
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
@@ -217,9 +218,9 @@ def test_more_queries_or_more_keys(kernels, dtype, d, sq, skv, window, sinks):
     ws = kernels.mi355x_attn_bwd_sink_workspace_bytes(1, 2, 1, sq, skv, d, window, sinks)
     hold = torch.full((ws,), 255, dtype=torch.uint8, device="cuda")
     torch.cuda.synchronize()
-    ok("forward", kernels.mi355x_attn_fwd_sink(o.data_ptr(), st(o), lse.data_ptr(), *at(*dev[:3]), 1, 2, 1, sq, skv, d,
+    ok("forward", kernels.mi355x_attn_fwd_sink(o.data_ptr(), st(o), None, lse.data_ptr(), *at(*dev[:3]), 1, 2, 1, sq, skv, d,
                                                d ** -0.5, window, sinks, code, None))
-    ok("backward", kernels.mi355x_attn_bwd_sink(*at(dq, dk, dv, dev[3], *dev[:3], o), lse.data_ptr(), 1, 2, 1, sq, skv, d,
+    ok("backward", kernels.mi355x_attn_bwd_sink(*at(dq, dk, dv, dev[3], *dev[:3], o), None, lse.data_ptr(), 1, 2, 1, sq, skv, d,
                                                 d ** -0.5, window, sinks, code, hold.data_ptr(), ws, None))
     torch.cuda.synchronize()
     # the same with n queries and n keys, those that are not there without weight or gradient
@@ -243,3 +244,25 @@ def test_more_queries_or_more_keys(kernels, dtype, d, sq, skv, window, sinks):
         check(got, want[name], np.full(want[name].shape, bound[name][1].max()), name)
     empty = ~seen.any(-1)[:sq]
     assert (np64(o)[:, :, empty] == 0).all() and (np64(dq)[:, :, empty] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128), (BF, 256), (BF, 96)])
+def test_what_rounding_takes_from_the_output_is_kept(dtype, d):
+    """Two visible keys a query: dP - D is a small difference, and D from the
+    rounded output alone makes dQ and dK worse."""
+    from paged_cases import np64
+    from torch_mojo_backend.eager_kernels import aten_fast
+
+    x = window_cases.inputs(1, 2, 2, 300, d, dtype)
+    want = window_cases.expected(*x, 1, 1)
+    q, k, v, do = (y.to("mojo") for y in x)
+    errors = []
+    for low in (None, aten_fast.alloc_bthd(1, 2, 300, d, dtype, q._device)):
+        out, lse = aten_fast.attention_forward(q, k, v, True, 1, None, 1, low)
+        dq, dk, _ = aten_fast.attention_backward(do, q, k, v, out, lse, True, 1, None, 1, low)
+        errors.append([abs(np64(g) - want[n][0]).sum() for g, n in ((dq, "dq"), (dk, "dk"))])
+        if low is not None:  # of half a step of the output at most
+            assert (abs(np64(low)) <= window_cases.STEP[dtype] * abs(np64(out)) + 2.0 ** -25).all()
+            both = np64(out) + np64(low)
+            assert abs(both - want["out"][0]).sum() < abs(np64(out) - want["out"][0]).sum()
+    assert all(kept < 0.85 * alone for alone, kept in zip(*errors)), errors

@@ -119,13 +119,13 @@ def test_windows_that_are_refused(lib):
     s = bht(64 * 64, 64, 64)
 
     def fwd(**over):
-        a = dict(o=P, os=s, lse=P, q=P, qs=s, k=P, ks=s, v=P, vs=s, batch=1, heads=2, hk=2, sq=64, skv=64, d=64, scale=0.1,
+        a = dict(o=P, os=s, low=None, lse=P, q=P, qs=s, k=P, ks=s, v=P, vs=s, batch=1, heads=2, hk=2, sq=64, skv=64, d=64, scale=0.1,
                  window=8, sinks=1, dtype=BF16, stream=None)
         assert not set(over) - set(a)
         return lib.mi355x_attn_fwd_sink(*{**a, **over}.values())
 
     def bwd(ws=None, **over):
-        a = dict(dq=P, dqs=s, dk=P, dks=s, dv=P, dvs=s, do=P, dos=s, q=P, qs=s, k=P, ks=s, v=P, vs=s, o=P, os=s, lse=P, batch=1,
+        a = dict(dq=P, dqs=s, dk=P, dks=s, dv=P, dvs=s, do=P, dos=s, q=P, qs=s, k=P, ks=s, v=P, vs=s, o=P, os=s, low=None, lse=P, batch=1,
                  heads=2, hk=2, sq=64, skv=64, d=64, scale=0.1, window=8, sinks=1, dtype=BF16, ws=ws, wsb=0, stream=None)
         assert not set(over) - set(a)
         return lib.mi355x_attn_bwd_sink(*{**a, **over}.values())

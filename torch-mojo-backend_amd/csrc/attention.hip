@@ -477,7 +477,8 @@ constexpr float kSlack = 8.f;
 // 512: 52 -> 36 us; 16 queries a wave in twice the blocks 39).
 // At 256, where two stages of K and V leave room for one block a CU, KH = 2 has
 // the same from eight waves: each half of them takes half of a tile's keys, and
-// they join at the end ([1, 4 over 1, 4096, 256], window 512: 31 -> 25 us).
+// they join at the end ([1, 4 over 1, 4096, 256], window 512: 31 -> 25 us, and 3
+// more where o_low is kept).
 template <typename T, int D, bool POS, int NW, int QPW, bool SINK = false, int KH = 1>
 __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : SINK && D == 128 && POS ? 2 : 1) attn_fwd_v2(AttnArgs p) {
   constexpr int QT = QPW / 16, QPB = NW / KH * QPW;  // 16-query tiles per wave, queries per block
@@ -718,6 +719,12 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
 #pragma unroll
       for (int e = 0; e < 4; ++e) o4.v[e] = (T)(oacc[dt][qt][e] * inv);
       *(V4<T>*)(O + qi * p.o_s + dt * 16 + lg * 4) = o4;
+      if constexpr (SINK)
+        if (p.o_low) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o4.v[e] = (T)(oacc[dt][qt][e] * inv - to_f32(o4.v[e]));
+          *(V4<T>*)((T*)p.o_low + b * p.o_b + h * p.o_h + qi * p.o_s + dt * 16 + lg * 4) = o4;
+        }
     }
     if (lg == 0)
       p.lse[(b * p.H + h) * p.Sq + qi] = l[qt] > 0.f ? (m[qt] + log2f(l[qt])) * kLn2 : -INFINITY;
@@ -728,8 +735,13 @@ __global__ void __launch_bounds__(64 * NW, D == 64 ? ATTN_FWD_BLOCKS * NW / 4 : 
 // backward
 // ---------------------------------------------------------------------------
 // D_i = sum_d dO[i, d] * O[i, d]: D/8 lanes per row, one 16-byte load of
-// each operand per lane, reduced across the row's lanes.
-template <typename T, int D>
+// each operand per lane, reduced across the row's lanes.  LOW: O with what its
+// rounding left out, where that is kept.  The rounding's part of D is the same
+// for all of a row's keys and grows beside dP - D where a window leaves few of
+// them: of 60 bf16 rows of 64 with a window of 1 and a sink dQ is 3.8e-3 off in
+// the 2-norm without it, 2.5e-3 with it, 2.4e-3 from an exact D (worked out in
+// f64 with the kernels' roundings).
+template <typename T, int D, bool LOW = false>
 __global__ void __launch_bounds__(kThreads) attn_bwd_delta(AttnBwdArgs p) {
   constexpr int CPR = D / 8;              // lanes per row
   constexpr int RPB = kThreads / CPR;     // rows per block
@@ -746,6 +758,11 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_delta(AttnBwdArgs p) {
     const V8<T> d = *(const V8<T>*)((const T*)p.dout + b * p.do_b + h * p.do_h + i * p.do_s + ch * 8);
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc += to_f32(o.v[e]) * to_f32(d.v[e]);
+    if constexpr (LOW) {
+      const V8<T> l = *(const V8<T>*)((const T*)p.f.o_low + b * p.f.o_b + h * p.f.o_h + i * p.f.o_s + ch * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc += to_f32(l.v[e]) * to_f32(d.v[e]);
+    }
   }
 #pragma unroll
   for (int off = CPR / 2; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
@@ -1431,9 +1448,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_b
 // rounds.  Blocks of one head stand side by side on an XCD (they read the same
 // rows): the hardware deals blocks to the 8 in turn, and each takes a
 // contiguous run of a kind.
-// bf16, [1, 12, 8192, 64], window 1024, 4 sinks: 136 us and 8 for D, 5.5 for the
-// sums, 430 TFLOP/s of the pairs seen.  [1, 4 over 1, 4096, 256], window 512: 85,
-// 6 and 12.7 us, 200 TFLOP/s; there a block takes a CU and a wave a SIMD, whose
+// bf16, [1, 12, 8192, 64], window 1024, 4 sinks: 136 us and 9 for D, 5.5 for the
+// sums, 400 TFLOP/s of the pairs seen.  [1, 4 over 1, 4096, 256], window 512: 85,
+// 9 and 12.7 us, 190 TFLOP/s; there a block takes a CU and a wave a SIMD, whose
 // waits for LDS are bare (the matrix units are busy a seventh of the time).
 // Eight waves that split a step's channels or its queries' tiles took 80 to 95.
 // 16-row tiles of a wave: two, or one of keys at head_dim 256, where the dK and
@@ -1916,7 +1933,8 @@ template <typename T, int D>
 int window_bwd_launch(AttnBwdArgs a, hipStream_t s) {
   const int64_t rows = a.f.B * a.f.H * a.f.Sq;
   MI_REQUIRE(rows < (1ll << 31), "mi355x_attn_bwd_sink: batch x heads x query rows must be below 2^31");
-  attn_bwd_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
+  auto delta = a.f.o_low ? attn_bwd_delta<T, D, true> : attn_bwd_delta<T, D>;
+  delta<<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
   auto k = attn_bwd_window<T, D>;
   static std::once_flag once;
   static hipError_t attr_err = hipSuccess;
@@ -2003,17 +2021,17 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
 // MFMA forward and backward of a window with sinks, called by
 // mi355x_attn_fwd_sink and mi355x_attn_bwd_sink (attention_generic.hip); -1
 // for inputs they do not take.
-int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
+int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, void* o_low, float* lse, const void* q, const int64_t* q_bhs,
                        const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs, int64_t batch,
                        int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
                        int64_t window, int64_t sinks, int dtype, hipStream_t stream) {
   if ((dtype != MI355X_BF16 && dtype != MI355X_F16) || (d != 64 && d != 128 && d != 256)) return -1;
   if (!(strides_ok(q, q_bhs) && strides_ok(k, k_bhs) && strides_ok(v, v_bhs))) return -1;
-  if ((uintptr_t)o % 8 || o_bhs[0] % 4 || o_bhs[1] % 4 || o_bhs[2] % 4) return -1;
+  if (((uintptr_t)o | (uintptr_t)o_low) % 8 || o_bhs[0] % 4 || o_bhs[1] % 4 || o_bhs[2] % 4) return -1;
   AttnArgs a{(void*)o, o_bhs[0], o_bhs[1], o_bhs[2], lse, q, q_bhs[0], q_bhs[1], q_bhs[2],
              k, k_bhs[0], k_bhs[1], k_bhs[2], v, v_bhs[0], v_bhs[1], v_bhs[2],
              batch, heads, sq, skv, (float)(scale * 1.4426950408889634), (float)scale, 1,
-             heads / kv_heads, window, sinks};
+             heads / kv_heads, window, sinks, o_low};
   const bool bf = dtype == MI355X_BF16;
   if (d == 64) return bf ? fwd_launch<bf16, 64, true>(a, stream) : fwd_launch<f16, 64, true>(a, stream);
   if (d == 128) return bf ? fwd_launch<bf16, 128, true>(a, stream) : fwd_launch<f16, 128, true>(a, stream);
@@ -2029,14 +2047,16 @@ int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t sk
 int attn_bwd_sink_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
                        const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
                        const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
-                       const void* o, const int64_t* o_bhs, const float* lse, int64_t batch, int64_t heads,
+                       const void* o, const int64_t* o_bhs, const void* o_low, const float* lse, int64_t batch, int64_t heads,
                        int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
                        int64_t sinks, int dtype, void* workspace, hipStream_t stream) {
   if ((dtype != MI355X_BF16 && dtype != MI355X_F16) || (d != 64 && d != 128 && d != 256)) return -1;
-  if (!bwd_operands_ok(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs))
+  if (!bwd_operands_ok(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs) ||
+      (uintptr_t)o_low % 16)
     return -1;
   AttnBwdArgs a = bwd_args(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
                            batch, heads, kv_heads, sq, skv, scale, 1, window, sinks, workspace);
+  a.f.o_low = (void*)o_low;
   window_parts(a, d);
   const bool bf = dtype == MI355X_BF16;
   if (d == 64) return bf ? window_bwd_launch<bf16, 64>(a, stream) : window_bwd_launch<f16, 64>(a, stream);

@@ -58,6 +58,7 @@ struct GenArgs {
   int causal;
   int64_t window;
   int64_t sinks;  // with a window: first keys that every later query sees
+  void* o_low;    // null, or (with o's strides) what rounding took from o
 };
 
 __device__ __forceinline__ bool visible(const GenArgs& p, int64_t i, int64_t j) {
@@ -187,6 +188,11 @@ __global__ void __launch_bounds__(kGT) gen_fwd(GenArgs p) {
 #pragma unroll
   for (int t = 0; t < E; ++t) o[t] *= inv;
   store_row<T>((T*)p.o + b * p.o_b + h * p.o_h + qi * p.o_s, o, part, p.D, E);
+  if (p.o_low) {
+#pragma unroll
+    for (int t = 0; t < E; ++t) o[t] -= to_f32(from_f32<T>(o[t]));
+    store_row<T>((T*)p.o_low + b * p.o_b + h * p.o_h + qi * p.o_s, o, part, p.D, E);
+  }
   if (part == 0) p.lse[(b * p.H + h) * p.Sq + qi] = l > 0.f ? (m + log2f(l)) * kLn2G : -INFINITY;
 }
 
@@ -207,6 +213,11 @@ __global__ void __launch_bounds__(kGT) gen_bwd_delta(GenArgs p) {
   float acc = 0.f;
 #pragma unroll
   for (int t = 0; t < E; ++t) acc = fmaf(ov[t], dv[t], acc);
+  if (p.o_low) {
+    load_row<T, E>(ov, (const T*)p.o_low + b * p.o_b + h * p.o_h + i * p.o_s, part, p.D, ok);
+#pragma unroll
+    for (int t = 0; t < E; ++t) acc = fmaf(ov[t], dv[t], acc);
+  }
   acc = row_sum8(acc);
   if (ok && part == 0) p.delta[row] = acc;
 }
@@ -450,15 +461,15 @@ int attn_bwd_grouped_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64
                           hipStream_t stream);
 int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
                             int64_t sinks);
-int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
+int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, void* o_low, float* lse, const void* q, const int64_t* q_bhs,
                        const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs, int64_t batch,
                        int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
                        int64_t window, int64_t sinks, int dtype, hipStream_t stream);
 int attn_bwd_sink_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
                        const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
                        const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
-                       const void* o, const int64_t* o_bhs, const float* lse, int64_t batch, int64_t heads,
-                       int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
+                       const void* o, const int64_t* o_bhs, const void* o_low, const float* lse, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale, int64_t window,
                        int64_t sinks, int dtype, void* workspace, hipStream_t stream);
 }  // namespace mi
 
@@ -475,7 +486,7 @@ extern "C" int64_t mi355x_attn_bwd_gen_workspace_bytes(int64_t batch, int64_t he
 static int attn_bwd_any(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
                                    const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
                                    const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
-                                   const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
+                                   const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const void* o_low, const float* lse,
                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
                                    int64_t d, double scale, int causal, int64_t window, int64_t sinks /* -1: not asked for */,
                                    int dtype, void* workspace, int64_t ws_bytes, int64_t need, const char* what,
@@ -487,7 +498,7 @@ static int attn_bwd_any(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
     return fail(MI355X_EWORKSPACE, "%s: workspace %lld < %lld", what, (long long)ws_bytes, (long long)need);
   const int mrc =
       sinks >= 0 ? attn_bwd_sink_mfma(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o,
-                                      o_bhs, lse, batch, heads, kv_heads, sq, skv, d, scale, window, sinks, dtype,
+                                      o_bhs, o_low, lse, batch, heads, kv_heads, sq, skv, d, scale, window, sinks, dtype,
                                       workspace, (hipStream_t)stream)
                  : attn_bwd_grouped_mfma(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs,
                                          o, o_bhs, lse, batch, heads, kv_heads, sq, skv, d, scale, causal, window, dtype,
@@ -501,6 +512,7 @@ static int attn_bwd_any(void* dq, const int64_t* dq_bhs, void* dk, const int64_t
   a.dk = dk; a.dk_b = dk_bhs[0]; a.dk_h = dk_bhs[1]; a.dk_s = dk_bhs[2];
   a.dv = dv; a.dv_b = dv_bhs[0]; a.dv_h = dv_bhs[1]; a.dv_s = dv_bhs[2];
   a.delta = (float*)workspace;
+  a.o_low = (void*)o_low;
   AttnF32 f;
   if (f32_args(a, dtype, &f, sinks >= 0)) {
     rc = sinks >= 0 ? attn_f32_window_bwd(f, d, (hipStream_t)stream) : attn_f32_bwd(f, d, (hipStream_t)stream);
@@ -516,7 +528,7 @@ extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, co
                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
                                    int64_t d, double scale, int causal, int64_t window, int dtype,
                                    void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
-  return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
+  return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, nullptr, lse,
                       batch, heads, kv_heads, sq, skv, d, scale, causal, window, -1, dtype, workspace, ws_bytes,
                       mi355x_attn_bwd_gen_workspace_bytes(batch, heads, kv_heads, sq, skv, d), "mi355x_attn_bwd_gen",
                       stream);
@@ -530,7 +542,7 @@ static void clip_window(int64_t& window, int64_t& sinks, int64_t sq, int64_t skv
 
 // A window with sinks: causal, query i sees key j iff i - j < window or j <
 // sinks.
-extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, const void* q, const int64_t* q_bhs,
+extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, void* o_low, float* lse, const void* q, const int64_t* q_bhs,
                                     const void* k, const int64_t* k_bhs, const void* v, const int64_t* v_bhs,
                                     int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
                                     int64_t d, double scale, int64_t window, int64_t sinks, int dtype,
@@ -540,12 +552,14 @@ extern "C" int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, float* lse, c
   MI_REQUIRE(o && lse && q && k && v, "mi355x_attn_fwd_sink: null pointer");
   MI_REQUIRE(window > 0 && sinks >= 0, "mi355x_attn_fwd_sink: window must be positive, sinks not negative");
   clip_window(window, sinks, sq, skv);
-  rc = attn_fwd_sink_mfma(o, o_bhs, lse, q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale,
+  if (dtype == MI355X_F32) o_low = nullptr;
+  rc = attn_fwd_sink_mfma(o, o_bhs, o_low, lse, q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale,
                           window, sinks, dtype, (hipStream_t)stream);
   if (rc >= 0) return rc;
   GenArgs a = gen_args(q, q_bhs, k, k_bhs, v, v_bhs, batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks);
   a.o = o; a.o_b = o_bhs[0]; a.o_h = o_bhs[1]; a.o_s = o_bhs[2];
   a.lse = lse;
+  a.o_low = o_low;
   AttnF32 f;
   if (f32_args(a, dtype, &f, true)) {
     rc = attn_f32_window_fwd(f, d, (hipStream_t)stream);
@@ -564,13 +578,14 @@ extern "C" int64_t mi355x_attn_bwd_sink_workspace_bytes(int64_t batch, int64_t h
 extern "C" int mi355x_attn_bwd_sink(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,
                                     const int64_t* dv_bhs, const void* dout, const int64_t* do_bhs, const void* q,
                                     const int64_t* q_bhs, const void* k, const int64_t* k_bhs, const void* v,
-                                    const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const float* lse,
+                                    const int64_t* v_bhs, const void* o, const int64_t* o_bhs, const void* o_low, const float* lse,
                                     int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
                                     int64_t d, double scale, int64_t window, int64_t sinks, int dtype,
                                     void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
   MI_REQUIRE(window > 0 && sinks >= 0, "mi355x_attn_bwd_sink: window must be positive, sinks not negative");
   clip_window(window, sinks, sq, skv);
-  return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, lse,
+  if (dtype == MI355X_F32) o_low = nullptr;
+  return attn_bwd_any(dq, dq_bhs, dk, dk_bhs, dv, dv_bhs, dout, do_bhs, q, q_bhs, k, k_bhs, v, v_bhs, o, o_bhs, o_low, lse,
                       batch, heads, kv_heads, sq, skv, d, scale, 1, window, sinks, dtype, workspace, ws_bytes,
                       mi355x_attn_bwd_sink_workspace_bytes(batch, heads, kv_heads, sq, skv, d, window, sinks),
                       "mi355x_attn_bwd_sink", stream);

@@ -32,6 +32,7 @@ struct AttnArgs {
   int64_t group;   // query heads per K/V head (grouped-query attention), >= 1
   int64_t window;  // > 0: query i sees keys i-window+1 .. i (causal only); 0: none
   int64_t sinks;   // with a window: first keys that every later query sees
+  void* o_low;     // null, or (with o's strides) what rounding took from o
 };
 
 struct AttnBwdArgs {

@@ -278,7 +278,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mi355x_attn_fwd_sink": (
         c_int,
         [
-            c_vp, P_i64, c_vp, c_vp, P_i64, c_vp, P_i64, c_vp, P_i64,
+            c_vp, P_i64, c_vp, c_vp, c_vp, P_i64, c_vp, P_i64, c_vp, P_i64,
             c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_double, c_i64, c_i64, c_int, c_vp,
         ],
     ),
@@ -287,7 +287,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [
             c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp, P_i64,
-            c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp,
+            c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp, P_i64, c_vp, c_vp,
             c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_double, c_i64, c_i64, c_int,
             c_vp, c_i64, c_vp,
         ],

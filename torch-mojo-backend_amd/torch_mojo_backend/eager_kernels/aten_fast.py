@@ -2198,12 +2198,13 @@ def _mfma_bwd_ok(q: MT, group, window) -> bool:
     return q._dtype in _MFMA_DTYPES and group == 1 and window == 0 and q._shape[3] in _FUSED_FA_HEAD_DIMS
 
 
-def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=None):
+def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=None, low=None):
     """(out [B,H,Sq,D] over BTHD storage, lse f32 [B,H,Sq]) of causal / full
     attention with optional grouped K/V heads (k, v with H / g heads) and a
     causal sliding window: MFMA kernels where they apply, else the f32
     kernels.  With `sinks` (0 too) the window's own kernels, which leave that
-    many first keys visible."""
+    many first keys visible, and in `low`, laid out like the output, what
+    rounding took from it."""
     b, h, sq, d = q._shape
     hk, skv = k._shape[1], k._shape[2]
     scale_value = float(scale) if scale is not None else 1.0 / math.sqrt(d)
@@ -2214,7 +2215,7 @@ def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=None):
         q, k, v = rows(q), rows(k), rows(v)
         check(
             "mi355x_attn_fwd_sink",
-            lib().mi355x_attn_fwd_sink(out._ptr, _bhs(out), lse._ptr, q._ptr, _bhs(q), k._ptr, _bhs(k),
+            lib().mi355x_attn_fwd_sink(out._ptr, _bhs(out), low._ptr if low is not None else None, lse._ptr, q._ptr, _bhs(q), k._ptr, _bhs(k),
                                        v._ptr, _bhs(v), b, h, hk, sq, skv, d, scale_value, int(window), int(sinks),
                                        _code(q._dtype), _STREAM),
         )
@@ -2237,7 +2238,7 @@ def attention_forward(q: MT, k: MT, v: MT, causal, window, scale, sinks=None):
     return out, lse
 
 
-def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, window, scale, sinks=None):
+def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, window, scale, sinks=None, low=None):
     """(dq, dk, dv) of attention_forward: dk/dv have k's heads (the query
     heads of each group summed)."""
     b, h, sq, d = q._shape
@@ -2260,6 +2261,8 @@ def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, 
         dv = alloc_bthd(b, hk, skv, d, q._dtype, q._device)
     if window and sinks is not None:
         rows = _fa_head_contig if q._dtype in _MFMA_DTYPES and d in _MFMA_EX_HEAD_DIMS else _unit_head_stride
+        if low is not None and (rows(out) is not out or low._strides != out._strides):
+            low = None  # D from `out` alone
         q, k, v, out, dout = rows(q), rows(k), rows(v), rows(out), rows(grad_out)
         ws = lib().mi355x_attn_bwd_sink_workspace_bytes(b, h, hk, sq, skv, d, int(window), int(sinks))
         hold, wptr = _workspace(ws, q._device)
@@ -2267,7 +2270,8 @@ def attention_backward(grad_out, q: MT, k: MT, v: MT, out: MT, lse: MT, causal, 
             "mi355x_attn_bwd_sink",
             lib().mi355x_attn_bwd_sink(
                 dq._ptr, _bhs(dq), dk._ptr, _bhs(dk), dv._ptr, _bhs(dv), dout._ptr, _bhs(dout),
-                q._ptr, _bhs(q), k._ptr, _bhs(k), v._ptr, _bhs(v), out._ptr, _bhs(out), lse._ptr,
+                q._ptr, _bhs(q), k._ptr, _bhs(k), v._ptr, _bhs(v), out._ptr, _bhs(out),
+                low._ptr if low is not None else None, lse._ptr,
                 b, h, hk, sq, skv, d, scale_value, int(window), int(sinks), _code(q._dtype), wptr, ws, _STREAM,
             ),
         )

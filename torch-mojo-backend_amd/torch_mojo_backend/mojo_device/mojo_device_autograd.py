@@ -89,17 +89,20 @@ class _FusedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, window, scale, sinks=None):
         with torch._C._AutoDispatchBelowAutograd():
-            out, lse = aten_fast.attention_forward(q, k, v, causal, window, scale, sinks)
-        ctx.save_for_backward(q, k, v, out, lse)
+            low = None  # of a 16-bit output: what rounding took from it, for the backward's row terms
+            if sinks is not None and window and q._dtype is not torch.float32:
+                low = aten_fast.alloc_bthd(*q._shape, q._dtype, q._device)
+            out, lse = aten_fast.attention_forward(q, k, v, causal, window, scale, sinks, low)
+        ctx.save_for_backward(q, k, v, out, lse, low)
         ctx.args = (causal, window, scale, sinks)
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, low = ctx.saved_tensors
         causal, window, scale, sinks = ctx.args
         with torch._C._AutoDispatchBelowAutograd():
-            dq, dk, dv = aten_fast.attention_backward(grad, q, k, v, out, lse, causal, window, scale, sinks)
+            dq, dk, dv = aten_fast.attention_backward(grad, q, k, v, out, lse, causal, window, scale, sinks, low)
         return dq, dk, dv, None, None, None, None
 
 
