@@ -127,6 +127,15 @@ def test_attention_over_a_long_sequence(dtype, bits, d):
     _attention(c, 4, [9000, 129], [1, 1], 1, dtype, window=4096, sinks=100)
 
 
+@pytest.mark.parametrize("dtype,bits", [(BF, None), (F32, None), (BF, 4), (HF, 4)])
+@pytest.mark.parametrize("d,hk,h,page", [(64, 1, 4, 16), (128, 2, 4, 24), (256, 1, 2, 64), (80, 1, 2, 16)])
+def test_attention_of_a_prompt(dtype, bits, d, hk, h, page):
+    d = 96 if bits and d == 80 else d  # 4-bit rows are multiples of 32 channels
+    c = Case([700, 431], page=page, bits=bits, device="mojo", d=d, hk=hk, dtype=dtype)
+    _attention(c, h, [100, 0], [600, 431], 600, dtype)
+    _attention(c, h, [100, 0], [600, 431], 600, dtype, window=64, sinks=20)
+
+
 @pytest.mark.parametrize("d,h", [(64, 2), (128, 4), (256, 4), (64, 20), (128, 20)])
 @pytest.mark.parametrize("page", [16, 24])
 def test_f16_queries_over_4_bits_round_nothing_but_the_result(d, h, page):

@@ -203,6 +203,8 @@ def test_refusals(device):
         (ValueError, lambda: PagedKVCache(x, x[:1])),
         (ValueError, lambda: PagedKVCache(x.expand(2, 2, 1, 64)[:, :1].expand(2, 2, 1, 64), x)),
         (ValueError, lambda: PagedKVCache(x[..., :20], x[..., :20])),
+        (ValueError, lambda: PagedKVCache(x, x)),
+        (ValueError, lambda: PagedKVCache(x, x[:])),
         (TypeError, lambda: PagedKVCache(x.int(), x.int())),
         (ValueError, lambda: PagedKVCache.zeros(2, 4, 1, 64, bits=8, device=device)),
         (ValueError, lambda: PagedKVCache.zeros(2, 4, 1, 48, bits=4, device=device)),

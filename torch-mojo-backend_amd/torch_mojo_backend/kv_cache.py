@@ -70,6 +70,9 @@ class PagedKVCache:
                 raise ValueError("PagedKVCache: rows of pages must be contiguous")
             if _overlaps(t):
                 raise ValueError("PagedKVCache: rows of pages must not overlap")
+        where = [t._ptr if isinstance(t, TorchMojoTensor) else t.data_ptr() for t in tensors]
+        if len(set(where)) < len(where):
+            raise ValueError("PagedKVCache: pages of keys, of values and scales must not be the same memory")
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
         self.tensors = tuple(tensors)
         self.scale = self.head_dim ** -0.5  # attention's default
