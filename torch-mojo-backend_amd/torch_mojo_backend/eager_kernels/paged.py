@@ -63,7 +63,7 @@ def rows_ok(cache, t, batch, like=None) -> bool:
             and (dtype is cache.dtype if cache.bits != 4 else dtype in _FLOATS if like is None else dtype is like._dtype))
 
 
-def _on_device(device: int, call, *args):
+def on_device(device: int, call, *args):
     """call(*args) with `device` current: a launch on the null stream goes to
     the current device."""
     if _tensor_mod.storage_kind() == "cuda" and torch._C._cuda_getDevice() != device:
@@ -92,7 +92,7 @@ def append(cache, table, starts, k, v, cos, sin, q, counts):
     if lazy_live():
         materialize_touched((*cache.tensors, table, starts, k, v, cos, sin, q, counts), None, True)
     dev = k._device
-    out = _on_device(dev, _append, cache, table, starts, k, v, cos, sin, q, counts, dev)
+    out = on_device(dev, _append, cache, table, starts, k, v, cos, sin, q, counts, dev)
     torch._C._increment_version(cache.tensors)
     return out
 
@@ -120,7 +120,7 @@ def _append(cache, table, starts, k, v, cos, sin, q, counts, dev):
 def gather(cache, table, starts, length, counts, dtype):
     if lazy_live():
         materialize_touched((*cache.tensors, table, starts, counts), None, False)
-    return _on_device(table._device, _gather, cache, table, starts, length, counts, dtype, table._device)
+    return on_device(table._device, _gather, cache, table, starts, length, counts, dtype, table._device)
 
 
 def _gather(cache, table, starts, length, counts, dtype, dev):
@@ -137,7 +137,7 @@ def _gather(cache, table, starts, length, counts, dtype, dev):
 def attention(q, cache, table, starts, counts, window, sinks, scale):
     if lazy_live():
         materialize_touched((q, *cache.tensors, table, starts, counts), None, False)
-    return _on_device(q._device, _attention, q, cache, table, starts, counts, window, sinks, scale, q._device)
+    return on_device(q._device, _attention, q, cache, table, starts, counts, window, sinks, scale, q._device)
 
 
 def _attention(q, cache, table, starts, counts, window, sinks, scale, dev):

@@ -40,7 +40,7 @@ from __future__ import annotations
 
 import torch
 
-from ..eager_kernels import aten_fast
+from ..eager_kernels import aten_fast, paged
 from .torch_mojo_tensor import TorchMojoTensor
 
 _registered = False
@@ -102,7 +102,8 @@ class _FusedAttention(torch.autograd.Function):
         q, k, v, out, lse, low = ctx.saved_tensors
         causal, window, scale, sinks = ctx.args
         with torch._C._AutoDispatchBelowAutograd():
-            dq, dk, dv = aten_fast.attention_backward(grad, q, k, v, out, lse, causal, window, scale, sinks, low)
+            dq, dk, dv = paged.on_device(q._device, aten_fast.attention_backward, grad, q, k, v, out, lse, causal, window,
+                                         scale, sinks, low)
         return dq, dk, dv, None, None, None, None
 
 

@@ -134,11 +134,11 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
             sinks = min(sinks, t)
         if not _needs_grad(q, k, v):
             materialize_touched((q, k, v), None, False)
-            return aten_fast.attention_forward(q, k, v, True, window, scale, sinks)[0]
+            return paged.on_device(q._device, aten_fast.attention_forward, q, k, v, True, window, scale, sinks)[0]
         from .mojo_device.mojo_device_autograd import _FusedAttention
 
         materialize_touched((q, k, v), None, False)
-        return _FusedAttention.apply(q, k, v, True, window, scale, sinks)
+        return paged.on_device(q._device, _FusedAttention.apply, q, k, v, True, window, scale, sinks)
     if not q.numel():
         return q * 1.0
     return F.scaled_dot_product_attention(
