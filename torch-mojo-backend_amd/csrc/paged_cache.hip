@@ -188,10 +188,10 @@ __device__ __forceinline__ bool place_of(const AppendArgs& a, int64_t b, int64_t
 // kHeads rows of one token and of one kind (query, key or value, the same for
 // a block): the angles are read once for all of them, and their loads are all
 // in flight before the first is used.  Four prompts of 2048 tokens, 16 query
-// and 8 K/V heads of 128 at most, into 4 bits (89 MB): one row a thread 38.7 us,
-// whose waves are too short to hide the lookup of their page, two 42.4, four
-// 36.8; the f64 rotation of the keys and the packing bound it, a copy would take
-// 17.  Five of 333 at most into f32 pages (13 MB) 6.2 us, one token 3.0, a launch.
+// and 8 K/V heads of 128 at most, into 4 bits (89 MB): 34.6 us (eight rows a
+// thread 12 more, one or two up to 5 more); the f64 rotation of the keys and the
+// packing bound it, a copy would take 17.  Five of 333 at most into f32 pages
+// (13 MB) 6.2 us, one token 3.0, a launch.
 constexpr int kHeads = 4;
 
 template <typename T, typename RT, bool FOUR>
@@ -202,11 +202,13 @@ __global__ void __launch_bounds__(kThreads) paged_append_heads(AppendArgs a) {
   if (token >= (uint32_t)a.tokens) return;
   const uint32_t bi = token / a.seq, t = token - bi * a.seq;
   const int64_t b = bi;
-  // blockIdx.y: groups of query heads, then of K heads, then of V heads
-  const int nq = (a.heads + kHeads - 1) / kHeads, nk = (a.kv_heads + kHeads - 1) / kHeads;
+  // blockIdx.y: groups of K heads, then of V heads, then of query heads, so that
+  // in 4 bits the blocks that pack do not come last (39 us so, for the prompts
+  // above; 38 with the kinds side by side)
+  const int nk = (a.kv_heads + kHeads - 1) / kHeads;
   int group = blockIdx.y;
-  const bool is_q = group < nq, is_k = !is_q && group < nq + nk;
-  if (!is_q) group -= is_k ? nq : nq + nk;
+  const bool is_k = group < nk, is_q = group >= 2 * nk;
+  if (!is_k) group -= is_q ? 2 * nk : nk;
   const int h0 = group * kHeads, n = min(kHeads, (is_q ? a.heads : a.kv_heads) - h0);
   const Rows& src = is_q ? a.q : is_k ? a.k : a.v;
   const T* x = row_of<T>(src, b, h0, t) + ch;
