@@ -300,3 +300,31 @@ def test_captured_and_replayed(kernels):
         ks.append(np64(k)[0, :, 0]), vs.append(np64(v)[0, :, 0])
         want = oracle.attend(np64(q)[0], np.stack(ks, 1), np.stack(vs, 1), [i])
         check(o, want[None], STEP[BF] * np.abs(want[None]) + 1e-4, f"replay {i}")
+
+
+@pytest.mark.parametrize("dtype,bits,d,page", [(BF, None, 64, 16), (F32, None, 128, 24), (HF, 4, 256, 16), (BF, None, 96, 16),
+                                               (F32, 4, 64, 5)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (9, 3)])
+def test_positions_past_the_table_see_what_it_holds(dtype, bits, d, page, window, sinks):
+    """A query behind the table's last place: an error at the next read, the
+    table's keys alone, and no more work than they take."""
+    n = 3 * page
+    c = Case([n, n], page=page, bits=bits, device="mojo", d=d, hk=1, dtype=dtype)
+    q = c.queries(4, 2, dtype)
+    for far in (n - 1, n, 40 * n, 2 ** 30, 2 ** 31 - 300):
+        out = ops.paged_attention(q.to("mojo"), c.cache, c.dev_table, c.ints([far, n - 2]), window=window, sinks=sinks)
+        with pytest.raises(IndexError, match="paged cache"):
+            out.cpu()
+        want, bound = c.expected(q, [far, n - 2], [0, 2], window, sinks)
+        k, v = (x[0] for x in c.values)
+        for t in range(2):  # the query sees j <= far + t < ..., of which the table has n
+            j = np.arange(n)
+            keep = (j <= far + t) & ((far + t - j < window) | (j < sinks) if window else True)
+            if keep.any():
+                s = d ** -0.5 * np64(q)[0, :, t] @ k[0, keep].T
+                p = np.exp(s - s.max(-1, keepdims=True))
+                want[0, :, t] = p / p.sum(-1, keepdims=True) @ v[0, keep]
+        # the bound of the sequence beside it, of as many keys and the same spread, twice
+        bound[0] = 2 * bound[1].max() + STEP[dtype] * np.abs(want[0])
+        check(out, want, bound, f"position {far}")
+    c.cache.k.cpu()  # the flag is cleared

@@ -246,3 +246,16 @@ def test_a_copy_of_a_cache_is_its_own(device, bits):
     ops.paged_append(other, zero.view(1, 1), zero, x, x)
     assert (ops.paged_gather(c, zero.view(1, 1), zero, 1)[0].cpu() == 0).all()
     assert (ops.paged_gather(other, zero.view(1, 1), zero, 1)[0].cpu() == 1).all()
+
+
+@pytest.mark.parametrize("far", [12, 500, 2 ** 30, 2 ** 31 - 2])
+def test_positions_past_the_table_raise(device, far):
+    c = Case([12, 12], page=4, device=device, dtype=torch.float32)
+    x = torch.zeros(2, 2, 1, 64).to(device)
+    for call in (lambda: ops.paged_append(c.cache, c.dev_table, c.ints([0, far]), x, x),
+                 lambda: ops.paged_gather(c.cache, c.dev_table, c.ints([0, far]), 1),
+                 lambda: ops.paged_attention(x, c.cache, c.dev_table, c.ints([0, far])),
+                 lambda: ops.paged_attention(x, c.cache, c.dev_table, c.ints([0, far]), window=3, sinks=2)):
+        with pytest.raises(IndexError, match="paged cache"):
+            call()
+            c.cache.k.cpu()

@@ -13,6 +13,7 @@
 // masked with 0x000f000f gives channels 2 i and 2 i + 1 as two 16-bit halves.
 #pragma once
 #include "common.h"
+#include "paged_span.h"
 
 namespace mi {
 
@@ -20,10 +21,6 @@ constexpr int kKvGroup = 32;  // channels per (scale, minimum) pair
 // Values are clamped to this before they are packed: minimum + 15 * scale,
 // both rounded to f16, then stays finite in f16 (61440 + 122880 * 2^-11 < 65504).
 constexpr double kKvLimit = 61440.0;
-
-// Positions end a little below 2^31, so that 32-bit sums with a tile's length
-// do not pass it.
-constexpr int64_t kMaxPosition = 0x7fffff00;
 
 // Quotients of 31-bit positions by the page size: one multiply-high and a
 // shift instead of the division's twenty instructions.  For a divisor that is
@@ -52,6 +49,7 @@ struct PagedSeqs {
   const int32_t* counts; // tokens of each sequence, the rest is padding (null: all)
   PageDiv page;
   int32_t num_pages;
+  int32_t end;           // positions from here on are past the table
   int32_t* error;        // set to 1 by a page or position out of range (may be null)
 };
 

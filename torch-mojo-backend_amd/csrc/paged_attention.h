@@ -23,22 +23,6 @@ struct DecodeArgs {
   int64_t row_groups, units;  // matrix cores: blocks of query rows per K/V head; (batch, K/V head, split) triples
 };
 
-// The keys that queries at positions first .. last can see, in tiles of
-// `tile` keys: the sinks' tiles, then the window's from tile `low` on.
-struct KeySpan {
-  int sink_tiles, low, tiles;
-  __device__ __forceinline__ KeySpan(int first, int last, int window, int sinks, int tile) {
-    low = window > 0 ? max(first - window + 1, 0) / tile : 0;
-    const int s = window > 0 ? min(sinks, last + 1) : 0;
-    sink_tiles = min((s + tile - 1) / tile, low);
-    tiles = last < 0 ? 0 : sink_tiles + last / tile + 1 - low;
-  }
-  __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : low + i - sink_tiles; }
-};
-__device__ __forceinline__ bool visible(int pos, int j, int window, int sinks) {
-  return j <= pos && (window <= 0 || pos - j < window || j < sinks);
-}
-
 // Whether the matrix-core kernel takes these pages with queries of dtype.
 bool paged_mfma_takes(const mi355x_paged_cache& c, int dtype);
 int paged_mfma_row_tiles(int64_t rows, int64_t d);

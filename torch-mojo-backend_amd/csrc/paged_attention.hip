@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_rows(DecodeArgs a) {
   const bool real = (int)t < seq_count(a.s, b, a.seq);
   const int64_t at = (int64_t)a.s.starts[b] + t;
   int pos = real && at >= 0 && at <= kMaxPosition ? (int)at : -1;
-  if (real && pos < 0 && a.s.error) *a.s.error = 1;
-  const KeySpan span(pos, pos, a.window, a.sinks, 16);
+  if (real && (pos < 0 || pos >= a.s.end) && a.s.error) *a.s.error = 1;
+  const KeySpan span(pos, pos, a.window, a.sinks, a.s.end, 16);
   const int per = (span.tiles + a.splits - 1) / a.splits, first = blockIdx.y * per;
   const int last = min(first + per, span.tiles);
   float q[2][8], o[2][8], m = -INFINITY, l = 0.f;

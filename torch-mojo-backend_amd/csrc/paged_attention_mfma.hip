@@ -553,16 +553,17 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
     const int64_t at = start + t;
     const bool real = r < rows && t < count;
     const bool ok = real && at >= 0 && at <= kMaxPosition;
-    if (real && !ok && a.s.error) *a.s.error = 1;
+    if (real && (!ok || at >= a.s.end) && a.s.error) *a.s.error = 1;
     pos[qt] = ok ? (int)at : -1;
     F::load_query(q[qt], (const T*)a.q + b * a.q_b + h * a.q_h + t * a.q_t, ok, g, a.scale_log2);
   }
   // positions of the block's first and last row (rows are token by token)
   const int t0 = r0 / a.group, t1 = min(min((r0 + 16 * QT - 1) / a.group, count - 1), a.seq - 1);
   const int64_t last64 = t1 >= t0 ? start + t1 : -1, first64 = start + t0;
-  const int last = last64 >= 0 && last64 <= kMaxPosition ? (int)last64 : -1;
+  const int last = (int)min(max(last64, (int64_t)-1), kMaxPosition);
   const int first = (int)min(max(first64, (int64_t)-1), kMaxPosition);
-  const KeySpan span(first, last, a.window, a.sinks, TK);
+  const KeySpan span(first, last, a.window, a.sinks, a.s.end, TK);
+  const int top_key = min(last, a.s.end - 1);  // a position past the table is an error, and sees what the table has
   const int low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
   const int per = (span.tiles + a.splits - 1) / a.splits;
   const int end = min((split + 1) * per, span.tiles);
@@ -570,10 +571,10 @@ __global__ void __launch_bounds__(64 * NW, (waves_of<F, QT>())) paged_attn_mfma(
   auto look_up = [&](int i) {
     Places p{0, 0, 0};
     const int j = span.tile(i) * TK + (lane & (TK - 1));
-    bool live = j <= last && (j >= low || j < a.sinks);
+    bool live = j <= top_key && (j >= low || j < a.sinks);
     // 16 keys of one page: its number is wanted if any of them is live
     const int j16 = j & ~15;
-    const bool wanted = P16 ? j16 <= last && (j16 + 15 >= low || j16 < a.sinks) : live;
+    const bool wanted = P16 ? j16 <= top_key && (j16 + 15 >= low || j16 < a.sinks) : live;
     if (wanted) {
       uint32_t slot;
       const int page = page_of(a.s, b, (uint32_t)j, &slot);

@@ -53,7 +53,7 @@ int paged_args(const char* what, const mi355x_paged_cache* c, const int32_t* tab
     MI_REQUIRE(((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) % 4 == 0, "%s: scales must be 4-byte aligned", what);
   }
   *s = PagedSeqs{table, table_stride, (uint32_t)table_width, starts, counts, page_div(c->page_size),
-                 (int32_t)c->num_pages, error};
+                 (int32_t)c->num_pages, table_end(table_width, c->page_size), error};
   return MI355X_OK;
 }
 
