@@ -328,3 +328,31 @@ def test_positions_past_the_table_see_what_it_holds(dtype, bits, d, page, window
         bound[0] = 2 * bound[1].max() + STEP[dtype] * np.abs(want[0])
         check(out, want, bound, f"position {far}")
     c.cache.k.cpu()  # the flag is cleared
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+@pytest.mark.parametrize("d,turned", [(64, False), (64, True), (32, False), (96, True)])
+def test_codes_are_of_clamped_values(dtype, d, turned):
+    """Values on both sides of +-61440: the codes, too, are those of the clamped ones."""
+    big = {F32: 70000.0, BF: 69632.0, HF: 65504.0}[dtype]
+    low = {F32: 61425.0, BF: 61440.0, HF: 61408.0}[dtype]
+    rows = torch.full((1, 1, 8, d), low)
+    rows[..., 1::2] = big                    # the minimum's f16 is the limit
+    rows[0, 0, 1] = -rows[0, 0, 1]
+    rows[0, 0, 2, ::3] = -big                # both ends past it
+    rows[0, 0, 3, 5:] = 0.0
+    rows[0, 0, 4] = big
+    rows[0, 0, 5] = torch.linspace(-2 * big, 2 * big, d)
+    if dtype is F32:
+        rows[0, 0, 6, 4:] = 3e38
+    rows = rows.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max).to(dtype)
+    cos, sin = torch.ones(8, d), torch.zeros(8, d)  # turned by nothing: the values in f64
+    c = PagedKVCache.zeros(1, 8, 1, d, bits=4)
+    zero = torch.zeros(1, 1, dtype=torch.int32).to("mojo")
+    args = (cos.to("mojo"), sin.to("mojo")) if turned else ()
+    ops.paged_append(c, zero, zero.view(1), rows.to("mojo"), rows.to("mojo"), *args)
+    codes, scale, base = oracle.quantize(np64(rows))
+    want = oracle.values(codes, scale, base)
+    assert np.abs(want).max() <= 61440 + 16 + 15 * 2  # half a step of the minimum, and 15 of the scale
+    for got in ops.paged_gather(c, zero, zero.view(1), 8):
+        assert (np64(got) == want.astype(np.float32)).all()

@@ -122,7 +122,7 @@ __device__ __forceinline__ f16 to_f16_by_f32(double x) {
 // settles those.  (The 64-bit quotients took 8 us of 42 for the prompts above
 // paged_append_heads.)
 template <typename W>
-__device__ __forceinline__ void pack_row(const W (&x)[8], uint32_t* codes, f16* scales, int ch, int d) {
+__device__ __forceinline__ void pack_row(W (&x)[8], uint32_t* codes, f16* scales, int ch, int d) {
   const W limit = (W)kKvLimit;
   W lo = x[0], hi = x[0], nan = (W)0;
 #pragma unroll
@@ -137,7 +137,11 @@ __device__ __forceinline__ void pack_row(const W (&x)[8], uint32_t* codes, f16* 
     hi = fmax(hi, __shfl_xor(hi, off, 64));
     bad |= __shfl_xor(bad, off, 64);
   }
-  lo = fmin(fmax(lo, -limit), limit), hi = fmin(fmax(hi, -limit), limit);
+  if (lo < -limit || hi > limit) {  // the codes, too, are those of clamped values
+    lo = fmin(fmax(lo, -limit), limit), hi = fmin(fmax(hi, -limit), limit);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmin(fmax(x[e], -limit), limit);
+  }
   // times 1 / 15 is within 2^-53 of the quotient, which f32 does not resolve
   const f16 step16 = bad ? (f16)NAN : to_f16_by_f32(((double)hi - (double)lo) * (1.0 / 15.0));
   const f16 base16 = bad ? (f16)NAN : to_f16_by_f32(lo);
