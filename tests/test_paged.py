@@ -259,3 +259,43 @@ def test_positions_past_the_table_raise(device, far):
         with pytest.raises(IndexError, match="paged cache"):
             call()
             c.cache.k.cpu()
+
+
+def test_pages_that_share_memory_are_refused(device):
+    base = torch.zeros(9, 2, 4, 64).to(device)
+    both = torch.zeros(8, 2, 2, 4, 64).to(device)
+    codes = torch.zeros(4, 2, 8, 32, dtype=torch.uint8).to(device)
+    scales = torch.zeros(5, 2, 8, 2, 2, dtype=torch.float16).to(device)
+    other = torch.zeros(4, 2, 8, 2, 2, dtype=torch.float16).to(device)
+    for k, v in ((base, base), (base[:2], base[1:3]), (base[:8], base[1:]), (base[:4, :1], base[3:7, :1]),
+                 (base[:, :, :3], base[:, :, 1:]), (base[..., :32], base[..., 16:48]), (base[::2][:4], base[2::2])):
+        with pytest.raises(ValueError, match="share memory"):
+            PagedKVCache(k, v)
+    with pytest.raises(ValueError, match="share memory"):
+        PagedKVCache(codes, codes.clone(), scales[1:], scales[:4])
+    for k, v in ((base[:4], base[4:8]), (base[::2][:4], base[1::2]), (base[:, :1], base[:, 1:]), (base[:, :, :2], base[:, :, 2:]),
+                 (base[..., :32], base[..., 32:]), (both[:, 0], both[:, 1]), (both[:, :, 0], both[:, :, 1])):
+        PagedKVCache(k, v)
+    PagedKVCache(codes, codes.clone(), scales[:4], other)
+
+
+def test_sharing_is_told_as_it_is():
+    from torch_mojo_backend.kv_cache import _share
+
+    g = np.random.default_rng(0)
+    found = [0, 0]
+    for _ in range(2000):
+        flat = torch.zeros(4000, dtype=torch.uint8)
+
+        def view():
+            width, shape = int(g.integers(1, 9)), [int(n) for n in g.integers(1, 5, size=3)]
+            strides = [int(g.choice([width + int(g.integers(0, 5)), 12, 40, 100, 130, 300])) for _ in range(3)]
+            return flat.as_strided((*shape, width), (*strides, 1), int(g.integers(0, 200)))
+
+        a, b = view(), view()
+        places = [{int(i) for i in np.lib.stride_tricks.as_strided(np.arange(4000), x.shape, [8 * s for s in x.stride()])
+                   .ravel() + x.storage_offset()} for x in (a, b)]
+        want = bool(places[0] & places[1])
+        assert _share(a, b) == _share(b, a) == want
+        found[want] += 1
+    assert min(found) > 200

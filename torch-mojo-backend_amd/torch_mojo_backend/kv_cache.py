@@ -70,9 +70,8 @@ class PagedKVCache:
                 raise ValueError("PagedKVCache: rows of pages must be contiguous")
             if _overlaps(t):
                 raise ValueError("PagedKVCache: rows of pages must not overlap")
-        where = [t._ptr if isinstance(t, TorchMojoTensor) else t.data_ptr() for t in tensors]
-        if len(set(where)) < len(where):
-            raise ValueError("PagedKVCache: pages of keys, of values and scales must not be the same memory")
+        if any(_share(a, b) for i, a in enumerate(tensors) for b in tensors[:i]):
+            raise ValueError("PagedKVCache: pages of keys, of values and scales must not share memory")
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
         self.tensors = tuple(tensors)
         self.scale = self.head_dim ** -0.5  # attention's default
@@ -118,6 +117,46 @@ def _overlaps(t) -> bool:
             return True
         extent += (size - 1) * stride
     return False
+
+
+def _share(a, b) -> bool:
+    """Whether two tensors with contiguous rows share memory; also where that
+    takes too long to tell, which layouts of pages do not.
+
+    A byte of both is a solution of sum n_s * s = the distance of their first
+    bytes, give or take a row, with a term for each stride s: of a, of b
+    negated, or of both.  From the largest on, a stride's multiples are tried
+    that the smaller ones can make up for: one or two of them, in tensors
+    whose dimensions lie inside one another."""
+    at = [t._ptr if isinstance(t, TorchMojoTensor) else t.data_ptr() for t in (a, b)]
+    rows = [t.shape[-1] * t.element_size() for t in (a, b)]
+    terms = {}  # stride in bytes -> the least and the greatest n
+    for t, sign in ((a, 1), (b, -1)):
+        for size, stride in zip(t.shape[:-1], t.stride()):
+            low, high = terms.get(stride * t.element_size(), (0, 0))
+            n = sign * (size - 1)
+            terms[stride * t.element_size()] = (low + min(n, 0), high + max(n, 0))
+    terms = sorted(terms.items(), reverse=True)
+    reach = [(1 - rows[1], rows[0] - 1)]  # of the row, then of the smaller strides as well
+    for s, (low, high) in reversed(terms):
+        reach.append((reach[-1][0] + low * s, reach[-1][1] + high * s))
+    reach.reverse()
+    tries = 0
+
+    def solve(i, rest) -> bool:
+        nonlocal tries
+        tries += 1
+        low, high = reach[i]
+        if not low <= rest <= high or tries > 20000:
+            return tries > 20000
+        if i == len(terms):
+            return True
+        (s, (least, most)), (low, high) = terms[i], reach[i + 1]
+        if s == 0:
+            return solve(i + 1, rest)
+        return any(solve(i + 1, rest - n * s) for n in range(max(least, -((high - rest) // s)), min(most, (rest - low) // s) + 1))
+
+    return solve(0, at[1] - at[0])
 
 
 # ---------------------------------------------------------------------------
