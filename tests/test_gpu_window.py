@@ -266,3 +266,13 @@ def test_what_rounding_takes_from_the_output_is_kept(dtype, d):
             both = np64(out) + np64(low)
             assert abs(both - want["out"][0]).sum() < abs(np64(out) - want["out"][0]).sum()
     assert all(kept < 0.85 * alone for alone, kept in zip(*errors)), errors
+
+
+@pytest.mark.parametrize("dtype,d,hk", [(BF, 64, 2), (HF, 128, 1), (BF, 256, 1), (F32, 64, 2), (F32, 128, 1)])
+@pytest.mark.parametrize("t,window,sinks", [(2300, 40, 150), (1700, 100, 190), (1500, 64, 20), (1500, 1, 250), (700, 300, 400),
+                                            (701, 300, 400)])
+def test_partials_of_many_sinks(dtype, d, hk, t, window, sinks):
+    """Last blocks of sinks of one wave, of two, of more, with several chunks of
+    queries; sinks and window that hide nothing, and one key."""
+    x = window_cases.inputs(1, 2, hk, t, d, dtype)
+    compare(run(x, window, sinks), window_cases.expected(*x, window, sinks))

@@ -138,3 +138,19 @@ def test_windows_that_are_refused(lib):
     size = lib.mi355x_attn_bwd_sink_workspace_bytes
     # positions past the sequence change nothing
     assert size(1, 2, 2, 64, 64, 64, 1 << 62, 1 << 62) == size(1, 2, 2, 64, 64, 64, 64, 64) > 0
+
+
+def test_workspaces_of_many_sinks(lib):
+    """Nothing for sinks that hide nothing, and for others no multiple of what they are."""
+    def size(b, h, hk, t, d, window, sinks):
+        return lib.mi355x_attn_bwd_sink_workspace_bytes(b, h, hk, t, t, d, window, sinks)
+
+    for b, h, hk, t, d, window, sinks in ((1, 12, 12, 8192, 64, 16, 8192), (1, 12, 12, 8192, 64, 16, 8176), (1, 4, 2, 500, 128, 400, 100)):
+        assert size(b, h, hk, t, d, window, sinks) == size(b, h, hk, t, d, t, 0)
+    assert size(1, 12, 12, 8192, 64, 16, 8175) > size(1, 12, 12, 8192, 64, 16, 0)
+    for b, h, hk, t, d, window, sinks in ((1, 32, 32, 32768, 128, 512, 1024), (1, 12, 12, 32768, 64, 512, 4096), (1, 12, 12, 8192, 64, 16, 4000),
+                                          (8, 16, 4, 32768, 64, 256, 65), (1, 4, 1, 4096, 256, 512, 4), (64, 64, 64, 100000, 64, 1, 64)):
+        more = size(b, h, hk, t, d, window, sinks) - size(b, h, hk, t, d, window, 0)
+        # 4096 blocks of 128 keys and each block's own, four times the last one's, dK and dV in f32
+        assert 0 < more <= 2 * 4 * d * (4 * 4096 * 128 + 2 * b * h * sinks), (t, sinks)
+    assert size(0, 2, 2, 64, 64, 8, 1) >= 0

@@ -1195,7 +1195,8 @@ __device__ __forceinline__ void dkv_body(const AttnBwdArgs& p, WindowPos at, cha
       int64_t plane = 0;
       if (extra || (!p.kv_part && kj < f.sinks)) {
         if (kj >= f.sinks) continue;
-        pk = sink_slot(p, extra ? 1 + 4 * at.chunk + part : 0, b, h, kj, D), plane = sink_plane(p, D);
+        const SinkRows rows = sink_rows(p);
+        pk = p.sink_part + rows.at(b * f.H + h, kj, at.chunk, part, 4 * KW) * D, plane = rows.count() * D;
       } else if (p.kv_part) {
         const int64_t hkn = f.H / f.group, gi = h - hk * f.group;
         pk = p.kv_part + (((gi * f.B + b) * hkn + hk) * f.Skv + kj) * D, plane = f.B * f.H * f.Skv * D;
@@ -2041,7 +2042,8 @@ int attn_fwd_sink_mfma(const void* o, const int64_t* o_bhs, void* o_low, float* 
 // Bytes of the sinks' partials, behind the workspace's other parts.
 int64_t attn_bwd_sink_bytes(int64_t batch, int64_t heads, int64_t sq, int64_t skv, int64_t d, int64_t window,
                             int64_t sinks) {
-  return 2 * (4 * (int64_t)sink_chunks(sq, window, sinks) + 1) * batch * heads * sink_keys(skv, sinks) * d * (int64_t)sizeof(float) + 256;
+  const SinkRows rows{batch * heads, (int)sink_keys(skv, sinks), sink_chunks(batch * heads, sq, window, sinks)};
+  return 2 * rows.count() * d * (int64_t)sizeof(float) + 256;
 }
 
 int attn_bwd_sink_mfma(void* dq, const int64_t* dq_bhs, void* dk, const int64_t* dk_bhs, void* dv,

@@ -477,13 +477,12 @@ __device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t t
   }
   if (kj >= p.Skv) return;
   if constexpr (WIN) {  // partials: of sinks, and of a head of a group
-    const int64_t keys = p.sink_keys, slots = 4 * (int64_t)p.sink_chunks + 1;
+    const SinkRows rows{p.B * p.H, p.sink_keys, p.sink_chunks};
     if (extra || (!p.kv_part && kj < p.sinks)) {
       if (kj >= p.sinks) return;
-      const int64_t slot = extra ? 1 + 4 * chunk + part : 0;
-      float* pk = p.sink_part + (((slot * p.B + b) * p.H + h) * keys + kj) * D;
+      float* pk = p.sink_part + rows.at(b * p.H + h, kj, extra ? chunk : -1, part, kBlk) * D;
       T::store(pk, dk, lg, 1.f);
-      return T::store(pk + slots * p.B * p.H * keys * D, dv, lg, 1.f);
+      return T::store(pk + rows.count() * D, dv, lg, 1.f);
     }
     if (p.kv_part) {
       const int64_t hkn = p.H / p.group, gi = h - hk * p.group;

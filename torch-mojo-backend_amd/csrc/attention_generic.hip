@@ -535,9 +535,12 @@ extern "C" int mi355x_attn_bwd_gen(void* dq, const int64_t* dq_bhs, void* dk, co
 }
 
 // A window past the queries and sinks past the keys mask what the clipped ones
-// do, and sums of positions with them stay in range.
+// do, and sums of positions with them stay in range.  Where the last query sees
+// all keys up to its own, nothing but the causal order hides any: no sinks, whose
+// gradients' partials take memory and time.
 static void clip_window(int64_t& window, int64_t& sinks, int64_t sq, int64_t skv) {
   window = std::min(window, std::max(sq, (int64_t)1)), sinks = std::min(sinks, skv);
+  if (sq <= window + sinks) window = std::max(sq, (int64_t)1), sinks = 0;
 }
 
 // A window with sinks: causal, query i sees key j iff i - j < window or j <

@@ -47,27 +47,38 @@ struct AttnBwdArgs {
   float* sink_part;    // sinks: f32 partials of their dK, dV (dkv_body)
   int sink_blocks;     // blocks of keys that hold sinks
   int sink_chunks;     // further blocks for each, which share the queries behind its window
-  int sink_keys;       // rows of a slot of sink_part
+  int sink_keys;       // how many sinks there are
   // (stored negated: the dK/dV and dQ steps add them, which saves a negation
   // per score)
 };
 
-// Slots of sink_part: 0 for the window of a block of sinks (grouped heads have
-// that in kv_part), then four (one a wave) for each chunk.
-__device__ __forceinline__ float* sink_slot(const AttnBwdArgs& p, int64_t slot, int64_t b, int64_t h, int64_t key, int D) {
-  return p.sink_part + (((slot * p.f.B + b) * p.f.H + h) * p.sink_keys + key) * D;
-}
-__host__ __device__ inline int64_t sink_plane(const AttnBwdArgs& p, int D) {  // from dK's slots to dV's
-  return (4 * (int64_t)p.sink_chunks + 1) * p.f.B * p.f.H * p.sink_keys * D;
-}
+// Rows of the sinks' f32 partials, of dK and then of dV: of the window of a
+// block of sinks (grouped heads have that in kv_part) and of each chunk, and,
+// of a last block of at most two waves, up to three more a chunk, since four or
+// two waves then share a key.
+struct SinkRows {
+  int64_t heads;  // in all of the batch
+  int keys, chunks;
+  __host__ __device__ int shared() const { return keys < 64 ? keys : 64; }
+  __host__ __device__ int64_t count() const {
+    return heads * ((int64_t)keys * (chunks + 1) + (int64_t)shared() * 3 * chunks);
+  }
+  // Of head bh of the batch and a key in a block of `block`, from its window
+  // (chunk -1) or a chunk, by the part-th of the waves that share the key.
+  __device__ __forceinline__ int64_t at(int64_t bh, int64_t key, int chunk, int part, int block) const {
+    if (part == 0) return ((int64_t)(chunk + 1) * heads + bh) * keys + key;
+    return heads * keys * (chunks + 1) + ((int64_t)(3 * chunk + part - 1) * heads + bh) * shared() + key % block;
+  }
+};
+__device__ __forceinline__ SinkRows sink_rows(const AttnBwdArgs& p) { return {p.f.B * p.f.H, p.sink_keys, p.sink_chunks}; }
 
 // KW: keys of a wave of the kernel that left the partials, which has four.
 //
 // dK = scale * the sum of its f32 partials, dV likewise.  The first `plain`
 // blocks take the keys that are no sinks of grouped heads, four head-dim
 // elements per thread: the sum over the group's query heads, in head order.
-// Each further block takes one sink, whose partials are many (a slot a wave of
-// the blocks that shared its queries, and each head): its threads sum every
+// Each further block takes one sink, whose partials are many (a row of each
+// block, or wave, that shared its queries, and each head): its threads sum every
 // kSlices-th of them, and the slices are added in order.  (One thread for all
 // of them waited for 112 loads in turn: 36 us for Gemma's local layer at 4096
 // tokens, 15 with four slices of 64 threads each, 12.7 with sixteen.)
@@ -100,8 +111,9 @@ __global__ void __launch_bounds__(kSumThreads) attn_bwd_window_sum(AttnBwdArgs p
   __shared__ f32x4 part[2][kSumThreads];
   const int64_t row = blockIdx.x - plain, key = row % p.sink_keys, bhk = row / p.sink_keys, hk = bhk % hkn, b = bhk / hkn;
   const int slice = threadIdx.x / (D / 4), d = (int)(threadIdx.x % (D / 4)) * 4;
-  const int64_t splane = sink_plane(p, D);
-  // of a chunk's four slots, those that waves of the sink's block wrote
+  const SinkRows rows = sink_rows(p);
+  const int64_t splane = rows.count() * D;
+  // the waves that shared the sink's block
   const int waves = (int)min((int64_t)4, (p.sink_keys - key / (4 * KW) * (4 * KW) + KW - 1) / KW);
   const int parts = waves == 1 ? 4 : waves == 2 ? 2 : 1;
   const int each = 1 + p.sink_chunks * parts, total = (int)f.group * each;  // partials of a head, of all
@@ -110,7 +122,7 @@ __global__ void __launch_bounds__(kSumThreads) attn_bwd_window_sum(AttnBwdArgs p
     const int g = i / each, n = i - g * each, c = (n - 1) / parts;
     const int64_t h = hk * f.group + g;
     const float* pk = n == 0 && p.kv_part ? p.kv_part + (((g * f.B + b) * hkn + hk) * f.Skv + key) * D
-                                          : sink_slot(p, n == 0 ? 0 : 1 + 4 * c + (n - 1 - c * parts), b, h, key, D);
+                                          : p.sink_part + rows.at(b * f.H + h, key, n == 0 ? -1 : c, n == 0 ? 0 : n - 1 - c * parts, 4 * KW) * D;
     sk += *(const f32x4*)(pk + d), sv += *(const f32x4*)(pk + d + (n == 0 && p.kv_part ? plane : splane));
   }
   part[0][threadIdx.x] = sk, part[1][threadIdx.x] = sv;
@@ -122,10 +134,14 @@ __global__ void __launch_bounds__(kSumThreads) attn_bwd_window_sum(AttnBwdArgs p
 
 // Blocks that share the steps behind the window of a block of sinks: eight
 // steps each, which their four waves share where there are few sinks, so that
-// one is shorter than a block of a window of 512 and more.
-inline int sink_chunks(int64_t sq, int64_t window, int64_t sinks) {
+// one is shorter than a block of a window of 512 and more.  Fewer and longer
+// ones where there would be more than 4096, sixteen a CU, in all: each leaves
+// partials of its sinks.
+inline int sink_chunks(int64_t heads, int64_t sq, int64_t window, int64_t sinks) {
   const int64_t rest = (sq + 63) / 64 - window / 64;
-  return sinks <= 0 || rest <= 0 ? 0 : (int)std::min<int64_t>((rest + 7) / 8, 1024);
+  if (sinks <= 0 || rest <= 0) return 0;
+  const int64_t blocks = std::max<int64_t>(1, heads * ((sinks + 63) / 64));
+  return (int)std::min<int64_t>((rest + 7) / 8, std::max<int64_t>(1, std::min<int64_t>(1024, 4096 / blocks)));
 }
 inline int64_t sink_keys(int64_t skv, int64_t sinks) { return std::min(skv, sinks); }
 
@@ -133,7 +149,7 @@ inline int64_t sink_keys(int64_t skv, int64_t sinks) { return std::min(skv, sink
 // other parts.
 inline void window_parts(AttnBwdArgs& a, int64_t d) {
   const int64_t rows = a.f.B * a.f.H * a.f.Sq;
-  a.sink_chunks = sink_chunks(a.f.Sq, a.f.window, a.f.sinks), a.sink_keys = (int)sink_keys(a.f.Skv, a.f.sinks);
+  a.sink_chunks = sink_chunks(a.f.B * a.f.H, a.f.Sq, a.f.window, a.f.sinks), a.sink_keys = (int)sink_keys(a.f.Skv, a.f.sinks);
   float* end = a.kv_part ? a.kv_part + 2 * a.f.B * a.f.H * a.f.Skv * d : a.ndelta + 2 * rows;
   a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
 }
