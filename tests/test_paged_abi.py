@@ -154,3 +154,14 @@ def test_workspaces_of_many_sinks(lib):
         # 4096 blocks of 128 keys and each block's own, four times the last one's, dK and dV in f32
         assert 0 < more <= 2 * 4 * d * (4 * 4096 * 128 + 2 * b * h * sinks), (t, sinks)
     assert size(0, 2, 2, 64, 64, 8, 1) >= 0
+
+
+@pytest.mark.parametrize("dtype,h,hk,t,d,sinks", [
+    (F32, 64, 64, 131072, 64, 65536), (BF16, 64, 64, 131072, 64, 65536), (BF16, 32, 1, 2 ** 27, 64, 1),
+    (BF16, 4096, 4096, 2 ** 18, 64, 0)])
+def test_window_backwards_of_too_many_blocks(lib, dtype, h, hk, t, d, sinks):
+    """Sums in 1024 threads, of sinks and of grouped heads, and blocks: refused before the first launch."""
+    s = bht(t * d, d, d)
+    assert lib.mi355x_attn_bwd_sink(P, s, P, s, P, s, P, s, P, s, P, s, P, s, P, s, None, P, 1, h, hk, t, t, d, 0.1, 1, sinks, dtype, P,
+                                    1 << 62, None) == EINVAL
+    assert b"blocks" in lib.mi355x_last_error() or b"sums" in lib.mi355x_last_error() or b"threads" in lib.mi355x_last_error()

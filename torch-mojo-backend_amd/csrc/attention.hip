@@ -1932,10 +1932,13 @@ int gqa_bwd_launch(const AttnBwdArgs& a, hipStream_t s) {
 
 template <typename T, int D>
 int window_bwd_launch(AttnBwdArgs a, hipStream_t s) {
+  constexpr int KB = 64 * kKeyTiles<D>, QB = 64 * kQueryTiles;
+  a.sink_blocks = (a.sink_keys + KB - 1) / KB;
   const int64_t rows = a.f.B * a.f.H * a.f.Sq;
-  MI_REQUIRE(rows < (1ll << 31), "mi355x_attn_bwd_sink: batch x heads x query rows must be below 2^31");
-  auto delta = a.f.o_low ? attn_bwd_delta<T, D, true> : attn_bwd_delta<T, D>;
-  delta<<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
+  const int64_t nkx = (a.f.Skv + KB - 1) / KB, nqx = (a.f.Sq + QB - 1) / QB, bh = a.f.H * a.f.B;
+  const int64_t blocks = bh * (nkx + nqx + (int64_t)a.sink_blocks * a.sink_chunks);
+  const int rc = window_launches(a, D, rows * (D / 8), blocks);
+  if (rc) return rc;
   auto k = attn_bwd_window<T, D>;
   static std::once_flag once;
   static hipError_t attr_err = hipSuccess;
@@ -1944,14 +1947,10 @@ int window_bwd_launch(AttnBwdArgs a, hipStream_t s) {
   });
   if (attr_err != hipSuccess)
     return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_sink: cannot raise the LDS limit: %s", hipGetErrorString(attr_err));
-  constexpr int KB = 64 * kKeyTiles<D>, QB = 64 * kQueryTiles;
-  a.sink_blocks = (a.sink_keys + KB - 1) / KB;
-  const int64_t nkx = (a.f.Skv + KB - 1) / KB, nqx = (a.f.Sq + QB - 1) / QB, bh = a.f.H * a.f.B;
-  const int64_t blocks = bh * (nkx + nqx + (int64_t)a.sink_blocks * a.sink_chunks);
-  MI_REQUIRE(blocks < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)blocks);
+  auto delta = a.f.o_low ? attn_bwd_delta<T, D, true> : attn_bwd_delta<T, D>;
+  delta<<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, s>>>(a);
   k<<<(unsigned)blocks, kThreads, kWindowLds<D>, s>>>(a, (uint32_t)nkx, (uint32_t)nqx);
-  const int rc = window_sum_launch<T, D, 16 * kKeyTiles<D>>(a, s);
-  if (rc) return rc;
+  window_sum_launch<T, D, 16 * kKeyTiles<D>>(a, s);
   return check_launch("mi355x_attn_bwd_sink");
 }
 

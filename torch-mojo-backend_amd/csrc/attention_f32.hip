@@ -554,10 +554,7 @@ int run_window_fwd(const AttnF32& p, hipStream_t s) {
 
 template <int D>
 int run_window_bwd(AttnF32 p, hipStream_t s) {
-  static const bool ok = opt_in((const void*)bwd_window_f32<D>, lds_bytes<D>(true));
-  if (!ok) return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_sink: cannot reserve %zu bytes of LDS", lds_bytes<D>(true));
   const int64_t rows = p.B * p.H * p.Sq;
-  delta_f32<D><<<ceil_div(rows * kChains<D>, kNT), kNT, 0, s>>>(p, rows);
   AttnBwdArgs a{};
   a.f.B = p.B, a.f.H = p.H, a.f.Sq = p.Sq, a.f.Skv = p.Skv, a.f.scale = p.scale, a.f.group = p.group;
   a.f.window = p.window, a.f.sinks = p.sinks;
@@ -570,11 +567,15 @@ int run_window_bwd(AttnF32 p, hipStream_t s) {
   p.sink_chunks = a.sink_chunks, p.sink_keys = a.sink_keys, p.sink_blocks = (a.sink_keys + kBlk - 1) / kBlk;
   const int64_t kblk = (p.Skv + kBlk - 1) / kBlk, qblk = (p.Sq + kBlk - 1) / kBlk, heads = p.B * p.H;
   const int64_t extra = (int64_t)p.sink_blocks * p.sink_chunks;
-  MI_REQUIRE((kblk + qblk + extra) * heads < (1ll << 24), "mi355x_attn_bwd_sink: too many blocks");
+  const int rc = window_launches(a, D, rows * kChains<D>, (kblk + qblk + extra) * heads);
+  if (rc) return rc;
+  static const bool ok = opt_in((const void*)bwd_window_f32<D>, lds_bytes<D>(true));
+  if (!ok) return fail(MI355X_ELAUNCH, "mi355x_attn_bwd_sink: cannot reserve %zu bytes of LDS", lds_bytes<D>(true));
+  delta_f32<D><<<ceil_div(rows * kChains<D>, kNT), kNT, 0, s>>>(p, rows);
   bwd_window_f32<D><<<(unsigned)((kblk + qblk + extra) * heads), kNT, lds_bytes<D>(true), s>>>(
       p, (uint32_t)(kblk * heads), (uint32_t)(extra * heads), (uint32_t)kblk, (uint32_t)qblk);
-  const int rc = window_sum_launch<float, D, 16>(a, s);
-  return rc ? rc : check_launch("mi355x_attn_bwd_sink");
+  window_sum_launch<float, D, 16>(a, s);
+  return check_launch("mi355x_attn_bwd_sink");
 }
 
 // Tiles are loaded and rows stored 16 bytes at a time.

@@ -154,14 +154,27 @@ inline void window_parts(AttnBwdArgs& a, int64_t d) {
   a.sink_part = (float*)(((uintptr_t)end + 255) & ~(uintptr_t)255);
 }
 
-template <typename T, int D, int KW>
-inline int window_sum_launch(const AttnBwdArgs& a, hipStream_t s) {
-  const int64_t kvh = a.f.B * (a.f.H / a.f.group);
-  const unsigned plain = a.kv_part ? ceil_div(kvh * (a.f.Skv - a.sink_keys) * (D / 4), kSumThreads) : 0;
-  const int64_t sums = plain + kvh * a.sink_keys;
-  MI_REQUIRE(sums < (1ll << 24), "mi355x_attn_bwd_sink: %lld blocks", (long long)sums);
-  if (sums) attn_bwd_window_sum<T, D, KW><<<(unsigned)sums, kSumThreads, 0, s>>>(a, plain);
+// Blocks of the two kinds of attn_bwd_window_sum.
+inline int64_t window_sum_plain(const AttnBwdArgs& a, int D) {
+  return a.kv_part ? (a.f.B * (a.f.H / a.f.group) * (a.f.Skv - a.sink_keys) * (D / 4) + kSumThreads - 1) / kSumThreads : 0;
+}
+inline int64_t window_sum_blocks(const AttnBwdArgs& a, int D) {
+  return window_sum_plain(a, D) + a.f.B * (a.f.H / a.f.group) * a.sink_keys;
+}
+
+// What a launch can have, 2^32 threads, for all of a backward's before its first.
+inline int window_launches(const AttnBwdArgs& a, int D, int64_t delta_threads, int64_t blocks) {
+  const int64_t sums = window_sum_blocks(a, D);
+  MI_REQUIRE(delta_threads < (1ll << 32) - kThreads, "mi355x_attn_bwd_sink: %lld threads", (long long)delta_threads);
+  MI_REQUIRE(blocks < (1ll << 32) / kThreads, "mi355x_attn_bwd_sink: %lld blocks", (long long)blocks);
+  MI_REQUIRE(sums < (1ll << 32) / kSumThreads, "mi355x_attn_bwd_sink: %lld sums of sinks and heads", (long long)sums);
   return MI355X_OK;
+}
+
+template <typename T, int D, int KW>
+inline void window_sum_launch(const AttnBwdArgs& a, hipStream_t s) {
+  const int64_t sums = window_sum_blocks(a, D);
+  if (sums) attn_bwd_window_sum<T, D, KW><<<(unsigned)sums, kSumThreads, 0, s>>>(a, (uint32_t)window_sum_plain(a, D));
 }
 
 }  // namespace
