@@ -6,6 +6,7 @@ import torch
 
 import decode_cases as cases
 import paged_standin  # noqa: F401
+from torch_mojo_backend.kv_cache import PagedKVCache
 
 
 @pytest.fixture(params=["cpu", "mojo"])
@@ -50,3 +51,26 @@ def test_one_cache_a_layer(device):
     table = torch.zeros(1, 1, dtype=torch.int32).to(device)
     with pytest.raises(ValueError):
         m.forward_cached(torch.zeros(1, 1, dtype=torch.int64).to(device), m.caches(1, 4)[:2], table, table.view(1))
+
+
+@pytest.mark.parametrize("weights", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("pages", [None, torch.float32, torch.bfloat16, 4])
+def test_under_autocast(device, weights, pages):
+    """Rows leave the projections in autocast's type; pages keep their own."""
+    m, ref = cases.model(weights, device)
+    if pages is not None:
+        kw = {"bits": 4} if pages == 4 else {"dtype": pages}
+        m.caches = lambda n, size, *, bits=None: [
+            PagedKVCache.zeros(n, size, m.cfg.kv_heads, m.cfg.head_dim, device=device, **kw) for _ in m.blocks]
+    idx = cases.tokens(2, 20)
+    with torch.no_grad():
+        want = ref(idx)
+        with torch.autocast(device, dtype=torch.bfloat16):
+            whole = m(idx.to(device)).cpu().double()
+            got = cases.run(m, idx, STEPS, device)
+        plain = cases.run(m, idx, STEPS, device)
+    lim = cases.bound(torch.bfloat16, want, 97)
+    assert (whole - want).abs().max() <= lim
+    for x in (got, plain):
+        assert torch.isfinite(x).all()
+        assert pages == 4 or (x - want).abs().max() <= lim

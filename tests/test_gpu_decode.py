@@ -61,3 +61,16 @@ def test_many_calls(dtype, bits, d, page):
             o = ops.paged_attention(turned, cache, c.dev_table, c.ints(at), counts=c.ints(counts), window=window, sinks=sinks)
             check(o, *c.expected(turned.cpu(), at, counts, window, sinks), f"{counts} window {window}")
         at = ends
+
+
+@pytest.mark.parametrize("weights", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [None, 4])
+def test_under_autocast(weights, bits):
+    m, ref = cases.model(weights, "mojo", head_dim=64, window=7)
+    idx = cases.tokens(3, 60)
+    with torch.no_grad():
+        want = ref(idx)
+        with torch.autocast("mojo", dtype=torch.bfloat16):
+            got = cases.run(m, idx, [[30, 1, 7], [1, 1, 1], [29, 58, 52]], "mojo", bits=bits)
+    assert torch.isfinite(got).all()
+    assert bits == 4 or (got - want).abs().max() <= cases.bound(torch.bfloat16, want, 4 * 64)

@@ -117,9 +117,12 @@ class Attention(nn.Module):
         b, t, _ = x.shape
         c = self.cfg
         q, k, v = self._qkv(x)
+        dtype = q.dtype
+        if cache.bits != 4:  # under autocast, or over pages of a type of their own
+            q, k, v = q.to(cache.dtype), k.to(cache.dtype), v.to(cache.dtype)
         q = ops.paged_append(cache, page_table, starts, k, v, *rope, q=q, counts=counts)
         window, sinks = (c.window, c.sinks) if self.local else (0, 0)
-        y = ops.paged_attention(q, cache, page_table, starts, counts=counts, window=window, sinks=sinks)
+        y = ops.paged_attention(q, cache, page_table, starts, counts=counts, window=window, sinks=sinks).to(dtype)
         return self.o_proj(y.transpose(1, 2).reshape(b, t, c.heads * c.head_dim))
 
 
@@ -211,10 +214,14 @@ class Gemma3(nn.Module):
         pages]); these are put there too.  Tokens from counts[b] on are padding."""
         c = self.cfg
         dev, dt = idx.device, self.embed.weight.dtype
-        need, key = page_table.shape[1] * caches[0].page_size, (str(dev), dt)
+        # angles in the type of the rows that they turn where that is the weights', else in f32
+        rows = torch.get_autocast_dtype(dev.type) if torch.is_autocast_enabled(dev.type) else dt
+        same = all((rows if cache.bits == 4 else cache.dtype) == dt for cache in caches)
+        angles = dt if same else torch.float32
+        need, key = page_table.shape[1] * caches[0].page_size, (str(dev), angles)
         rope = self._cached_tables.get(key)
         if rope is None or rope[0][0].shape[0] < need:
-            rope = tuple(rope_tables(need, c.head_dim, base, dev, dt) for base in (c.rope_local_base, c.rope_global_base))
+            rope = tuple(rope_tables(need, c.head_dim, base, dev, angles) for base in (c.rope_local_base, c.rope_global_base))
             self._cached_tables = {key: rope}
         x = self.embed(idx) * torch.tensor(c.hidden ** 0.5, dtype=dt, device=dev)
         for blk, cache in zip(self.blocks, caches, strict=True):
