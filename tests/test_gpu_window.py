@@ -276,3 +276,14 @@ def test_partials_of_many_sinks(dtype, d, hk, t, window, sinks):
     queries; sinks and window that hide nothing, and one key."""
     x = window_cases.inputs(1, 2, hk, t, d, dtype)
     compare(run(x, window, sinks), window_cases.expected(*x, window, sinks))
+
+
+@pytest.mark.parametrize("dtype,d,hk", [(BF, 64, 2), (F32, 256, 1)])
+def test_a_gradient_of_the_gradient_is_refused(dtype, d, hk):
+    x = window_cases.inputs(1, 2, hk, 90, d, dtype)
+    q, k, v = (y.to("mojo").requires_grad_() for y in x[:3])
+    out = ops.sliding_window_attention(q, k, v, 20, sinks=2)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), x[3].to("mojo"), create_graph=True)
+    compare({"out": out, "dq": dq, "dk": dk, "dv": dv}, window_cases.expected(*x, 20, 2))
+    with pytest.raises(RuntimeError, match="second time"):
+        (out.float().sum() + (dk.float() * dk.float()).sum()).backward()

@@ -78,3 +78,16 @@ def test_refusals(device):
             att(q, k.cpu(), v.cpu(), 3)
         with pytest.raises(NotImplementedError):
             att(q.double(), k.double(), v.double(), 3)
+
+
+@pytest.mark.parametrize("window,sinks", [(3, 0), (3, 2), (30, 0)])
+def test_a_gradient_of_the_gradient_is_refused(device, window, sinks):
+    """Where it is not known: a second term of a loss must not be left out in silence."""
+    x = window_cases.inputs(1, 2, 1, 9, 16, torch.float32)
+    q, k, v = (leaf(y, device) for y in x[:3])
+    out = ops.sliding_window_attention(q, k, v, window, sinks=sinks)
+    dq, = torch.autograd.grad(out.sum(), q, create_graph=True)
+    assert dq.requires_grad
+    check(dq, *window_cases.expected(*x[:3], torch.ones_like(x[3]), window, sinks)["dq"])
+    with pytest.raises(RuntimeError, match="differentia|derivative"):
+        (out.sum() + (dq * dq).sum()).backward()

@@ -104,7 +104,23 @@ class _FusedAttention(torch.autograd.Function):
         with torch._C._AutoDispatchBelowAutograd():
             dq, dk, dv = paged.on_device(q._device, aten_fast.attention_backward, grad, q, k, v, out, lse, causal, window,
                                          scale, sinks, low)
+        if torch.is_grad_enabled():  # create_graph
+            dq, dk, dv = _OneGradient.apply(dq, dk, dv, q, k, v, grad)
         return dq, dk, dv, None, None, None, None
+
+
+class _OneGradient(torch.autograd.Function):
+    """dq, dk, dv as they are, with an error for a graph that the fused
+    kernels do not leave: without one, a loss with a term of the gradient
+    would lose that term in silence."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, *inputs):
+        return dq.view_as(dq), dk.view_as(dk), dv.view_as(dv)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradient of fused attention is not differentiable a second time")
 
 
 def register_autograd_ops() -> None:
