@@ -287,3 +287,17 @@ def test_a_gradient_of_the_gradient_is_refused(dtype, d, hk):
     compare({"out": out, "dq": dq, "dk": dk, "dv": dv}, window_cases.expected(*x, 20, 2))
     with pytest.raises(RuntimeError, match="second time"):
         (out.float().sum() + (dk.float() * dk.float()).sum()).backward()
+
+
+@pytest.mark.parametrize("dtype,d,h,hk", [(F32, 64, 2, 2), (F32, 32, 4, 2), (F32, 256, 2, 1), (BF, 128, 4, 1), (HF, 256, 2, 2), (BF, 96, 2, 1),
+                                          (BF, 64, 2, 2), (HF, 64, 4, 2)])
+@pytest.mark.parametrize("t,window", [(300, 32), (130, 129), (130, 200)])
+def test_masks_without_sinks(dtype, d, h, hk, t, window):
+    """The kernels of ops.sliding_window_attention, but for 16-bit types at head_dim 64."""
+    x = window_cases.inputs(1, h, hk, t, d, dtype)
+    got = run(x, window, 0, mask=sliding_window_causal_mask(t, window, "mojo"))
+    compare(got, window_cases.expected(*x, window, 0))
+    if t > window and (dtype is F32 or d != 64):
+        op = run(x, window, 0)
+        for n in op:
+            assert torch.equal(op[n].detach().cpu(), got[n].detach().cpu()), n

@@ -91,3 +91,17 @@ def test_a_gradient_of_the_gradient_is_refused(device, window, sinks):
     check(dq, *window_cases.expected(*x[:3], torch.ones_like(x[3]), window, sinks)["dq"])
     with pytest.raises(RuntimeError, match="differentia|derivative"):
         (out.sum() + (dq * dq).sum()).backward()
+
+
+@pytest.mark.parametrize("dtype,d,sinks,new", [(torch.float32, 64, 0, True), (torch.bfloat16, 128, 0, True), (torch.float16, 256, 0, True),
+                                               (torch.bfloat16, 96, 0, True), (torch.bfloat16, 64, 0, False), (torch.float16, 64, 0, False),
+                                               (torch.bfloat16, 64, 1, True), (torch.float32, 32, 0, True)])
+def test_masks_reach_the_windows_kernels(mojo, monkeypatch, dtype, d, sinks, new):
+    from torch_mojo_backend.eager_kernels import aten_fast
+
+    if mojo != "host":
+        pytest.skip("the stand-in is for machines without a GPU")
+    x = [y.to("mojo") for y in window_cases.inputs(1, 2, 1, 9, d, dtype)[:3]]
+    mask = sliding_window_causal_mask(9, 3, "mojo", sinks=sinks)
+    seen = aten_fast.fused_fa_ex_inputs(*x, mask, 0.0, False, None, True)
+    assert seen[3:] == (True, 3, sinks if new else None)

@@ -2408,7 +2408,18 @@ def fused_fa_ex_inputs(query, key, value, attn_mask, dropout_p, is_causal, scale
         w = window_and_sinks_of(attn_mask)
         if w is None or is_causal or sq != skv or attn_mask.shape[-1] != skv:
             return None
-        causal, window, sinks = True, w[0], w[1] or None
+        causal, window, sinks = True, w[0], w[1]
+        # Without sinks the window's kernels, as in ops.sliding_window_attention,
+        # but for 16-bit types at head_dim 64, where those of plain windows are
+        # faster by up to a tenth.  Forward + backward, plain windows' against
+        # these: bf16 [8, 16 over 4, 4096, 64], window 256, 88 + 353 against 110 +
+        # 372 us, [2, 12, 255, 64] 11 + 19 against 11 + 21 (a long window gains
+        # from these: [1, 12, 8192, 64], 1024, 48 + 170 against 55 + 116); head_dim
+        # 128 [2, 16 over 4, 2000], 512, 48 + 139 against 35 + 141, 256 [1, 4 over
+        # 1, 4096], 512, 27 + 97 against 24 + 92; f32 [2, 12, 255, 64], 64, 35 + 80
+        # against 13 + 21, [4, 16 over 4, 2000, 128], 512, 1538 + 5322 against 359 + 1139.
+        if not sinks and q._dtype in _MFMA_DTYPES and q._shape[3] == 64:
+            sinks = None
     return q, k, v, causal, window, sinks
 
 

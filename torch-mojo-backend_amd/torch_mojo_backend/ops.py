@@ -108,7 +108,8 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
     h // (H // H_kv); scale defaults to D ** -0.5.  Differentiable in q, k and
     v.  The scores of what is not visible are not computed, and no mask is
     held: F.scaled_dot_product_attention with a mask of
-    masks.sliding_window_causal_mask runs the same kernels."""
+    masks.sliding_window_causal_mask runs the same kernels, but for bf16 and f16
+    at head_dim 64 without sinks, where it keeps those of plain windows."""
     what = "sliding_window_attention"
     window, sinks = int(window), int(sinks)
     if window <= 0 or sinks < 0:
