@@ -694,7 +694,8 @@ typedef struct {
 /* Writes the tokens' keys (turned by the angles of their positions: row p of
  * the dense [rope_len][d] tables of rope_dtype, as in mi355x_rope; null: as
  * they are) and values to their pages; q, if given, is turned into q_out,
- * zero at padding.  *_bht: (batch, head, token) strides in elements.
+ * zero at padding.  *_bht: (batch, head, token) strides in elements.  The
+ * rows must not lie in the pages.
  * 4 bits: per 32 channels minimum = f16(f32(min)), scale = f16(f32((max -
  * min) / 15)), code = clamp(rint((x - minimum) / scale), 0, 15) in f64, with x clamped to
  * +-61440; a group with a NaN or an infinity reads back as NaN. */

@@ -356,3 +356,16 @@ def test_codes_are_of_clamped_values(dtype, d, turned):
     assert np.abs(want).max() <= 61440 + 16 + 15 * 2  # half a step of the minimum, and 15 of the scale
     for got in ops.paged_gather(c, zero, zero.view(1), 8):
         assert (np64(got) == want.astype(np.float32)).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (F32, 96)])
+def test_tokens_moved_within_the_pages(dtype, d):
+    """Rows that are views of the pages are read before any is written."""
+    n, hk = 4096, 3
+    g = torch.Generator().manual_seed(7)
+    old = [torch.randn(1, hk, n, d, generator=g).to(dtype) for _ in range(2)]
+    c = PagedKVCache(*(x.to("mojo") for x in old))
+    zero = torch.zeros(1, 1, dtype=torch.int32).to("mojo")
+    ops.paged_append(c, zero, zero.view(1) + 1, c.k[:, :, :-1], c.v[:, :, :-1])
+    for x, was in zip((c.k.cpu(), c.v.cpu()), old):
+        assert torch.equal(x[:, :, 1:], was[:, :, :-1]) and torch.equal(x[:, :, :1], was[:, :, :1])

@@ -299,3 +299,35 @@ def test_sharing_is_told_as_it_is():
         assert _share(a, b) == _share(b, a) == want
         found[want] += 1
     assert min(found) > 200
+
+
+@pytest.mark.parametrize("what", ["k", "v", "q", "none"])
+def test_rows_of_the_pages_themselves(device, monkeypatch, what):
+    """Tokens moved within the cache: the rows are read before any is written."""
+    if device == "mojo":
+        from host_standin import HostStandIn
+
+        call, seen = HostStandIn.mi355x_paged_append, []
+
+        def watched(self, cache, table, tst, width, starts, counts, *rest):
+            seen.append([r.value if hasattr(r, "value") else r for r in (rest[0], rest[2], rest[6])])
+            return call(self, cache, table, tst, width, starts, counts, *rest)
+
+        monkeypatch.setattr(HostStandIn, "mi355x_paged_append", watched)
+    n = 8
+    c = PagedKVCache(*(torch.randn(1, 2, n, 64, generator=torch.Generator().manual_seed(i)).to(device) for i in range(2)))
+    old = [x.cpu().clone() for x in (c.k, c.v)]
+    rows = {x: torch.ones(1, 2, n - 1, 64).to(device) for x in "kvq"}
+    if what != "none":
+        rows[what] = (c.v if what == "v" else c.k)[:, :, :-1]
+    cos, sin = torch.ones(n, 64).to(device), torch.zeros(n, 64).to(device)
+    zero = torch.zeros(1, 1, dtype=torch.int32).to(device)
+    out = ops.paged_append(c, zero, zero.view(1) + 1, rows["k"], rows["v"], cos, sin, q=rows["q"])
+    for name, x, was in (("k", c.k, old[0]), ("v", c.v, old[1])):
+        want = was[:, :, :-1] if what == name else torch.ones(1, 2, n - 1, 64)
+        assert torch.equal(x.cpu()[:, :, 1:], want) and torch.equal(x.cpu()[:, :, :1], was[:, :, :1])
+    assert torch.equal(out.cpu(), old[0][:, :, :-1] if what == "q" else torch.ones(1, 2, n - 1, 64))
+    if device == "mojo":
+        pages = [(t.data_ptr() if not hasattr(t, "_ptr") else t._ptr) for t in (c.k, c.v)]
+        for ptr in seen[0]:
+            assert not any(p <= ptr < p + 4 * 2 * n * 64 for p in pages)

@@ -72,10 +72,12 @@ def on_device(device: int, call, *args):
     return call(*args)
 
 
-def _rows(t: MT) -> MT:
-    """t itself when its rows can be read 16 bytes at a time, else a copy."""
+def _rows(t: MT, written=()) -> MT:
+    """t itself when its rows can be read 16 bytes at a time and do not lie in
+    a storage that the call writes (moved tokens: views of the pages), else a
+    copy."""
     st, n = t._strides, t._itemsize
-    if st[3] == 1 and not (t._ptr | st[0] * n | st[1] * n | st[2] * n) & 15:
+    if st[3] == 1 and not (t._ptr | st[0] * n | st[1] * n | st[2] * n) & 15 and id(t._holder) not in written:
         return t
     return materialize_contiguous(t)
 
@@ -99,11 +101,11 @@ def append(cache, table, starts, k, v, cos, sin, q, counts):
 
 def _append(cache, table, starts, k, v, cos, sin, q, counts, dev):
     b, _, t, d = k._shape
-    k, v = _rows(k), _rows(v)
+    k, v = _rows(k, cache.holders), _rows(v, cache.holders)
     out, q_args, rope = None, (None, None, None, None), (None, None, 0, 0)
     heads = 0
     if q is not None:
-        q, heads = _rows(q), q._shape[1]
+        q, heads = _rows(q, cache.holders), q._shape[1]
         out = alloc_bthd(b, heads, t, d, q._dtype, dev)
         q_args = out._ptr, _bht(out), q._ptr, _bht(q)
     if cos is not None:

@@ -86,6 +86,7 @@ class PagedKVCache:
             from .eager_kernels import paged
 
             self._desc = paged.describe(self)
+            self.holders = frozenset(id(t._holder) for t in tensors)  # their storages, which live as long as the cache
 
     def __reduce__(self):  # the kernels' description holds addresses
         return type(self), (self.k, self.v, self.k_scales, self.v_scales)

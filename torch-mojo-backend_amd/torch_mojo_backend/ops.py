@@ -191,7 +191,8 @@ def paged_append(cache, page_table, starts, k, v, cos=None, sin=None, *, q=None,
     One kernel.  A position outside the page table, a page that does not exist
     or a position outside cos raises IndexError (on the mojo device at the next
     device-to-host read) and is not written.  Two tokens of one call must not
-    name the same slot."""
+    name the same slot; rows that are views of the pages are read before any
+    is written."""
     if (paged.seqs_ok(cache, page_table, starts, counts) and paged.rows_ok(cache, k, page_table._shape[0])
             and paged.rows_ok(cache, v, page_table._shape[0], k) and k._shape[1] == cache.kv_heads and k._shape == v._shape
             and (cos is None) == (sin is None) == (q is None)
