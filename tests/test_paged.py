@@ -331,3 +331,15 @@ def test_rows_of_the_pages_themselves(device, monkeypatch, what):
         pages = [(t.data_ptr() if not hasattr(t, "_ptr") else t._ptr) for t in (c.k, c.v)]
         for ptr in seen[0]:
             assert not any(p <= ptr < p + 4 * 2 * n * 64 for p in pages)
+
+
+@pytest.mark.parametrize("bits", [None, 4])
+def test_a_caches_tensors_are_fixed(device, bits):
+    """The kernels would go on using the old ones."""
+    c = PagedKVCache.zeros(2, 4, 1, 64, dtype=torch.float32, bits=bits, device=device)
+    for name in ("k", "v", "k_scales", "v_scales"):
+        old = getattr(c, name)
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(c, name, old)
+        assert getattr(c, name) is old
+    c.note = 1  # other attributes are the user's

@@ -88,6 +88,12 @@ class PagedKVCache:
             self._desc = paged.describe(self)
             self.holders = frozenset(id(t._holder) for t in tensors)  # their storages, which live as long as the cache
 
+    def __setattr__(self, name, value):
+        # the kernels go by the addresses of the tensors that the cache was made with
+        if name in ("k", "v", "k_scales", "v_scales") and name in self.__dict__:
+            raise AttributeError(f"PagedKVCache: {name} is fixed: copy into it, or make another cache")
+        super().__setattr__(name, value)
+
     def __reduce__(self):  # the kernels' description holds addresses
         return type(self), (self.k, self.v, self.k_scales, self.v_scales)
 
