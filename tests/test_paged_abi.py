@@ -165,3 +165,11 @@ def test_window_backwards_of_too_many_blocks(lib, dtype, h, hk, t, d, sinks):
     assert lib.mi355x_attn_bwd_sink(P, s, P, s, P, s, P, s, P, s, P, s, P, s, P, s, None, P, 1, h, hk, t, t, d, 0.1, 1, sinks, dtype, P,
                                     1 << 62, None) == EINVAL
     assert b"blocks" in lib.mi355x_last_error() or b"sums" in lib.mi355x_last_error() or b"threads" in lib.mi355x_last_error()
+
+
+def test_windows_past_every_position_share_keys_as_none(lib):
+    size = lib.mi355x_paged_attn_workspace_bytes
+    none = size(cache(), 1000, 1, 2, 1, 0, 0, BF16)
+    for window, sinks in ((1 << 62, 1 << 62), ((1 << 63) - 1, 1), (1, (1 << 63) - 1), (1 << 20, 0)):
+        assert size(cache(), 1000, 1, 2, 1, window, sinks, BF16) == none > 0
+    assert size(cache(), 1000, 1, 2, 1, 100, 4, BF16) == 0

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join(DecodeArgs a) {
 int64_t most_keys(const mi355x_paged_cache& c, int64_t width, int64_t window, int64_t sinks) {
   int64_t n = width * c.page_size;
   if (n > kMaxPosition) n = kMaxPosition;
-  return window > 0 && window + sinks < n ? window + sinks : n;
+  return window > 0 && window < n && sinks < n - window ? window + sinks : n;
 }
 
 // Blocks that share the keys of a row, where rows alone are too few to fill
