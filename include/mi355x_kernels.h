@@ -663,7 +663,9 @@ int mi355x_attn_bwd_noalloc(void* dq, const int64_t* dq_bhs, void* dk,
  * in page table[b * table_stride + p / page_size], slot p % page_size.  Its row
  * of d channels (unit stride) is d values of `dtype` (bits = 0), or with
  * bits = 4 d / 2 bytes of codes and d / 32 pairs (scale, minimum) of f16, value
- * = minimum + scale * code.  32-bit word g * (d / 32) + s of a row of codes
+ * = minimum + scale * code, all within +-65504 and scale from 0 to 8192 (as
+ * mi355x_paged_append makes them; attention takes values in f16, where others may
+ * become infinities and NaN).  32-bit word g * (d / 32) + s of a row of codes
  * (g < 4) holds channels 32 s + 8 g + e (e < 8), channel e in nibble
  * e / 2 + 4 (e % 2).  *_phs: (page, head, slot) strides, of k and v in values
  * (bytes for codes), of the scales in f16 values.  Rows must be 16-byte

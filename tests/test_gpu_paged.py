@@ -369,3 +369,17 @@ def test_tokens_moved_within_the_pages(dtype, d):
     ops.paged_append(c, zero, zero.view(1) + 1, c.k[:, :, :-1], c.v[:, :, :-1])
     for x, was in zip((c.k.cpu(), c.v.cpu()), old):
         assert torch.equal(x[:, :, 1:], was[:, :, :-1]) and torch.equal(x[:, :, :1], was[:, :, :1])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("d,h", [(64, 1), (128, 20), (256, 4)])
+def test_4_bit_values_at_the_ends_of_the_range(dtype, d, h):
+    c = Case([90, 33], page=16, bits=4, device="mojo", d=d, hk=1, dtype=dtype)
+    g = torch.Generator().manual_seed(9)
+    v = ((torch.rand(2, 1, 90, d, generator=g) - 0.5) * 1e6).to(F32).to("mojo")  # most are clamped
+    k, _ = ops.paged_gather(c.cache, c.dev_table, c.ints([0, 0]), 90, counts=c.ints([90, 33]))
+    ops.paged_append(c.cache, c.dev_table, c.ints([0, 0]), k, v, counts=c.ints([90, 33]))
+    c.values = [np64(x) for x in ops.paged_gather(c.cache, c.dev_table, c.ints([0, 0]), 90, counts=c.ints([90, 33]))]
+    assert np.abs(c.values[1]).max() == 61440
+    _attention(c, h, [89, 32], [1, 1], 1, dtype)
+    _attention(c, h, [86, 29], [4, 4], 4, dtype, window=30, sinks=2)

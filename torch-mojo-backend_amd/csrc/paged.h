@@ -19,7 +19,8 @@ namespace mi {
 
 constexpr int kKvGroup = 32;  // channels per (scale, minimum) pair
 // Values are clamped to this before they are packed: minimum + 15 * scale,
-// both rounded to f16, then stays finite in f16 (61440 + 122880 * 2^-11 < 65504).
+// both rounded to f16, then stays finite in f16 (61440 + 122880 * 2^-11 < 65504),
+// as do twice the scale and 7.5 times it, which attention forms in f16.
 constexpr double kKvLimit = 61440.0;
 
 // Quotients of 31-bit positions by the page size: one multiply-high and a

@@ -5,14 +5,17 @@ A `PagedKVCache` is the storage of one attention layer: a page holds
 which pages a sequence owns, in order, so sequences of different lengths share
 one allocation and grow a page at a time.  `torch_mojo_backend.ops` has the
 operations on it: `paged_append`, `paged_attention`, `paged_gather`.  They run
-one gfx950 kernel each on the mojo device and the plain formulas below
-elsewhere (the CPU reference).
+one gfx950 kernel each on the mojo device (attention a second one, where blocks
+share the keys of a row) and the plain formulas below elsewhere (the CPU
+reference).
 
 With `bits=4` a row of `head_dim` channels is held as 4-bit codes with a scale
 and a minimum in float16 for each 32 channels (5 bits a value): minimum =
 min, scale = (max - min) / 15, value = minimum + scale * code.  Inputs are
 clamped to +-61440; 32 channels with a NaN or an infinity among them read back
-as NaN.
+as NaN.  Attention takes such values in float16: pages that were not filled by
+`paged_append` must keep to its range, minimum + scale * code within +-65504 and
+scale from 0 to 8192, or their values may become infinities and NaN there.
 """
 
 from __future__ import annotations
