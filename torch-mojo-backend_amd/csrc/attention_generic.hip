@@ -61,26 +61,31 @@ struct GenArgs {
   void* o_low;    // null, or (with o's strides) what rounding took from o
 };
 
+// SINK, here and below: a window with sinks.  Kernels of their own, since the
+// sinks' tests and tiles cost all others 1 to 4 % (f32 [2, 8 over 2,
+// 512, 64] forward 161 against 167 us, bf16 [4, 8, 512, 96] 332 against 341).
+template <bool SINK>
 __device__ __forceinline__ bool visible(const GenArgs& p, int64_t i, int64_t j) {
   if (j >= p.Skv) return false;
   if (p.causal && j > i) return false;
-  if (p.window > 0 && i - j >= p.window && j >= p.sinks) return false;
+  if (p.window > 0 && i - j >= p.window && !(SINK && j < p.sinks)) return false;
   return true;
 }
 
 // First key of the block's `it`-th tile: the tiles of sinks that lie before
 // kbeg, the window's first tile, then those from kbeg on.
+template <bool SINK>
 struct GenTiles {
   int64_t kbeg, ns;
   __device__ __forceinline__ GenTiles(const GenArgs& p, int64_t kb, int tile) {
     kbeg = kb / tile * tile;
-    ns = p.window > 0 ? min((min(p.sinks, p.Skv) + tile - 1) / tile, kbeg / tile) : 0;
+    ns = SINK ? min((min(p.sinks, p.Skv) + tile - 1) / tile, kbeg / tile) : 0;
   }
   __device__ __forceinline__ int64_t count(int64_t kend, int tile) const {
     return ns + (kend > kbeg ? (kend - kbeg + tile - 1) / tile : 0);
   }
   __device__ __forceinline__ int64_t key(int64_t it, int tile) const {
-    return it < ns ? it * tile : kbeg + (it - ns) * tile;
+    return SINK && it < ns ? it * tile : kbeg + (it - ns) * tile;
   }
 };
 
@@ -125,7 +130,7 @@ __device__ __forceinline__ void store_row(T* row, const float* x, int part, int6
 // ---------------------------------------------------------------------------
 // forward: a block owns 32 queries of one (batch, head)
 // ---------------------------------------------------------------------------
-template <typename T, int E>
+template <typename T, int E, bool SINK>
 __global__ void __launch_bounds__(kGT) gen_fwd(GenArgs p) {
   constexpr int DP = E * kTPR, kTile = kTileOf<E>;
   __shared__ float Ks[kTile * DP];
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kGT) gen_fwd(GenArgs p) {
   int64_t kbeg = 0, kend = p.Skv;
   if (p.causal) kend = min(kend, qlast + 1);
   if (p.window > 0) kbeg = max((int64_t)0, q0 - p.window + 1);
-  const GenTiles tiles(p, kbeg, kTile);
+  const GenTiles<SINK> tiles(p, kbeg, kTile);
   const int64_t nt = tiles.count(kend, kTile);
   for (int64_t it = 0; it < nt; ++it) {
     const int64_t kb0 = tiles.key(it, kTile);
@@ -165,7 +170,7 @@ __global__ void __launch_bounds__(kGT) gen_fwd(GenArgs p) {
 #pragma unroll
       for (int t = 0; t < E; ++t) acc = fmaf(qv[t], Ks[j * DP + part + kTPR * t], acc);
       acc = row_sum8(acc);
-      s[j] = visible(p, qi, kb0 + j) ? acc : -INFINITY;
+      s[j] = visible<SINK>(p, qi, kb0 + j) ? acc : -INFINITY;
       mx = fmaxf(mx, s[j]);
     }
     if (mx == -INFINITY) continue;  // nothing visible to this row in the tile
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_delta(GenArgs p) {
 }
 
 // dQ: a block owns 32 queries of one (batch, head) and walks the visible keys
-template <typename T, int E>
+template <typename T, int E, bool SINK>
 __global__ void __launch_bounds__(kGT) gen_bwd_dq(GenArgs p) {
   constexpr int DP = E * kTPR, kTile = kTileOf<E>;
   __shared__ float Ks[kTile * DP];
@@ -247,7 +252,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dq(GenArgs p) {
   int64_t kbeg = 0, kend = p.Skv;
   if (p.causal) kend = min(kend, qlast + 1);
   if (p.window > 0) kbeg = max((int64_t)0, q0 - p.window + 1);
-  const GenTiles tiles(p, kbeg, kTile);
+  const GenTiles<SINK> tiles(p, kbeg, kTile);
   const int64_t nt = tiles.count(kend, kTile);
   for (int64_t it = 0; it < nt; ++it) {
     const int64_t kb0 = tiles.key(it, kTile);
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dq(GenArgs p) {
       }
       sa = row_sum8(sa);
       pa = row_sum8(pa);
-      const float pj = (qok && visible(p, qi, kb0 + j)) ? exp2f(sa - lse2) : 0.f;
+      const float pj = (qok && visible<SINK>(p, qi, kb0 + j)) ? exp2f(sa - lse2) : 0.f;
       const float ds = pj * (pa - di);
 #pragma unroll
       for (int t = 0; t < E; ++t) dq[t] = fmaf(ds, Ks[j * DP + part + kTPR * t], dq[t]);
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dq(GenArgs p) {
 
 // dK/dV: a block owns 32 keys of one (batch, K/V head) and walks, for each
 // query head of its group, the queries that can see them
-template <typename T, int E>
+template <typename T, int E, bool SINK>
 __global__ void __launch_bounds__(kGT) gen_bwd_dkv(GenArgs p) {
   constexpr int DP = E * kTPR, kTile = kTileOf<E>;
   __shared__ float Qs[kTile * DP];
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dkv(GenArgs p) {
   const int64_t klast = min(p.Skv, k0 + kRows) - 1;
   int64_t qbeg = 0, qend = p.Sq;
   if (p.causal) qbeg = k0;
-  if (p.window > 0 && k0 >= p.sinks) qend = min(qend, klast + p.window);
+  if (p.window > 0 && !(SINK && k0 < p.sinks)) qend = min(qend, klast + p.window);
   qbeg = qbeg / kTile * kTile;
   for (int64_t r = 0; r < g; ++r) {
     const int64_t h = hk * g + r;
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(kGT) gen_bwd_dkv(GenArgs p) {
         sa = row_sum8(sa);
         pa = row_sum8(pa);
         const int64_t qi = qb0 + i;
-        const float pi = (kok && qi < p.Sq && visible(p, qi, kj)) ? exp2f(sa - lse_s[i]) : 0.f;
+        const float pi = (kok && qi < p.Sq && visible<SINK>(p, qi, kj)) ? exp2f(sa - lse_s[i]) : 0.f;
         const float ds = pi * (pa - del_s[i]);
 #pragma unroll
         for (int t = 0; t < E; ++t) {
@@ -362,21 +367,30 @@ int gen_check(int64_t B, int64_t H, int64_t HK, int64_t Sq, int64_t Skv, int64_t
   return MI355X_OK;
 }
 
+template <typename T, int E, bool SINK>
+void gen_fwd_kernels(const GenArgs& a, hipStream_t s) {
+  gen_fwd<T, E, SINK><<<dim3(ceil_div(a.Sq, kRows), (unsigned)a.H, (unsigned)a.B), kGT, 0, s>>>(a);
+}
+
 template <typename T, int E>
 int gen_fwd_launch(const GenArgs& a, hipStream_t s) {
-  gen_fwd<T, E><<<dim3(ceil_div(a.Sq, kRows), (unsigned)a.H, (unsigned)a.B), kGT, 0, s>>>(a);
+  a.sinks > 0 ? gen_fwd_kernels<T, E, true>(a, s) : gen_fwd_kernels<T, E, false>(a, s);
   return check_launch("mi355x_attn_fwd_gen");
+}
+
+template <typename T, int E, bool SINK>
+void gen_bwd_kernels(const GenArgs& a, hipStream_t s) {
+  gen_bwd_delta<T, E><<<ceil_div(a.B * a.H * a.Sq, kRows), kGT, 0, s>>>(a);
+  gen_bwd_dq<T, E, SINK><<<dim3(ceil_div(a.Sq, kRows), (unsigned)a.H, (unsigned)a.B), kGT, 0, s>>>(a);
+  gen_bwd_dkv<T, E, SINK><<<dim3(ceil_div(a.Skv, kRows), (unsigned)a.HK, (unsigned)a.B), kGT, 0, s>>>(a);
 }
 
 template <typename T, int E>
 int gen_bwd_launch(const GenArgs& a, hipStream_t s) {
-  gen_bwd_delta<T, E><<<ceil_div(a.B * a.H * a.Sq, kRows), kGT, 0, s>>>(a);
-  gen_bwd_dq<T, E><<<dim3(ceil_div(a.Sq, kRows), (unsigned)a.H, (unsigned)a.B), kGT, 0, s>>>(a);
-  gen_bwd_dkv<T, E><<<dim3(ceil_div(a.Skv, kRows), (unsigned)a.HK, (unsigned)a.B), kGT, 0, s>>>(a);
+  a.sinks > 0 ? gen_bwd_kernels<T, E, true>(a, s) : gen_bwd_kernels<T, E, false>(a, s);
   return check_launch("mi355x_attn_bwd_gen");
 }
 
-// dispatch on dtype and the per-lane element count (8, 16 or 32)
 #define MI_GEN_DISPATCH(dtype, D, FN, ...)                                      \
   do {                                                                          \
     const int e_ = D <= 64 ? 8 : (D <= 128 ? 16 : 32);                          \
