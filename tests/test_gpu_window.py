@@ -301,3 +301,21 @@ def test_masks_without_sinks(dtype, d, h, hk, t, window):
         op = run(x, window, 0)
         for n in op:
             assert torch.equal(op[n].detach().cpu(), got[n].detach().cpu()), n
+
+
+@pytest.mark.parametrize("dtype,d,h,hk", [(BF, 64, 8, 8), (HF, 128, 8, 2), (BF, 256, 4, 4), (BF, 96, 8, 4)])
+@pytest.mark.parametrize("t,window", [(3, 3), (3, 100), (2, 2 ** 40)])
+def test_windows_of_all_tokens_keep_what_rounding_takes(dtype, d, h, hk, t, window):
+    """As narrow ones do: with few keys a row the row terms dO . O decide."""
+    from paged_cases import np64
+    from torch_mojo_backend.eager_kernels import aten_fast
+
+    x = window_cases.inputs(8, h, hk, t, d, dtype)
+    want = window_cases.expected(*x, t, 0)
+    got = run(x, window, 4)
+    compare(got, want)
+    q, k, v, do = (y.to("mojo") for y in x)
+    out, lse = aten_fast.attention_forward(q, k, v, True, t, None, 0, None)
+    alone = aten_fast.attention_backward(do, q, k, v, out, lse, True, t, None, 0, None)
+    for n, a in zip(("dq", "dk"), alone):
+        assert abs(np64(got[n]) - want[n][0]).sum() < 0.85 * abs(np64(a) - want[n][0]).sum(), n

@@ -129,10 +129,10 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
         if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or q.shape[3] > 256:
             raise NotImplementedError(f"{what}: {q.dtype} with head_dim {q.shape[3]} is not supported"
                                       " (float32, bfloat16, float16, head_dim up to 256)")
-        if t <= window:
-            window, sinks = 0, None  # plain causal attention
-        else:
-            sinks = min(sinks, t)
+        # (a window of all tokens too: plain causal attention would take its
+        # row terms from the rounded output, dQ and dK of 6 tokens 3.3e-3 off
+        # instead of 2.4e-3)
+        window, sinks = min(window, t), min(sinks, t)
         if not _needs_grad(q, k, v):
             materialize_touched((q, k, v), None, False)
             return paged.on_device(q._device, aten_fast.attention_forward, q, k, v, True, window, scale, sinks)[0]
