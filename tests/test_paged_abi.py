@@ -173,3 +173,15 @@ def test_windows_past_every_position_share_keys_as_none(lib):
     for window, sinks in ((1 << 62, 1 << 62), ((1 << 63) - 1, 1), (1, (1 << 63) - 1), (1 << 20, 0)):
         assert size(cache(), 1000, 1, 2, 1, window, sinks, BF16) == none > 0
     assert size(cache(), 1000, 1, 2, 1, 100, 4, BF16) == 0
+
+
+@pytest.mark.parametrize("kw,dtype,alone", [(dict(d=64), BF16, 384), (dict(d=128), F16, 384), (dict(d=256), BF16, 256), (dict(d=64, dtype=F32), F32, 384),
+                                            (dict(d=128, dtype=F32), F32, 256), (dict(d=256, dtype=F32), F32, 128), (dict(d=96), BF16, 128),
+                                            (dict(d=128, bits=4), BF16, 384), (dict(d=256, bits=4), F16, 256), (dict(d=128, bits=4), F32, 128)])
+def test_keys_that_one_block_takes(lib, kw, dtype, alone):
+    c = cache(heads=1, **kw)
+    size = lambda keys, window=0: lib.mi355x_paged_attn_workspace_bytes(c, keys // 16, 1, 4, 1, window, 0, dtype)  # noqa: E731
+    assert size(alone) == 0 and size(10 ** 5, alone) == 0
+    assert size(alone + 16) > 0 and size(10 ** 5, alone + 1) > 0
+    many = lambda keys: lib.mi355x_paged_attn_workspace_bytes(c, keys // 16, 200, 4, 1, 0, 0, dtype)  # noqa: E731
+    assert many(384) == 0 and many(400) > 0

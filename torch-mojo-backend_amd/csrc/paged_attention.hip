@@ -190,22 +190,39 @@ int64_t most_keys(const mi355x_paged_cache& c, int64_t width, int64_t window, in
   return window > 0 && window < n && sinks < n - window ? window + sinks : n;
 }
 
+// Keys up to which one block does a row: a second launch costs 3.5 us and as
+// long again to reach the GPU, a block's tiles of 32 keys (16 in f32) about 2 us
+// for each that a wave has.  Calls replayed one after another, us with one block
+// and with splits: rows of 256 bytes and less 384 keys bf16 [8, 32 over 8, 128]
+// 9.6 and 9.9, [1, 12, 64] 7.9 and 8.7 (f32 [3 x 4, 12, 64] 333 keys 11.4 and
+// 10.2, but 11.9 and 14.1 as calls of their own); of 512 bytes bf16 [1, 4 over 1,
+// 256] 256 keys 11.6 and 11.9, 384 keys 13.8 and 12.2; of 1024 bytes 256 keys f32
+// [1, 4 over 1, 256] 20.3 and 17.3; an element a lane f32 [1, 4, 96] 128 keys 10.0
+// and 10.0, 256 keys 15.9 and 13.0.  All of it for few rows: with more blocks than
+// `few` below the parts cost more than they save up to 384 keys (bf16 [64, 4 over
+// 1, 256] 14.8 and 13.2, [256] 21.7 and 36.1; f32 [16, 32, 96] 38 and 31, [32] 48 and
+// 61).  The host knows the table's capacity, not the lengths: a short context in a
+// wide table is split all the same.
+int64_t keys_of_a_block(const mi355x_paged_cache& c, int dtype) {
+  if (!paged_mfma_takes(c, dtype)) return 128;
+  const int64_t bytes = c.d * (dtype == MI355X_F32 ? 4 : 2);
+  return bytes <= 256 ? 384 : bytes <= 512 ? 256 : 128;
+}
+
 // Blocks that share the keys of a row, where rows alone are too few to fill
 // the 256 CUs: eight blocks a CU in all (lengths differ, and the last round is
 // shorter than with four: 282 against 276 us for the batch above
-// paged_attn_mfma), of at least 128 keys each.  Up to 384 keys one block does
-// it: the second launch takes 3.5 us and as long again to reach the GPU, which
-// is what the three tiles of 32 keys (six of 16) that a wave then has take
-// ([3 x 4, 12, 64] f32 over 333 keys: 7.8 + 3.6 us and a launch between, or 12.4).
+// paged_attn_mfma), of at least 128 keys each.
 int plan_splits(const mi355x_paged_cache& c, int64_t width, int64_t batch, int64_t heads, int64_t seq, int64_t window,
                 int64_t sinks, int dtype) {
   const int64_t keys = most_keys(c, width, window, sinks);
-  int64_t blocks = batch * heads * seq;
+  int64_t blocks = batch * heads * seq, few = 512;
   if (paged_mfma_takes(c, dtype)) {
+    few = 128;
     const int64_t rows = heads / c.kv_heads * seq, per = 16 * paged_mfma_row_tiles(rows, c.d);
     blocks = batch * c.kv_heads * ((rows + per - 1) / per);
   }
-  if (keys <= 384) return 1;
+  if (keys <= 384 && (keys <= keys_of_a_block(c, dtype) || blocks > few)) return 1;
   int64_t n = blocks > 0 ? (2048 + blocks - 1) / blocks : 1;
   if (n > (keys + 127) / 128) n = (keys + 127) / 128;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
