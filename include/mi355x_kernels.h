@@ -622,7 +622,8 @@ int mi355x_attn_fwd_sink(void* o, const int64_t* o_bhs, void* o_low, float* lse,
                          int64_t kv_heads, int64_t sq, int64_t skv, int64_t d, double scale,
                          int64_t window, int64_t sinks, int dtype, mi355x_stream_t stream);
 /* Workspace: that of mi355x_attn_bwd_gen, and f32 partials of the sinks'
- * gradients, whose queries are shared by several blocks. */
+ * gradients, whose queries are shared by several blocks (of at most 4096; none
+ * where window and sinks hide nothing). */
 int64_t mi355x_attn_bwd_sink_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
                                              int64_t sq, int64_t skv, int64_t d, int64_t window,
                                              int64_t sinks);

@@ -1453,7 +1453,13 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? ATTN_BWD_WAVES : 1) attn_b
 // sums, 400 TFLOP/s of the pairs seen.  [1, 4 over 1, 4096, 256], window 512: 85,
 // 9 and 12.7 us, 190 TFLOP/s; there a block takes a CU and a wave a SIMD, whose
 // waits for LDS are bare (the matrix units are busy a seventh of the time).
-// Eight waves that split a step's channels or its queries' tiles took 80 to 95.
+// Eight waves that split a step's channels took 80 to 87 us from run to run, no
+// sure gain, and eight that split its queries' tiles 95, with spilled registers.
+// P and dS are rounded to the type before their products, as in the kernels
+// above: half a step each (2^-8 in bf16), so that gradients are 2.4e-3 off in the
+// 2-norm where unrounded ones are 1.7e-3 off, the result's own rounding (the f16
+// forward 2.6e-4 against 2.0e-4).  Two halves of each would be 14 D MFMA operations
+// a pair instead of 10, and their conversions, beside the softmax that bounds this.
 // 16-row tiles of a wave: two, or one of keys at head_dim 256, where the dK and
 // dV of two would take all of its registers.
 template <int D>

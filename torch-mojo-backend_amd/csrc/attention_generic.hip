@@ -1,9 +1,9 @@
 // Fused attention for the inputs the MFMA kernels do not take: any head_dim
 // up to 256, f32 with grouped K/V heads or a window, and the backward of
 // grouped-K/V-head and sliding-window attention.  Everything is computed in
-// f32.  Plain f32 attention at head_dim 32, 64 and 128, and a window with sinks
-// at 256 as well, goes on from these entry points to the matrix cores
-// (attention_f32.hip).
+// f32.  Plain f32 attention at head_dim 32, 64 and 128, and the windows of the
+// _sink entry points at 256 and with grouped heads as well, go on from these
+// entry points to the matrix cores (attention_f32.hip).
 //
 // Semantics are those of attention.hip: S = scale Q K^T over the visible keys
 // (top-left causal: key j visible to query i iff j <= i; with a window w > 0

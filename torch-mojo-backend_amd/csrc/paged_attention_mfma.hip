@@ -20,7 +20,10 @@
 // g) is the operand layout of P^T, for tiles in the order of the keys.
 //
 // P is split in two halves of the pages' type, so its rounding (2^-8 in bf16)
-// does not show beside the result's; the second product costs nothing here.
+// does not show beside the result's; for a few new tokens the second product
+// costs nothing (for a prompt it is a third of the MFMAs).  Exponentials are the
+// hardware's, within a step of f32: f32 results are 3.1e-7 off in the 2-norm where
+// the plain form's are 2.1e-7.
 //
 // 4-bit rows are turned into f16 in registers: masked nibbles under f16's
 // exponent of 512, less 512, are half the codes, two a register.  For bf16
@@ -35,11 +38,14 @@
 // Blocks split the keys of long sequences; paged_attn_join adds the parts.
 //
 // 32 sequences of up to 16384 keys, 32 query heads over 8 of 128: 275 us in
-// bf16, 5.6 TB/s, as fast as memory is read here by anything.  In 4 bits 139 us,
-// 3.8 TB/s: turning the codes takes 57% of the issue slots and the waits on the
+// bf16, 5.7 TB/s (a pass that only reads reaches 6.3 here).  In 4 bits 139 us, 3.5
+// TB/s: turning the codes takes 57% of the issue slots and the waits on the
 // lookups and loads of a tile most of the rest (164 us with f16 queries).  One
 // token over 516 keys of 4 heads over 1 of 256, bf16: 9.9 us, of which a tile of
-// 32 keys is 2; over 8191 in 4 bits 9.7.
+// 32 keys is 2; over 8191 in 4 bits 9.7.  A prompt runs here too, 16 or 32 rows a
+// block, which read each K and V row again: [1, 32 over 8, 2048, 128] bf16 137 us
+// where attention over rows laid out densely takes 88, [1, 4 over 1, 2048, 256] 212
+// and 70; over 4 bits 143 and 137 (f16 queries 188 and 253).
 #include <math.h>
 
 #include <type_traits>

@@ -192,10 +192,13 @@ __device__ __forceinline__ bool place_of(const AppendArgs& a, int64_t b, int64_t
 // kHeads rows of one token and of one kind (query, key or value, the same for
 // a block): the angles are read once for all of them, and their loads are all
 // in flight before the first is used.  Four prompts of 2048 tokens, 16 query
-// and 8 K/V heads of 128 at most, into 4 bits (89 MB): 34.6 us (eight rows a
-// thread 12 more, one or two up to 5 more); the f64 rotation of the keys and the
-// packing bound it, a copy would take 17.  Five of 333 at most into f32 pages
-// (13 MB) 6.2 us, one token 3.0, a launch.
+// and 8 K/V heads of 128 at most, into 4 bits (89 MB): 35 us (eight rows a
+// thread 12 more, one or two up to 5 more), where a copy takes 17.  Waiting bounds
+// it: four waves a SIMD (116 registers), twice over, load, pack and store one
+// after another, and a wave waits for memory in 61% of its cycles; VALU work
+// issues in about a third of them (the f64 rotation is little of it), LDS in 2%, and
+// the 76 MB that pass HBM are 2.2 TB/s.  Five of 333 at most into f32 pages (13 MB)
+// 6.2 us, one token 3.0, a launch.
 constexpr int kHeads = 4;
 
 template <typename T, typename RT, bool FOUR>
@@ -369,8 +372,11 @@ struct GatherArgs {
   uint32_t per_token;  // 2 kv_heads * d / 8
 };
 
-// Eight channels a thread, bound by the bytes written: the rows of the prompts
-// above from 4 bits to f32, 61 MB, in 17.5 us.
+// Eight channels a thread.  Padding is written as well, zeros: the rows of the
+// prompts above from 4 bits to f32, 67 MB written and 13 read, in 17.5 us, 4.6
+// TB/s, as a copy.  Full rows of 4 sequences of 2048, 8 heads of 128: f32 24 us, 5.6
+// TB/s; bf16 15 us, 4.6; 4 bits to f32 20 us, 3.8, to 16 bits 17 us, 2.5, where
+// unpacking is as long.
 // T: the type of the values written; CT: of the pages (uint8_t: 4 bits).
 template <typename T, typename CT>
 __global__ void __launch_bounds__(kThreads) paged_gather_kernel(GatherArgs a) {
