@@ -118,11 +118,14 @@ class Attention(nn.Module):
         c = self.cfg
         q, k, v = self._qkv(x)
         dtype = q.dtype
-        if cache.bits != 4:  # under autocast, or over pages of a type of their own
+        cast = cache.bits != 4 and dtype != cache.dtype  # under autocast, or pages of a type of their own
+        if cast:
             q, k, v = q.to(cache.dtype), k.to(cache.dtype), v.to(cache.dtype)
         q = ops.paged_append(cache, page_table, starts, k, v, *rope, q=q, counts=counts)
         window, sinks = (c.window, c.sinks) if self.local else (0, 0)
-        y = ops.paged_attention(q, cache, page_table, starts, counts=counts, window=window, sinks=sinks).to(dtype)
+        y = ops.paged_attention(q, cache, page_table, starts, counts=counts, window=window, sinks=sinks)
+        if cast:
+            y = y.to(dtype)
         return self.o_proj(y.transpose(1, 2).reshape(b, t, c.heads * c.head_dim))
 
 
