@@ -727,6 +727,45 @@ int mi355x_paged_attn(void* o, const int64_t* o_bht, const void* q, const int64_
                       int64_t heads, int64_t seq, double scale, int64_t window, int64_t sinks, int dtype,
                       void* workspace, int64_t ws_bytes, int32_t* error, mi355x_stream_t stream);
 
+/* ---- packed sequences --------------------------------------------------
+ * Sequences of different lengths laid end to end: sequence i of a batch is rows
+ * offsets[i] .. offsets[i + 1] - 1 of [tokens][heads][d].  Lengths may be zero;
+ * rows before the first and behind the last sequence are padding.  The
+ * reference has no counterpart: it trains on rectangular batches
+ * (current_bench/bench_nanogpt_train.py:90-108), and its attention knows no
+ * sequence borders (aten_fast.py:7462-7530). */
+/* Makes the plan of a batch (16-byte aligned device memory, which every
+ * call below reads) from its sequences + 1 offsets (int32 in device memory), and
+ * each row's position in its sequence (0 in padding).  Offsets that fall or
+ * leave 0 .. tokens set *error (may be null) to 1; every row is then padding. */
+int64_t mi355x_packed_plan_bytes(int64_t sequences, int64_t tokens);
+int mi355x_packed_plan(void* plan, int64_t plan_bytes, int32_t* positions, const int32_t* offsets,
+                       int64_t sequences, int64_t tokens, int32_t* error, mi355x_stream_t stream);
+/* Causal attention within each sequence: row i sees rows j <= i of its own
+ * sequence and, with a window > 0, only i - j < window.  Query head h reads K/V
+ * head h / (heads / kv_heads).  lse: [heads][tokens], the natural logarithm of
+ * each row's sum, -inf in padding, where o is zero.  o_low may be null or laid
+ * out as o: what rounding took from a 16-bit o, for the backward's row terms.
+ * *_th: (row, head) strides in elements, rows 16-byte aligned; d a multiple of 8
+ * up to 256; f32, bf16 and f16. */
+int mi355x_packed_attn_fwd(void* o, const int64_t* o_th, void* o_low, float* lse, const void* q,
+                           const int64_t* q_th, const void* k, const int64_t* k_th, const void* v,
+                           const int64_t* v_th, const void* plan, int64_t sequences, int64_t tokens,
+                           int64_t heads, int64_t kv_heads, int64_t d, double scale, int64_t window,
+                           int dtype, mi355x_stream_t stream);
+/* dQ, dK, dV (written, zero in padding); those of a K/V head are the sums over
+ * its query heads, in head order.  The workspace holds two floats a query row
+ * and, where a group's heads are shared out, f32 partials of dK and dV. */
+int64_t mi355x_packed_attn_bwd_workspace_bytes(int64_t sequences, int64_t tokens, int64_t heads,
+                                               int64_t kv_heads, int64_t d);
+int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, const int64_t* dk_th, void* dv,
+                           const int64_t* dv_th, const void* dout, const int64_t* do_th, const void* q,
+                           const int64_t* q_th, const void* k, const int64_t* k_th, const void* v,
+                           const int64_t* v_th, const void* o, const int64_t* o_th, const void* o_low,
+                           const float* lse, const void* plan, int64_t sequences, int64_t tokens,
+                           int64_t heads, int64_t kv_heads, int64_t d, double scale, int64_t window,
+                           int dtype, void* workspace, int64_t ws_bytes, mi355x_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

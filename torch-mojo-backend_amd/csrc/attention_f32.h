@@ -2,6 +2,7 @@
 // of attention_generic.hip.
 #pragma once
 #include "common.h"
+#include "packed.h"
 
 namespace mi {
 
@@ -25,6 +26,8 @@ struct AttnF32 {
   int64_t group, window, sinks;
   float *kv_part, *sink_part;  // the backward's partials (attention_window.h)
   int sink_blocks, sink_chunks, sink_keys;
+  int64_t kv_plane;  // from kv_part's dK to its dV
+  int d;             // channels, of packed sequences alone
 };
 
 // -1 when the inputs are not taken (other head dims, unaligned rows).
@@ -34,5 +37,17 @@ int attn_f32_bwd(const AttnF32& p, int64_t d, hipStream_t s);
 // backward's workspace: D and one more float per query row, then the partials.
 int attn_f32_window_fwd(const AttnF32& p, int64_t d, hipStream_t s);
 int attn_f32_window_bwd(const AttnF32& p, int64_t d, hipStream_t s);
+
+
+// Packed sequences, forward or backward.  p: strides of rows and heads, Sq = all
+// rows, H = the query heads, whose terms lie in lse and delta [H][Sq], B = 1,
+// window 0 for none, d up to 256 (16-byte rows), with grouped heads kv_part.
+struct PackedF32 {
+  const PackedHeader* head;
+  const PackedTile* tiles;  // of 64 rows
+  int64_t cap;              // entries that the list may have
+  uint32_t heads, kv_heads;
+};
+int attn_f32_packed(const AttnF32& p, const PackedF32& k, bool backward, hipStream_t s);
 
 }  // namespace mi

@@ -57,15 +57,18 @@ struct Tile {
   static constexpr int H = NF / W;             // transposed reads per row
   static __device__ __forceinline__ int swz(int row) { return D >= 64 ? (row & 15) : ((row >> 1) & 7); }
 
-  // rows row0 .. row0 + 31 (past the end: the last one) of a [rows, D] operand
-  static __device__ __forceinline__ void load(const float* src, int64_t stride, int64_t row0, int64_t rows, char* dst) {
+  // rows row0 .. row0 + 31 (past the end: the last one) of a [rows, D] operand;
+  // RAG: of its first d channels, the others' place in LDS is left alone
+  template <bool RAG = false>
+  static __device__ __forceinline__ void load(const float* src, int64_t stride, int64_t row0, int64_t rows, char* dst, int d = D) {
     constexpr int RPI = 64 / CH;  // rows per wave instruction
     const int lane = threadIdx.x & 63, wave = wave_id();
     const unsigned lds = lds_base_of(dst) + wave * 1024;
 #pragma unroll
     for (int it = 0; it < D / 32; ++it) {
       const int r = (it * 4 + wave) * RPI + lane / CH;
-      dma_b128(src + min(row0 + r, rows - 1) * stride + ((lane % CH) ^ swz(r)) * 4, lds + it * 4096);
+      const int c = ((lane % CH) ^ swz(r)) * 4;
+      if (!RAG || c < d) dma_b128(src + min(row0 + r, rows - 1) * stride + c, lds + it * 4096);
     }
   }
   // lane (lr, lg): 4 consecutive elements 16 ks + 4 lg of row r
@@ -86,8 +89,10 @@ struct Tile {
       }
     }
   }
-  // Write a wave's [D, 16] accumulators (column lr) times `f` to the row at p.
-  static __device__ __forceinline__ void store(float* p, const f32x4 (&acc)[NF], int lg, float f) {
+  // Write a wave's [D, 16] accumulators (column lr) times `f` to the row at p
+  // (RAG: its first d channels).
+  template <bool RAG = false>
+  static __device__ __forceinline__ void store(float* p, const f32x4 (&acc)[NF], int lg, float f, int d = D) {
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -96,9 +101,9 @@ struct Tile {
           f32x4 v;
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] = acc[h * 4 + i][e] * f;
-          *(f32x4*)(p + h * 64 + 4 * (4 * lg + e)) = v;
+          if (!RAG || h * 64 + 4 * (4 * lg + e) < d) *(f32x4*)(p + h * 64 + 4 * (4 * lg + e)) = v;
         } else {
-          *(float2*)(p + 2 * (4 * lg + e)) = make_float2(acc[0][e] * f, acc[1][e] * f);
+          if (!RAG || 2 * (4 * lg + e) < d) *(float2*)(p + 2 * (4 * lg + e)) = make_float2(acc[0][e] * f, acc[1][e] * f);
         }
       }
   }
@@ -189,11 +194,15 @@ __device__ __forceinline__ float group_max(float v) {
   return fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
-// This lane's fragments of one row of q, k, v or dO (times f).
-template <int D>
-__device__ __forceinline__ void load_frags(const float* row, int lg, float f, f32x4 (&x)[D / 16]) {
+// This lane's fragments of one row of q, k, v or dO (times f; RAG: zeros past
+// channel d).
+template <int D, bool RAG = false>
+__device__ __forceinline__ void load_frags(const float* row, int lg, float f, f32x4 (&x)[D / 16], int d = D) {
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) x[ks] = *(const f32x4*)(row + ks * 16 + lg * 4) * f;
+  for (int ks = 0; ks < D / 16; ++ks) {
+    if (RAG && ks * 16 + lg * 4 >= d) x[ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+    else x[ks] = *(const f32x4*)(row + ks * 16 + lg * 4) * f;
+  }
 }
 
 // WIN, a causal window (with sinks or without) and grouped K/V heads: the
@@ -225,21 +234,19 @@ __device__ __forceinline__ bool win_some(const AttnF32& p, int64_t w0, int64_t k
   return k0 < w0 + 15 - p.window + 1;
 }
 
-template <int D, bool WIN = false>
-__global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint32_t nblk) {
+// Block x of 64 queries of head h.
+template <int D, bool WIN, bool RAG = false>
+__device__ __forceinline__ void fwd_body(const AttnF32& p, int64_t b, int64_t h, uint32_t x) {
   typedef Tile<D> T;
   char* const lds = attn_f32_smem;  // 2 stages of a K and a V tile
-  uint32_t bh, x;
-  block_of(blockIdx.x, gridDim.x, nblk, &bh, &x);
-  if (p.causal) x = nblk - 1 - x;  // the longest rows first
-  const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, q0 = (int64_t)x * kBlk;
+  const int64_t q0 = (int64_t)x * kBlk;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int64_t w0 = q0 + wave_id() * 16, qi = w0 + lr;
   const int64_t hk = WIN ? h / p.group : h;
   const float* K = p.k + b * p.k_b + hk * p.k_h;
   const float* V = p.v + b * p.v_b + hk * p.v_h;
   f32x4 q[T::NF], o[T::NF];
-  load_frags<D>(p.q + b * p.q_b + h * p.q_h + min(qi, p.Sq - 1) * p.q_s, lg, p.scale_log2, q);
+  load_frags<D, RAG>(p.q + b * p.q_b + h * p.q_h + min(qi, p.Sq - 1) * p.q_s, lg, p.scale_log2, q, p.d);
 #pragma unroll
   for (int n = 0; n < T::NF; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
@@ -250,8 +257,8 @@ __global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint
   const int64_t nt = WIN ? tiles.count : (kend + kRow - 1) / kRow;
   auto key = [&](int64_t i) { return WIN ? tiles.key(i) : i * kRow; };
   if (!WIN || nt > 0) {
-    T::load(K, p.k_s, key(0), p.Skv, lds);
-    T::load(V, p.v_s, key(0), p.Skv, lds + T::BYTES);
+    T::template load<RAG>(K, p.k_s, key(0), p.Skv, lds, p.d);
+    T::template load<RAG>(V, p.v_s, key(0), p.Skv, lds + T::BYTES, p.d);
   }
   int cur = 0;
   for (int64_t i = 0; i < nt; ++i, cur ^= 1) {
@@ -259,8 +266,8 @@ __global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
     if (i + 1 < nt) {
-      T::load(K, p.k_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES);
-      T::load(V, p.v_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES);
+      T::template load<RAG>(K, p.k_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES, p.d);
+      T::template load<RAG>(V, p.v_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES, p.d);
     }
     if (k0 >= wend || (WIN && win_none(p, w0, k0))) continue;
     const char* kt = lds + cur * 2 * T::BYTES;
@@ -301,8 +308,17 @@ __global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint
   }
   l = group_sum(l);
   if (qi >= p.Sq) return;
-  T::store(p.o + b * p.o_b + h * p.o_h + qi * p.o_s, o, lg, l > 0.f ? 1.f / l : 0.f);
+  T::template store<RAG>(p.o + b * p.o_b + h * p.o_h + qi * p.o_s, o, lg, l > 0.f ? 1.f / l : 0.f, p.d);
   if (lg == 0) p.lse[(b * p.H + h) * p.Sq + qi] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+template <int D, bool WIN = false>
+__global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint32_t nblk) {
+  uint32_t bh, x;
+  block_of(blockIdx.x, gridDim.x, nblk, &bh, &x);
+  if (p.causal) x = nblk - 1 - x;  // the longest rows first
+  const int64_t b = bh / (uint32_t)p.H;
+  fwd_body<D, WIN>(p, b, bh - b * p.H, x);
 }
 
 // D_i = sum_d dO[i, d] O[i, d], in the order of scores(): a lane per partial
@@ -311,7 +327,7 @@ __global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) fwd_f32(AttnF32 p, uint
 // is in exact arithmetic: in another order it is the rounding of both sums
 // (one key: dQ and dK 1e-8 of |dO||V| instead of 0; [1, 2, 3, 64] against 135
 // keys, causal: 2-norm error of dQ 7.1e-7, 3.8e-7 in the element-per-lane kernels).
-template <int D>
+template <int D, bool RAG = false>
 __global__ void __launch_bounds__(kNT) delta_f32(AttnF32 p, int64_t rows) {
   constexpr int N = kChains<D>;
   const int64_t row = ((int64_t)blockIdx.x * kNT + threadIdx.x) / N;
@@ -326,7 +342,8 @@ __global__ void __launch_bounds__(kNT) delta_f32(AttnF32 p, int64_t rows) {
     for (int t = 0; t < D / 4; t += N) {
       const int at = (t + c) / 4 * 16 + (t + c) % 4;
 #pragma unroll
-      for (int g = 0; g < 16; g += 4) v = fmaf(o[at + g], d[at + g], v);
+      for (int g = 0; g < 16; g += 4)
+        if (!RAG || at + g < p.d) v = fmaf(o[at + g], d[at + g], v);
     }
   }
 #pragma unroll
@@ -335,22 +352,19 @@ __global__ void __launch_bounds__(kNT) delta_f32(AttnF32 p, int64_t rows) {
 }
 
 // dQ of 64 queries: dS^T = P^T (dP^T - D), dQ^T = scale K^T dS^T.
-template <int D, bool WIN = false>
-__device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk) {
+template <int D, bool WIN, bool RAG = false>
+__device__ __forceinline__ void dq_body(const AttnF32& p, int64_t b, int64_t h, uint32_t x) {
   typedef Tile<D> T;
   char* const lds = attn_f32_smem;
-  uint32_t bh, x;
-  block_of(L, total, nblk, &bh, &x);
-  if (p.causal) x = nblk - 1 - x;
-  const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, q0 = (int64_t)x * kBlk;
+  const int64_t q0 = (int64_t)x * kBlk;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int64_t w0 = q0 + wave_id() * 16, qi = w0 + lr, qc = min(qi, p.Sq - 1);
   const int64_t hk = WIN ? h / p.group : h;
   const float* K = p.k + b * p.k_b + hk * p.k_h;
   const float* V = p.v + b * p.v_b + hk * p.v_h;
   f32x4 q[T::NF], dO[T::NF], dq[T::NF];
-  load_frags<D>(p.q + b * p.q_b + h * p.q_h + qc * p.q_s, lg, p.scale_log2, q);
-  load_frags<D>(p.dout + b * p.do_b + h * p.do_h + qc * p.do_s, lg, 1.f, dO);
+  load_frags<D, RAG>(p.q + b * p.q_b + h * p.q_h + qc * p.q_s, lg, p.scale_log2, q, p.d);
+  load_frags<D, RAG>(p.dout + b * p.do_b + h * p.do_h + qc * p.do_s, lg, 1.f, dO, p.d);
 #pragma unroll
   for (int n = 0; n < T::NF; ++n) dq[n] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float lse2 = p.lse[(b * p.H + h) * p.Sq + qc] * kLog2e;
@@ -362,8 +376,8 @@ __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t to
   const int64_t nt = WIN ? tiles.count : (kend + kRow - 1) / kRow;
   auto key = [&](int64_t i) { return WIN ? tiles.key(i) : i * kRow; };
   if (!WIN || nt > 0) {
-    T::load(K, p.k_s, key(0), p.Skv, lds);
-    T::load(V, p.v_s, key(0), p.Skv, lds + T::BYTES);
+    T::template load<RAG>(K, p.k_s, key(0), p.Skv, lds, p.d);
+    T::template load<RAG>(V, p.v_s, key(0), p.Skv, lds + T::BYTES, p.d);
   }
   int cur = 0;
   for (int64_t i = 0; i < nt; ++i, cur ^= 1) {
@@ -371,8 +385,8 @@ __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t to
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
     if (i + 1 < nt) {
-      T::load(K, p.k_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES);
-      T::load(V, p.v_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES);
+      T::template load<RAG>(K, p.k_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES, p.d);
+      T::template load<RAG>(V, p.v_s, key(i + 1), p.Skv, lds + (cur ^ 1) * 2 * T::BYTES + T::BYTES, p.d);
     }
     if (k0 >= wend || (WIN && win_none(p, w0, k0))) continue;
     const char* kt = lds + cur * 2 * T::BYTES;
@@ -394,22 +408,27 @@ __device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t to
       }
     accumulate<D>(kt, s, lr, lg, dq);
   }
-  if (qi < p.Sq) T::store(p.dq + b * p.dq_b + h * p.dq_h + qi * p.dq_s, dq, lg, p.scale);
+  if (qi < p.Sq) T::template store<RAG>(p.dq + b * p.dq_b + h * p.dq_h + qi * p.dq_s, dq, lg, p.scale, p.d);
+}
+
+template <int D, bool WIN = false>
+__device__ __forceinline__ void dq_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk) {
+  uint32_t bh, x;
+  block_of(L, total, nblk, &bh, &x);
+  if (p.causal) x = nblk - 1 - x;
+  const int64_t b = bh / (uint32_t)p.H;
+  dq_body<D, WIN>(p, b, bh - b * p.H, x);
 }
 
 // dK, dV of 64 keys: dV^T = dO^T P, dK^T = scale Q^T dS.  WIN: of one query
 // head, and (extra) of one chunk of the queries behind the window of a block of
 // sinks, as attention.hip's dkv_body.
-template <int D, bool WIN = false>
-__device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk, bool extra = false) {
+template <int D, bool WIN, bool RAG = false>
+__device__ __forceinline__ void dkv_body(const AttnF32& p, int64_t b, int64_t h, uint32_t x, int chunk, bool extra) {
   typedef Tile<D> T;
   char* const lds = attn_f32_smem;                    // 2 stages of a Q and a dO tile
   float* const terms = (float*)(lds + 4 * T::BYTES);  // 2 stages of 32 LSE, 32 D
-  uint32_t bh, x;
-  block_of(L, total, nblk, &bh, &x);
-  int chunk = 0;
-  if (WIN && extra) chunk = x / p.sink_blocks, x -= chunk * p.sink_blocks;
-  const int64_t b = bh / (uint32_t)p.H, h = bh - b * p.H, hk = WIN ? h / p.group : h, k0 = (int64_t)x * kBlk;
+  const int64_t hk = WIN ? h / p.group : h, k0 = (int64_t)x * kBlk;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   int wave_key = wave_id(), part = 0, parts = 1;  // of a chunk: the wave's keys, and its share of the steps
   if (WIN && extra) {
@@ -422,8 +441,8 @@ __device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t t
   const float* dO = p.dout + b * p.do_b + h * p.do_h;
   const float* rt = (lane < 32 ? p.lse : p.delta) + (b * p.H + h) * p.Sq;  // this lane's row term
   f32x4 k[T::NF], v[T::NF], dk[T::NF], dv[T::NF];
-  load_frags<D>(p.k + b * p.k_b + hk * p.k_h + kc * p.k_s, lg, p.scale_log2, k);
-  load_frags<D>(p.v + b * p.v_b + hk * p.v_h + kc * p.v_s, lg, 1.f, v);
+  load_frags<D, RAG>(p.k + b * p.k_b + hk * p.k_h + kc * p.k_s, lg, p.scale_log2, k, p.d);
+  load_frags<D, RAG>(p.v + b * p.v_b + hk * p.v_h + kc * p.v_s, lg, 1.f, v, p.d);
 #pragma unroll
   for (int n = 0; n < T::NF; ++n) dk[n] = dv[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -438,8 +457,8 @@ __device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t t
     }
   }
   auto issue = [&](int64_t r0, int st) {
-    T::load(Q, p.q_s, r0, p.Sq, lds + st * 2 * T::BYTES);
-    T::load(dO, p.do_s, r0, p.Sq, lds + st * 2 * T::BYTES + T::BYTES);
+    T::template load<RAG>(Q, p.q_s, r0, p.Sq, lds + st * 2 * T::BYTES, p.d);
+    T::template load<RAG>(dO, p.do_s, r0, p.Sq, lds + st * 2 * T::BYTES + T::BYTES, p.d);
     if (wave_id() == 0) dma_b32(rt + min(r0 + (lane & 31), p.Sq - 1), lds_base_of(terms + st * 64));
   };
   if (qbeg < qend) issue(qbeg, 0);
@@ -488,11 +507,21 @@ __device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t t
       const int64_t hkn = p.H / p.group, gi = h - hk * p.group;
       float* pk = p.kv_part + (((gi * p.B + b) * hkn + hk) * p.Skv + kj) * D;
       T::store(pk, dk, lg, 1.f);
-      return T::store(pk + p.B * p.H * p.Skv * D, dv, lg, 1.f);
+      return T::store(pk + p.kv_plane, dv, lg, 1.f);
     }
   }
-  T::store(p.dk + b * p.dk_b + hk * p.dk_h + kj * p.dk_s, dk, lg, p.scale);
-  T::store(p.dv + b * p.dv_b + hk * p.dv_h + kj * p.dv_s, dv, lg, 1.f);
+  T::template store<RAG>(p.dk + b * p.dk_b + hk * p.dk_h + kj * p.dk_s, dk, lg, p.scale, p.d);
+  T::template store<RAG>(p.dv + b * p.dv_b + hk * p.dv_h + kj * p.dv_s, dv, lg, 1.f, p.d);
+}
+
+template <int D, bool WIN = false>
+__device__ __forceinline__ void dkv_f32(const AttnF32& p, uint32_t L, uint32_t total, uint32_t nblk, bool extra = false) {
+  uint32_t bh, x;
+  block_of(L, total, nblk, &bh, &x);
+  int chunk = 0;
+  if (WIN && extra) chunk = x / p.sink_blocks, x -= chunk * p.sink_blocks;
+  const int64_t b = bh / (uint32_t)p.H;
+  dkv_body<D, WIN>(p, b, bh - b * p.H, x, chunk, extra);
 }
 
 // Both in one launch: the first `ndkv` blocks do dK and dV, the rest dQ, so
@@ -563,7 +592,7 @@ int run_window_bwd(AttnF32 p, hipStream_t s) {
   a.ndelta = p.delta;
   if (p.group > 1) a.kv_part = (float*)(((uintptr_t)(p.delta + 2 * rows) + 255) & ~(uintptr_t)255);
   window_parts(a, D);
-  p.kv_part = a.kv_part, p.sink_part = a.sink_part;
+  p.kv_part = a.kv_part, p.sink_part = a.sink_part, p.kv_plane = p.B * p.H * p.Skv * D;
   p.sink_chunks = a.sink_chunks, p.sink_keys = a.sink_keys, p.sink_blocks = (a.sink_keys + kBlk - 1) / kBlk;
   const int64_t kblk = (p.Skv + kBlk - 1) / kBlk, qblk = (p.Sq + kBlk - 1) / kBlk, heads = p.B * p.H;
   const int64_t extra = (int64_t)p.sink_blocks * p.sink_chunks;
@@ -576,6 +605,87 @@ int run_window_bwd(AttnF32 p, hipStream_t s) {
       p, (uint32_t)(kblk * heads), (uint32_t)(extra * heads), (uint32_t)kblk, (uint32_t)qblk);
   window_sum_launch<float, D, 16>(a, s);
   return check_launch("mi355x_attn_bwd_sink");
+}
+
+// ---------------------------------------------------------------------------
+// packed sequences (attention_packed.hip): a block takes a tile of 64 rows of
+// one sequence and one head, and p describes the whole batch (Sq: its rows).
+// ---------------------------------------------------------------------------
+// The same of the block's own sequence and head, whose causal attention is a
+// window's without sinks.
+__device__ __forceinline__ AttnF32 sequence_of(AttnF32 p, const PackedAt& at) {
+  const int64_t r = at.t.start, terms = (int64_t)at.h * p.Sq + r;
+  p.q += r * p.q_s + at.h * p.q_h, p.o += r * p.o_s + at.h * p.o_h;
+  p.k += r * p.k_s + at.hk * p.k_h, p.v += r * p.v_s + at.hk * p.v_h;
+  p.dout += r * p.do_s + at.h * p.do_h, p.dq += r * p.dq_s + at.h * p.dq_h;
+  p.dk += r * p.dk_s + at.hk * p.dk_h, p.dv += r * p.dv_s + at.hk * p.dv_h;
+  p.lse += terms, p.delta += terms;
+  p.window = p.window > 0 ? min(p.window, (int64_t)at.t.len) : at.t.len;
+  p.Sq = p.Skv = at.t.len, p.B = p.H = p.group = 1;
+  return p;
+}
+__device__ __forceinline__ void zero_rows(float* x, int64_t stride, int rows, int d) {
+  for (int i = threadIdx.x; i < rows * (d / 4); i += kNT)
+    *(f32x4*)(x + (int64_t)(i / (d / 4)) * stride + i % (d / 4) * 4) = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+template <int D, bool RAG>
+__device__ __forceinline__ void clear_tiles() {
+  if constexpr (RAG) {
+    for (int i = threadIdx.x * 16; i < 4 * Tile<D>::BYTES; i += kNT * 16) *(f32x4*)(attn_f32_smem + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+  }
+}
+
+template <int D, bool RAG>
+__global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) packed_fwd_f32(AttnF32 p, PackedF32 k) {
+  const PackedAt at = packed_at(k.tiles, k.head->count[1], blockIdx.x, k.heads, k.kv_heads);
+  if (!at.live) return;
+  const AttnF32 a = sequence_of(p, at);
+  if (at.t.tile < 0) {
+    for (int i = threadIdx.x; i < at.t.len; i += kNT) a.lse[i] = -INFINITY;
+    return zero_rows(a.o, a.o_s, at.t.len, p.d);
+  }
+  clear_tiles<D, RAG>();
+  fwd_body<D, true, RAG>(a, 0, 0, at.t.tile);
+}
+
+// Keys of a query head's first (with grouped heads their gradients go through
+// partials, which packed_sum adds), then queries.
+template <int D, bool RAG>
+__global__ void __launch_bounds__(kNT, D == 256 ? 1 : 2) packed_bwd_f32(AttnF32 p, PackedF32 k, uint32_t nkv) {
+  const bool keys = blockIdx.x < nkv;
+  const PackedAt at = packed_at(k.tiles, k.head->count[1], blockIdx.x - (keys ? 0 : nkv), k.heads, k.kv_heads);
+  if (!at.live) return;
+  AttnF32 a = sequence_of(p, at);
+  if (at.t.tile < 0) {
+    if (!keys) return zero_rows(a.dq, a.dq_s, at.t.len, p.d);
+    zero_rows(a.dk, a.dk_s, at.t.len, p.d);  // (of a group's heads each the same)
+    return zero_rows(a.dv, a.dv_s, at.t.len, p.d);
+  }
+  clear_tiles<D, RAG>();
+  if (!keys) return dq_body<D, true, RAG>(a, 0, 0, at.t.tile);
+  if (a.kv_part) {
+    const int g = at.h - at.hk * (k.heads / k.kv_heads);
+    a.kv_part += (((int64_t)g * k.kv_heads + at.hk) * p.Sq + at.t.start) * D;
+  }
+  dkv_body<D, true, RAG>(a, 0, 0, (at.t.len - 1) / kBlk - at.t.tile, 0, false);
+}
+
+template <int D, bool RAG>
+int run_packed(const AttnF32& p, const PackedF32& k, bool backward, hipStream_t s) {
+  const char* what = backward ? "mi355x_packed_attn_bwd" : "mi355x_packed_attn_fwd";
+  const int64_t blocks = k.cap * k.heads, rows = p.Sq * k.heads;
+  MI_REQUIRE(2 * blocks < (1ll << 24) && rows < (1ll << 29), "%s: too many rows and heads", what);
+  const size_t bytes = lds_bytes<D>(backward);
+  const void* kernel = backward ? (const void*)packed_bwd_f32<D, RAG> : (const void*)packed_fwd_f32<D, RAG>;
+  if (!opt_in(kernel, bytes)) return fail(MI355X_ELAUNCH, "%s: cannot reserve %zu bytes of LDS", what, bytes);
+  if (!backward) {
+    packed_fwd_f32<D, RAG><<<(unsigned)blocks, kNT, bytes, s>>>(p, k);
+  } else {
+    delta_f32<D, RAG><<<ceil_div(rows * kChains<D>, kNT), kNT, 0, s>>>(p, rows);
+    packed_bwd_f32<D, RAG><<<(unsigned)(2 * blocks), kNT, bytes, s>>>(p, k, (uint32_t)blocks);
+  }
+  return check_launch(what);
 }
 
 // Tiles are loaded and rows stored 16 bytes at a time.
@@ -597,6 +707,14 @@ bool takes_grads(const AttnF32& p) {
 }
 
 }  // namespace
+
+int attn_f32_packed(const AttnF32& p, const PackedF32& k, bool backward, hipStream_t s) {
+  switch (p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256) {
+    case 64: return p.d == 64 ? run_packed<64, false>(p, k, backward, s) : run_packed<64, true>(p, k, backward, s);
+    case 128: return p.d == 128 ? run_packed<128, false>(p, k, backward, s) : run_packed<128, true>(p, k, backward, s);
+    default: return p.d == 256 ? run_packed<256, false>(p, k, backward, s) : run_packed<256, true>(p, k, backward, s);
+  }
+}
 
 int attn_f32_window_fwd(const AttnF32& p, int64_t d, hipStream_t s) {
   if (!takes(p)) return -1;

@@ -1329,8 +1329,9 @@ _ERROR_KINDS = (
     (IndexError, "index out of range in self"),
     (IndexError, "Target is out of bounds"),
     (IndexError, "a position or page of a paged cache is out of range"),
+    (IndexError, "offsets of packed sequences fall or leave the rows"),
 )
-_INDEX_ERROR, _TARGET_ERROR, _PAGE_ERROR = 0, 1, 2
+_INDEX_ERROR, _TARGET_ERROR, _PAGE_ERROR, _PACKING_ERROR = 0, 1, 2, 3
 _error_flags: dict = {}      # device index -> int32 [len(_ERROR_KINDS)] flag tensor
 _errors_pending: set = set()  # devices with a flag launch since the last read
 

@@ -40,7 +40,8 @@ from __future__ import annotations
 
 import torch
 
-from ..eager_kernels import aten_fast, paged
+from ..eager_kernels import aten_fast, packed, paged
+from ..eager_kernels import materialize_touched
 from .torch_mojo_tensor import TorchMojoTensor
 
 _registered = False
@@ -107,6 +108,30 @@ class _FusedAttention(torch.autograd.Function):
         if torch.is_grad_enabled():  # create_graph
             dq, dk, dv = _OneGradient.apply(dq, dk, dv, q, k, v, grad)
         return dq, dk, dv, None, None, None, None
+
+
+class _PackedAttention(torch.autograd.Function):
+    """Causal attention within packed sequences (ops.packed_attention): the
+    forward saves the rows' log-sum-exp and what rounding took from a 16-bit
+    output, the backward recomputes the weights from them."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, sequences, window, scale):
+        with torch._C._AutoDispatchBelowAutograd():
+            out, lse, low = packed.attention_forward(q, k, v, sequences, window, scale, keep_low=True)
+        ctx.save_for_backward(q, k, v, out, lse, low)
+        ctx.args = (sequences, window, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        q, k, v, out, lse, low = ctx.saved_tensors
+        materialize_touched((grad, q, k, v, out), None, False)
+        with torch._C._AutoDispatchBelowAutograd():
+            dq, dk, dv = paged.on_device(q._device, packed.attention_backward, grad, q, k, v, out, lse, low, *ctx.args)
+        if torch.is_grad_enabled():  # create_graph
+            dq, dk, dv = _OneGradient.apply(dq, dk, dv, q, k, v, grad)
+        return dq, dk, dv, None, None, None
 
 
 class _OneGradient(torch.autograd.Function):

@@ -17,8 +17,8 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import kv_cache
-from .eager_kernels import aten_fast, materialize_touched, paged
+from . import kv_cache, packing
+from .eager_kernels import aten_fast, materialize_touched, packed, paged
 from .masks import sliding_window_causal_mask
 from .mojo_device.torch_mojo_tensor import TorchMojoTensor
 
@@ -144,6 +144,58 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
         return q * 1.0
     return F.scaled_dot_product_attention(
         q, k, v, attn_mask=sliding_window_causal_mask(t, min(window, t), q.device, sinks=sinks), scale=scale, enable_gqa=True)
+
+
+# ---------------------------------------------------------------------------
+# packed sequences (torch_mojo_backend.packing)
+# ---------------------------------------------------------------------------
+def packed_attention(q, k, v, sequences, *, window=0, scale=None):
+    """Causal attention within each of a batch's packed sequences: row i of q
+    [tokens, heads, head_dim] sees the rows j <= i of k, v [tokens, kv_heads,
+    head_dim] of its own sequence and, with a window > 0, only those with i - j <
+    window.  Query head h reads K/V head h // (heads // kv_heads); scale defaults
+    to head_dim ** -0.5.  Rows that belong to no sequence give zero, whatever
+    they hold, and get zero gradients.  Differentiable in q, k and v.
+
+    `sequences` is a packing.PackedSequences of the batch, on its device.  On the
+    mojo device head_dim is a multiple of 8 up to 256, of float32, bfloat16 or
+    float16.  Nothing of a sequence reaches another one; a NaN or an infinity in a
+    row may reach the other rows of its own sequence, also earlier ones, as 0 *
+    NaN does in the plain formula."""
+    what = "packed_attention"
+    if not isinstance(sequences, packing.PackedSequences):
+        raise TypeError(f"{what}: sequences must be a PackedSequences, got {type(sequences).__name__}")
+    if any(x.dim() != 3 for x in (q, k, v)) or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] \
+            or q.shape[0] != sequences.tokens:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, heads,"
+                         f" head_dim] of the same head_dim and of the batch's {sequences.tokens} rows")
+    if not q.shape[1] or not k.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{what}: {q.shape[1]} heads over {k.shape[1]} K/V heads")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"{what}: q, k and v are of {q.dtype}, {k.dtype} and {v.dtype}, expected one dtype")
+    if not q.device == k.device == v.device == sequences.device or _on_mojo(q, k, v) != sequences.on_mojo:
+        raise ValueError(f"{what}: q, k and v are on {q.device}, {k.device} and {v.device}, the sequences on {sequences.device}")
+    window = int(window)
+    if window < 0:
+        raise ValueError(f"{what}: window {window} must not be negative")
+    if scale is not None:
+        scale = float(scale)
+        if not abs(scale) < 1e38:
+            raise ValueError(f"{what}: scale {scale} must be finite in 32 bits")
+    window = min(window, sequences.tokens)
+    if not q.numel():
+        return q * 1.0
+    if not sequences.on_mojo:
+        return packing.attention_plain(q, k, v, sequences, window, scale)
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or q.shape[2] > 256 or q.shape[2] % 8:
+        raise NotImplementedError(f"{what}: {q.dtype} with head_dim {q.shape[2]} is not supported"
+                                  " (float32, bfloat16, float16, head_dim a multiple of 8 up to 256)")
+    if not _needs_grad(q, k, v):
+        return packed.attention(q, k, v, sequences, window, scale)
+    from .mojo_device.mojo_device_autograd import _PackedAttention
+
+    materialize_touched((q, k, v), None, False)
+    return paged.on_device(q._device, _PackedAttention.apply, q, k, v, sequences, window, scale)
 
 
 # ---------------------------------------------------------------------------
