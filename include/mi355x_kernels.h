@@ -765,6 +765,44 @@ int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, const int64
                            const float* lse, const void* plan, int64_t sequences, int64_t tokens,
                            int64_t heads, int64_t kv_heads, int64_t d, double scale, int64_t window,
                            int dtype, void* workspace, int64_t ws_bytes, mi355x_stream_t stream);
+/* Rotary positions from the positions themselves.  Pair j of a row's first
+ * `turned` channels (channels j and j + turned / 2, or interleaved 2j and 2j + 1)
+ * is turned by the angle p * frequencies[j] of its position p and scaled; the
+ * channels behind are copied.  inverse = 1 turns the other way, with the same
+ * scale: the backward.  q and k (either may have no heads) go through one
+ * launch.  *_bht: (batch, head, token) strides in elements, channels of stride 1;
+ * positions: int32 or int64 [seq] of each batch, positions_stride elements apart
+ * (0: the same); frequencies: f64 [turned / 2] in device memory, radians a
+ * position.  Angles are taken in f64.  The reference's models build their angles
+ * in PyTorch and run under torch.compile (demo_scripts/gemma3.py:11). */
+int mi355x_rope_at(void* q_out, const int64_t* qo_bht, const void* q, const int64_t* q_bht, int64_t heads,
+                   void* k_out, const int64_t* ko_bht, const void* k, const int64_t* k_bht, int64_t kv_heads,
+                   const void* positions, int positions_dtype, int64_t positions_stride,
+                   const double* frequencies, int64_t batch, int64_t seq, int64_t d, int64_t turned,
+                   int interleaved, double scale, int inverse, int dtype, mi355x_stream_t stream);
+
+/* ---- log-probabilities of given tokens ----------------------------------
+ * Of each row of logits [n][c] (rows at logits + i * ld): logprobs[i] =
+ * log_softmax(row)[tokens[i]] (0 where tokens[i] is ignore_index; a token outside
+ * [0, c) sets *error, which may be null, and gives 0), entropy[i] = -sum p log p,
+ * and the `top` (up to 64) largest entries, NaN first and equal ones by index:
+ * top_logprobs, top_tokens [n][top].  logprobs and entropy may be null.  stats
+ * [n][2]: the row's maximum and the logarithm of the sum of exp(x - maximum).
+ * The reference composes these from log_softmax and gather
+ * (aten_fast.py:5792-5825, 9332-9368) and has no top entries. */
+int64_t mi355x_token_logprobs_workspace_bytes(int64_t n, int64_t c, int top, int dtype);
+int mi355x_token_logprobs_fwd(float* logprobs, float* entropy, float* stats, float* top_logprobs,
+                              int64_t* top_tokens, const void* logits, int dtype, int64_t ld,
+                              const int64_t* tokens, int64_t n, int64_t c, int top, int64_t ignore_index,
+                              int32_t* error, void* workspace, int64_t ws_bytes, mi355x_stream_t stream);
+/* The gradient of the three with respect to the logits, from f32 gradients of
+ * each (null: none), in the logits' dtype; rows at dx + i * ld_dx, 16-byte
+ * aligned, columns [c, ld_dx) written as zero. */
+int mi355x_token_logprobs_bwd(void* dx, int64_t ld_dx, const void* logits, int dtype, int64_t ld,
+                              const float* stats, const float* entropy, const int64_t* tokens,
+                              const int64_t* top_tokens, int top, const float* d_logprobs,
+                              const float* d_entropy, const float* d_top, int64_t n, int64_t c,
+                              int64_t ignore_index, mi355x_stream_t stream);
 
 #ifdef __cplusplus
 }

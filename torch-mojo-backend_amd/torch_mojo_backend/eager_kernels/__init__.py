@@ -325,6 +325,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             c_i64, c_i64, c_i64, c_double, c_i64, c_i64, c_int, c_vp, c_i64, c_vp, c_vp,
         ],
     ),
+    "mi355x_rope_at": (
+        c_int,
+        [
+            c_vp, P_i64, c_vp, P_i64, c_i64, c_vp, P_i64, c_vp, P_i64, c_i64, c_vp, c_int, c_i64, c_vp,
+            c_i64, c_i64, c_i64, c_i64, c_int, c_double, c_int, c_int, c_vp,
+        ],
+    ),
+    "mi355x_token_logprobs_workspace_bytes": (c_i64, [c_i64, c_i64, c_int, c_int]),
+    "mi355x_token_logprobs_fwd": (
+        c_int,
+        [
+            c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_vp, c_i64, c_i64, c_int, c_i64, c_vp, c_vp, c_i64, c_vp,
+        ],
+    ),
+    "mi355x_token_logprobs_bwd": (
+        c_int,
+        [
+            c_vp, c_i64, c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
+        ],
+    ),
     "mi355x_packed_plan_bytes": (c_i64, [c_i64, c_i64]),
     "mi355x_packed_plan": (c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp]),
     "mi355x_packed_attn_fwd": (

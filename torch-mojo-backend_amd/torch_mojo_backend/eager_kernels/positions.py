@@ -1,0 +1,100 @@
+"""Calls of the rotary positions' and the token log-probabilities' kernels
+(csrc/rope_at.hip, csrc/logprobs.hip) on mojo tensors.
+
+Arguments are checked in `torch_mojo_backend.ops`.  Outputs and workspaces are
+allocated here; launches go to the null stream of the tensors' device.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import check
+from . import native_lib as lib
+from .aten_fast import (
+    _STREAM, _TARGET_ERROR, _alloc, _code, _contig, _error_slot, _workspace, alloc_bthd, materialize_contiguous,
+)
+from ..mojo_device.torch_mojo_tensor import TorchMojoTensor as MT
+
+
+def _bht(t: MT):
+    """(batch, head, token) strides of [batch, heads, tokens, d] or [tokens, heads, d]."""
+    st = t._strides
+    return st[:3] if len(st) == 4 else (0, st[1], st[0])
+
+
+def _side(t):
+    """(out, its pointer and strides, t's pointer and strides, heads) for t or None."""
+    if t is None:
+        return None, (None, (0, 0, 0), None, (0, 0, 0), 0)
+    if t._strides[-1] != 1:
+        t = materialize_contiguous(t)
+    out = alloc_bthd(*t._shape, t._dtype, t._device) if len(t._shape) == 4 else _alloc(t._shape, t._dtype, t._device)
+    return out, (out._ptr, _bht(out), t._ptr, _bht(t), t._shape[1])
+
+
+def rotary(q, k, positions: MT, frequencies: MT, interleaved, scale, inverse):
+    """(q, k) turned; either may be None."""
+    like = q if q is not None else k
+    batch, seq = (like._shape[0], like._shape[2]) if len(like._shape) == 4 else (1, like._shape[0])
+    if positions._strides and positions._strides[-1] != 1 and positions._shape[-1] > 1:
+        positions = materialize_contiguous(positions)
+    frequencies = _contig(frequencies)
+    (qo, qa), (ko, ka) = _side(q), _side(k)
+    check(
+        "mi355x_rope_at",
+        lib().mi355x_rope_at(*qa, *ka, positions._ptr, _code(positions._dtype),
+                             positions._strides[0] if len(positions._shape) == 2 else 0, frequencies._ptr, batch, seq,
+                             like._shape[-1], 2 * frequencies._shape[0], int(interleaved), scale, int(inverse),
+                             _code(like._dtype), _STREAM),
+    )
+    return qo, ko
+
+
+def logprobs_forward(x: MT, tokens, top, entropy, ignore_index):
+    """(logprobs, entropy, top_logprobs, top_tokens, stats) of x [n, vocab]."""
+    if x._strides[1] != 1 and x._shape[1] > 1 or x._strides[0] < 0:
+        x = materialize_contiguous(x)
+    (n, c), dev = x._shape, x._device
+    code, library = _code(x._dtype), lib()
+    f32 = torch.float32
+    picked = _alloc((n,), f32, dev) if tokens is not None else None
+    spread = _alloc((n,), f32, dev) if entropy else None
+    best, order = (_alloc((n, top), f32, dev), _alloc((n, top), torch.int64, dev)) if top else (None, None)
+    stats = _alloc((n, 2), f32, dev)
+    ws = library.mi355x_token_logprobs_workspace_bytes(n, c, top, code)
+    hold, wptr = _workspace(ws, dev)
+    at = lambda t: t._ptr if t is not None else None  # noqa: E731
+    check(
+        "mi355x_token_logprobs_fwd",
+        library.mi355x_token_logprobs_fwd(at(picked), at(spread), stats._ptr, at(best), at(order), x._ptr, code,
+                                          x._strides[0], at(_contig(tokens)) if tokens is not None else None, n, c, top,
+                                          ignore_index, _error_slot(dev, _TARGET_ERROR), wptr, ws, _STREAM),
+    )
+    return picked, spread, best, order, stats
+
+
+def logprobs_backward(x: MT, tokens, stats, spread, order, d_picked, d_spread, d_best, ignore_index):
+    """d_logits of x's dtype, its rows padded to 16 bytes (as the GEMMs behind it read them)."""
+    if x._strides[1] != 1 and x._shape[1] > 1 or x._strides[0] < 0:
+        x = materialize_contiguous(x)
+    (n, c), dev = x._shape, x._device
+    ld = (c + 7) // 8 * 8
+    dense = _alloc((n, ld), x._dtype, dev)
+    dx = MT._view_of(dense, (n, c), (ld, 1), 0, ld == c)
+
+    def grad(t):
+        if t is None:
+            return None
+        return _contig(t) if t._dtype is torch.float32 else materialize_contiguous(t, torch.float32)
+
+    d_picked, d_spread, d_best = grad(d_picked), grad(d_spread), grad(d_best)
+    at = lambda t: t._ptr if t is not None else None  # noqa: E731
+    check(
+        "mi355x_token_logprobs_bwd",
+        lib().mi355x_token_logprobs_bwd(dx._ptr, ld, x._ptr, _code(x._dtype), x._strides[0], stats._ptr, at(spread),
+                                        at(_contig(tokens)) if tokens is not None else None, at(order),
+                                        order._shape[1] if order is not None else 0, at(d_picked), at(d_spread),
+                                        at(d_best), n, c, ignore_index, _STREAM),
+    )
+    return dx

@@ -40,7 +40,7 @@ from __future__ import annotations
 
 import torch
 
-from ..eager_kernels import aten_fast, packed, paged
+from ..eager_kernels import aten_fast, packed, paged, positions
 from ..eager_kernels import materialize_touched
 from .torch_mojo_tensor import TorchMojoTensor
 
@@ -132,6 +132,50 @@ class _PackedAttention(torch.autograd.Function):
         if torch.is_grad_enabled():  # create_graph
             dq, dk, dv = _OneGradient.apply(dq, dk, dv, q, k, v, grad)
         return dq, dk, dv, None, None, None
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    """ops.token_logprobs of logits [n, vocab]: one read of them forward, one
+    more and the gradient's write backward."""
+
+    @staticmethod
+    def forward(ctx, x, tokens, top, entropy, ignore_index):
+        with torch._C._AutoDispatchBelowAutograd():
+            picked, spread, best, order, stats = positions.logprobs_forward(x, tokens, top, entropy, ignore_index)
+        ctx.save_for_backward(x, tokens, stats, spread, order)
+        ctx.ignore_index = ignore_index
+        ctx.set_materialize_grads(False)
+        if order is not None:
+            ctx.mark_non_differentiable(order)
+        return picked, spread, best, order
+
+    @staticmethod
+    def backward(ctx, d_picked, d_spread, d_best, _):
+        x, tokens, stats, spread, order = ctx.saved_tensors
+        grads = [g for g in (d_picked, d_spread, d_best) if g is not None]
+        if not grads:
+            return None, None, None, None, None
+        materialize_touched((x, tokens, *grads), None, False)
+        with torch._C._AutoDispatchBelowAutograd():
+            dx = paged.on_device(x._device, positions.logprobs_backward, x, tokens, stats, spread, order, d_picked,
+                                 d_spread, d_best, ctx.ignore_index)
+        if torch.is_grad_enabled():  # create_graph
+            dx = _OnceOnly.apply("token_logprobs", dx, x, *grads)
+        return dx, None, None, None, None
+
+
+class _OnceOnly(torch.autograd.Function):
+    """A gradient as it is, with an error for a graph that its kernel does not
+    leave (as _OneGradient)."""
+
+    @staticmethod
+    def forward(ctx, what, dx, *inputs):
+        ctx.what = what
+        return dx.view_as(dx)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"the gradient of {ctx.what} is not differentiable a second time")
 
 
 class _OneGradient(torch.autograd.Function):

@@ -17,8 +17,8 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import kv_cache, packing
-from .eager_kernels import aten_fast, materialize_touched, packed, paged
+from . import kv_cache, logprobs, packing, rotary
+from .eager_kernels import aten_fast, materialize_touched, packed, paged, positions as _positions
 from .masks import sliding_window_causal_mask
 from .mojo_device.torch_mojo_tensor import TorchMojoTensor
 
@@ -147,8 +147,78 @@ def sliding_window_attention(q, k, v, window, *, sinks=0, scale=None):
 
 
 # ---------------------------------------------------------------------------
-# packed sequences (torch_mojo_backend.packing)
+# rotary positions, and packed sequences (torch_mojo_backend.packing)
 # ---------------------------------------------------------------------------
+class _RotaryAt(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, interleaved, scale, inverse):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.args = (interleaved, scale, inverse)
+        ctx.set_materialize_grads(False)
+        with torch._C._AutoDispatchBelowAutograd():
+            return _positions.rotary(q, k, positions, frequencies, interleaved, scale, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        if dq is None and dk is None:
+            return (None,) * 7
+        positions, frequencies = ctx.saved_tensors
+        interleaved, scale, inverse = ctx.args
+        given = [g for g in (dq, dk) if g is not None]
+        materialize_touched((*given, positions, frequencies), None, False)
+        turn = _RotaryAt.apply if _needs_grad(*given) else _positions.rotary
+        dq, dk = paged.on_device(given[0]._device, turn, dq, dk, positions, frequencies, interleaved, scale, not inverse)
+        return dq, dk, None, None, None, None, None
+
+
+def rotary_at(q, k, positions, frequencies, *, interleaved=False, scale=1.0):
+    """q and k (or None) with their first channels turned by the angles of the
+    rows' positions: pair j of the first n = 2 * len(frequencies) channels,
+    channels j and j + n / 2, or with `interleaved` 2j and 2j + 1, becomes scale *
+    (a cos - b sin, b cos + a sin) with the angle position * frequencies[j]; the
+    channels behind are copied.  Differentiable in q and k.
+
+    q and k are [tokens, heads, head_dim] with positions [tokens] (packed
+    sequences: PackedSequences.positions), or [batch, heads, tokens, head_dim]
+    with positions [tokens] or [batch, tokens]; positions are int32 or int64.
+    frequencies is f64 (`rotary.rotary_frequencies`, with the scale that goes with
+    stretched contexts): angles are taken in 64 bits and good at any position
+    below 2 ** 31.  One kernel on the mojo device."""
+    what = "rotary_at"
+    rows = [x for x in (q, k) if x is not None]
+    if not rows:
+        raise ValueError(f"{what}: neither q nor k")
+    like = rows[0]
+    if like.dim() not in (3, 4):
+        raise ValueError(f"{what}: rows must be [tokens, heads, head_dim] or [batch, heads, tokens, head_dim], got {tuple(like.shape)}")
+    outer = (lambda x: (x.shape[0],)) if like.dim() == 3 else (lambda x: (x.shape[0], x.shape[2]))
+    if any(x.dim() != like.dim() or outer(x) != outer(like) or x.shape[-1] != like.shape[-1] for x in rows):
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} must have the same tokens and head_dim")
+    if any(x.dtype != like.dtype for x in rows):
+        raise TypeError(f"{what}: q is of {q.dtype}, k of {k.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in (outer(like), outer(like)[-1:]):
+        raise ValueError(f"{what}: positions must be int32 or int64 {' or '.join(str(list(s)) for s in {outer(like), outer(like)[-1:]})},"
+                         f" got {tuple(positions.shape)} of {positions.dtype}")
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or 2 * frequencies.shape[0] > like.shape[-1]:
+        raise ValueError(f"{what}: frequencies must be float64 [pairs] of at most {like.shape[-1] // 2} pairs, got"
+                         f" {tuple(frequencies.shape)} of {frequencies.dtype}")
+    if any(x.device != like.device for x in (*rows, positions, frequencies)):
+        raise ValueError(f"{what}: q, k, positions and frequencies must be on one device")
+    scale = float(scale)
+    if not abs(scale) < 1e38:
+        raise ValueError(f"{what}: scale {scale} must be finite in 32 bits")
+    if not _on_mojo(*rows, positions, frequencies):
+        at = lambda x: x if x is None else rotary.turn_plain(  # noqa: E731
+            x if x.dim() == 4 else x.transpose(0, 1), positions, frequencies, interleaved, scale)
+        return tuple(x if x is None or x.dim() == 4 else x.transpose(0, 1) for x in (at(q), at(k)))
+    if like.dtype not in (torch.float32, torch.bfloat16, torch.float16) or like.shape[-1] > 4096:
+        raise NotImplementedError(f"{what}: {like.dtype} with head_dim {like.shape[-1]} is not supported"
+                                  " (float32, bfloat16, float16, head_dim up to 4096)")
+    materialize_touched((*rows, positions, frequencies), None, False)
+    turn = _RotaryAt.apply if _needs_grad(*rows) else _positions.rotary
+    return paged.on_device(like._device, turn, q, k, positions, frequencies, bool(interleaved), scale, False)
+
+
 def packed_attention(q, k, v, sequences, *, window=0, scale=None):
     """Causal attention within each of a batch's packed sequences: row i of q
     [tokens, heads, head_dim] sees the rows j <= i of k, v [tokens, kv_heads,
@@ -196,6 +266,51 @@ def packed_attention(q, k, v, sequences, *, window=0, scale=None):
 
     materialize_touched((q, k, v), None, False)
     return paged.on_device(q._device, _PackedAttention.apply, q, k, v, sequences, window, scale)
+
+
+def token_logprobs(logits, tokens=None, *, top=0, entropy=False, ignore_index=-100):
+    """Of each row of logits [..., vocab]: the log-probability of the given token
+    (tokens [...], int64; 0 where it is ignore_index), with `entropy` the
+    distribution's entropy in nats, and the `top` largest log-probabilities with
+    their tokens, largest first, equal ones by token (a NaN before all others).
+    Returns a logprobs.TokenLogprobs, float32 whatever the logits' dtype (f64 of
+    f64); differentiable in logits, whose gradient is of their dtype.
+
+    On the mojo device the logits are read once, and once more for the gradient;
+    `top` goes up to 64.  A token outside the vocabulary raises IndexError, on
+    the mojo device at the next device-to-host read."""
+    what = "token_logprobs"
+    top = int(top)
+    if logits.dim() < 1 or not logits.shape[-1]:
+        raise ValueError(f"{what}: logits must be [..., vocab], got {tuple(logits.shape)}")
+    if not logits.dtype.is_floating_point:
+        raise TypeError(f"{what}: logits of {logits.dtype} are not supported")
+    if not 0 <= top <= logits.shape[-1]:
+        raise ValueError(f"{what}: {top} top entries of {logits.shape[-1]}")
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1]:
+            raise ValueError(f"{what}: tokens must be int64 {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)} of {tokens.dtype}")
+        if tokens.device != logits.device:
+            raise ValueError(f"{what}: tokens are on {tokens.device}, the logits on {logits.device}")
+    if not _on_mojo(logits) or (tokens is not None and not _on_mojo(tokens)):
+        return logprobs.plain(logits, tokens, top, entropy, ignore_index)
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16) or top > 64:
+        raise NotImplementedError(f"{what}: {logits.dtype} with {top} top entries is not supported (float32, bfloat16,"
+                                  " float16, top up to 64)")
+    lead = logits.shape[:-1]
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    if tokens is not None and tokens.dim() != 1:
+        tokens = tokens.reshape(-1)
+    materialize_touched((x, tokens), None, False)
+    if _needs_grad(x):
+        from .mojo_device.mojo_device_autograd import _TokenLogprobs
+
+        got = paged.on_device(x._device, _TokenLogprobs.apply, x, tokens, top, bool(entropy), int(ignore_index))
+    else:
+        got = paged.on_device(x._device, _positions.logprobs_forward, x, tokens, top, bool(entropy), int(ignore_index))[:4]
+    if len(lead) != 1:
+        got = [y if y is None else y.view((*lead, *y.shape[1:])) for y in got]
+    return logprobs.TokenLogprobs(*got)
 
 
 # ---------------------------------------------------------------------------
