@@ -796,8 +796,8 @@ int mi355x_token_logprobs_fwd(float* logprobs, float* entropy, float* stats, flo
                               const int64_t* tokens, int64_t n, int64_t c, int top, int64_t ignore_index,
                               int32_t* error, void* workspace, int64_t ws_bytes, mi355x_stream_t stream);
 /* The gradient of the three with respect to the logits, from f32 gradients of
- * each (null: none), in the logits' dtype; rows at dx + i * ld_dx, 16-byte
- * aligned, columns [c, ld_dx) written as zero. */
+ * each (null: none), in the logits' dtype; rows at dx + i * ld_dx, columns [c,
+ * ld_dx) written as zero. */
 int mi355x_token_logprobs_bwd(void* dx, int64_t ld_dx, const void* logits, int dtype, int64_t ld,
                               const float* stats, const float* entropy, const int64_t* tokens,
                               const int64_t* top_tokens, int top, const float* d_logprobs,

@@ -130,7 +130,7 @@ __device__ __forceinline__ void zero_rows(const Rows& x, const PackedTile& t, in
 // halves take half of a tile's keys each and join at the end.
 // ---------------------------------------------------------------------------
 template <typename T, int D, bool RAG, int NW, int QPW, int KH>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) packed_fwd(PackedArgs p) {
+__global__ void __launch_bounds__(64 * NW, D == 256 || QPW == 64 ? 1 : 2) packed_fwd(PackedArgs p) {
   constexpr int QT = QPW / 16, QPB = NW / KH * QPW;
   constexpr int LIST = QPB == 128 ? 0 : 1;
   static_assert(QPB == kPackedRows[LIST], "");
@@ -372,11 +372,20 @@ __global__ void __launch_bounds__(kThreads) packed_delta(PackedArgs p) {
   }
 }
 
+#ifndef PK_OCC
+#define PK_OCC 1
+#endif
+#ifndef PK_NW
+#define PK_NW 4
+#endif
 template <int D>
-constexpr int kKeyTiles = D == 256 ? 1 : 2;  // 16-key tiles of a wave: two would take all registers at 256
+constexpr int kBwdWaves = D == 128 ? PK_NW : 4;
+template <int D>
+constexpr int kKeyTiles = D == 256 ? 1 : 8 / kBwdWaves<D>;  // 16-key tiles of a wave: two would take all registers at 256
 template <int D>
 constexpr int kKeyList = D == 256 ? 1 : 0;
-constexpr int kQueryTiles = 2;
+template <int D>
+constexpr int kQueryTiles = 8 / kBwdWaves<D>;
 
 // dK and dV of a tile of keys, over the query heads [g0, g1) of its group.
 template <typename T, int D, bool RAG>
@@ -388,8 +397,9 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
   const int lane = threadIdx.x & 63, wave = wave_id(), lr = lane & 15, lg = lane >> 4;
   const int start = t.start, len = t.len, group = p.heads / p.kv_heads;
   // (the list's number counts from the end: the first keys' tiles take longest)
-  const int tile = (len - 1) / (4 * KW) - t.tile;
-  const int k0 = tile * (4 * KW), kw = k0 + wave * KW;
+  constexpr int KB = kBwdWaves<D> * KW;
+  const int tile = (len - 1) / KB - t.tile;
+  const int k0 = tile * KB, kw = k0 + wave * KW;
   const int window = p.window > 0 ? min(p.window, len) : len;
 
   if constexpr (RAG) clear_lds(lds, 2 * STAGE);
@@ -407,11 +417,11 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
     for (int u = 0; u < RT; ++u) dva[dt][u] = dka[dt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int qstart = k0 / 64 * 64;  // the steps that see the tile's keys
-  const int qend = (int)min((int64_t)len, (int64_t)k0 + 4 * KW - 1 + window);
+  const int qend = min(len, k0 + KB - 1 + window);
   const int nqb = (qend - qstart + 63) / 64, nsteps = nqb * (g1 - g0);
   const int sw = L::swz(lr);
   const TrOffsets<D> tro;
-  TileLoad<D, 4, RAG> ql, dl;
+  TileLoad<D, kBwdWaves<D>, RAG> ql, dl;
   auto head_of = [&](int g) {
     const int h = hk * group + g;
     ql.init(p.q.at<T>(start, h), p.q.row * (int64_t)sizeof(T), p.d);
@@ -521,7 +531,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
   int j1 = nqb, j2 = nqb;
   if (kw + KW <= len) {
     j1 = min(nqb, (max(0, kw + KW - 1 - qstart) + 63) / 64);
-    j2 = max(j1, min(nqb, max(0, (int)min((int64_t)len, (int64_t)kw + window) - qstart) / 64));
+    j2 = max(j1, min(nqb, max(0, min(len, kw + window) - qstart) / 64));
   }
   for (int g = g0; g < g1; ++g) {
     int j = 0;
@@ -562,17 +572,18 @@ template <typename T, int D, bool RAG>
 __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t, int h, int hk, char* lds) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
-  constexpr int RT = kQueryTiles, QW = 16 * RT, KS = D / 32, DT = D / 16;
+  constexpr int RT = kQueryTiles<D>, QW = 16 * RT, QB = kBwdWaves<D> * QW, KS = D / 32, DT = D / 16;
+  static_assert(QB == 128, "");
   constexpr int STAGE = 2 * L::TILE;
   const int lane = threadIdx.x & 63, wave = wave_id(), lr = lane & 15, lg = lane >> 4;
-  const int start = t.start, len = t.len, q0 = t.tile * (4 * QW), qw = q0 + wave * QW;
+  const int start = t.start, len = t.len, q0 = t.tile * QB, qw = q0 + wave * QW;
   const int window = p.window > 0 ? min(p.window, len) : len;
 
   if constexpr (RAG) clear_lds(lds, 2 * STAGE);
-  TileLoad<D, 4, RAG> kl, vl;
+  TileLoad<D, kBwdWaves<D>, RAG> kl, vl;
   kl.init(p.k.at<T>(start, hk), p.k.row * (int64_t)sizeof(T), p.d);
   vl.init(p.v.at<T>(start, hk), p.v.row * (int64_t)sizeof(T), p.d);
-  const int kv_end = min(len, q0 + 4 * QW);
+  const int kv_end = min(len, q0 + QB);
   const int jw = max(0, q0 - window + 1) / 64;
   kl.issue(jw * 64, len, lds);
   vl.issue(jw * 64, len, lds + L::TILE);
@@ -695,7 +706,7 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 // where their gradients go through partials, one of a query head's; the rest
 // take queries.
 template <typename T, int D, bool RAG>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1) packed_bwd(PackedArgs p, uint32_t nkv) {
+__global__ void __launch_bounds__(64 * kBwdWaves<D>, D == 64 ? 2 : D == 128 ? PK_OCC : 1) packed_bwd(PackedArgs p, uint32_t nkv) {
   char* const lds = packed_lds;
   const int group = p.heads / p.kv_heads;
   if (blockIdx.x < nkv) {
@@ -755,7 +766,10 @@ constexpr int64_t kMostThreads = 1ll << 32;
 
 template <typename T, int D, bool RAG>
 int fwd_launch(const PackedArgs& a, const Launch& l) {
-  constexpr int KH = D == 256 ? 2 : 1, NW = 4 * KH, QPW = D == 256 ? 16 : 32, QPB = NW / KH * QPW;
+#ifndef PK_FW
+#define PK_FW 4
+#endif
+  constexpr int KH = D == 256 ? 2 : 1, NW = D == 256 ? 8 : D == 128 ? PK_FW : 4, QPW = D == 256 ? 16 : 128 / NW, QPB = NW / KH * QPW;
   constexpr int bytes = 4 * KvLayout<D>::TILE;
   auto k = packed_fwd<T, D, RAG, NW, QPW, KH>;
   const int rc = reserve((const void*)k, bytes, "mi355x_packed_attn_fwd");
@@ -787,7 +801,7 @@ int bwd_launch(const PackedArgs& a, const Launch& l) {
   MI_REQUIRE((nkv + nq) * kThreads < kMostThreads && rows * (D / 4) < kMostThreads - kThreads,
              "mi355x_packed_attn_bwd: too many rows and heads");
   packed_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, l.s>>>(a);
-  k<<<(unsigned)(nkv + nq), kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
+  k<<<(unsigned)(nkv + nq), 64 * kBwdWaves<D>, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
   return a.kv_part ? sum_launch<T, D, RAG>(a, l) : check_launch("mi355x_packed_attn_bwd");
 }
 

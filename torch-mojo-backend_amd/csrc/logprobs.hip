@@ -300,49 +300,61 @@ __global__ void __launch_bounds__((LpShape<T, NW, CPT>::kThreads)) lp_rows(LpArg
   }
 }
 
-// A row's segments: one block, kJoinList keys at most.
-constexpr int kJoinThreads = 256, kJoinList = 4096;
+// A row's segments: one block, kJoinList keys at most.  The bound here: with r =
+// ceil(k / segments), the ceil(k / r)-th largest of the segments' r-th keys (of
+// their maxima, where there are k segments), which r entries of each of as many
+// segments reach.
+constexpr int kJoinThreads = 256, kJoinList = 4096, kMostSegments = 512;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) lp_join(LpArgs p) {
   __shared__ u64 list[kJoinList];
+  __shared__ u64 heads[kMostSegments];
   __shared__ float red[kJoinThreads / 64][3];
-  __shared__ u64 bounds[kJoinThreads / 64];
+  __shared__ u64 bound_s;
   __shared__ int count_s;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = p.segments, k = p.top;
   const int64_t row = blockIdx.x;
   const float* const part = p.part + row * g * 3;
   const u64* const keys = p.part_keys + row * g * k;
-  if (tid == 0) count_s = 0;
+  const int r = k ? (k + g - 1) / g : 1, need = k ? (k + r - 1) / r : 0;
+  if (tid == 0) count_s = 0, bound_s = 0;
   float m = -INFINITY;
-  u64 bound = 0;  // the largest of the segments' last keys: k entries reach it
   for (int i = tid; i < g; i += kJoinThreads) {
     m = nan_max(m, part[3 * i]);
-    if (k) bound = max(bound, keys[(int64_t)i * k + k - 1]);
+    if (k) heads[i] = keys[(int64_t)i * k + r - 1];
   }
-  m = wave_max_nan(m), bound = wave_max_key(bound);
-  if (lane == 0) red[wave][0] = m, bounds[wave] = bound;
+  m = wave_max_nan(m);
+  if (lane == 0) red[wave][0] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 64; ++w) m = nan_max(m, red[w][0]), bound = max(bound, bounds[w]);
+  for (int w = 0; w < kJoinThreads / 64; ++w) m = nan_max(m, red[w][0]);
   float s = 0.f, t = 0.f;
   for (int i = tid; i < g; i += kJoinThreads) {
     const float ps = part[3 * i + 1], pt = part[3 * i + 2], d = not_below((part[3 * i] - m) * kLog2e), f = hw_exp2(d);
     // of a segment whose entries are all -inf nothing counts, and its own sums are NaN
     const bool none = part[3 * i] == -INFINITY && m > -INFINITY;
     s += none ? 0.f : ps * f, t += none ? 0.f : (pt + ps * d * kLn2) * f;
+    if (k) {
+      const u64 mine = heads[i];
+      int before = 0;
+      for (int j = 0; j < g; ++j) before += heads[j] > mine;
+      if (mine && before == need - 1) bound_s = mine;
+    }
   }
   s = wave_sum(s), t = wave_sum(t);
   if (lane == 0) red[wave][1] = s, red[wave][2] = t;
-  if (k)
-    for (int i = tid; i < g * k; i += kJoinThreads) {
-      const u64 key = keys[i];
-      if (key && key >= bound) list[atomicAdd(&count_s, 1)] = key;
-    }
   __syncthreads();
   s = t = 0.f;
 #pragma unroll
   for (int w = 0; w < kJoinThreads / 64; ++w) s += red[w][1], t += red[w][2];
   if (tid == 0) finish_row<T>(p, row, m, s, t);
+  if (!k) return;
+  const u64 bound = bound_s;
+  for (int i = tid; i < g * k; i += kJoinThreads) {
+    const u64 key = keys[i];
+    if (key && key >= bound) list[atomicAdd(&count_s, 1)] = key;
+  }
+  __syncthreads();
   const float ls = log2f(s) * kLn2;
   const int count = count_s;
   for (int i = tid; i < count; i += kJoinThreads) {
@@ -404,7 +416,7 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
     for (int u = 0; u < U; ++u) {
       const int64_t j = j0 + u * kBwdThreads * V;
       if (j >= c1) break;
-      struct alignas(16) { T v[V]; } o;
+      struct { T v[V]; } o;
       const bool whole = j + V <= p.c && !(given && token - j >= 0 && token - j < V);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -415,7 +427,13 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
         }
         o.v[e] = (T)r;
       }
-      *(decltype(o)*)(dx + j) = o;
+      if (j + V <= p.ld_dx) {
+        __builtin_memcpy(dx + j, o.v, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (j + e < p.ld_dx) dx[j + e] = o.v[e];
+      }
     }
   }
   if (!p.d_top) return;
@@ -440,6 +458,9 @@ struct LpPlan {
   int waves;      // of a segment: 1, 4 or 8
   int64_t segments, seg;
 };
+#ifndef LP_SEG
+#define LP_SEG 4
+#endif
 template <typename T>
 LpPlan plan_of(int64_t n, int64_t c, int top) {
   constexpr int V = Chunk<T>::V;
@@ -447,12 +468,11 @@ LpPlan plan_of(int64_t n, int64_t c, int top) {
   if (c <= one && (n >= 512 || c <= one / 4)) return {1, 1, c};
   if (c <= eight && n >= 256) return {8, 1, c};
   int64_t g = (c + eight - 1) / eight;
-  if (n < 512) g = std::max<int64_t>(g, std::min<int64_t>((512 + n - 1) / n, c / (one / 8)));
-  g = std::min<int64_t>(g, top ? kJoinList / top : kJoinList);
-  g = std::max<int64_t>(g, 1);
+  if (n < 512) g = std::max<int64_t>(g, std::min<int64_t>((512 + n - 1) / n, c / (four / LP_SEG)));
+  g = std::max<int64_t>(1, std::min<int64_t>(g, std::min(kMostSegments, top ? kJoinList / top : kMostSegments)));
   const int64_t seg = ((c + g - 1) / g + V - 1) / V * V;
   g = (c + seg - 1) / seg;
-  return {seg <= one / 4 ? 1 : seg <= four ? 4 : 8, g, g == 1 ? c : seg};
+  return {seg <= one / 8 ? 1 : seg <= four ? 4 : 8, g, g == 1 ? c : seg};
 }
 
 template <typename T, int NW, int CPT>
@@ -485,7 +505,7 @@ template <typename T>
 int lp_bwd_launch(LpBwd a, hipStream_t s) {
   constexpr int64_t V = Chunk<T>::V;
   // a block a row, or where rows are few, 512 blocks in all of 2048 chunks at least
-  int64_t parts = a.n < 512 ? std::min<int64_t>((512 + a.n - 1) / a.n, (a.ld_dx / V + 2047) / 2048) : 1;
+  int64_t parts = a.n < 512 ? std::min<int64_t>((512 + a.n - 1) / a.n, a.ld_dx / V / 2048 + 1) : 1;
   a.share = ((a.ld_dx + parts - 1) / parts + V - 1) / V * V;
   parts = (a.ld_dx + a.share - 1) / a.share;
   lp_bwd<T><<<dim3((unsigned)a.n, (unsigned)parts), kBwdThreads, 0, s>>>(a);
@@ -540,8 +560,7 @@ extern "C" int mi355x_token_logprobs_bwd(void* dx, int64_t ld_dx, const void* lo
   if (rc || n == 0) return rc;
   MI_REQUIRE(dx && logits && stats && (!d_logprobs || tokens) && (!d_entropy || entropy) && (!d_top || !top || top_tokens),
              "mi355x_token_logprobs_bwd: null pointer");
-  MI_REQUIRE(ld_dx >= c && ld_dx * (int64_t)dtype_size(dtype) % 16 == 0 && (uintptr_t)dx % 16 == 0,
-             "mi355x_token_logprobs_bwd: rows of dx must be 16-byte aligned");
+  MI_REQUIRE(ld_dx >= c, "mi355x_token_logprobs_bwd: rows of dx %lld apart", (long long)ld_dx);
   LpBwd a{};
   a.dx = dx, a.x = logits, a.ld_dx = ld_dx, a.ld = ld, a.n = n, a.c = c, a.stats = stats, a.entropy = entropy;
   a.tokens = tokens, a.top_tokens = top_tokens, a.d_logprobs = d_logprobs, a.d_entropy = d_entropy;

@@ -19,6 +19,8 @@ from .aten_fast import _PACKING_ERROR, _STREAM, _alloc, _code, _contig, _error_s
 from .paged import on_device
 from ..mojo_device.torch_mojo_tensor import TorchMojoTensor as MT
 
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
 
 def plan(offsets: MT, tokens: int):
     """(plan, positions) of a batch."""
@@ -50,6 +52,18 @@ def _rows(t: MT) -> MT:
 
 def _th(t: MT):
     return t._strides[:2]
+
+
+def ready(q, k, v, sequences) -> bool:
+    """Whether a call needs no further look (the checks of
+    torch_mojo_backend.ops, which name what is wrong, take as long as a small
+    call's kernel)."""
+    if type(q) is not MT or type(k) is not MT or type(v) is not MT or not getattr(sequences, "on_mojo", False):
+        return False
+    qs, ks, dev, dtype = q._shape, k._shape, q._device, q._dtype
+    return (len(qs) == len(ks) == 3 and ks == v._shape and qs[0] == ks[0] == sequences.tokens and qs[2] == ks[2]
+            and qs[0] and ks[1] and qs[1] and qs[1] % ks[1] == 0 and 0 < qs[2] <= 256 and qs[2] % 8 == 0
+            and dtype in _FLOATS and dtype is k._dtype is v._dtype and dev == k._device == v._device == sequences._plan._device)
 
 
 def attention(q, k, v, sequences, window, scale):

@@ -16,11 +16,33 @@ from .aten_fast import (
 )
 from ..mojo_device.torch_mojo_tensor import TorchMojoTensor as MT
 
+_FLOATS, _INTS = (torch.bfloat16, torch.float16, torch.float32), (torch.int32, torch.int64)
+
 
 def _bht(t: MT):
     """(batch, head, token) strides of [batch, heads, tokens, d] or [tokens, heads, d]."""
     st = t._strides
     return st[:3] if len(st) == 4 else (0, st[1], st[0])
+
+
+def ready(q, k, positions, frequencies) -> bool:
+    """Whether a rotary call needs no further look (as packed.ready)."""
+    if type(q) is not MT or type(positions) is not MT or type(frequencies) is not MT or not (k is None or type(k) is MT):
+        return False
+    shape, dev, dtype, ps, fs = q._shape, q._device, q._dtype, positions._shape, frequencies._shape
+    if len(shape) == 4:
+        outer = (shape[0], shape[2])
+    elif len(shape) == 3:
+        outer = shape[:1]
+    else:
+        return False
+    if k is not None:
+        ks = k._shape
+        if not (len(ks) == len(shape) and ks[0] == shape[0] and ks[2] == shape[2] and ks[-1] == shape[-1]
+                and k._dtype is dtype and k._device == dev):
+            return False
+    return ((ps == outer or ps == outer[-1:]) and positions._dtype in _INTS and len(fs) == 1 and 2 * fs[0] <= shape[-1] <= 4096
+            and frequencies._dtype is torch.float64 and dtype in _FLOATS and dev == positions._device == frequencies._device)
 
 
 def _side(t):
@@ -74,12 +96,13 @@ def logprobs_forward(x: MT, tokens, top, entropy, ignore_index):
     return picked, spread, best, order, stats
 
 
-def logprobs_backward(x: MT, tokens, stats, spread, order, d_picked, d_spread, d_best, ignore_index):
-    """d_logits of x's dtype, its rows padded to 16 bytes (as the GEMMs behind it read them)."""
+def logprobs_backward(x: MT, tokens, stats, spread, order, d_picked, d_spread, d_best, ignore_index, dense_rows):
+    """d_logits of x's dtype: dense, as a leaf's gradient is kept, or its rows
+    padded to 8 elements, as the GEMMs behind a projection read them."""
     if x._strides[1] != 1 and x._shape[1] > 1 or x._strides[0] < 0:
         x = materialize_contiguous(x)
     (n, c), dev = x._shape, x._device
-    ld = (c + 7) // 8 * 8
+    ld = c if dense_rows else (c + 7) // 8 * 8
     dense = _alloc((n, ld), x._dtype, dev)
     dx = MT._view_of(dense, (n, c), (ld, 1), 0, ld == c)
 

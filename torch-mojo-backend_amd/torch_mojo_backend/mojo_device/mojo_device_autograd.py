@@ -41,7 +41,7 @@ from __future__ import annotations
 import torch
 
 from ..eager_kernels import aten_fast, packed, paged, positions
-from ..eager_kernels import materialize_touched
+from ..eager_kernels import lazy_live, materialize_touched
 from .torch_mojo_tensor import TorchMojoTensor
 
 _registered = False
@@ -119,16 +119,17 @@ class _PackedAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, sequences, window, scale):
         with torch._C._AutoDispatchBelowAutograd():
             out, lse, low = packed.attention_forward(q, k, v, sequences, window, scale, keep_low=True)
-        ctx.save_for_backward(q, k, v, out, lse, low)
-        ctx.args = (sequences, window, scale)
+        ctx.save_for_backward(q, k, v, out)
+        ctx.args = (lse, low, sequences, window, scale)  # (lse and low: nobody else's)
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        q, k, v, out, lse, low = ctx.saved_tensors
-        materialize_touched((grad, q, k, v, out), None, False)
+        q, k, v, out = ctx.saved_tensors
+        if lazy_live():
+            materialize_touched((grad, q, k, v, out), None, False)
         with torch._C._AutoDispatchBelowAutograd():
-            dq, dk, dv = paged.on_device(q._device, packed.attention_backward, grad, q, k, v, out, lse, low, *ctx.args)
+            dq, dk, dv = paged.on_device(q._device, packed.attention_backward, grad, q, k, v, out, *ctx.args)
         if torch.is_grad_enabled():  # create_graph
             dq, dk, dv = _OneGradient.apply(dq, dk, dv, q, k, v, grad)
         return dq, dk, dv, None, None, None
@@ -139,11 +140,11 @@ class _TokenLogprobs(torch.autograd.Function):
     more and the gradient's write backward."""
 
     @staticmethod
-    def forward(ctx, x, tokens, top, entropy, ignore_index):
+    def forward(ctx, x, tokens, top, entropy, ignore_index, leaf):
         with torch._C._AutoDispatchBelowAutograd():
             picked, spread, best, order, stats = positions.logprobs_forward(x, tokens, top, entropy, ignore_index)
         ctx.save_for_backward(x, tokens, stats, spread, order)
-        ctx.ignore_index = ignore_index
+        ctx.args = (ignore_index, leaf)
         ctx.set_materialize_grads(False)
         if order is not None:
             ctx.mark_non_differentiable(order)
@@ -154,14 +155,14 @@ class _TokenLogprobs(torch.autograd.Function):
         x, tokens, stats, spread, order = ctx.saved_tensors
         grads = [g for g in (d_picked, d_spread, d_best) if g is not None]
         if not grads:
-            return None, None, None, None, None
+            return (None,) * 6
         materialize_touched((x, tokens, *grads), None, False)
         with torch._C._AutoDispatchBelowAutograd():
             dx = paged.on_device(x._device, positions.logprobs_backward, x, tokens, stats, spread, order, d_picked,
-                                 d_spread, d_best, ctx.ignore_index)
+                                 d_spread, d_best, *ctx.args)
         if torch.is_grad_enabled():  # create_graph
             dx = _OnceOnly.apply("token_logprobs", dx, x, *grads)
-        return dx, None, None, None, None
+        return dx, None, None, None, None, None
 
 
 class _OnceOnly(torch.autograd.Function):

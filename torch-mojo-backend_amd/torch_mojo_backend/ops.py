@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import kv_cache, logprobs, packing, rotary
-from .eager_kernels import aten_fast, materialize_touched, packed, paged, positions as _positions
+from .eager_kernels import aten_fast, lazy_live, materialize_touched, packed, paged, positions as _positions
 from .masks import sliding_window_causal_mask
 from .mojo_device.torch_mojo_tensor import TorchMojoTensor
 
@@ -165,7 +165,8 @@ class _RotaryAt(torch.autograd.Function):
         positions, frequencies = ctx.saved_tensors
         interleaved, scale, inverse = ctx.args
         given = [g for g in (dq, dk) if g is not None]
-        materialize_touched((*given, positions, frequencies), None, False)
+        if lazy_live():
+            materialize_touched((*given, positions, frequencies), None, False)
         turn = _RotaryAt.apply if _needs_grad(*given) else _positions.rotary
         dq, dk = paged.on_device(given[0]._device, turn, dq, dk, positions, frequencies, interleaved, scale, not inverse)
         return dq, dk, None, None, None, None, None
@@ -184,6 +185,8 @@ def rotary_at(q, k, positions, frequencies, *, interleaved=False, scale=1.0):
     frequencies is f64 (`rotary.rotary_frequencies`, with the scale that goes with
     stretched contexts): angles are taken in 64 bits and good at any position
     below 2 ** 31.  One kernel on the mojo device."""
+    if type(scale) is float and -1e38 < scale < 1e38 and _positions.ready(q, k, positions, frequencies):
+        return _rotary_at(q, k, positions, frequencies, interleaved, scale)
     what = "rotary_at"
     rows = [x for x in (q, k) if x is not None]
     if not rows:
@@ -214,9 +217,14 @@ def rotary_at(q, k, positions, frequencies, *, interleaved=False, scale=1.0):
     if like.dtype not in (torch.float32, torch.bfloat16, torch.float16) or like.shape[-1] > 4096:
         raise NotImplementedError(f"{what}: {like.dtype} with head_dim {like.shape[-1]} is not supported"
                                   " (float32, bfloat16, float16, head_dim up to 4096)")
-    materialize_touched((*rows, positions, frequencies), None, False)
-    turn = _RotaryAt.apply if _needs_grad(*rows) else _positions.rotary
-    return paged.on_device(like._device, turn, q, k, positions, frequencies, bool(interleaved), scale, False)
+    return _rotary_at(q, k, positions, frequencies, interleaved, scale)
+
+
+def _rotary_at(q, k, positions, frequencies, interleaved, scale):
+    if lazy_live():
+        materialize_touched((q, k, positions, frequencies), None, False)
+    turn = _RotaryAt.apply if _needs_grad(q, k) else _positions.rotary
+    return paged.on_device(positions._device, turn, q, k, positions, frequencies, bool(interleaved), scale, False)
 
 
 def packed_attention(q, k, v, sequences, *, window=0, scale=None):
@@ -232,6 +240,8 @@ def packed_attention(q, k, v, sequences, *, window=0, scale=None):
     float16.  Nothing of a sequence reaches another one; a NaN or an infinity in a
     row may reach the other rows of its own sequence, also earlier ones, as 0 *
     NaN does in the plain formula."""
+    if type(window) is int and 0 <= window and scale is None and packed.ready(q, k, v, sequences):
+        return _packed_attention(q, k, v, sequences, min(window, sequences.tokens), None)
     what = "packed_attention"
     if not isinstance(sequences, packing.PackedSequences):
         raise TypeError(f"{what}: sequences must be a PackedSequences, got {type(sequences).__name__}")
@@ -260,11 +270,16 @@ def packed_attention(q, k, v, sequences, *, window=0, scale=None):
     if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or q.shape[2] > 256 or q.shape[2] % 8:
         raise NotImplementedError(f"{what}: {q.dtype} with head_dim {q.shape[2]} is not supported"
                                   " (float32, bfloat16, float16, head_dim a multiple of 8 up to 256)")
+    return _packed_attention(q, k, v, sequences, window, scale)
+
+
+def _packed_attention(q, k, v, sequences, window, scale):
     if not _needs_grad(q, k, v):
         return packed.attention(q, k, v, sequences, window, scale)
     from .mojo_device.mojo_device_autograd import _PackedAttention
 
-    materialize_touched((q, k, v), None, False)
+    if lazy_live():
+        materialize_touched((q, k, v), None, False)
     return paged.on_device(q._device, _PackedAttention.apply, q, k, v, sequences, window, scale)
 
 
@@ -305,7 +320,7 @@ def token_logprobs(logits, tokens=None, *, top=0, entropy=False, ignore_index=-1
     if _needs_grad(x):
         from .mojo_device.mojo_device_autograd import _TokenLogprobs
 
-        got = paged.on_device(x._device, _TokenLogprobs.apply, x, tokens, top, bool(entropy), int(ignore_index))
+        got = paged.on_device(x._device, _TokenLogprobs.apply, x, tokens, top, bool(entropy), int(ignore_index), logits.is_leaf)
     else:
         got = paged.on_device(x._device, _positions.logprobs_forward, x, tokens, top, bool(entropy), int(ignore_index))[:4]
     if len(lead) != 1:
