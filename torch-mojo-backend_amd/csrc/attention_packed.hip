@@ -52,41 +52,48 @@ struct PackedArgs {
   float* kv_part;      // dK and then dV of each query head [group][kv_heads][tokens][D] (f32), or null
 };
 
-// Loads of 64-row tiles into the layout of KvLayout by NW waves.  RAG: chunks
-// past d are left as they are, zeros that the block wrote before its first load.
+// Loads of 64-row tiles into the layout of KvLayout by NW waves.  A lane's rows
+// of a tile lie NW * RPI apart, and the chunk it takes of them is the same (of
+// rows 8 apart, at head_dim 256 in four waves, one of two), so that one or two
+// 32-bit offsets a lane serve all: addresses made lane by lane took 16 registers
+// of the backward's and an add a load.  RAG: chunks past d are left as they are,
+// zeros that the block wrote before its first load.
+constexpr int64_t kMostRowBytes = (1ll << 32) / 64 - 64;  // of 64 rows' offsets in 32 bits
 template <int D, int NW, bool RAG>
 struct TileLoad {
   typedef KvLayout<D> L;
-  static constexpr int IT = L::TILE / 1024 / NW;
+  static constexpr int IT = L::TILE / 1024 / NW, STEP = NW * L::RPI;
+  static constexpr int KINDS = (STEP & (D == 64 ? 7 : 15)) ? 2 : 1;
+  static_assert(STEP % 8 == 0, "");
   const char* g;
-  int64_t rs;
-  int64_t off[IT];
-  bool keep[RAG ? IT : 1];
-  static __device__ __forceinline__ int row_of(int it) { return (it * NW + wave_id()) * L::RPI + (int)(threadIdx.x & 63) / L::CH; }
-  static __device__ __forceinline__ int chunk_of(int row) { return ((int)(threadIdx.x & 63) % L::CH) ^ L::swz(row); }
+  uint32_t rs;
+  uint32_t off[KINDS];
+  bool keep[KINDS];
   __device__ __forceinline__ void init(const void* base, int64_t rs_bytes, int d) {
     g = (const char*)base;
-    rs = rs_bytes;
+    rs = (uint32_t)rs_bytes;
+    const int lane = threadIdx.x & 63, r = wave_id() * L::RPI + lane / L::CH;
 #pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      const int r = row_of(it), c = chunk_of(r);
-      off[it] = r * rs + c * 16;
-      if constexpr (RAG) keep[it] = c * 8 < d;
+    for (int k = 0; k < KINDS; ++k) {
+      const int c = (lane % L::CH) ^ L::swz(r + k * STEP);
+      off[k] = r * rs + c * 16;
+      keep[k] = !RAG || c * 8 < d;
     }
   }
   __device__ __forceinline__ void issue(int row0, int nrows, char* dst) const {
     const int wave = wave_id();
+    const char* tb = g + (int64_t)row0 * rs;
+    const unsigned lds = lds_base_of(dst) + wave * 1024;
     if (row0 + 64 <= nrows) {
-      const char* tb = g + row0 * rs;
 #pragma unroll
       for (int it = 0; it < IT; ++it)
-        if (!RAG || keep[it]) dma_b128(tb + off[it], lds_base_of(dst + (it * NW + wave) * 1024));
+        if (!RAG || keep[it % KINDS]) dma_b128_at(tb + (uint64_t)(it * STEP) * rs, off[it % KINDS], lds + it * (NW * 1024));
     } else {
+      const int r = wave * L::RPI + (int)(threadIdx.x & 63) / L::CH;
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
-        const int r = row_of(it);
-        const char* src = g + min(row0 + r, nrows - 1) * rs + chunk_of(r) * 16;
-        if (!RAG || keep[it]) dma_b128(src, lds_base_of(dst + (it * NW + wave) * 1024));
+        const uint32_t o = off[it % KINDS] - r * rs + min(r + it * STEP, nrows - 1 - row0) * rs;
+        if (!RAG || keep[it % KINDS]) dma_b128_at(tb, o, lds + it * (NW * 1024));
       }
     }
   }
@@ -130,7 +137,7 @@ __device__ __forceinline__ void zero_rows(const Rows& x, const PackedTile& t, in
 // halves take half of a tile's keys each and join at the end.
 // ---------------------------------------------------------------------------
 template <typename T, int D, bool RAG, int NW, int QPW, int KH>
-__global__ void __launch_bounds__(64 * NW, D == 256 || QPW == 64 ? 1 : 2) packed_fwd(PackedArgs p) {
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) packed_fwd(PackedArgs p) {
   constexpr int QT = QPW / 16, QPB = NW / KH * QPW;
   constexpr int LIST = QPB == 128 ? 0 : 1;
   static_assert(QPB == kPackedRows[LIST], "");
@@ -372,20 +379,11 @@ __global__ void __launch_bounds__(kThreads) packed_delta(PackedArgs p) {
   }
 }
 
-#ifndef PK_OCC
-#define PK_OCC 1
-#endif
-#ifndef PK_NW
-#define PK_NW 4
-#endif
 template <int D>
-constexpr int kBwdWaves = D == 128 ? PK_NW : 4;
-template <int D>
-constexpr int kKeyTiles = D == 256 ? 1 : 8 / kBwdWaves<D>;  // 16-key tiles of a wave: two would take all registers at 256
+constexpr int kKeyTiles = D == 256 ? 1 : 2;  // 16-key tiles of a wave: two would take all registers at 256
 template <int D>
 constexpr int kKeyList = D == 256 ? 1 : 0;
-template <int D>
-constexpr int kQueryTiles = 8 / kBwdWaves<D>;
+constexpr int kQueryTiles = 2;
 
 // dK and dV of a tile of keys, over the query heads [g0, g1) of its group.
 template <typename T, int D, bool RAG>
@@ -397,7 +395,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
   const int lane = threadIdx.x & 63, wave = wave_id(), lr = lane & 15, lg = lane >> 4;
   const int start = t.start, len = t.len, group = p.heads / p.kv_heads;
   // (the list's number counts from the end: the first keys' tiles take longest)
-  constexpr int KB = kBwdWaves<D> * KW;
+  constexpr int KB = 4 * KW;
   const int tile = (len - 1) / KB - t.tile;
   const int k0 = tile * KB, kw = k0 + wave * KW;
   const int window = p.window > 0 ? min(p.window, len) : len;
@@ -421,7 +419,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
   const int nqb = (qend - qstart + 63) / 64, nsteps = nqb * (g1 - g0);
   const int sw = L::swz(lr);
   const TrOffsets<D> tro;
-  TileLoad<D, kBwdWaves<D>, RAG> ql, dl;
+  TileLoad<D, 4, RAG> ql, dl;
   auto head_of = [&](int g) {
     const int h = hk * group + g;
     ql.init(p.q.at<T>(start, h), p.q.row * (int64_t)sizeof(T), p.d);
@@ -472,7 +470,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
       if (MASK && (qs * 32 + 31 < kq || qs * 32 >= kq + KW - 1 + window || qb0 + qs * 32 >= len)) continue;
-      f32x4 pt[2][RT], ds[2][RT];
+      frag pb[RT], sb[RT];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const int qt = 2 * qs + w;
@@ -500,21 +498,11 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
               x = (unsigned)(qr - lo[u]) < (unsigned)span[u] ? x : -INFINITY;
             }
             const float pv = fast_exp2(x);
-            pt[w][u][e] = pv;
-            ds[w][u][e] = pv * pa[e];
+            pb[u][4 * w + e] = (T)pv;
+            sb[u][4 * w + e] = (T)(pv * pa[e]);
           }
         }
       }
-      frag pb[RT], sb[RT];
-#pragma unroll
-      for (int u = 0; u < RT; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pb[u][e] = (T)pt[0][u][e];
-          pb[u][4 + e] = (T)pt[1][u][e];
-          sb[u][e] = (T)ds[0][u][e];
-          sb[u][4 + e] = (T)ds[1][u][e];
-        }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const frag dof = tr_frag_at<T, D>(dOt, tro, dt, 2 * qs, 2 * qs + 1);
@@ -572,7 +560,7 @@ template <typename T, int D, bool RAG>
 __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t, int h, int hk, char* lds) {
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
-  constexpr int RT = kQueryTiles<D>, QW = 16 * RT, QB = kBwdWaves<D> * QW, KS = D / 32, DT = D / 16;
+  constexpr int RT = kQueryTiles, QW = 16 * RT, QB = 4 * QW, KS = D / 32, DT = D / 16;
   static_assert(QB == 128, "");
   constexpr int STAGE = 2 * L::TILE;
   const int lane = threadIdx.x & 63, wave = wave_id(), lr = lane & 15, lg = lane >> 4;
@@ -580,7 +568,7 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
   const int window = p.window > 0 ? min(p.window, len) : len;
 
   if constexpr (RAG) clear_lds(lds, 2 * STAGE);
-  TileLoad<D, kBwdWaves<D>, RAG> kl, vl;
+  TileLoad<D, 4, RAG> kl, vl;
   kl.init(p.k.at<T>(start, hk), p.k.row * (int64_t)sizeof(T), p.d);
   vl.init(p.v.at<T>(start, hk), p.v.row * (int64_t)sizeof(T), p.d);
   const int kv_end = min(len, q0 + QB);
@@ -632,7 +620,7 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
       if (MASK && (ks2 * 32 > qk + QW - 1 || ks2 * 32 + 31 < qk - window + 1)) continue;
-      f32x4 ds[2][RT];
+      frag sb[RT];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const int kt = 2 * ks2 + w;
@@ -658,18 +646,10 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
               const int key = kt * 16 + 4 * lg + e;
               x = key < lim[u] && key >= lo[u] ? x : -INFINITY;
             }
-            ds[w][u][e] = fast_exp2(x) * pa[e];
+            sb[u][4 * w + e] = (T)(fast_exp2(x) * pa[e]);
           }
         }
       }
-      frag sb[RT];
-#pragma unroll
-      for (int u = 0; u < RT; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sb[u][e] = (T)ds[0][u][e];
-          sb[u][4 + e] = (T)ds[1][u][e];
-        }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const frag ktf = tr_frag_at<T, D>(Kt, tro, dt, 2 * ks2, 2 * ks2 + 1);
@@ -702,14 +682,18 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
   }
 }
 
-// Both in one launch: the first nkv blocks take keys, one of a K/V head's or,
-// where their gradients go through partials, one of a query head's; the rest
-// take queries.
-template <typename T, int D, bool RAG>
-__global__ void __launch_bounds__(64 * kBwdWaves<D>, D == 64 ? 2 : D == 128 ? PK_OCC : 1) packed_bwd(PackedArgs p, uint32_t nkv) {
+// KIND 0, both in one launch: the first nkv blocks take keys, one of a K/V
+// head's or, where their gradients go through partials, one of a query head's;
+// the rest take queries.  1: keys alone, 2: queries alone.  At head_dim 128 the
+// keys' blocks need 380 registers, a wave a SIMD, and the queries' 248, two; in
+// one launch both run at the first ([16384 rows, 32 over 8, 128] in 4 sequences:
+// 2370 us, 1335 + 774 in two).  Four tiles of keys a wave, two waves a block,
+// spill (4.9 ms, 39 registers of 512 short with the sums pinned in AGPRs); four of queries take 960.
+template <typename T, int D, bool RAG, int KIND>
+__global__ void __launch_bounds__(kThreads, D == 64 || (D == 128 && KIND == 2) ? 2 : 1) packed_bwd(PackedArgs p, uint32_t nkv) {
   char* const lds = packed_lds;
   const int group = p.heads / p.kv_heads;
-  if (blockIdx.x < nkv) {
+  if (KIND == 1 || (KIND == 0 && blockIdx.x < nkv)) {
     const PackedAt at = packed_at(p.tiles[kKeyList<D>], p.head->count[kKeyList<D>], blockIdx.x, p.kv_part ? p.heads : p.kv_heads, p.kv_heads);
     if (!at.live) return;
     const int g = p.kv_part ? at.h - at.hk * group : 0;
@@ -719,10 +703,12 @@ __global__ void __launch_bounds__(64 * kBwdWaves<D>, D == 64 ? 2 : D == 128 ? PK
     }
     return dkv_body<T, D, RAG>(p, at.t, at.hk, g, p.kv_part ? g + 1 : group, lds);
   }
-  const PackedAt at = packed_at(p.tiles[0], p.head->count[0], blockIdx.x - nkv, p.heads, p.kv_heads);
-  if (!at.live) return;
-  if (at.t.tile < 0) return zero_rows<T>(p.dq, at.t, at.h, p.d);
-  dq_body<T, D, RAG>(p, at.t, at.h, at.hk, lds);
+  if constexpr (KIND != 1) {
+    const PackedAt at = packed_at(p.tiles[0], p.head->count[0], blockIdx.x - nkv, p.heads, p.kv_heads);
+    if (!at.live) return;
+    if (at.t.tile < 0) return zero_rows<T>(p.dq, at.t, at.h, p.d);
+    dq_body<T, D, RAG>(p, at.t, at.h, at.hk, lds);
+  }
 }
 
 // dK and dV from the f32 partials of a group's query heads, added in head order.
@@ -766,10 +752,7 @@ constexpr int64_t kMostThreads = 1ll << 32;
 
 template <typename T, int D, bool RAG>
 int fwd_launch(const PackedArgs& a, const Launch& l) {
-#ifndef PK_FW
-#define PK_FW 4
-#endif
-  constexpr int KH = D == 256 ? 2 : 1, NW = D == 256 ? 8 : D == 128 ? PK_FW : 4, QPW = D == 256 ? 16 : 128 / NW, QPB = NW / KH * QPW;
+  constexpr int KH = D == 256 ? 2 : 1, NW = 4 * KH, QPW = D == 256 ? 16 : 32, QPB = NW / KH * QPW;
   constexpr int bytes = 4 * KvLayout<D>::TILE;
   auto k = packed_fwd<T, D, RAG, NW, QPW, KH>;
   const int rc = reserve((const void*)k, bytes, "mi355x_packed_attn_fwd");
@@ -793,15 +776,23 @@ constexpr int kBwdLds = 2 * (2 * KvLayout<D>::TILE + 512);
 
 template <typename T, int D, bool RAG>
 int bwd_launch(const PackedArgs& a, const Launch& l) {
-  auto k = packed_bwd<T, D, RAG>;
-  const int rc = reserve((const void*)k, kBwdLds<D>, "mi355x_packed_attn_bwd");
-  if (rc) return rc;
+  constexpr bool SPLIT = D == 128;
+  auto k0 = packed_bwd<T, D, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, D, RAG, SPLIT ? 2 : 0>;
+  for (auto k : {k0, k1}) {
+    const int rc = reserve((const void*)k, kBwdLds<D>, "mi355x_packed_attn_bwd");
+    if (rc) return rc;
+  }
   const int64_t nkv = l.cap(kPackedRows[kKeyList<D>]) * (a.kv_part ? a.heads : a.kv_heads), nq = l.cap(128) * a.heads;
   const int64_t rows = (int64_t)a.heads * a.tokens;
   MI_REQUIRE((nkv + nq) * kThreads < kMostThreads && rows * (D / 4) < kMostThreads - kThreads,
              "mi355x_packed_attn_bwd: too many rows and heads");
   packed_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, l.s>>>(a);
-  k<<<(unsigned)(nkv + nq), 64 * kBwdWaves<D>, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
+  if (SPLIT) {
+    k0<<<(unsigned)nkv, kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
+    k1<<<(unsigned)nq, kThreads, kBwdLds<D>, l.s>>>(a, 0);
+  } else {
+    k0<<<(unsigned)(nkv + nq), kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
+  }
   return a.kv_part ? sum_launch<T, D, RAG>(a, l) : check_launch("mi355x_packed_attn_bwd");
 }
 
@@ -856,7 +847,8 @@ AttnF32 f32_args(const PackedArgs& a) {
 
 // Rows that are read and written 16 bytes at a time.
 bool wide(const void* p, const int64_t* th, size_t es) {
-  return p && (uintptr_t)p % 16 == 0 && th[0] * (int64_t)es % 16 == 0 && th[1] * (int64_t)es % 16 == 0;
+  return p && (uintptr_t)p % 16 == 0 && th[0] * (int64_t)es % 16 == 0 && th[1] * (int64_t)es % 16 == 0 && th[0] >= 0 &&
+         th[1] >= 0 && th[0] * (int64_t)es <= kMostRowBytes;
 }
 
 }  // namespace
@@ -875,7 +867,7 @@ extern "C" int mi355x_packed_attn_fwd(void* o, const int64_t* o_th, void* o_low,
   MI_REQUIRE(lse && plan && (uintptr_t)plan % 16 == 0, "%s: lse or plan missing", what);
   const size_t es = dtype_size(dtype);
   MI_REQUIRE(wide(o, o_th, es) && wide(q, q_th, es) && wide(k, k_th, es) && wide(v, v_th, es) && (uintptr_t)o_low % 16 == 0,
-             "%s: rows must be 16-byte aligned", what);
+             "%s: rows must be 16-byte aligned, less than 64 MB apart", what);
   PackedArgs a{};
   a.q = {q, q_th[0], q_th[1]}, a.k = {k, k_th[0], k_th[1]}, a.v = {v, v_th[0], v_th[1]}, a.o = {o, o_th[0], o_th[1]};
   a.o_low = o_low, a.lse = lse, a.head = (const PackedHeader*)plan;
@@ -916,7 +908,7 @@ extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, 
   const size_t es = dtype_size(dtype);
   MI_REQUIRE(wide(o, o_th, es) && wide(q, q_th, es) && wide(k, k_th, es) && wide(v, v_th, es) && wide(dout, do_th, es) &&
                  wide(dq, dq_th, es) && wide(dk, dk_th, es) && wide(dv, dv_th, es) && (uintptr_t)o_low % 16 == 0,
-             "%s: rows must be 16-byte aligned", what);
+             "%s: rows must be 16-byte aligned, less than 64 MB apart", what);
   const int64_t need = mi355x_packed_attn_bwd_workspace_bytes(sequences, tokens, heads, kv_heads, d);
   if (!workspace || ws_bytes < need)
     return fail(MI355X_EWORKSPACE, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);

@@ -43,6 +43,10 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 __device__ __forceinline__ void dma_b128(const void* gptr, unsigned lds_base) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gptr), "s"(lds_base) : "memory", "m0");
 }
+// The same from a wave-uniform address plus each lane's 32-bit offset.
+__device__ __forceinline__ void dma_b128_at(const void* base, unsigned offset, unsigned lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_base) : "memory", "m0");
+}
 __device__ __forceinline__ void dma_b32(const void* gptr, unsigned lds_base) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" : : "v"(gptr), "s"(lds_base) : "memory", "m0");
 }
