@@ -787,7 +787,8 @@ int mi355x_rope_at(void* q_out, const int64_t* qo_bht, const void* q, const int6
  * [0, c) sets *error, which may be null, and gives 0), entropy[i] = -sum p log p,
  * and the `top` (up to 64) largest entries, NaN first and equal ones by index:
  * top_logprobs, top_tokens [n][top].  logprobs and entropy may be null.  stats
- * [n][2]: the row's maximum and the logarithm of the sum of exp(x - maximum).
+ * [n][2], for the backward (may be null): the row's maximum and the logarithm of
+ * the sum of exp(x - maximum).
  * The reference composes these from log_softmax and gather
  * (aten_fast.py:5792-5825, 9332-9368) and has no top entries. */
 int64_t mi355x_token_logprobs_workspace_bytes(int64_t n, int64_t c, int top, int dtype);

@@ -20,7 +20,7 @@
 // P and dS are rounded to the type for their products, half a step each; what
 // rounding takes from a 16-bit O is kept (o_low) and D taken from both.
 #include <algorithm>
-#include <mutex>
+#include <atomic>
 
 #include "attention_f32.h"
 #include "attention_tile.h"
@@ -736,11 +736,22 @@ __global__ void __launch_bounds__(kThreads) packed_sum(PackedArgs p) {
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-int reserve(const void* kernel, int bytes, const char* what) {
-  if (bytes <= 65536) return MI355X_OK;
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == hipSuccess ? MI355X_OK : fail(MI355X_ELAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
-}
+// Opts a kernel into more than 64 KB of LDS, once for each device that is
+// current at a launch.
+struct Reserved {
+  std::atomic<uint64_t> devices{0};
+  int operator()(const void* kernel, int bytes, const char* what) {
+    if (bytes <= 65536) return MI355X_OK;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == hipSuccess && (devices.load(std::memory_order_relaxed) & bit)) return MI355X_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(MI355X_ELAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+    devices.fetch_or(bit, std::memory_order_relaxed);
+    return MI355X_OK;
+  }
+};
 
 struct Launch {
   int64_t sequences, tokens;
@@ -755,6 +766,7 @@ int fwd_launch(const PackedArgs& a, const Launch& l) {
   constexpr int KH = D == 256 ? 2 : 1, NW = 4 * KH, QPW = D == 256 ? 16 : 32, QPB = NW / KH * QPW;
   constexpr int bytes = 4 * KvLayout<D>::TILE;
   auto k = packed_fwd<T, D, RAG, NW, QPW, KH>;
+  static Reserved reserve;
   const int rc = reserve((const void*)k, bytes, "mi355x_packed_attn_fwd");
   if (rc) return rc;
   const int64_t blocks = l.cap(QPB) * a.heads;
@@ -778,10 +790,10 @@ template <typename T, int D, bool RAG>
 int bwd_launch(const PackedArgs& a, const Launch& l) {
   constexpr bool SPLIT = D == 128;
   auto k0 = packed_bwd<T, D, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, D, RAG, SPLIT ? 2 : 0>;
-  for (auto k : {k0, k1}) {
-    const int rc = reserve((const void*)k, kBwdLds<D>, "mi355x_packed_attn_bwd");
-    if (rc) return rc;
-  }
+  static Reserved reserve0, reserve1;
+  int rc = reserve0((const void*)k0, kBwdLds<D>, "mi355x_packed_attn_bwd");
+  if (!rc) rc = reserve1((const void*)k1, kBwdLds<D>, "mi355x_packed_attn_bwd");
+  if (rc) return rc;
   const int64_t nkv = l.cap(kPackedRows[kKeyList<D>]) * (a.kv_part ? a.heads : a.kv_heads), nq = l.cap(128) * a.heads;
   const int64_t rows = (int64_t)a.heads * a.tokens;
   MI_REQUIRE((nkv + nq) * kThreads < kMostThreads && rows * (D / 4) < kMostThreads - kThreads,
@@ -882,15 +894,18 @@ extern "C" int mi355x_packed_attn_fwd(void* o, const int64_t* o_th, void* o_low,
 }
 
 // Whether a K/V head's query heads go to blocks of their own, whose partials are
-// added after them: where one block for all of a group would leave CUs idle.
-static bool splits_group(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d) {
-  return heads > kv_heads;
+// added after them: below two blocks a CU, where one for all of a group would
+// leave CUs idle (bf16 forward and backward, one block a group against one a
+// head: 16384 rows in 16 sequences, 32 over 2 heads of 64 684 and 584 us; 8192 rows
+// in 4, 32 over 8 of 128 747 and 844; 16384 in 4, 16 over 4 of 256 3533 and 3740).
+static bool splits_group(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d) {
+  return heads > kv_heads && (tokens / kPackedRows[d > 128] + 1) * kv_heads < 512;
 }
 
 extern "C" int64_t mi355x_packed_attn_bwd_workspace_bytes(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                           int64_t d) {
   const int64_t terms = 2 * heads * tokens * (int64_t)sizeof(float) + 512;
-  return splits_group(sequences, tokens, heads, kv_heads, d) ? terms + 2 * heads * tokens * width_of(d) * (int64_t)sizeof(float) : terms;
+  return heads > kv_heads ? terms + 2 * heads * tokens * width_of(d) * (int64_t)sizeof(float) : terms;
 }
 
 extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, const int64_t* dk_th, void* dv,
@@ -922,7 +937,7 @@ extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, 
   set_scale(a, scale);
   a.ndelta = (float*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);
   a.nlse2 = a.ndelta + heads * tokens;
-  if (splits_group(sequences, tokens, heads, kv_heads, d))
+  if (dtype == MI355X_F32 ? heads > kv_heads : splits_group(tokens, heads, kv_heads, d))
     a.kv_part = (float*)(((uintptr_t)(a.nlse2 + heads * tokens) + 255) & ~(uintptr_t)255);
   const Launch l{sequences, tokens, (hipStream_t)stream};
   if (dtype == MI355X_F32) {

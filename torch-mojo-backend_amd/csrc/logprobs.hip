@@ -93,7 +93,7 @@ struct LpArgs {
   const int64_t* tokens;
   int64_t ignore;
   int32_t* error;
-  float *logprobs, *entropy, *stats, *top_logprobs;  // stats: [n][2], m and ln s
+  float *logprobs, *entropy, *stats, *top_logprobs;  // stats: [n][2], m and ln s, or null
   int64_t* top_tokens;
   int top;
   int segments;       // of a row; more than one: partials
@@ -106,7 +106,7 @@ struct LpArgs {
 template <typename T>
 __device__ __forceinline__ void finish_row(const LpArgs& p, int64_t row, float m, float s, float t) {
   const float ls = log2f(s) * kLn2;
-  p.stats[2 * row] = m, p.stats[2 * row + 1] = ls;
+  if (p.stats) p.stats[2 * row] = m, p.stats[2 * row + 1] = ls;
   if (p.entropy) p.entropy[row] = ls - t / s;
   if (p.logprobs) {
     const int64_t k = p.tokens[row];
@@ -145,7 +145,7 @@ struct LpShape {
   static constexpr int kList = NW == 1 ? 256 : 1024;
 };
 
-template <typename T, int NW, int CPT>
+template <typename T, int NW, int CPT, bool ENT>
 __global__ void __launch_bounds__((LpShape<T, NW, CPT>::kThreads)) lp_rows(LpArgs p) {
   typedef LpShape<T, NW, CPT> S;
   constexpr int V = Chunk<T>::V, LIST = S::kList;
@@ -202,8 +202,14 @@ __global__ void __launch_bounds__((LpShape<T, NW, CPT>::kThreads)) lp_rows(LpArg
     if (i >= nit) continue;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float d = not_below((ch[i].get(e) - m) * kLog2e), q = hw_exp2(d);
-      s += q, t = fmaf(q, d, t);
+      // (NaNs that the floor hides are in m)
+      const float d = (ch[i].get(e) - m) * kLog2e;
+      if constexpr (ENT) {
+        const float f = fmaxf(d, kFloor), q = hw_exp2(f);
+        s += q, t = fmaf(q, f, t);
+      } else {
+        s += hw_exp2(d);
+      }
     }
     ch[i].forget();
   }
@@ -298,6 +304,69 @@ __global__ void __launch_bounds__((LpShape<T, NW, CPT>::kThreads)) lp_rows(LpArg
     if (tid == 0) put(i, key);
     last = key;
   }
+}
+
+// Without top entries nothing is looked at twice: a block walks its segment with
+// a running maximum m, s = sum 2^f and t = sum 2^f f, f = (x - m) log2(e), which
+// move to a new maximum as t = (t + s d) 2^d, s = s 2^d.
+constexpr int kStreamThreads = 256;
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kStreamThreads) lp_stream(LpArgs p) {
+  constexpr int V = Chunk<T>::V, U = 4, W = kStreamThreads / 64;
+  __shared__ float red[W][3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t item = blockIdx.x, row = item / p.segments, e0 = (item - row * p.segments) * p.seg;
+  const int len = (int)min(p.seg, p.c - e0), nc = (len + V - 1) / V;
+  const T* const x = (const T*)p.x + row * p.ld + e0;
+  float m = -INFINITY, s = 0.f, t = 0.f;
+  bool nan = false;
+  for (int c0 = tid; c0 < nc; c0 += kStreamThreads * U) {
+    Chunk<T> ch[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = (c0 + u * kStreamThreads) * V;
+      if (i + V <= len) ch[u].load(x, i);
+      else ch[u].load_end(x, i, len);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = ch[u].get(e);
+      const float top = max_nan(v);
+      nan |= top != top;
+      if (top > m) {
+        const float d = fmaxf((m - top) * kLog2e, kFloor), f = hw_exp2(d);
+        if constexpr (ENT) t = fmaf(s, d, t) * f;
+        s *= f, m = top;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float f = fmaxf((v[e] - m) * kLog2e, kFloor), q = hw_exp2(f);
+        s += q;
+        if constexpr (ENT) t = fmaf(q, f, t);
+      }
+    }
+  }
+  if (nan) m = __uint_as_float(0x7fc00000u);
+  // to the block's maximum; what a NaN or an infinity makes of the sums is in m
+  float all = wave_max_nan(m);
+  if (lane == 0) red[wave][0] = all;
+  __syncthreads();
+  all = red[0][0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) all = nan_max(all, red[w][0]);
+  const float d = fmaxf((m - all) * kLog2e, kFloor), f = hw_exp2(d);
+  t = wave_sum(fmaf(s, d, t) * f), s = wave_sum(s * f);
+  if (lane == 0) red[wave][1] = s, red[wave][2] = t;
+  __syncthreads();
+  if (tid) return;
+  s = t = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) s += red[w][1], t += red[w][2];
+  t *= kLn2;
+  if (p.segments == 1) finish_row<T>(p, row, all, s, t);
+  else p.part[3 * item] = all, p.part[3 * item + 1] = s, p.part[3 * item + 2] = t;
 }
 
 // A row's segments: one block, kJoinList keys at most.  The bound here: with r =
@@ -452,41 +521,45 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
 // launches
 // ---------------------------------------------------------------------------
 // How rows are cut.  A row that one wave's, or one block's, registers hold is
-// not, where there are enough rows to fill the 256 CUs; else into segments of a
-// few KB for 512 blocks in all, of which the join takes kJoinList keys.
+// not, where there are enough rows to fill the 256 CUs; else into segments of 8 KB
+// and more for 512 blocks in all, of which the join takes kJoinList keys (one
+// bf16 row of 262144, 20 top entries: 9.8 us and 5.8 to join 64 segments, 11.4 and
+// 4.8 of 32, 8.5 and 8.3 of 128).  Rows of 8192 x 50257 bf16 stream in 214 us, 0.82
+// GB: a lane's ten instructions an element, an exponential among them, take 150 of
+// them, reading alone would; held in registers 239, in blocks of 16 waves 346.
 struct LpPlan {
-  int waves;      // of a segment: 1, 4 or 8
+  int waves;      // of a segment: 1, 4 or 8; 0: lp_stream's block
   int64_t segments, seg;
 };
-#ifndef LP_SEG
-#define LP_SEG 4
-#endif
 template <typename T>
 LpPlan plan_of(int64_t n, int64_t c, int top) {
   constexpr int V = Chunk<T>::V;
   constexpr int64_t one = LpShape<T, 1, 16>::kMost, four = LpShape<T, 4, 8>::kMost, eight = LpShape<T, 8, 16>::kMost;
   if (c <= one && (n >= 512 || c <= one / 4)) return {1, 1, c};
+  if (!top && n >= 512) return {0, 1, c};
   if (c <= eight && n >= 256) return {8, 1, c};
   int64_t g = (c + eight - 1) / eight;
-  if (n < 512) g = std::max<int64_t>(g, std::min<int64_t>((512 + n - 1) / n, c / (four / LP_SEG)));
+  if (n < 512) g = std::max<int64_t>(g, std::min<int64_t>((512 + n - 1) / n, c / (four / 4)));
   g = std::max<int64_t>(1, std::min<int64_t>(g, std::min(kMostSegments, top ? kJoinList / top : kMostSegments)));
   const int64_t seg = ((c + g - 1) / g + V - 1) / V * V;
   g = (c + seg - 1) / seg;
-  return {seg <= one / 8 ? 1 : seg <= four ? 4 : 8, g, g == 1 ? c : seg};
+  return {!top ? 0 : seg <= one / 8 ? 1 : seg <= four ? 4 : 8, g, g == 1 ? c : seg};
 }
 
 template <typename T, int NW, int CPT>
 void lp_launch(const LpArgs& a, hipStream_t s) {
   typedef LpShape<T, NW, CPT> S;
-  lp_rows<T, NW, CPT><<<ceil_div(a.n * a.segments, S::kUnits), S::kThreads, 0, s>>>(a);
+  const unsigned blocks = ceil_div(a.n * a.segments, S::kUnits);
+  if (a.entropy) lp_rows<T, NW, CPT, true><<<blocks, S::kThreads, 0, s>>>(a);
+  else lp_rows<T, NW, CPT, false><<<blocks, S::kThreads, 0, s>>>(a);
 }
 
 template <typename T>
 int lp_fwd(LpArgs a, void* workspace, int64_t ws_bytes, hipStream_t s) {
   const LpPlan g = plan_of<T>(a.n, a.c, a.top);
   a.segments = (int)g.segments, a.seg = g.seg;
-  MI_REQUIRE((g.seg <= LpShape<T, 8, 16>::kMost), "mi355x_token_logprobs_fwd: %lld columns", (long long)a.c);
-  MI_REQUIRE(a.n * g.segments < (1ll << 32) / 512, "mi355x_token_logprobs_fwd: %lld rows", (long long)a.n);
+  MI_REQUIRE((g.waves == 0 || g.seg <= LpShape<T, 8, 16>::kMost), "mi355x_token_logprobs_fwd: %lld columns", (long long)a.c);
+  MI_REQUIRE(a.n * g.segments < (1ll << 32) / 1024, "mi355x_token_logprobs_fwd: %lld rows", (long long)a.n);
   if (g.segments > 1) {
     const int64_t items = a.n * g.segments, need = items * (8 * (int64_t)a.top + 12) + 16;
     if (!workspace || ws_bytes < need)
@@ -494,7 +567,11 @@ int lp_fwd(LpArgs a, void* workspace, int64_t ws_bytes, hipStream_t s) {
     a.part_keys = (u64*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);
     a.part = (float*)(a.part_keys + items * a.top);
   }
-  if (g.waves == 1) lp_launch<T, 1, 16>(a, s);
+  if (g.waves == 0) {
+    const unsigned blocks = (unsigned)(a.n * g.segments);
+    if (a.entropy) lp_stream<T, true><<<blocks, kStreamThreads, 0, s>>>(a);
+    else lp_stream<T, false><<<blocks, kStreamThreads, 0, s>>>(a);
+  } else if (g.waves == 1) lp_launch<T, 1, 16>(a, s);
   else if (g.waves == 4) lp_launch<T, 4, 8>(a, s);
   else lp_launch<T, 8, 16>(a, s);
   if (g.segments > 1) lp_join<T><<<(unsigned)a.n, kJoinThreads, 0, s>>>(a);
@@ -539,7 +616,7 @@ extern "C" int mi355x_token_logprobs_fwd(float* logprobs, float* entropy, float*
                                          int32_t* error, void* workspace, int64_t ws_bytes, mi355x_stream_t stream) {
   const int rc = lp_check("mi355x_token_logprobs_fwd", n, c, ld, top, dtype);
   if (rc || n == 0) return rc;
-  MI_REQUIRE(logits && stats && (!logprobs || tokens) && (!top || (top_logprobs && top_tokens)),
+  MI_REQUIRE(logits && (!logprobs || tokens) && (!top || (top_logprobs && top_tokens)),
              "mi355x_token_logprobs_fwd: null pointer");
   LpArgs a{};
   a.x = logits, a.ld = ld, a.n = n, a.c = c, a.tokens = tokens, a.ignore = ignore_index, a.error = error;

@@ -73,8 +73,18 @@ def rotary(q, k, positions: MT, frequencies: MT, interleaved, scale, inverse):
     return qo, ko
 
 
-def logprobs_forward(x: MT, tokens, top, entropy, ignore_index):
-    """(logprobs, entropy, top_logprobs, top_tokens, stats) of x [n, vocab]."""
+def logprobs_ready(x, tokens, top) -> bool:
+    """Whether token_logprobs of rows needs no further look (as packed.ready)."""
+    if type(x) is not MT or type(top) is not int or not (tokens is None or type(tokens) is MT):
+        return False
+    shape = x._shape
+    return (len(shape) == 2 and 0 <= top <= 64 and 0 < shape[1] >= top and x._dtype in _FLOATS
+            and (tokens is None or (tokens._dtype is torch.int64 and tokens._shape == shape[:1] and tokens._device == x._device)))
+
+
+def logprobs_forward(x: MT, tokens, top, entropy, ignore_index, keep=False):
+    """(logprobs, entropy, top_logprobs, top_tokens, stats) of x [n, vocab]; the
+    rows' statistics where they are to be kept for the backward."""
     if x._strides[1] != 1 and x._shape[1] > 1 or x._strides[0] < 0:
         x = materialize_contiguous(x)
     (n, c), dev = x._shape, x._device
@@ -83,13 +93,13 @@ def logprobs_forward(x: MT, tokens, top, entropy, ignore_index):
     picked = _alloc((n,), f32, dev) if tokens is not None else None
     spread = _alloc((n,), f32, dev) if entropy else None
     best, order = (_alloc((n, top), f32, dev), _alloc((n, top), torch.int64, dev)) if top else (None, None)
-    stats = _alloc((n, 2), f32, dev)
+    stats = _alloc((n, 2), f32, dev) if keep else None
     ws = library.mi355x_token_logprobs_workspace_bytes(n, c, top, code)
     hold, wptr = _workspace(ws, dev)
     at = lambda t: t._ptr if t is not None else None  # noqa: E731
     check(
         "mi355x_token_logprobs_fwd",
-        library.mi355x_token_logprobs_fwd(at(picked), at(spread), stats._ptr, at(best), at(order), x._ptr, code,
+        library.mi355x_token_logprobs_fwd(at(picked), at(spread), at(stats), at(best), at(order), x._ptr, code,
                                           x._strides[0], at(_contig(tokens)) if tokens is not None else None, n, c, top,
                                           ignore_index, _error_slot(dev, _TARGET_ERROR), wptr, ws, _STREAM),
     )

@@ -142,9 +142,10 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, top, entropy, ignore_index, leaf):
         with torch._C._AutoDispatchBelowAutograd():
-            picked, spread, best, order, stats = positions.logprobs_forward(x, tokens, top, entropy, ignore_index)
-        ctx.save_for_backward(x, tokens, stats, spread, order)
+            picked, spread, best, order, stats = positions.logprobs_forward(x, tokens, top, entropy, ignore_index, True)
+        ctx.save_for_backward(x, tokens, spread, order)
         ctx.args = (ignore_index, leaf)
+        ctx.stats = stats  # (nobody else's)
         ctx.set_materialize_grads(False)
         if order is not None:
             ctx.mark_non_differentiable(order)
@@ -152,13 +153,14 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_picked, d_spread, d_best, _):
-        x, tokens, stats, spread, order = ctx.saved_tensors
+        x, tokens, spread, order = ctx.saved_tensors
         grads = [g for g in (d_picked, d_spread, d_best) if g is not None]
         if not grads:
             return (None,) * 6
-        materialize_touched((x, tokens, *grads), None, False)
+        if lazy_live():
+            materialize_touched((x, tokens, *grads), None, False)
         with torch._C._AutoDispatchBelowAutograd():
-            dx = paged.on_device(x._device, positions.logprobs_backward, x, tokens, stats, spread, order, d_picked,
+            dx = paged.on_device(x._device, positions.logprobs_backward, x, tokens, ctx.stats, spread, order, d_picked,
                                  d_spread, d_best, *ctx.args)
         if torch.is_grad_enabled():  # create_graph
             dx = _OnceOnly.apply("token_logprobs", dx, x, *grads)

@@ -294,6 +294,8 @@ def token_logprobs(logits, tokens=None, *, top=0, entropy=False, ignore_index=-1
     On the mojo device the logits are read once, and once more for the gradient;
     `top` goes up to 64.  A token outside the vocabulary raises IndexError, on
     the mojo device at the next device-to-host read."""
+    if type(ignore_index) is int and _positions.logprobs_ready(logits, tokens, top):
+        return logprobs.TokenLogprobs(*_token_logprobs(logits, tokens, top, entropy, ignore_index, logits))
     what = "token_logprobs"
     top = int(top)
     if logits.dim() < 1 or not logits.shape[-1]:
@@ -316,16 +318,20 @@ def token_logprobs(logits, tokens=None, *, top=0, entropy=False, ignore_index=-1
     x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if tokens is not None and tokens.dim() != 1:
         tokens = tokens.reshape(-1)
-    materialize_touched((x, tokens), None, False)
-    if _needs_grad(x):
-        from .mojo_device.mojo_device_autograd import _TokenLogprobs
-
-        got = paged.on_device(x._device, _TokenLogprobs.apply, x, tokens, top, bool(entropy), int(ignore_index), logits.is_leaf)
-    else:
-        got = paged.on_device(x._device, _positions.logprobs_forward, x, tokens, top, bool(entropy), int(ignore_index))[:4]
+    got = _token_logprobs(x, tokens, top, entropy, int(ignore_index), logits)
     if len(lead) != 1:
         got = [y if y is None else y.view((*lead, *y.shape[1:])) for y in got]
     return logprobs.TokenLogprobs(*got)
+
+
+def _token_logprobs(x, tokens, top, entropy, ignore_index, logits):
+    if lazy_live():
+        materialize_touched((x, tokens), None, False)
+    if not _needs_grad(x):
+        return paged.on_device(x._device, _positions.logprobs_forward, x, tokens, top, bool(entropy), ignore_index)[:4]
+    from .mojo_device.mojo_device_autograd import _TokenLogprobs
+
+    return paged.on_device(x._device, _TokenLogprobs.apply, x, tokens, top, bool(entropy), ignore_index, logits.is_leaf)
 
 
 # ---------------------------------------------------------------------------
