@@ -15,10 +15,13 @@ import torch
 
 from . import check, lazy_live, materialize_touched
 from . import native_lib as lib
-from .aten_fast import _PACKING_ERROR, _STREAM, _alloc, _code, _contig, _error_slot, _workspace, materialize_contiguous
+from .aten_fast import (
+    _PACKING_ERROR, _STREAM, _alloc, _code, _contig, _error_slot, _mark_cat_ready, _workspace, materialize_contiguous,
+)
 from .paged import on_device
 from ..mojo_device.torch_mojo_tensor import TorchMojoTensor as MT
 
+_MOST_ROW_BYTES = 2 ** 26 - 64
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -43,9 +46,10 @@ def _plan(offsets, tokens, dev):
 
 
 def _rows(t: MT) -> MT:
-    """t itself when its rows can be read 16 bytes at a time, else a copy."""
+    """t itself when its rows can be read 16 bytes at a time and lie less than
+    64 MB apart (the kernels' offsets in a tile of 64 have 32 bits), else a copy."""
     st, n = t._strides, t._itemsize
-    if st[2] == 1 and not (t._ptr | st[0] * n | st[1] * n) & 15:
+    if st[2] == 1 and not (t._ptr | st[0] * n | st[1] * n) & 15 and st[0] * n <= _MOST_ROW_BYTES:
         return t
     return materialize_contiguous(t)
 
@@ -91,13 +95,21 @@ def attention_forward(q: MT, k: MT, v: MT, sequences, window, scale, keep_low=Fa
 
 
 def attention_backward(grad: MT, q: MT, k: MT, v: MT, out: MT, lse: MT, low, sequences, window, scale):
-    """(dq, dk, dv), dense."""
+    """(dq, dk, dv): dense, or the parts of one dense tensor."""
     if grad._dtype != q._dtype:
         grad = materialize_contiguous(grad, q._dtype)
+    together = q._holder is k._holder is v._holder
     grad, q, k, v = _rows(grad), _rows(q), _rows(k), _rows(v)
     t, h, d = q._shape
     hk, code, library = k._shape[1], _code(q._dtype), lib()
-    dq, dk, dv = (_alloc(x._shape, q._dtype, q._device) for x in (q, k, v))
+    if together and hk == h:
+        # slices of one projection: side by side, so that the backward of its
+        # split is a view (aten_fast._mark_cat_ready)
+        rows = _alloc((t, 3, h, d), q._dtype, q._device)
+        dq, dk, dv = (MT._view_of(rows, (t, h, d), (3 * h * d, d, 1), i * h * d) for i in range(3))
+        _mark_cat_ready(rows)
+    else:
+        dq, dk, dv = (_alloc(x._shape, q._dtype, q._device) for x in (q, k, v))
     ws = library.mi355x_packed_attn_bwd_workspace_bytes(sequences.count, t, h, hk, d)
     hold, wptr = _workspace(ws, q._device)
     check(

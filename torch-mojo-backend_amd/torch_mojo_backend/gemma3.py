@@ -1,5 +1,6 @@
-"""A Gemma-3-1B-shaped decoder (forward only): prefill of whole sequences, and
-new tokens against a paged key/value cache.
+"""A Gemma-3-1B-shaped decoder: prefill of whole sequences, of sequences of
+different lengths packed end to end, and new tokens against a paged key/value
+cache.
 
 The shapes are those of Gemma 3 1B: 26 layers, d_model 1152, 4 query heads
 sharing 1 K/V head (grouped-query attention), head_dim 256, GeGLU MLP with
@@ -18,7 +19,11 @@ grouped-query windowed flash forward, RoPE and GeGLU -> their fused kernels
 device).  `Gemma3.forward_cached` takes the tokens of each call, one or many a
 sequence, into a paged cache (ops.paged_append, which also turns q and k) and
 attends over its pages (ops.paged_attention).  With `sinks` the local layers
-keep a sequence's first tokens visible beside the window.
+keep a sequence's first tokens visible beside the window.  `Gemma3.forward_packed`
+and `score_packed` take a batch of sequences without padding between them
+(packing.PackedSequences): q and k are turned by the rows' own positions
+(ops.rotary_at), attention keeps to their sequences (ops.packed_attention), and
+scores are ops.token_logprobs; all three are differentiable.
 """
 
 from __future__ import annotations
@@ -33,6 +38,7 @@ import torch.nn.functional as F
 from . import ops
 from .kv_cache import PagedKVCache
 from .masks import sliding_window_causal_mask
+from .rotary import rotary_frequencies
 
 
 @dataclass
@@ -49,6 +55,7 @@ class Gemma3Config:
     global_every: int = 6  # layers 5, 11, 17, 23 are global: five local to one global
     rope_local_base: float = 10000.0
     rope_global_base: float = 1000000.0
+    rope_global_factor: float = 1.0  # global layers' positions are divided by it, for contexts as many times as long
     eps: float = 1e-6
 
 
@@ -65,9 +72,9 @@ class RMSNorm(nn.Module):
         return ops.rms_norm(x, self.weight, self.eps, weight_offset=1.0)
 
 
-def rope_tables(seq_len, dim, base, device, dtype):
+def rope_tables(seq_len, dim, base, device, dtype, factor=1.0):
     """cos, sin [seq_len, dim] of the half-split rotary embedding."""
-    inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float64) / dim))
+    inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float64) / dim)) / factor
     ang = torch.arange(seq_len, dtype=torch.float64)[:, None] * inv[None, :]
     ang = torch.cat([ang, ang], dim=-1)
     return ang.cos().to(dtype).to(device), ang.sin().to(dtype).to(device)
@@ -129,6 +136,16 @@ class Attention(nn.Module):
         return self.o_proj(y.transpose(1, 2).reshape(b, t, c.heads * c.head_dim))
 
 
+    def forward_packed(self, x, frequencies, sequences):
+        c, t = self.cfg, x.shape[0]
+        q, k, v = (y[0].transpose(0, 1) for y in self._qkv(x[None]))  # [tokens, heads, head_dim]
+        if not q.dtype == k.dtype == v.dtype:  # under autocast the norms' results are wider
+            q, k = q.to(v.dtype), k.to(v.dtype)
+        q, k = ops.rotary_at(q, k, sequences.positions, frequencies)
+        y = ops.packed_attention(q, k, v, sequences, window=c.window if self.local else 0, scale=1.0 / math.sqrt(c.head_dim))
+        return self.o_proj(y.reshape(t, c.heads * c.head_dim))
+
+
 class MLP(nn.Module):
     def __init__(self, cfg: Gemma3Config):
         super().__init__()
@@ -162,6 +179,12 @@ class Block(nn.Module):
         return x + self.post_ffw_norm(self.mlp(self.pre_ffw_norm(x)))
 
 
+    def forward_packed(self, x, frequencies_local, frequencies_global, sequences):
+        frequencies = frequencies_local if self.local else frequencies_global
+        x = x + self.post_attn_norm(self.attn.forward_packed(self.input_norm(x), frequencies, sequences))
+        return x + self.post_ffw_norm(self.mlp(self.pre_ffw_norm(x)))
+
+
 class Gemma3(nn.Module):
     def __init__(self, cfg: Gemma3Config):
         super().__init__()
@@ -179,6 +202,7 @@ class Gemma3(nn.Module):
         # more than a third of a prefill's host time when rebuilt per call
         self._tables = {}
         self._cached_tables = {}  # the same for forward_cached: of the most positions seen
+        self._frequencies = {}  # and forward_packed's, of the last device seen
 
     def _rope_and_mask(self, t, dev, dt):
         key = (t, str(dev), dt)
@@ -186,7 +210,7 @@ class Gemma3(nn.Module):
         if hit is None:
             c = self.cfg
             hit = (rope_tables(t, c.head_dim, c.rope_local_base, dev, dt),
-                   rope_tables(t, c.head_dim, c.rope_global_base, dev, dt),
+                   rope_tables(t, c.head_dim, c.rope_global_base, dev, dt, c.rope_global_factor),
                    sliding_window_causal_mask(t, c.window, dev, c.sinks))
             self._tables = {key: hit}
         return hit
@@ -202,6 +226,30 @@ class Gemma3(nn.Module):
             x = blk(x, rope_local, rope_global, mask)
         x = self.norm(x)
         return F.linear(x, self.embed.weight)
+
+    def forward_packed(self, idx, sequences):
+        """Logits [tokens, vocab] of a batch of packed sequences: token ids idx
+        [tokens], whose rows belong to `sequences` (packing.PackedSequences)."""
+        c = self.cfg
+        if c.sinks:
+            raise NotImplementedError("Gemma3.forward_packed: local layers of packed sequences keep no sinks")
+        dev, dt = idx.device, self.embed.weight.dtype
+        frequencies = self._frequencies.get(str(dev))
+        if frequencies is None:
+            frequencies = tuple(rotary_frequencies(c.head_dim, base, scaling="linear", factor=factor, device=dev).frequencies
+                                for base, factor in ((c.rope_local_base, 1.0), (c.rope_global_base, c.rope_global_factor)))
+            self._frequencies = {str(dev): frequencies}
+        x = self.embed(idx) * torch.tensor(c.hidden ** 0.5, dtype=dt, device=dev)
+        for blk in self.blocks:
+            x = blk.forward_packed(x, *frequencies, sequences)
+        return F.linear(self.norm(x), self.embed.weight)
+
+    def score_packed(self, idx, sequences, *, top=0, entropy=False):
+        """logprobs.TokenLogprobs of a batch of packed sequences: of each row the
+        log-probability of the token behind it in its sequence (0 of the last one,
+        and of rows without a sequence), and where asked for the entropy and the
+        `top` likeliest tokens."""
+        return ops.token_logprobs(self.forward_packed(idx, sequences), sequences.next_tokens(idx), top=top, entropy=entropy)
 
     def caches(self, num_pages, page_size, *, bits=None):
         """Empty pages for each layer: of the weights' type, or of 4 bits."""
@@ -224,7 +272,8 @@ class Gemma3(nn.Module):
         need, key = page_table.shape[1] * caches[0].page_size, (str(dev), angles)
         rope = self._cached_tables.get(key)
         if rope is None or rope[0][0].shape[0] < need:
-            rope = tuple(rope_tables(need, c.head_dim, base, dev, angles) for base in (c.rope_local_base, c.rope_global_base))
+            rope = tuple(rope_tables(need, c.head_dim, base, dev, angles, factor) for base, factor in
+                         ((c.rope_local_base, 1.0), (c.rope_global_base, c.rope_global_factor)))
             self._cached_tables = {key: rope}
         x = self.embed(idx) * torch.tensor(c.hidden ** 0.5, dtype=dt, device=dev)
         for blk, cache in zip(self.blocks, caches, strict=True):

@@ -9,7 +9,9 @@ and training semantics: pre-LayerNorm blocks, fused qkv projection, causal
 lm_head tied to the token embedding, N(0, 0.02) init with the residual
 projections scaled by 1/sqrt(2*n_layer), cross-entropy over the vocabulary,
 and AdamW with decay on >=2-D parameters only.  It is plain PyTorch: it runs
-unchanged on "cpu" (the fp32 oracle run) and on "mojo".
+unchanged on "cpu" (the fp32 oracle run) and on "mojo".  With a
+packing.PackedSequences it takes documents of different lengths laid end to end
+(ops.packed_attention) instead of equal blocks.
 """
 
 from __future__ import annotations
@@ -20,6 +22,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from . import ops
 
 
 @dataclass
@@ -41,7 +45,11 @@ class CausalSelfAttention(nn.Module):
         self.n_head = cfg.n_head
         self.n_embd = cfg.n_embd
 
-    def forward(self, x):
+    def forward(self, x, sequences=None):
+        if sequences is not None:  # x [tokens, C]
+            T, C = x.shape
+            q, k, v = (y.view(T, self.n_head, C // self.n_head) for y in self.c_attn(x).split(self.n_embd, dim=1))
+            return self.c_proj(ops.packed_attention(q, k, v, sequences).reshape(T, C))
         B, T, C = x.shape
         q, k, v = self.c_attn(x).split(self.n_embd, dim=2)
         hd = C // self.n_head
@@ -72,8 +80,8 @@ class Block(nn.Module):
         self.ln_2 = nn.LayerNorm(cfg.n_embd, bias=cfg.bias)
         self.mlp = MLP(cfg)
 
-    def forward(self, x):
-        x = x + self.attn(self.ln_1(x))
+    def forward(self, x, sequences=None):
+        x = x + self.attn(self.ln_1(x), sequences)
         x = x + self.mlp(self.ln_2(x))
         return x
 
@@ -109,12 +117,16 @@ class GPT(nn.Module):
     def num_params(self) -> int:
         return sum(p.numel() for p in self.parameters())
 
-    def forward(self, idx, targets=None):
-        b, t = idx.shape
-        pos = torch.arange(0, t, dtype=torch.long, device=idx.device)
+    def forward(self, idx, targets=None, sequences=None):
+        """Logits and loss of idx [B, T], or of packed documents' idx [tokens]
+        with their sequences (targets [tokens]: sequences.next_tokens(idx, -1))."""
+        if sequences is None:
+            pos = torch.arange(0, idx.shape[1], dtype=torch.long, device=idx.device)
+        else:
+            pos = sequences.positions.long()
         x = self.transformer.wte(idx) + self.transformer.wpe(pos)
         for block in self.transformer.h:
-            x = block(x)
+            x = block(x, sequences)
         x = self.transformer.ln_f(x)
         logits = self.lm_head(x)
         loss = None
@@ -153,14 +165,16 @@ def make_batches(batch_size, block_size, vocab_size, count, seed, device):
 
 
 def training_step(model, optimizer, inputs, targets, autocast_dtype=None, device_type="mojo",
-                  grad_clip=GRAD_CLIP):
+                  grad_clip=GRAD_CLIP, sequences=None):
     """nanoGPT's train.py loop body: forward (optionally under autocast),
-    backward, clip_grad_norm_, optimizer step, zero_grad(set_to_none)."""
+    backward, clip_grad_norm_, optimizer step, zero_grad(set_to_none).  With
+    `sequences` inputs and targets are those of packed documents."""
+    packed = () if sequences is None else (sequences,)
     if autocast_dtype is not None:
         with torch.autocast(device_type=device_type, dtype=autocast_dtype):
-            _, loss = model(inputs, targets)
+            _, loss = model(inputs, targets, *packed)
     else:
-        _, loss = model(inputs, targets)
+        _, loss = model(inputs, targets, *packed)
     loss.backward()
     if grad_clip:
         torch.nn.utils.clip_grad_norm_(model.parameters(), grad_clip)

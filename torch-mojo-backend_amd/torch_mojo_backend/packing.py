@@ -71,6 +71,18 @@ class PackedSequences:
         return cls(torch.tensor(at, dtype=torch.int32).to(device), tokens)
 
 
+    def next_tokens(self, tokens, ignore_index=-100):
+        """For each row of tokens [tokens] the token behind it in its sequence,
+        ignore_index where there is none: what a model's row predicts."""
+        if tokens.dim() != 1 or tokens.shape[0] != self.tokens:
+            raise ValueError(f"PackedSequences: tokens must be [{self.tokens}], got {tuple(tokens.shape)}")
+        if not self.tokens:
+            return tokens.clone()
+        # (a row whose position is 0 begins a sequence, or belongs to none)
+        behind = torch.where(self.positions[1:] > 0, tokens[1:], torch.full_like(tokens[1:], ignore_index))
+        return torch.cat([behind, torch.full_like(tokens[:1], ignore_index)])
+
+
 def attention_plain(q, k, v, sequences, window, scale):
     """The plain formula of `ops.packed_attention`, in 32 bits at least."""
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
