@@ -68,6 +68,27 @@ def test_gradients(dtype, n, c, top, entropy, picked):
     train(*cases.logits(n, c, dtype), top, entropy, picked)
 
 
+@pytest.mark.parametrize("dtype,top", [(BF, 0), (BF, 3), (F32, 0)])
+def test_a_gradient_larger_than_the_cache(dtype, top):
+    """A row's gradient is the same in a batch whose gradient has over 256 MB."""
+    n, times, c = 600, 5, 50257
+    x, tokens = cases.logits(n, c, dtype)
+
+    def grad(x, tokens):
+        leaf = x.to("mojo").requires_grad_()
+        got = ops.token_logprobs(leaf, tokens.to("mojo"), top=top, entropy=True)
+        weight = torch.linspace(-1, 1, n).repeat(len(tokens) // n).to("mojo")
+        loss = (got.logprobs * weight).sum() + (got.entropy * weight).sum()
+        if top:
+            loss = loss + (got.top_logprobs * weight[:, None]).sum()
+        loss.backward()
+        return leaf.grad.cpu()
+
+    want, got = grad(x, tokens), grad(x.repeat(times, 1), tokens.repeat(times))
+    for part in got.chunk(times):
+        assert torch.equal(part, want)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("n,c", [(2, 50), (600, 3000), (3, 50257), (300, 50257)])
 def test_ties(dtype, n, c):
