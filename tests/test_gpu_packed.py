@@ -70,13 +70,15 @@ def test_forward_and_backward(dtype, d, h, hk, lengths):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("d,h,hk", [(8, 1, 1), (40, 3, 1), (72, 2, 2), (96, 4, 2), (136, 2, 1), (248, 2, 2)])
+@pytest.mark.parametrize("d,h,hk", [(8, 1, 1), (40, 3, 1), (72, 2, 2), (88, 2, 1), (96, 4, 2), (112, 2, 2), (136, 2, 1), (160, 3, 3),
+                                    (192, 4, 2), (200, 2, 1), (248, 2, 2)])
 def test_other_head_dims(dtype, d, h, hk):
     at, x = cases.inputs([70, 0, 1, 190, 64], h, hk, d, dtype, before=2, behind=70)
     compare(run(at, x), cases.expected(at, *x))
 
 
-@pytest.mark.parametrize("dtype,d,h,hk", [(BF, 64, 2, 2), (BF, 128, 4, 2), (HF, 256, 2, 1), (F32, 64, 2, 1), (F32, 256, 1, 1)])
+@pytest.mark.parametrize("dtype,d,h,hk", [(BF, 64, 2, 2), (BF, 128, 4, 2), (HF, 256, 2, 1), (BF, 96, 2, 1), (BF, 192, 2, 2),
+                                         (F32, 64, 2, 1), (F32, 256, 1, 1)])
 @pytest.mark.parametrize("window", [1, 17, 64, 100, 128, 2 ** 40])
 def test_windows(dtype, d, h, hk, window):
     at, x = cases.inputs([300, 1, 64, 190], h, hk, d, dtype, behind=9)
@@ -96,7 +98,26 @@ def test_long_sequences(dtype, d, h, hk):
     compare(run(at, x), cases.expected(at, *x))
 
 
-@pytest.mark.parametrize("dtype,d", [(BF, 64), (BF, 128), (HF, 256), (F32, 64), (BF, 96), (F32, 96)])
+@pytest.mark.parametrize("dtype,d,h,hk,window", [(BF, 256, 32, 4, 0), (HF, 192, 32, 32, 0), (BF, 160, 32, 2, 100), (BF, 256, 32, 32, 65),
+                                                 (BF, 96, 32, 8, 0)])
+def test_many_blocks(dtype, d, h, hk, window):
+    at, x = cases.inputs([300, 1, 0, 260, 700, 128, 64, 127, 500], h, hk, d, dtype, behind=30)
+    compare(run(at, x, window), cases.expected(at, *x, window))
+
+
+def test_nothing_reaches_another_sequence_of_many_blocks():
+    lengths, h, d = [300, 700, 1100], 32, 192
+    at, x = cases.inputs(lengths, h, 4, d, BF, behind=60, junk=float("nan"))
+    want = cases.expected(at, *x)
+    for y, value in zip(x, (float("inf"), float("nan"), float("-inf"), float("nan"))):
+        y[at[1] + 3:at[2]:4] = value
+    got = {n: y.detach().cpu() for n, y in run(at, x).items()}
+    for name, y in got.items():
+        for a, b in ((0, at[1]), (at[2], x[0].shape[0])):
+            check(y[a:b], *(z[a:b] for z in want[name]), name)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (BF, 128), (HF, 256), (F32, 64), (BF, 96), (F32, 96), (BF, 192), (HF, 160)])
 def test_nothing_reaches_another_sequence(dtype, d):
     """NaN and infinities in the rows of no sequence and in one of three sequences."""
     lengths = [45, 30, 81]

@@ -15,8 +15,9 @@
 //   dK, dV   S = Q K^T (keys are columns), dV^T += dO^T P, dK^T += Q^T dS;
 //   dQ       S^T = K Q^T, dQ^T += K^T dS^T.
 // The transposed operands are read from row-major tiles (ds_read_b64_tr_b16).
-// head_dim is any multiple of 8: RAG kernels of the next of 64, 128 and 256 fill
-// the channels past it with zeros.
+// head_dim is any multiple of 8.  Kernels are made for the widths W of 64, 96, 128,
+// 192 and 256 channels, with rows of D = 64, 128 or 256 in LDS; a head_dim between
+// two runs those of the next (RAG), with zeros in the channels past it.
 // P and dS are rounded to the type for their products, half a step each; what
 // rounding takes from a 16-bit O is kept (o_low) and D taken from both.
 #include <algorithm>
@@ -56,11 +57,15 @@ struct PackedArgs {
 // of a tile lie NW * RPI apart, and the chunk it takes of them is the same (of
 // rows 8 apart, at head_dim 256 in four waves, one of two), so that one or two
 // 32-bit offsets a lane serve all: addresses made lane by lane took 16 registers
-// of the backward's and an add a load.  RAG: chunks past d are left as they are,
-// zeros that the block wrote before its first load.
+// of the backward's and an add a load.  Chunks past d are left as they are: RAG,
+// zeros that the block wrote before its first load, or past W, never read.
 constexpr int64_t kMostRowBytes = (1ll << 32) / 64 - 64;  // of 64 rows' offsets in 32 bits
-template <int D, int NW, bool RAG>
+template <int W>
+constexpr int kLayout = W <= 64 ? 64 : W <= 128 ? 128 : 256;
+template <int W, int NW, bool RAG>
 struct TileLoad {
+  static constexpr int D = kLayout<W>;
+  static constexpr bool PART = RAG || W < D;
   typedef KvLayout<D> L;
   static constexpr int IT = L::TILE / 1024 / NW, STEP = NW * L::RPI;
   static constexpr int KINDS = (STEP & (D == 64 ? 7 : 15)) ? 2 : 1;
@@ -77,7 +82,7 @@ struct TileLoad {
     for (int k = 0; k < KINDS; ++k) {
       const int c = (lane % L::CH) ^ L::swz(r + k * STEP);
       off[k] = r * rs + c * 16;
-      keep[k] = !RAG || c * 8 < d;
+      keep[k] = !PART || c * 8 < d;
     }
   }
   __device__ __forceinline__ void issue(int row0, int nrows, char* dst) const {
@@ -87,13 +92,13 @@ struct TileLoad {
     if (row0 + 64 <= nrows) {
 #pragma unroll
       for (int it = 0; it < IT; ++it)
-        if (!RAG || keep[it % KINDS]) dma_b128_at(tb + (uint64_t)(it * STEP) * rs, off[it % KINDS], lds + it * (NW * 1024));
+        if (!PART || keep[it % KINDS]) dma_b128_at(tb + (uint64_t)(it * STEP) * rs, off[it % KINDS], lds + it * (NW * 1024));
     } else {
       const int r = wave * L::RPI + (int)(threadIdx.x & 63) / L::CH;
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
         const uint32_t o = off[it % KINDS] - r * rs + min(r + it * STEP, nrows - 1 - row0) * rs;
-        if (!RAG || keep[it % KINDS]) dma_b128_at(tb, o, lds + it * (NW * 1024));
+        if (!PART || keep[it % KINDS]) dma_b128_at(tb, o, lds + it * (NW * 1024));
       }
     }
   }
@@ -107,10 +112,10 @@ __device__ __forceinline__ void clear_lds(char* lds, int bytes) {
 
 // 16 rows' fragments of a wave: row lr, channels 32 ks + 8 lg .. + 7 (zeros past
 // d), times +-1 or 0.
-template <typename T, int D, bool RAG>
-__device__ __forceinline__ void load_frags(const T* row, bool there, int lg, int d, float sign, typename Mfma<T>::frag (&f)[D / 32]) {
+template <typename T, int W, bool RAG>
+__device__ __forceinline__ void load_frags(const T* row, bool there, int lg, int d, float sign, typename Mfma<T>::frag (&f)[W / 32]) {
 #pragma unroll
-  for (int ks = 0; ks < D / 32; ++ks) {
+  for (int ks = 0; ks < W / 32; ++ks) {
     f[ks] = there && (!RAG || ks * 32 + lg * 8 < d) ? *(const typename Mfma<T>::frag*)(row + ks * 32 + lg * 8) : zero_frag<T>();
     if (sign != 1.f)
 #pragma unroll
@@ -136,14 +141,15 @@ __device__ __forceinline__ void zero_rows(const Rows& x, const PackedTile& t, in
 // forward.  NW waves take QPW queries each, QPB in all; with KH = 2 the waves'
 // halves take half of a tile's keys each and join at the end.
 // ---------------------------------------------------------------------------
-template <typename T, int D, bool RAG, int NW, int QPW, int KH>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) packed_fwd(PackedArgs p) {
+template <typename T, int W, bool RAG, int NW, int QPW, int KH>
+__global__ void __launch_bounds__(64 * NW, W > 128 ? 1 : 2) packed_fwd(PackedArgs p) {
+  constexpr int D = kLayout<W>;
   constexpr int QT = QPW / 16, QPB = NW / KH * QPW;
   constexpr int LIST = QPB == 128 ? 0 : 1;
   static_assert(QPB == kPackedRows[LIST], "");
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
-  constexpr int KS = D / 32, DT = D / 16;
+  constexpr int KS = W / 32, DT = W / 16;
   constexpr int STAGE = 2 * L::TILE;
   constexpr int KN = 64 / KH;
   char* const lds = packed_lds;
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) packed_fwd(PackedAr
   const int window = p.window > 0 ? min(p.window, len) : len;
 
   if constexpr (RAG) clear_lds(lds, 2 * STAGE);
-  TileLoad<D, NW, RAG> kl, vl;
+  TileLoad<W, NW, RAG> kl, vl;
   kl.init(p.k.at<T>(start, at.hk), p.k.row * (int64_t)sizeof(T), p.d);
   vl.init(p.v.at<T>(start, at.hk), p.v.row * (int64_t)sizeof(T), p.d);
   const int kv_end = min(len, q0 + QPB);
@@ -177,7 +183,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) packed_fwd(PackedAr
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int qi = qw + qt * 16 + lr;
-    load_frags<T, D, RAG>(p.q.at<T>(start + min(qi, len - 1), h), qi < len, lg, p.d, p.sign, qf[qt]);
+    load_frags<T, W, RAG>(p.q.at<T>(start + min(qi, len - 1), h), qi < len, lg, p.d, p.sign, qf[qt]);
   }
   frag ones;
 #pragma unroll
@@ -379,18 +385,21 @@ __global__ void __launch_bounds__(kThreads) packed_delta(PackedArgs p) {
   }
 }
 
-template <int D>
-constexpr int kKeyTiles = D == 256 ? 1 : 2;  // 16-key tiles of a wave: two would take all registers at 256
-template <int D>
-constexpr int kKeyList = D == 256 ? 1 : 0;
+// 16-key tiles of a wave: two would take all registers at 256 (794 spilled); at
+// 192 they take 436 (16384 rows, 8 over 2 heads, in 4 sequences: 971 us, one 1100).
+template <int W>
+constexpr int kKeyTiles = W > 192 ? 1 : 2;
+template <int W>
+constexpr int kKeyList = kKeyTiles<W> == 1 ? 1 : 0;
 constexpr int kQueryTiles = 2;
 
 // dK and dV of a tile of keys, over the query heads [g0, g1) of its group.
-template <typename T, int D, bool RAG>
+template <typename T, int W, bool RAG>
 __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& t, int hk, int g0, int g1, char* lds) {
+  constexpr int D = kLayout<W>;
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
-  constexpr int RT = kKeyTiles<D>, KW = 16 * RT, KS = D / 32, DT = D / 16;
+  constexpr int RT = kKeyTiles<W>, KW = 16 * RT, KS = W / 32, DT = W / 16;
   constexpr int STAGE = 2 * L::TILE + 512;  // a Q and a dO tile, -LSE log2(e)[64], -D[64]
   const int lane = threadIdx.x & 63, wave = wave_id(), lr = lane & 15, lg = lane >> 4;
   const int start = t.start, len = t.len, group = p.heads / p.kv_heads;
@@ -405,8 +414,8 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
     const int kj = kw + u * 16 + lr, row = start + min(kj, len - 1);
-    load_frags<T, D, RAG>(p.k.at<T>(row, hk), kj < len, lg, p.d, p.sign, kf[u]);
-    load_frags<T, D, RAG>(p.v.at<T>(row, hk), kj < len, lg, p.d, 1.f, vf[u]);
+    load_frags<T, W, RAG>(p.k.at<T>(row, hk), kj < len, lg, p.d, p.sign, kf[u]);
+    load_frags<T, W, RAG>(p.v.at<T>(row, hk), kj < len, lg, p.d, 1.f, vf[u]);
   }
   f32x4 dva[DT][RT], dka[DT][RT];
 #pragma unroll
@@ -419,7 +428,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
   const int nqb = (qend - qstart + 63) / 64, nsteps = nqb * (g1 - g0);
   const int sw = L::swz(lr);
   const TrOffsets<D> tro;
-  TileLoad<D, 4, RAG> ql, dl;
+  TileLoad<W, 4, RAG> ql, dl;
   auto head_of = [&](int g) {
     const int h = hk * group + g;
     ql.init(p.q.at<T>(start, h), p.q.row * (int64_t)sizeof(T), p.d);
@@ -556,11 +565,12 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
 }
 
 // dQ of a tile of 128 queries of one head.
-template <typename T, int D, bool RAG>
+template <typename T, int W, bool RAG>
 __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t, int h, int hk, char* lds) {
+  constexpr int D = kLayout<W>;
   typedef typename Mfma<T>::frag frag;
   typedef KvLayout<D> L;
-  constexpr int RT = kQueryTiles, QW = 16 * RT, QB = 4 * QW, KS = D / 32, DT = D / 16;
+  constexpr int RT = kQueryTiles, QW = 16 * RT, QB = 4 * QW, KS = W / 32, DT = W / 16;
   static_assert(QB == 128, "");
   constexpr int STAGE = 2 * L::TILE;
   const int lane = threadIdx.x & 63, wave = wave_id(), lr = lane & 15, lg = lane >> 4;
@@ -568,7 +578,7 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
   const int window = p.window > 0 ? min(p.window, len) : len;
 
   if constexpr (RAG) clear_lds(lds, 2 * STAGE);
-  TileLoad<D, 4, RAG> kl, vl;
+  TileLoad<W, 4, RAG> kl, vl;
   kl.init(p.k.at<T>(start, hk), p.k.row * (int64_t)sizeof(T), p.d);
   vl.init(p.v.at<T>(start, hk), p.v.row * (int64_t)sizeof(T), p.d);
   const int kv_end = min(len, q0 + QB);
@@ -581,8 +591,8 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
     const int qi = qw + u * 16 + lr, qc = min(qi, len - 1);
-    load_frags<T, D, RAG>(p.q.at<T>(start + qc, h), qi < len, lg, p.d, p.sign, qf[u]);
-    load_frags<T, D, RAG>(p.dout.at<T>(start + qc, h), qi < len, lg, p.d, 1.f, df[u]);
+    load_frags<T, W, RAG>(p.q.at<T>(start + qc, h), qi < len, lg, p.d, p.sign, qf[u]);
+    load_frags<T, W, RAG>(p.dout.at<T>(start + qc, h), qi < len, lg, p.d, 1.f, df[u]);
     lse2[u] = p.nlse2[(int64_t)h * p.tokens + start + qc];
     dlt[u] = p.ndelta[(int64_t)h * p.tokens + start + qc];
   }
@@ -688,26 +698,29 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 // keys' blocks need 380 registers, a wave a SIMD, and the queries' 248, two; in
 // one launch both run at the first ([16384 rows, 32 over 8, 128] in 4 sequences:
 // 2370 us, 1335 + 774 in two).  Four tiles of keys a wave, two waves a block,
-// spill (4.9 ms, 39 registers of 512 short with the sums pinned in AGPRs); four of queries take 960.
-template <typename T, int D, bool RAG, int KIND>
-__global__ void __launch_bounds__(kThreads, D == 64 || (D == 128 && KIND == 2) ? 2 : 1) packed_bwd(PackedArgs p, uint32_t nkv) {
+// spill (4.9 ms, 39 registers of 512 short with the sums pinned in AGPRs); four of
+// queries take 960.  At 64 and 96 both run at two in one launch (96 channels
+// 570 us of 16384 rows, 12 heads, in 4 sequences; 564 in two, 781 as 128).
+template <typename T, int W, bool RAG, int KIND>
+__global__ void __launch_bounds__(kThreads, W <= 96 || (W == 128 && KIND == 2) ? 2 : 1) packed_bwd(PackedArgs p, uint32_t nkv) {
+  constexpr int D = kLayout<W>;
   char* const lds = packed_lds;
   const int group = p.heads / p.kv_heads;
   if (KIND == 1 || (KIND == 0 && blockIdx.x < nkv)) {
-    const PackedAt at = packed_at(p.tiles[kKeyList<D>], p.head->count[kKeyList<D>], blockIdx.x, p.kv_part ? p.heads : p.kv_heads, p.kv_heads);
+    const PackedAt at = packed_at(p.tiles[kKeyList<W>], p.head->count[kKeyList<W>], blockIdx.x, p.kv_part ? p.heads : p.kv_heads, p.kv_heads);
     if (!at.live) return;
     const int g = p.kv_part ? at.h - at.hk * group : 0;
     if (at.t.tile < 0) {
       if (g == 0) zero_rows<T>(p.dk, at.t, at.hk, p.d), zero_rows<T>(p.dv, at.t, at.hk, p.d);
       return;
     }
-    return dkv_body<T, D, RAG>(p, at.t, at.hk, g, p.kv_part ? g + 1 : group, lds);
+    return dkv_body<T, W, RAG>(p, at.t, at.hk, g, p.kv_part ? g + 1 : group, lds);
   }
   if constexpr (KIND != 1) {
     const PackedAt at = packed_at(p.tiles[0], p.head->count[0], blockIdx.x - nkv, p.heads, p.kv_heads);
     if (!at.live) return;
     if (at.t.tile < 0) return zero_rows<T>(p.dq, at.t, at.h, p.d);
-    dq_body<T, D, RAG>(p, at.t, at.h, at.hk, lds);
+    dq_body<T, W, RAG>(p, at.t, at.h, at.hk, lds);
   }
 }
 
@@ -761,21 +774,32 @@ struct Launch {
 
 constexpr int64_t kMostThreads = 1ll << 32;
 
-template <typename T, int D, bool RAG>
-int fwd_launch(const PackedArgs& a, const Launch& l) {
-  constexpr int KH = D == 256 ? 2 : 1, NW = 4 * KH, QPW = D == 256 ? 16 : 32, QPB = NW / KH * QPW;
-  constexpr int bytes = 4 * KvLayout<D>::TILE;
-  auto k = packed_fwd<T, D, RAG, NW, QPW, KH>;
+template <typename T, int W, bool RAG, int NW, int QPW, int KH>
+int fwd_start(const PackedArgs& a, const Launch& l) {
+  constexpr int bytes = 4 * KvLayout<kLayout<W>>::TILE;
+  auto k = packed_fwd<T, W, RAG, NW, QPW, KH>;
   static Reserved reserve;
   const int rc = reserve((const void*)k, bytes, "mi355x_packed_attn_fwd");
   if (rc) return rc;
-  const int64_t blocks = l.cap(QPB) * a.heads;
+  const int64_t blocks = l.cap(NW / KH * QPW) * a.heads;
   MI_REQUIRE(blocks * 64 * NW < kMostThreads, "mi355x_packed_attn_fwd: %lld blocks", (long long)blocks);
   k<<<(unsigned)blocks, 64 * NW, bytes, l.s>>>(a);
   return check_launch("mi355x_packed_attn_fwd");
 }
 
-template <typename T, int D, bool>
+// Above 128 channels a block fills a CU, with 8 waves of 16 queries: 128 queries
+// where that gives 512 blocks, else 64, the keys of a step in two halves (256
+// channels, 4096 rows in 3 sequences: 8 heads 71 us and 59, 16 heads 95 and 106;
+// 16384 rows in 30, 4 heads, 66 and 82.  Four waves of 32 queries read half as
+// much from LDS, one a SIMD: 826 us where 8 take 746 and halves 878).
+template <typename T, int W, bool RAG>
+int fwd_launch(const PackedArgs& a, const Launch& l) {
+  if constexpr (W <= 128) return fwd_start<T, W, RAG, 4, 32, 1>(a, l);
+  else if (l.tokens / 128 * a.heads >= 512) return fwd_start<T, W, RAG, 8, 16, 1>(a, l);
+  else return fwd_start<T, W, RAG, 8, 16, 2>(a, l);
+}
+
+template <typename T, int D>
 int sum_launch(const PackedArgs& a, const Launch& l) {
   const int64_t sums = (int64_t)a.kv_heads * a.tokens * (D / 4);
   MI_REQUIRE(sums < kMostThreads - kThreads, "mi355x_packed_attn_bwd: too many rows and heads");
@@ -786,15 +810,16 @@ int sum_launch(const PackedArgs& a, const Launch& l) {
 template <int D>
 constexpr int kBwdLds = 2 * (2 * KvLayout<D>::TILE + 512);
 
-template <typename T, int D, bool RAG>
+template <typename T, int W, bool RAG>
 int bwd_launch(const PackedArgs& a, const Launch& l) {
-  constexpr bool SPLIT = D == 128;
-  auto k0 = packed_bwd<T, D, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, D, RAG, SPLIT ? 2 : 0>;
+  constexpr int D = kLayout<W>;
+  constexpr bool SPLIT = W == 128;
+  auto k0 = packed_bwd<T, W, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, W, RAG, SPLIT ? 2 : 0>;
   static Reserved reserve0, reserve1;
   int rc = reserve0((const void*)k0, kBwdLds<D>, "mi355x_packed_attn_bwd");
   if (!rc) rc = reserve1((const void*)k1, kBwdLds<D>, "mi355x_packed_attn_bwd");
   if (rc) return rc;
-  const int64_t nkv = l.cap(kPackedRows[kKeyList<D>]) * (a.kv_part ? a.heads : a.kv_heads), nq = l.cap(128) * a.heads;
+  const int64_t nkv = l.cap(kPackedRows[kKeyList<W>]) * (a.kv_part ? a.heads : a.kv_heads), nq = l.cap(128) * a.heads;
   const int64_t rows = (int64_t)a.heads * a.tokens;
   MI_REQUIRE((nkv + nq) * kThreads < kMostThreads && rows * (D / 4) < kMostThreads - kThreads,
              "mi355x_packed_attn_bwd: too many rows and heads");
@@ -805,16 +830,20 @@ int bwd_launch(const PackedArgs& a, const Launch& l) {
   } else {
     k0<<<(unsigned)(nkv + nq), kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
   }
-  return a.kv_part ? sum_launch<T, D, RAG>(a, l) : check_launch("mi355x_packed_attn_bwd");
+  return a.kv_part ? sum_launch<T, D>(a, l) : check_launch("mi355x_packed_attn_bwd");
 }
 
-int width_of(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+int layout_of(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+int width_of(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 
-#define MI_PACKED(FN, T, a, l)                                                                       \
-  switch (width_of((a).d)) {                                                                         \
-    case 64: return (a).d == 64 ? FN<T, 64, false>(a, l) : FN<T, 64, true>(a, l);                    \
-    case 128: return (a).d == 128 ? FN<T, 128, false>(a, l) : FN<T, 128, true>(a, l);                \
-    default: return (a).d == 256 ? FN<T, 256, false>(a, l) : FN<T, 256, true>(a, l);                 \
+#define MI_PACKED_WIDTH(FN, T, W, a, l) (a).d == W ? FN<T, W, false>(a, l) : FN<T, W, true>(a, l)
+#define MI_PACKED(FN, T, a, l)                                   \
+  switch (width_of((a).d)) {                                     \
+    case 64: return MI_PACKED_WIDTH(FN, T, 64, a, l);            \
+    case 96: return MI_PACKED_WIDTH(FN, T, 96, a, l);            \
+    case 128: return MI_PACKED_WIDTH(FN, T, 128, a, l);          \
+    case 192: return MI_PACKED_WIDTH(FN, T, 192, a, l);          \
+    default: return MI_PACKED_WIDTH(FN, T, 256, a, l);           \
   }
 
 int check_shape(const char* what, int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, double scale,
@@ -853,7 +882,7 @@ AttnF32 f32_args(const PackedArgs& a) {
   f.dv = (float*)a.dv.p, f.dv_s = a.dv.row, f.dv_h = a.dv.head;
   f.delta = a.ndelta, f.B = 1, f.H = a.heads, f.Sq = f.Skv = a.tokens;
   f.scale = a.scale, f.scale_log2 = a.scale * kLog2e, f.causal = 1, f.group = 1, f.window = a.window;
-  f.kv_part = a.kv_part, f.kv_plane = (int64_t)a.heads * a.tokens * (a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256), f.d = a.d;
+  f.kv_part = a.kv_part, f.kv_plane = (int64_t)a.heads * a.tokens * layout_of(a.d), f.d = a.d;
   return f;
 }
 
@@ -899,13 +928,13 @@ extern "C" int mi355x_packed_attn_fwd(void* o, const int64_t* o_th, void* o_low,
 // head: 16384 rows in 16 sequences, 32 over 2 heads of 64 684 and 584 us; 8192 rows
 // in 4, 32 over 8 of 128 747 and 844; 16384 in 4, 16 over 4 of 256 3533 and 3740).
 static bool splits_group(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d) {
-  return heads > kv_heads && (tokens / kPackedRows[d > 128] + 1) * kv_heads < 512;
+  return heads > kv_heads && (tokens / kPackedRows[d > 192] + 1) * kv_heads < 512;
 }
 
 extern "C" int64_t mi355x_packed_attn_bwd_workspace_bytes(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                           int64_t d) {
   const int64_t terms = 2 * heads * tokens * (int64_t)sizeof(float) + 512;
-  return heads > kv_heads ? terms + 2 * heads * tokens * width_of(d) * (int64_t)sizeof(float) : terms;
+  return heads > kv_heads ? terms + 2 * heads * tokens * layout_of(d) * (int64_t)sizeof(float) : terms;
 }
 
 extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, const int64_t* dk_th, void* dv,
@@ -943,7 +972,8 @@ extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, 
   if (dtype == MI355X_F32) {
     const int r = attn_f32_packed(f32_args(a), {a.head, a.tiles[1], l.cap(64), (uint32_t)heads, (uint32_t)kv_heads}, true, l.s);
     if (r || !a.kv_part) return r;
-    MI_PACKED(sum_launch, float, a, l);
+    const int w = layout_of(d);
+    return w == 64 ? sum_launch<float, 64>(a, l) : w == 128 ? sum_launch<float, 128>(a, l) : sum_launch<float, 256>(a, l);
   }
   if (dtype == MI355X_BF16) MI_PACKED(bwd_launch, bf16, a, l);
   MI_PACKED(bwd_launch, f16, a, l);
