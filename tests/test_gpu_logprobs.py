@@ -117,6 +117,25 @@ def test_masked_vocabulary(dtype, n, c):
     assert torch.isneginf(got.cpu()).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("n,c,entropy", [(600, 9001, True), (600, 9001, False), (8, 50257, True), (8, 50257, False)])
+def test_far_and_masked_rows_without_top_entries(dtype, n, c, entropy):
+    """What a row's walk meets late, early or everywhere: large values, -inf, the type's lowest."""
+    x, tokens = cases.logits(n, c, dtype)
+    low = torch.finfo(dtype).min
+    x[0, :], x[0, c - 2] = -torch.inf, 3.0
+    x[1, :] = low
+    x[2, 1::2] = low
+    x[3, c // 2] = 40000.0
+    x[4, :] = -40000.0
+    x[5, :c // 2], x[5, c // 2:] = -30000.0, 30000.0
+    x[6, c - 1] = 60000.0
+    x[7, :4000] = -torch.inf
+    tokens[:8] = torch.tensor([c - 2, 7, 8, c // 2, c - 1, c - 1, c - 1, 4000])
+    run(x, tokens, 0, entropy)
+    train(x, tokens, 0, entropy)
+
+
 @pytest.mark.parametrize("n,c", [(3, 100), (600, 1000), (2, 50257), (300, 50257)])
 def test_nan_and_infinity(n, c):
     """A NaN makes its row NaN and comes first; so do a +inf, and a row of -inf."""

@@ -48,11 +48,11 @@ struct Chunk {
   u32x4 w;
   // whole elements i .. i + V - 1
   __device__ __forceinline__ void load(const T* row, int64_t i) { __builtin_memcpy(&w, row + i, 16); }
-  // those of them that lie before n, the others -inf
-  __device__ __forceinline__ void load_end(const T* row, int64_t i, int64_t n) {
+  // those of them that lie before n and from `first` on, for the others `rest`
+  __device__ __forceinline__ void load_end(const T* row, int64_t i, int64_t n, int64_t first = 0, float rest = -INFINITY) {
     union { T v[V]; u32x4 w; } u;
 #pragma unroll
-    for (int e = 0; e < V; ++e) u.v[e] = i + e < n ? row[i + e] : (T)-INFINITY;
+    for (int e = 0; e < V; ++e) u.v[e] = i + e >= first && i + e < n ? row[i + e] : (T)rest;
     w = u.w;
   }
   __device__ __forceinline__ float get(int e) const {
@@ -74,6 +74,11 @@ struct Chunk {
     }
   }
 };
+
+// Elements between a 16-byte boundary and p (a row of an odd number of 16-bit
+// elements begins anywhere; loads that do not lie on 4 bytes run at 90% of the others' rate).
+template <typename T>
+__device__ __forceinline__ int lead_of(const T* p) { return (int)((uintptr_t)p & 15) / (int)sizeof(T); }
 
 // Where a value stands among f32 values, and the key that a larger value, or of
 // equal ones the lower index, has the larger of.  0 is no entry's key.
@@ -308,28 +313,77 @@ __global__ void __launch_bounds__((LpShape<T, NW, CPT>::kThreads)) lp_rows(LpArg
 
 // Without top entries nothing is looked at twice: a block walks its segment with
 // a running maximum m, s = sum 2^f and t = sum 2^f f, f = (x - m) log2(e), which
-// move to a new maximum as t = (t + s d) 2^d, s = s 2^d.
+// move to a new maximum as t = (t + s d) 2^d, s = s 2^d.  An exponential an element
+// and what stands around it bound the walk, so f is one instruction, x log2(e) -
+// r with r = m log2(e) as rounded, and what r is off by is taken out of the sums at
+// the end; that holds for the finite x below kNear, and -inf makes 2^f f a NaN.  A
+// wave that meets anything else takes its batch again, and those that follow,
+// with f as it is defined, an exponent of -200 for all below it (8192 x 50257
+// bf16, 0.82 GB, 160 us with that for all, 149 so, 5.5 TB/s).
 constexpr int kStreamThreads = 256;
+constexpr float kNear = 32768.f;
+// What fills a row's last chunk: 2^f of it is 0 for every m below kNear.
+template <typename T>
+constexpr float kFill = -1e30f;
+template <>
+constexpr float kFill<f16> = -65504.f;
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kStreamThreads) lp_stream(LpArgs p) {
   constexpr int V = Chunk<T>::V, U = 4, W = kStreamThreads / 64;
   __shared__ float red[W][3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t item = blockIdx.x, row = item / p.segments, e0 = (item - row * p.segments) * p.seg;
-  const int len = (int)min(p.seg, p.c - e0), nc = (len + V - 1) / V;
-  const T* const x = (const T*)p.x + row * p.ld + e0;
-  float m = -INFINITY, s = 0.f, t = 0.f;
-  bool nan = false;
+  // chunks are cut where memory is, from up to V - 1 elements before the segment
+  const T* const begin = (const T*)p.x + row * p.ld + e0;
+  const int first = lead_of(begin), len = first + (int)min(p.seg, p.c - e0), nc = (len + V - 1) / V;
+  const T* const x = begin - first;
+  float m = -INFINITY, r = 0.f, s = 0.f, t = 0.f;
+  bool nan = false, near = true;
+  auto settle = [&]() {  // the sums with f = (x - m) log2(e): by 2^-e, e = m log2(e) - r
+    if (m == -INFINITY) return;
+    const float e = fmaf(m, kLog2e, -r), k = e * kLn2, g = fmaf(0.5f * k, k, -k);
+    t = fmaf(-e, s, t);
+    t = fmaf(g, t, t), s = fmaf(g, s, s);
+  };
   for (int c0 = tid; c0 < nc; c0 += kStreamThreads * U) {
     Chunk<T> ch[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = (c0 + u * kStreamThreads) * V;
-      if (i + V <= len) ch[u].load(x, i);
-      else ch[u].load_end(x, i, len);
+      if (i >= first && i + V <= len) ch[u].load(x, i);
+      else ch[u].load_end(x, i, len, first, kFill<T>);
+    }
+    if (near) {
+      const float m0 = m, r0 = r, s0 = s, t0 = t;
+      bool far = false;
+      float v[U * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u * V + e] = ch[u].get(e);
+      const float top = max_nan(v);
+      if (top > m) {
+        const float r1 = top * kLog2e, d = m == -INFINITY ? kFloor : fmaxf(r - r1, kFloor), f = hw_exp2(d);
+        if constexpr (ENT) t = fmaf(s, d, t) * f;
+        s *= f, m = top, r = r1;
+        far = !(fabsf(top) < kNear);
+      }
+#pragma unroll
+      for (int e = 0; e < U * V; ++e) {
+        const float f = fmaf(v[e], kLog2e, -r), q = hw_exp2(f);
+        s += q;
+        if constexpr (ENT) t = fmaf(q, f, t);
+      }
+      const float sum = ENT ? t : s;
+      if (!__builtin_amdgcn_ballot_w64(far || sum != sum)) continue;
+      m = m0, r = r0, s = s0, t = t0;
+      settle();
+      near = false;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const int i = (c0 + u * kStreamThreads) * V;
+      if (i < first || i + V > len) ch[u].load_end(x, i, len, first);
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = ch[u].get(e);
@@ -348,6 +402,7 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream(LpArgs p) {
       }
     }
   }
+  if (near) settle();
   if (nan) m = __uint_as_float(0x7fc00000u);
   // to the block's maximum; what a NaN or an infinity makes of the sums is in m
   float all = wave_max_nan(m);
@@ -456,10 +511,11 @@ using Chunk8 = uint32_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 
 // Rows go last first: the forward has read those last, and what of them the 256
 // MB cache still holds is not read from memory again.  A gradient that does not
-// fit that cache is stored past it, or it would push the logits out and be
-// written back during the next kernel (8192 x 50257 bf16, forward and
-// backward, 2.47 GB: 582 us first to last, 560 last to first, 525 with both; a small
-// gradient stays for the product that reads it next).
+// fit that cache is stored past it, or it would push the logits out and be written
+// back during the next kernel (8192 x 50257 bf16, forward and backward, 2.47 GB:
+// 582 us first to last, 560 last to first, 525 with both, 496 with chunks that lie
+// on 16 bytes and the forward's shorter exponent; a small gradient stays for the
+// product that reads it next).
 constexpr int64_t kMemoryCache = 256ll << 20;
 constexpr int kBwdThreads = 256;
 template <typename T>
@@ -482,33 +538,36 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
     const float z = not_below(fmaf(v - m, kLog2e, -l2));
     return -hw_exp2(z) * fmaf(slope, z, base);
   };
-  for (int64_t j0 = c0 + tid * V; j0 < c1; j0 += kBwdThreads * V * U) {
+  // chunks lie on 16 bytes where those of the row and of its gradient can
+  const int64_t begin = c0 - (((uintptr_t)(x + c0) ^ (uintptr_t)(dx + c0)) & 15 ? 0 : lead_of(x + c0));
+  for (int64_t j0 = begin + tid * V; j0 < c1; j0 += kBwdThreads * V * U) {
     Chunk<T> ch[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-    {
+    for (int u = 0; u < U; ++u) {
       const int64_t j = j0 + u * kBwdThreads * V;
       if (j < c1) {
-        if (j + V <= p.c) ch[u].load(x, j);
-        else ch[u].load_end(x, j, p.c);
+        if (j >= c0 && j + V <= p.c) ch[u].load(x, j);
+        else ch[u].load_end(x, j, p.c, c0);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t j = j0 + u * kBwdThreads * V;
       if (j >= c1) break;
+      float r[V];
       struct { T v[V]; } o;
-      const bool whole = j + V <= p.c && !(given && token - j >= 0 && token - j < V);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float r = at(ch[u].get(e));
-        if (!whole) {
-          if (given && j + e == token) r += g;
-          if (j + e >= p.c) r = 0.f;  // the columns that pad a row
+      for (int e = 0; e < V; ++e) r[e] = at(ch[u].get(e));
+      if (j + V > p.c || (uint64_t)(token - j) < V) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (given && j + e == token) r[e] += g;
+          if (j + e >= p.c) r[e] = 0.f;  // the columns that pad a row
         }
-        o.v[e] = (T)r;
       }
-      if (j + V <= p.ld_dx) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.v[e] = (T)r[e];
+      if (j >= c0 && j + V <= c1) {
         Chunk8<T> w;
         __builtin_memcpy(&w, o.v, 16);
         if (p.past) __builtin_nontemporal_store(w, (Chunk8<T>*)(dx + j));
@@ -516,7 +575,7 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (j + e < p.ld_dx) dx[j + e] = o.v[e];
+          if (j + e >= c0 && j + e < c1) dx[j + e] = o.v[e];
       }
     }
   }
@@ -539,9 +598,8 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
 // not, where there are enough rows to fill the 256 CUs; else into segments of 8 KB
 // and more for 512 blocks in all, of which the join takes kJoinList keys (one
 // bf16 row of 262144, 20 top entries: 9.8 us and 5.8 to join 64 segments, 11.4 and
-// 4.8 of 32, 8.5 and 8.3 of 128).  Rows of 8192 x 50257 bf16 stream in 214 us, 0.82
-// GB: a lane's ten instructions an element, an exponential among them, take 150 of
-// them, reading alone would; held in registers 239, in blocks of 16 waves 346.
+// 4.8 of 32, 8.5 and 8.3 of 128).  Rows of 8192 x 50257 bf16 stream in 149 us; held
+// in registers they took 239, in blocks of 16 waves 346.
 struct LpPlan {
   int waves;      // of a segment: 1, 4 or 8; 0: lp_stream's block
   int64_t segments, seg;
