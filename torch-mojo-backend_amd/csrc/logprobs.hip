@@ -11,7 +11,9 @@
 // segment of one, in registers, so that the maximum, the sums and the search for
 // the largest entries are passes over registers.  Long rows and few rows are cut
 // into segments, whose results a second kernel joins.  The backward reads the
-// logits once and writes the gradient once.
+// logits once and writes the gradient once.  1000 x 50257 f32 with entropy and 5
+// top entries: 51.5 us and 5 to join, 201 MB; the gradient of 8192 x 50257 bf16 320
+// us, 1.65 GB, 5.1 TB/s.
 //
 // Largest entries: a lane's maximum is known from the first pass.  The k-th
 // largest of a wave's 64 is a bound that k entries of the row reach, and so is

@@ -12,7 +12,7 @@ constexpr int kClasses = 512;  // tile numbers that are told apart; all later on
 // themselves is that of arrival, and moves no result.  With sequence i's number
 // of tiles m_i, number k has as many entries as there are m_i > k: a count of
 // the m_i, then two suffix sums.
-// 48 sequences of 16384 rows 10 us, 16384 sequences of one row 76.
+// 16384 rows: one sequence 5 us, 16 of 1024 rows 11, 48 of 341 14, 16384 of one row 45.
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedHeader* head, PackedTile* list0, PackedTile* list1,
                                                                    const int32_t* offsets, int64_t n, int tokens,
                                                                    int32_t* error) {
