@@ -1,6 +1,8 @@
 """Fused ops of the Gemma-3-shaped workload: rotary embedding, GeGLU and
-RMSNorm with a weight offset, attention over a sliding window with sinks; and
-serving's: appending to a paged key/value cache and attention over it.
+RMSNorm with a weight offset, attention over a sliding window with sinks; those of
+packed sequences: rotary positions, attention within each sequence and
+log-probabilities of tokens; and serving's: appending to a paged key/value cache
+and attention over it.
 
 Torch has no single aten op for these (a model writes them as chains of
 slice / neg / cat / mul / add, gelu + mul, and rms_norm with `1 + w`); the
