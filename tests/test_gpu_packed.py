@@ -192,3 +192,64 @@ def test_only_padding():
     _, x = cases.inputs([], 2, 1, 64, F32, behind=100, junk=float("nan"))
     got = run([0], x)
     assert all(not y.detach().cpu().abs().any() for y in got.values())
+
+
+def test_one_tensor_for_all_and_gradients_of_some():
+    at, x = cases.inputs([70, 1, 100], 2, 2, 64, BF)
+    seqs = sequences(at, 171)
+    want = cases.expected(at, x[0], x[0], x[0], x[3])
+    leaf = x[0].to("mojo").requires_grad_()
+    ops.packed_attention(leaf, leaf, leaf, seqs).backward(x[3].to("mojo"))
+    value = sum(want[n][0] for n in ("dq", "dk", "dv"))
+    # (each rounded, and two sums of them)
+    bound = sum(want[n][1] for n in ("dq", "dk", "dv")) + 2.0 ** -8 * (abs(value) + abs(want["dq"][0] + want["dk"][0]) + abs(want["dk"][0] + want["dv"][0]))
+    check(leaf.grad, value, bound)
+    want = cases.expected(at, *x)
+    q, k, v = (y.to("mojo") for y in x[:3])
+    k.requires_grad_()
+    out = ops.packed_attention(q, k, v, seqs)
+    for _ in range(2):  # the graph is kept
+        dk, = torch.autograd.grad(out, k, x[3].to("mojo"), retain_graph=True)
+        check(dk, *want["dk"])
+    with torch.no_grad():
+        out.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, k, x[3].to("mojo"))
+
+
+def test_leaves_of_one_buffer_keep_their_gradients():
+    at, x = cases.inputs([40, 30], 2, 2, 64, F32)
+    whole = torch.cat(x[:3], dim=1).to("mojo")
+    q, k, v = (y.detach().requires_grad_() for y in whole.split(2, dim=1))
+    ops.packed_attention(q, k, v, sequences(at, 70)).backward(x[3].to("mojo"))
+    before = k.grad.clone()
+    torch.cat([q.grad, k.grad, v.grad], dim=1).mul_(3)
+    assert torch.equal(before.cpu(), k.grad.cpu())
+    check(k.grad, *cases.expected(at, *x)["dk"])
+
+
+def test_many_short_sequences_and_far_rows():
+    """As many tiles as rows, and rows that lie further apart than the kernels' offsets reach."""
+    n, h, d = 30000, 2, 8
+    at, x = cases.inputs([1] * n, h, 1, d, BF)
+    got = run(at, x)
+    assert torch.equal(got["out"].cpu(), x[2].expand(n, h, d))  # a row that sees itself
+    # dS = P (dP - D) is 0 but for dP and D, the same 8 products added in f32 in two
+    # orders: 8 roundings each, and their difference's and the next product's
+    q, k, v, dy = (y.double() for y in x)
+    off = d ** -0.5 * 20 * 2.0 ** -24 * (dy * v).abs().sum(-1, keepdim=True)
+    assert (got["dq"].cpu().double().abs() <= off * k.abs()).all()
+    assert (got["dk"].cpu().double().abs() <= (off * q.abs()).sum(1, keepdim=True)).all()
+    check(got["dv"], x[3].double().sum(1, keepdim=True).numpy(), 2.0 ** -8 * x[3].double().sum(1, keepdim=True).abs().numpy() + 2.0 ** -22)
+    at, x = cases.inputs([5, 3], 1, 1, 64, BF)
+    far = torch.zeros(8, 2 ** 25 + 64, dtype=BF, device="mojo")
+    far[:, :64] = x[1].view(8, 64).to("mojo")
+    k = far[:, :64].view(8, 1, 64)
+    with torch.no_grad():
+        check(ops.packed_attention(x[0].to("mojo"), k, x[2].to("mojo"), sequences(at, 8)), *cases.expected(at, *x)["out"])
+
+
+def test_no_sequences():
+    at, x = cases.inputs([], 2, 1, 64, BF, behind=70)
+    for y in run(at, x).values():
+        assert not y.detach().cpu().any()

@@ -68,6 +68,20 @@ def test_gemma_scores():
     assert (got.top_tokens.cpu() == want.top_tokens).float().mean() > 0.99  # f32 may order a near tie either way
 
 
+def test_of_no_rows_and_of_other_batches():
+    """One model, batches one after another, one of no rows among them."""
+    m, ref = decode_cases.model(F32, "mojo", sinks=0)
+    for lengths, rows in (([5, 0, 9], 14), ([], 0), ([], 3), ([64, 1], 70)):
+        idx = torch.randint(0, 97, (rows,), generator=torch.Generator().manual_seed(rows))
+        with torch.no_grad():
+            got = m.score_packed(idx.to("mojo"), PackedSequences.of_lengths(lengths, rows), top=1, entropy=True)
+            want = ref.score_packed(idx, PackedSequences.of_lengths(lengths, rows, device="cpu"), top=1, entropy=True)
+        assert got.logprobs.shape == (rows,) and got.top_tokens.shape == (rows, 1)
+        if rows:
+            close(got.logprobs, want.logprobs, 1e-4, "logprobs") if lengths else None
+            close(got.entropy, want.entropy, 1e-4, "entropy")
+
+
 @pytest.mark.parametrize("autocast", [None, BF])
 def test_gpt_training_steps(autocast):
     """Documents packed end to end: loss and gradients are those of the f64 model,

@@ -98,7 +98,8 @@ def attention_backward(grad: MT, q: MT, k: MT, v: MT, out: MT, lse: MT, low, seq
     """(dq, dk, dv): dense, or the parts of one dense tensor."""
     if grad._dtype != q._dtype:
         grad = materialize_contiguous(grad, q._dtype)
-    together = q._holder is k._holder is v._holder
+    # (a leaf's gradient is kept, and must not share memory with a cat of it)
+    together = q._holder is k._holder is v._holder and not (q.is_leaf or k.is_leaf or v.is_leaf)
     grad, q, k, v = _rows(grad), _rows(q), _rows(k), _rows(v)
     t, h, d = q._shape
     hk, code, library = k._shape[1], _code(q._dtype), lib()
