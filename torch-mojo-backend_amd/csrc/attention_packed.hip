@@ -396,6 +396,8 @@ __global__ void __launch_bounds__(kThreads) packed_delta(PackedArgs p) {
 
 // 16-key tiles of a wave: two would take all registers at 256 (794 spilled); at
 // 192 they take 436 (16384 rows, 8 over 2 heads, in 4 sequences: 971 us, one 1100).
+// Eight waves of one at 256 spill 28 (16384 rows, 16 over 4 heads, in 4 sequences:
+// keys 2427 us and queries 970 in two launches, 2581 in one as it is).
 template <int W>
 constexpr int kKeyTiles = W > 192 ? 1 : 2;
 template <int W>
