@@ -253,3 +253,17 @@ def test_no_sequences():
     at, x = cases.inputs([], 2, 1, 64, BF, behind=70)
     for y in run(at, x).values():
         assert not y.detach().cpu().any()
+
+
+@pytest.mark.parametrize("dtype,d,h,hk", [(BF, 64, 12, 12), (HF, 64, 12, 12), (BF, 128, 8, 2), (BF, 80, 8, 8), (BF, 256, 4, 4)])
+@pytest.mark.parametrize("lengths", [[2] * 40, [2, 3, 5, 7, 9] * 8])
+def test_gradients_of_few_terms(dtype, d, h, hk, lengths):
+    """The norm of what dQ and dK of short sequences are off by: that of rounding them,
+    whose error is spread evenly over half a step to either side, a root of three of
+    half a step at most.  (dS rounded once would add as much again.)"""
+    at, x = cases.inputs(lengths, h, hk, d, dtype)
+    got, want = run(at, x), cases.expected(at, *x)
+    for name in ("dq", "dk"):
+        value = torch.from_numpy(want[name][0])
+        off = (got[name].cpu().double() - value).norm() / value.norm()
+        assert off <= torch.finfo(dtype).eps / 2 / 3 ** 0.5, (name, off.item())

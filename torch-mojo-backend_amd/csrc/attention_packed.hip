@@ -403,9 +403,20 @@ constexpr int kKeyTiles = W > 192 ? 1 : 2;
 template <int W>
 constexpr int kKeyList = kKeyTiles<W> == 1 ? 1 : 0;
 constexpr int kQueryTiles = 2;
+// Sequences, or windows, of no more rows than this take what rounding took from dS
+// to a product of its own (FINE; all their steps are masked ones): a gradient of
+// few terms is off by its own rounding and by theirs, up to 1.9 times its own alone
+// in sequences of 2 to 9 rows.  In longer ones it is 1.45 times, and the product a
+// quarter of the queries' pass.  In a body of its own, and at 128 channels the keys
+// in a launch of their own: in one kernel their loop took 1.09 times as long (1397
+// us where it takes 1280), in one body 1.15.
+constexpr int kFine = 64;
+__device__ __forceinline__ bool is_fine(const PackedArgs& p, const PackedTile& t) {
+  return t.len <= kFine || (p.window > 0 && p.window <= kFine);
+}
 
 // dK and dV of a tile of keys, over the query heads [g0, g1) of its group.
-template <typename T, int W, bool RAG>
+template <typename T, int W, bool RAG, bool FINE>
 __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& t, int hk, int g0, int g1, char* lds) {
   constexpr int D = kLayout<W>;
   typedef typename Mfma<T>::frag frag;
@@ -490,7 +501,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs) {
       if (MASK && (qs * 32 + 31 < kq || qs * 32 >= kq + KW - 1 + window || qb0 + qs * 32 >= len)) continue;
-      frag pb[RT], sb[RT];
+      frag pb[RT], sb[RT], sl[FINE ? RT : 1];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const int qt = 2 * qs + w;
@@ -520,6 +531,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
             const float pv = fast_exp2(x);
             pb[u][4 * w + e] = (T)pv;
             sb[u][4 * w + e] = (T)(pv * pa[e]);
+            if constexpr (FINE) sl[u][4 * w + e] = (T)(pv * pa[e] - to_f32(sb[u][4 * w + e]));
           }
         }
       }
@@ -531,6 +543,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
         for (int u = 0; u < RT; ++u) {
           dva[dt][u] = Mfma<T>::mma(dof, pb[u], dva[dt][u]);
           dka[dt][u] = Mfma<T>::mma(qtf, sb[u], dka[dt][u]);
+          if constexpr (FINE) dka[dt][u] = Mfma<T>::mma(qtf, sl[u], dka[dt][u]);
         }
       }
     }
@@ -544,7 +557,8 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
   for (int g = g0; g < g1; ++g) {
     int j = 0;
     for (; j < j1; ++j) step(j, BoolTag<true>{});
-    for (; j < j2; ++j) step(j, BoolTag<false>{});
+    if constexpr (!FINE)
+      for (; j < j2; ++j) step(j, BoolTag<false>{});
     for (; j < nqb; ++j) step(j, BoolTag<true>{});
   }
 #pragma unroll
@@ -576,7 +590,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
 }
 
 // dQ of a tile of 128 queries of one head.
-template <typename T, int W, bool RAG>
+template <typename T, int W, bool RAG, bool FINE>
 __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t, int h, int hk, char* lds) {
   constexpr int D = kLayout<W>;
   typedef typename Mfma<T>::frag frag;
@@ -641,7 +655,7 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
       if (MASK && (ks2 * 32 > qk + QW - 1 || ks2 * 32 + 31 < qk - window + 1)) continue;
-      frag sb[RT];
+      frag sb[RT], sl[FINE ? RT : 1];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const int kt = 2 * ks2 + w;
@@ -667,7 +681,9 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
               const int key = kt * 16 + 4 * lg + e;
               x = key < lim[u] && key >= lo[u] ? x : -INFINITY;
             }
-            sb[u][4 * w + e] = (T)(fast_exp2(x) * pa[e]);
+            const float sv = fast_exp2(x) * pa[e];
+            sb[u][4 * w + e] = (T)sv;
+            if constexpr (FINE) sl[u][4 * w + e] = (T)(sv - to_f32(sb[u][4 * w + e]));
           }
         }
       }
@@ -675,7 +691,10 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
       for (int dt = 0; dt < DT; ++dt) {
         const frag ktf = tr_frag_at<T, D>(Kt, tro, dt, 2 * ks2, 2 * ks2 + 1);
 #pragma unroll
-        for (int u = 0; u < RT; ++u) dqa[dt][u] = Mfma<T>::mma(ktf, sb[u], dqa[dt][u]);
+        for (int u = 0; u < RT; ++u) {
+          dqa[dt][u] = Mfma<T>::mma(ktf, sb[u], dqa[dt][u]);
+          if constexpr (FINE) dqa[dt][u] = Mfma<T>::mma(ktf, sl[u], dqa[dt][u]);
+        }
       }
     }
   };
@@ -685,7 +704,8 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
   const int ju = qw + QW <= len ? max(jl, min(nkb, (qw + 1) / 64)) : jl;
   int j = jw;
   for (; j < jl; ++j) step(j, BoolTag<true>{});
-  for (; j < ju; ++j) step(j, BoolTag<false>{});
+  if constexpr (!FINE)
+    for (; j < ju; ++j) step(j, BoolTag<false>{});
   for (; j < nkb; ++j) step(j, BoolTag<true>{});
 #pragma unroll
   for (int u = 0; u < RT; ++u) {
@@ -705,8 +725,8 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 
 // KIND 0, both in one launch: the first nkv blocks take keys, one of a K/V
 // head's or, where their gradients go through partials, one of a query head's;
-// the rest take queries.  1: keys alone, 2: queries alone.  At head_dim 128 the
-// keys' blocks need 380 registers, a wave a SIMD, and the queries' 248, two; in
+// the rest take queries.  1: keys alone, but for FINE tiles, which 3 takes (4.8 us
+// where there are none), 2: queries alone.  At head_dim 128 the keys' blocks need 380 registers, a wave a SIMD, and the queries' 248, two; in
 // one launch both run at the first ([16384 rows, 32 over 8, 128] in 4 sequences:
 // 2370 us, 1335 + 774 in two).  Four tiles of keys a wave, two waves a block,
 // spill (4.9 ms, 39 registers of 512 short with the sums pinned in AGPRs); four of
@@ -717,21 +737,28 @@ __global__ void __launch_bounds__(kThreads, W <= 96 || (W == 128 && KIND == 2) ?
   constexpr int D = kLayout<W>;
   char* const lds = packed_lds;
   const int group = p.heads / p.kv_heads;
-  if (KIND == 1 || (KIND == 0 && blockIdx.x < nkv)) {
+  if (KIND % 2 || (KIND == 0 && blockIdx.x < nkv)) {
     const PackedAt at = packed_at(p.tiles[kKeyList<W>], p.head->count[kKeyList<W>], blockIdx.x, p.kv_part ? p.heads : p.kv_heads, p.kv_heads);
-    if (!at.live) return;
+    if (!at.live || (KIND == 3 && at.t.tile < 0)) return;
     const int g = p.kv_part ? at.h - at.hk * group : 0;
     if (at.t.tile < 0) {
       if (g == 0) zero_rows<T>(p.dk, at.t, at.hk, p.d), zero_rows<T>(p.dv, at.t, at.hk, p.d);
       return;
     }
-    return dkv_body<T, W, RAG>(p, at.t, at.hk, g, p.kv_part ? g + 1 : group, lds);
+    const int g1 = p.kv_part ? g + 1 : group;
+    if (is_fine(p, at.t)) {
+      if constexpr (KIND != 1) dkv_body<T, W, RAG, true>(p, at.t, at.hk, g, g1, lds);
+    } else {
+      if constexpr (KIND != 3) dkv_body<T, W, RAG, false>(p, at.t, at.hk, g, g1, lds);
+    }
+    return;
   }
-  if constexpr (KIND != 1) {
+  if constexpr (KIND % 2 == 0) {
     const PackedAt at = packed_at(p.tiles[0], p.head->count[0], blockIdx.x - nkv, p.heads, p.kv_heads);
     if (!at.live) return;
     if (at.t.tile < 0) return zero_rows<T>(p.dq, at.t, at.h, p.d);
-    dq_body<T, W, RAG>(p, at.t, at.h, at.hk, lds);
+    if (is_fine(p, at.t)) return dq_body<T, W, RAG, true>(p, at.t, at.h, at.hk, lds);
+    dq_body<T, W, RAG, false>(p, at.t, at.h, at.hk, lds);
   }
 }
 
@@ -825,10 +852,11 @@ template <typename T, int W, bool RAG>
 int bwd_launch(const PackedArgs& a, const Launch& l) {
   constexpr int D = kLayout<W>;
   constexpr bool SPLIT = W == 128;
-  auto k0 = packed_bwd<T, W, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, W, RAG, SPLIT ? 2 : 0>;
-  static Reserved reserve0, reserve1;
+  auto k0 = packed_bwd<T, W, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, W, RAG, SPLIT ? 2 : 0>, k2 = packed_bwd<T, W, RAG, SPLIT ? 3 : 0>;
+  static Reserved reserve0, reserve1, reserve2;
   int rc = reserve0((const void*)k0, kBwdLds<D>, "mi355x_packed_attn_bwd");
   if (!rc) rc = reserve1((const void*)k1, kBwdLds<D>, "mi355x_packed_attn_bwd");
+  if (!rc) rc = reserve2((const void*)k2, kBwdLds<D>, "mi355x_packed_attn_bwd");
   if (rc) return rc;
   const int64_t nkv = l.cap(kPackedRows[kKeyList<W>]) * (a.kv_part ? a.heads : a.kv_heads), nq = l.cap(128) * a.heads;
   const int64_t rows = (int64_t)a.heads * a.tokens;
@@ -837,6 +865,7 @@ int bwd_launch(const PackedArgs& a, const Launch& l) {
   packed_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, l.s>>>(a);
   if (SPLIT) {
     k0<<<(unsigned)nkv, kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
+    k2<<<(unsigned)nkv, kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
     k1<<<(unsigned)nq, kThreads, kBwdLds<D>, l.s>>>(a, 0);
   } else {
     k0<<<(unsigned)(nkv + nq), kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
