@@ -1,0 +1,51 @@
+"""Calls of rotary positions, packed attention and token log-probabilities on the
+MI355X whose arguments have to be copied first, or that take kernels of their own."""
+
+import pytest
+import torch
+
+import logprob_cases
+from paged_cases import check
+from torch_mojo_backend import ops
+from torch_mojo_backend.rotary import rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _mojo(mojo):
+    return mojo
+
+
+# ---------------------------------------------------------------------------
+# copies of arguments live until the call
+# ---------------------------------------------------------------------------
+def channels_apart(x):
+    """x's values in a tensor whose last stride is not 1."""
+    return x.transpose(-1, -2).contiguous().to("mojo").transpose(-1, -2)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("which", ["q", "k", "both"])
+def test_rotary_of_channels_apart(dtype, which):
+    f = rotary_frequencies(32, device="cpu").frequencies
+    g = torch.Generator().manual_seed(0)
+    x, y = (torch.randn(2, 4, 90, 64, generator=g).to(dtype) for _ in range(2))
+    pos = torch.arange(90)
+    q = channels_apart(x) if which != "k" else x.to("mojo")
+    k = channels_apart(y) if which != "q" else y.to("mojo")
+    got = ops.rotary_at(q, k, pos.to("mojo"), f.to("mojo"))
+    for name, z, value in (("q", x, got[0]), ("k", y, got[1])):
+        check(value, *logprob_cases.turned(z, pos, f, False, 1.0), name)
+
+
+def test_rotary_of_expanded_gradients():
+    f = rotary_frequencies(32, device="cpu").frequencies
+    pos = torch.arange(90)
+    q, k = (torch.zeros(1, 4, 90, 64).to("mojo").requires_grad_() for _ in range(2))
+    a, b = ops.rotary_at(q, k, pos.to("mojo"), f.to("mojo"))
+    (2 * a.sum() + 3 * b.sum()).backward()
+    for name, value, grad in (("q", 2.0, q.grad), ("k", 3.0, k.grad)):
+        check(grad, *logprob_cases.turned(torch.full((1, 4, 90, 64), value), pos, f, False, 1.0, True), name)

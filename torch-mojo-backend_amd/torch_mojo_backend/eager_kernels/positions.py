@@ -45,12 +45,16 @@ def ready(q, k, positions, frequencies) -> bool:
             and frequencies._dtype is torch.float64 and dtype in _FLOATS and dev == positions._device == frequencies._device)
 
 
+def _channels(t):
+    """t itself when its channels lie side by side, else a copy."""
+    return t if t is None or t._strides[-1] == 1 else materialize_contiguous(t)
+
+
 def _side(t):
-    """(out, its pointer and strides, t's pointer and strides, heads) for t or None."""
+    """(out, its pointer and strides, t's pointer and strides, heads) for t, of
+    channels side by side, or None."""
     if t is None:
         return None, (None, (0, 0, 0), None, (0, 0, 0), 0)
-    if t._strides[-1] != 1:
-        t = materialize_contiguous(t)
     out = alloc_bthd(*t._shape, t._dtype, t._device) if len(t._shape) == 4 else _alloc(t._shape, t._dtype, t._device)
     return out, (out._ptr, _bht(out), t._ptr, _bht(t), t._shape[1])
 
@@ -62,6 +66,7 @@ def rotary(q, k, positions: MT, frequencies: MT, interleaved, scale, inverse):
     if positions._strides and positions._strides[-1] != 1 and positions._shape[-1] > 1:
         positions = materialize_contiguous(positions)
     frequencies = _contig(frequencies)
+    q, k = _channels(q), _channels(k)  # (copies are held until the launch)
     (qo, qa), (ko, ka) = _side(q), _side(k)
     check(
         "mi355x_rope_at",
