@@ -49,3 +49,17 @@ def test_rotary_of_expanded_gradients():
     (2 * a.sum() + 3 * b.sum()).backward()
     for name, value, grad in (("q", 2.0, q.grad), ("k", 3.0, k.grad)):
         check(grad, *logprob_cases.turned(torch.full((1, 4, 90, 64), value), pos, f, False, 1.0, True), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logprobs_of_tokens_apart(dtype):
+    """Tokens in a column of a table."""
+    x, tokens = logprob_cases.logits(300, 50, dtype)
+    pair = torch.stack([tokens, tokens.flip(0)], dim=1).to("mojo")
+    d = torch.linspace(-1, 1, 300)
+    want = logprob_cases.expected(x, tokens, 0, (d, None, None))
+    leaf = x.to("mojo").requires_grad_()
+    got = ops.token_logprobs(leaf, pair[:, 0])
+    check(got.logprobs, *want["logprobs"])
+    got.logprobs.backward(d.to("mojo"))
+    check(leaf.grad, *want["dx"])

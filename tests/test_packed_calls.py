@@ -49,3 +49,21 @@ def test_rotary_of_expanded_gradients(device):
     (2 * a.sum() + 3 * b.sum()).backward()
     for name, value, grad in (("q", 2.0, q.grad), ("k", 3.0, k.grad)):
         check(grad, *logprob_cases.turned(torch.full((1, 4, 90, 64), value), pos, f, False, 1.0, True), name)
+
+
+@pytest.mark.parametrize("entropy", [False, True])
+def test_logprobs_of_tokens_apart(device, monkeypatch, entropy):
+    """Tokens in a column of a table, also by the first call that may raise at a host read."""
+    from torch_mojo_backend.eager_kernels import aten_fast
+
+    x, tokens = logprob_cases.logits(300, 50, F32)
+    pair = torch.stack([tokens, tokens.flip(0)], dim=1).to("mojo")
+    d = torch.linspace(-1, 1, 300)
+    want = logprob_cases.expected(x, tokens, 0, (d, None, None))
+    for flags in (aten_fast._error_flags, {}):
+        monkeypatch.setattr(aten_fast, "_error_flags", flags)
+        leaf = x.to("mojo").requires_grad_()
+        got = ops.token_logprobs(leaf, pair[:, 0], entropy=entropy)
+        check(got.logprobs, *want["logprobs"])
+        got.logprobs.backward(d.to("mojo"))
+        check(leaf.grad, *want["dx"])

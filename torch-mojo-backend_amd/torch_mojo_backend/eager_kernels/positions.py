@@ -101,12 +101,13 @@ def logprobs_forward(x: MT, tokens, top, entropy, ignore_index, keep=False):
     stats = _alloc((n, 2), f32, dev) if keep else None
     ws = library.mi355x_token_logprobs_workspace_bytes(n, c, top, code)
     hold, wptr = _workspace(ws, dev)
+    error = _error_slot(dev, _TARGET_ERROR)  # (the first one allocates)
+    tokens = _contig(tokens) if tokens is not None else None  # (a copy is held until the launch)
     at = lambda t: t._ptr if t is not None else None  # noqa: E731
     check(
         "mi355x_token_logprobs_fwd",
         library.mi355x_token_logprobs_fwd(at(picked), at(spread), at(stats), at(best), at(order), x._ptr, code,
-                                          x._strides[0], at(_contig(tokens)) if tokens is not None else None, n, c, top,
-                                          ignore_index, _error_slot(dev, _TARGET_ERROR), wptr, ws, _STREAM),
+                                          x._strides[0], at(tokens), n, c, top, ignore_index, error, wptr, ws, _STREAM),
     )
     return picked, spread, best, order, stats
 
@@ -127,12 +128,12 @@ def logprobs_backward(x: MT, tokens, stats, spread, order, d_picked, d_spread, d
         return _contig(t) if t._dtype is torch.float32 else materialize_contiguous(t, torch.float32)
 
     d_picked, d_spread, d_best = grad(d_picked), grad(d_spread), grad(d_best)
+    tokens = _contig(tokens) if tokens is not None else None
     at = lambda t: t._ptr if t is not None else None  # noqa: E731
     check(
         "mi355x_token_logprobs_bwd",
         lib().mi355x_token_logprobs_bwd(dx._ptr, ld, x._ptr, _code(x._dtype), x._strides[0], stats._ptr, at(spread),
-                                        at(_contig(tokens)) if tokens is not None else None, at(order),
-                                        order._shape[1] if order is not None else 0, at(d_picked), at(d_spread),
-                                        at(d_best), n, c, ignore_index, _STREAM),
+                                        at(tokens), at(order), order._shape[1] if order is not None else 0,
+                                        at(d_picked), at(d_spread), at(d_best), n, c, ignore_index, _STREAM),
     )
     return dx
