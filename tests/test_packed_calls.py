@@ -5,12 +5,14 @@ import pytest
 import torch
 
 import logprob_cases
+import packed_cases
 import packed_standin  # noqa: F401
 from paged_cases import check
 from torch_mojo_backend import ops
+from torch_mojo_backend.packing import PackedSequences
 from torch_mojo_backend.rotary import rotary_frequencies
 
-F32 = torch.float32
+BF, F32 = torch.bfloat16, torch.float32
 
 
 @pytest.fixture
@@ -67,3 +69,79 @@ def test_logprobs_of_tokens_apart(device, monkeypatch, entropy):
         check(got.logprobs, *want["logprobs"])
         got.logprobs.backward(d.to("mojo"))
         check(leaf.grad, *want["dx"])
+
+
+# ---------------------------------------------------------------------------
+# what a backward keeps is autograd's
+# ---------------------------------------------------------------------------
+def saved_by(call, give=lambda t: t.to("mojo")):
+    """The call's result, and the tensors that a saved-tensor hook sees of it, in
+    whose places the backward gets others of the same values."""
+    seen = []
+
+    def pack(t):
+        seen.append((tuple(t.shape), t.dtype))
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, give):
+        out = call()
+    return out, seen
+
+
+def test_saved_tensors_of_attention(device):
+    at, x = packed_cases.inputs([5, 0, 9], 4, 2, 16, BF, behind=2)
+    seqs = PackedSequences(torch.tensor(at, dtype=torch.int32).to("mojo"), 16)
+    q, k, v = (y.to("mojo").requires_grad_() for y in x[:3])
+    out, seen = saved_by(lambda: ops.packed_attention(q, k, v, seqs))
+    rows, kv = ((16, 4, 16), BF), ((16, 2, 16), BF)
+    assert sorted(seen, key=str) == sorted([rows, kv, kv, rows, ((4, 16), F32), rows], key=str)
+    out.backward(x[3].to("mojo"))
+    want = packed_cases.expected(at, *x)
+    for name, y in (("out", out), ("dq", q.grad), ("dk", k.grad), ("dv", v.grad)):
+        check(y, *want[name], name)
+
+
+def test_saved_tensors_of_logprobs(device):
+    x, tokens = logprob_cases.logits(6, 40, F32)
+    leaf = x.to("mojo").requires_grad_()
+    got, seen = saved_by(lambda: ops.token_logprobs(leaf, tokens.to("mojo"), top=3, entropy=True))
+    assert ((6, 2), F32) in seen and len(seen) == 5
+    ones = [torch.ones(6), torch.ones(6), torch.ones(6, 3)]
+    torch.autograd.backward(got[:3], [y.to("mojo") for y in ones])
+    check(leaf.grad, *logprob_cases.expected(x, tokens, 3, ones)["dx"])
+
+
+def test_saved_tensors_come_back_apart(device):
+    """From a hook that gives back every second element of a wider tensor."""
+    def apart(t):
+        return torch.stack([t, t], dim=-1).to("mojo")[..., 0]
+
+    at, x = packed_cases.inputs([5, 9], 4, 2, 16, BF)
+    seqs = PackedSequences(torch.tensor(at, dtype=torch.int32).to("mojo"), 14)
+    q, k, v = (y.to("mojo").requires_grad_() for y in x[:3])
+    saved_by(lambda: ops.packed_attention(q, k, v, seqs), apart)[0].backward(x[3].to("mojo"))
+    want = packed_cases.expected(at, *x)
+    for name, y in (("dq", q.grad), ("dk", k.grad), ("dv", v.grad)):
+        check(y, *want[name], name)
+    x, tokens = logprob_cases.logits(6, 40, F32)
+    leaf = x.to("mojo").requires_grad_()
+    got, _ = saved_by(lambda: ops.token_logprobs(leaf, tokens.to("mojo"), top=3, entropy=True), apart)
+    ones = [torch.ones(6), torch.ones(6), torch.ones(6, 3)]
+    torch.autograd.backward(got[:3], [y.to("mojo") for y in ones])
+    check(leaf.grad, *logprob_cases.expected(x, tokens, 3, ones)["dx"])
+
+
+def test_nothing_is_kept_behind_a_backward(device):
+    """A loss that a program keeps holds none of what the backward read."""
+    at, x = packed_cases.inputs([5, 9], 2, 2, 16, BF)
+    seqs = PackedSequences(torch.tensor(at, dtype=torch.int32).to("mojo"), 14)
+    out = ops.packed_attention(*(y.to("mojo").requires_grad_() for y in x[:3]), seqs)
+    logits, tokens = logprob_cases.logits(6, 40, F32)
+    lp = ops.token_logprobs(logits.to("mojo").requires_grad_(), tokens.to("mojo")).logprobs
+    for y in (out, lp):
+        node = y.grad_fn
+        y.sum().backward()
+        held = [z for z in vars(node).values() for z in (z if isinstance(z, tuple) else (z,)) if isinstance(z, torch.Tensor)]
+        assert not held, [tuple(z.shape) for z in held]
+        with pytest.raises(RuntimeError, match="second time"):
+            node.saved_tensors

@@ -101,6 +101,8 @@ def attention_backward(grad: MT, q: MT, k: MT, v: MT, out: MT, lse: MT, low, seq
     # (a leaf's gradient is kept, and must not share memory with a cat of it)
     together = q._holder is k._holder is v._holder and not (q.is_leaf or k.is_leaf or v.is_leaf)
     grad, q, k, v = _rows(grad), _rows(q), _rows(k), _rows(v)
+    # (as the forward made them, unless a saved-tensor hook gave back other ones)
+    out, lse, low = _contig(out), _contig(lse), _contig(low) if low is not None else None
     t, h, d = q._shape
     hk, code, library = k._shape[1], _code(q._dtype), lib()
     if together and hk == h:

@@ -128,7 +128,7 @@ def logprobs_backward(x: MT, tokens, stats, spread, order, d_picked, d_spread, d
         return _contig(t) if t._dtype is torch.float32 else materialize_contiguous(t, torch.float32)
 
     d_picked, d_spread, d_best = grad(d_picked), grad(d_spread), grad(d_best)
-    tokens = _contig(tokens) if tokens is not None else None
+    tokens, spread, order, stats = (t if t is None else _contig(t) for t in (tokens, spread, order, stats))
     at = lambda t: t._ptr if t is not None else None  # noqa: E731
     check(
         "mi355x_token_logprobs_bwd",

@@ -119,17 +119,17 @@ class _PackedAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, sequences, window, scale):
         with torch._C._AutoDispatchBelowAutograd():
             out, lse, low = packed.attention_forward(q, k, v, sequences, window, scale, keep_low=True)
-        ctx.save_for_backward(q, k, v, out)
-        ctx.args = (lse, low, sequences, window, scale)  # (lse and low: nobody else's)
+        ctx.save_for_backward(q, k, v, out, lse, low)
+        ctx.args = (sequences, window, scale)
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        q, k, v, out = ctx.saved_tensors
+        q, k, v, out, lse, low = ctx.saved_tensors
         if lazy_live():
-            materialize_touched((grad, q, k, v, out), None, False)
+            materialize_touched((grad, q, k, v, out, lse, low), None, False)
         with torch._C._AutoDispatchBelowAutograd():
-            dq, dk, dv = paged.on_device(q._device, packed.attention_backward, grad, q, k, v, out, *ctx.args)
+            dq, dk, dv = paged.on_device(q._device, packed.attention_backward, grad, q, k, v, out, lse, low, *ctx.args)
         if torch.is_grad_enabled():  # create_graph
             dq, dk, dv = _OneGradient.apply(dq, dk, dv, q, k, v, grad)
         return dq, dk, dv, None, None, None
@@ -143,9 +143,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, x, tokens, top, entropy, ignore_index, leaf):
         with torch._C._AutoDispatchBelowAutograd():
             picked, spread, best, order, stats = positions.logprobs_forward(x, tokens, top, entropy, ignore_index, True)
-        ctx.save_for_backward(x, tokens, spread, order)
+        ctx.save_for_backward(x, tokens, spread, order, stats)
         ctx.args = (ignore_index, leaf)
-        ctx.stats = stats  # (nobody else's)
         ctx.set_materialize_grads(False)
         if order is not None:
             ctx.mark_non_differentiable(order)
@@ -153,14 +152,14 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_picked, d_spread, d_best, _):
-        x, tokens, spread, order = ctx.saved_tensors
+        x, tokens, spread, order, stats = ctx.saved_tensors
         grads = [g for g in (d_picked, d_spread, d_best) if g is not None]
         if not grads:
             return (None,) * 6
         if lazy_live():
-            materialize_touched((x, tokens, *grads), None, False)
+            materialize_touched((x, tokens, spread, order, stats, *grads), None, False)
         with torch._C._AutoDispatchBelowAutograd():
-            dx = paged.on_device(x._device, positions.logprobs_backward, x, tokens, ctx.stats, spread, order, d_picked,
+            dx = paged.on_device(x._device, positions.logprobs_backward, x, tokens, stats, spread, order, d_picked,
                                  d_spread, d_best, *ctx.args)
         if torch.is_grad_enabled():  # create_graph
             dx = _OnceOnly.apply("token_logprobs", dx, x, *grads)
