@@ -145,3 +145,45 @@ def test_nothing_is_kept_behind_a_backward(device):
         assert not held, [tuple(z.shape) for z in held]
         with pytest.raises(RuntimeError, match="second time"):
             node.saved_tensors
+
+
+# ---------------------------------------------------------------------------
+# tangents
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(device, grad):
+    """No operator has a forward-mode derivative: a dual tensor is refused, not taken as a constant."""
+    from torch.autograd import forward_ad as fwd
+
+    at, x = packed_cases.inputs([5, 9], 2, 2, 16, F32)
+    seqs = PackedSequences(torch.tensor(at, dtype=torch.int32).to("mojo"), 14)
+    q, k, v, t = (y.to("mojo") for y in x)
+    logits, tokens = (y.to("mojo") for y in logprob_cases.logits(14, 32, F32))
+    f, pos = rotary_frequencies(16, device="cpu").frequencies.to("mojo"), seqs.positions
+    if grad:
+        for y in (q, k, v, logits):
+            y.requires_grad_()
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, t)
+        wide = fwd.make_dual(logits, t.reshape(14, 32))
+        for call in (
+            lambda: ops.packed_attention(dual, k, v, seqs),
+            lambda: ops.packed_attention(q, dual, v, seqs, window=3, scale=0.5),
+            lambda: ops.packed_attention(q, k, dual, seqs),
+            lambda: ops.rotary_at(dual, k, pos, f),
+            lambda: ops.rotary_at(q, dual, pos, f, scale=2),
+            lambda: ops.rotary_at(None, dual, pos, f),
+            lambda: ops.token_logprobs(wide, tokens),
+            lambda: ops.token_logprobs(wide.view(2, 7, 32), top=2),
+        ):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        if grad:  # nor have the backward passes
+            lp = ops.token_logprobs(logits, tokens).logprobs
+            for out, at, g in ((ops.packed_attention(q, k, v, seqs), q, t), (ops.rotary_at(q, None, pos, f)[0], q, t),
+                               (lp, logits, t[:, 0, 0])):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    torch.autograd.grad(out, at, fwd.make_dual(g.clone(), g.clone()))
+        assert ops.packed_attention(q, k, v, seqs).shape == (14, 2, 16)  # none of its inputs has a tangent
+        assert ops.rotary_at(q, k, pos, f)[0].shape == q.shape
+    assert ops.token_logprobs(logits, tokens).logprobs.shape == (14,)

@@ -11,6 +11,7 @@ allocated here and launches go to the null stream, that of the tensors' device.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import PagedCache, check, lazy_live, materialize_touched
 from . import native_lib as lib
@@ -70,6 +71,13 @@ def on_device(device: int, call, *args):
         with torch.cuda.device(device):
             return call(*args)
     return call(*args)
+
+
+def no_tangents(what, *ts) -> None:
+    """Refuses dual tensors: the kernels have no forward-mode derivative, and would
+    take them as constants."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not supported")
 
 
 def _rows(t: MT, written=()) -> MT:

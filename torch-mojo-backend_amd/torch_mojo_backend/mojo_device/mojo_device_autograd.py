@@ -126,6 +126,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         q, k, v, out, lse, low = ctx.saved_tensors
+        paged.no_tangents("packed_attention", grad)
         if lazy_live():
             materialize_touched((grad, q, k, v, out, lse, low), None, False)
         with torch._C._AutoDispatchBelowAutograd():
@@ -156,6 +157,7 @@ class _TokenLogprobs(torch.autograd.Function):
         grads = [g for g in (d_picked, d_spread, d_best) if g is not None]
         if not grads:
             return (None,) * 6
+        paged.no_tangents("token_logprobs", *grads)
         if lazy_live():
             materialize_touched((x, tokens, spread, order, stats, *grads), None, False)
         with torch._C._AutoDispatchBelowAutograd():

@@ -167,6 +167,7 @@ class _RotaryAt(torch.autograd.Function):
         positions, frequencies = ctx.saved_tensors
         interleaved, scale, inverse = ctx.args
         given = [g for g in (dq, dk) if g is not None]
+        paged.no_tangents("rotary_at", *given)
         if lazy_live():
             materialize_touched((*given, positions, frequencies), None, False)
         turn = _RotaryAt.apply if _needs_grad(*given) else _positions.rotary
@@ -223,6 +224,7 @@ def rotary_at(q, k, positions, frequencies, *, interleaved=False, scale=1.0):
 
 
 def _rotary_at(q, k, positions, frequencies, interleaved, scale):
+    paged.no_tangents("rotary_at", q, k)
     if lazy_live():
         materialize_touched((q, k, positions, frequencies), None, False)
     turn = _RotaryAt.apply if _needs_grad(q, k) else _positions.rotary
@@ -276,6 +278,7 @@ def packed_attention(q, k, v, sequences, *, window=0, scale=None):
 
 
 def _packed_attention(q, k, v, sequences, window, scale):
+    paged.no_tangents("packed_attention", q, k, v)
     if not _needs_grad(q, k, v):
         return packed.attention(q, k, v, sequences, window, scale)
     from .mojo_device.mojo_device_autograd import _PackedAttention
@@ -327,6 +330,7 @@ def token_logprobs(logits, tokens=None, *, top=0, entropy=False, ignore_index=-1
 
 
 def _token_logprobs(x, tokens, top, entropy, ignore_index, logits):
+    paged.no_tangents("token_logprobs", x)
     if lazy_live():
         materialize_touched((x, tokens), None, False)
     if not _needs_grad(x):
