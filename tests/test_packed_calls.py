@@ -4,6 +4,7 @@ arguments have to be copied first, or that autograd has to know of, off the GPU.
 import pytest
 import torch
 
+import decode_cases
 import logprob_cases
 import packed_cases
 import packed_standin  # noqa: F401
@@ -187,3 +188,17 @@ def test_tangents_are_refused(device, grad):
         assert ops.packed_attention(q, k, v, seqs).shape == (14, 2, 16)  # none of its inputs has a tangent
         assert ops.rotary_at(q, k, pos, f)[0].shape == q.shape
     assert ops.token_logprobs(logits, tokens).logprobs.shape == (14,)
+
+
+# ---------------------------------------------------------------------------
+# a model that has answered before it trains
+# ---------------------------------------------------------------------------
+def test_training_after_inference(device):
+    m, ref = decode_cases.model(F32, "mojo", sinks=0)
+    idx = torch.randint(0, 97, (12,), generator=torch.Generator().manual_seed(2)).to("mojo")
+    with torch.inference_mode():
+        m.forward_packed(idx, PackedSequences.of_lengths([5, 7]))
+    m.score_packed(idx, PackedSequences.of_lengths([5, 7])).logprobs.sum().backward()
+    ref.score_packed(idx.cpu(), PackedSequences.of_lengths([5, 7], device="cpu")).logprobs.sum().backward()
+    for (name, p), r in zip(m.named_parameters(), ref.parameters()):
+        check(p.grad, r.grad.numpy(), 2e-5 * max(1.0, r.grad.abs().max().item()) + 0 * r.grad.numpy(), name)

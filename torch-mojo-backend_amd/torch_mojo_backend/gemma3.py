@@ -236,8 +236,9 @@ class Gemma3(nn.Module):
         dev, dt = idx.device, self.embed.weight.dtype
         frequencies = self._frequencies.get(str(dev))
         if frequencies is None:
-            frequencies = tuple(rotary_frequencies(c.head_dim, base, scaling="linear", factor=factor, device=dev).frequencies
-                                for base, factor in ((c.rope_local_base, 1.0), (c.rope_global_base, c.rope_global_factor)))
+            with torch.inference_mode(False):  # (a training step may be the next to use them)
+                frequencies = tuple(rotary_frequencies(c.head_dim, base, scaling="linear", factor=factor, device=dev).frequencies
+                                    for base, factor in ((c.rope_local_base, 1.0), (c.rope_global_base, c.rope_global_factor)))
             self._frequencies = {str(dev): frequencies}
         x = self.embed(idx) * torch.tensor(c.hidden ** 0.5, dtype=dt, device=dev)
         for blk in self.blocks:
