@@ -202,3 +202,27 @@ def test_training_after_inference(device):
     ref.score_packed(idx.cpu(), PackedSequences.of_lengths([5, 7], device="cpu")).logprobs.sum().backward()
     for (name, p), r in zip(m.named_parameters(), ref.parameters()):
         check(p.grad, r.grad.numpy(), 2e-5 * max(1.0, r.grad.abs().max().item()) + 0 * r.grad.numpy(), name)
+
+
+@pytest.mark.parametrize("at,tokens", [([0], 0), ([3], 5), ([0, 0, 0], 0)])
+@pytest.mark.parametrize("where", ["cpu", "mojo"])
+def test_gradients_of_no_rows(device, where, at, tokens):
+    """Zeros for each of q, k and v, whichever of them takes one."""
+    seqs = PackedSequences(torch.tensor(at, dtype=torch.int32).to(where), tokens)
+    for some in ((0, 1, 2), (1,), (2,)):
+        x = [torch.full((tokens, h, 16), float("nan")).to(where) for h in (4, 2, 2)]
+        for i in some:
+            x[i].requires_grad_()
+        out = ops.packed_attention(*x, seqs)
+        out.sum().backward()
+        assert out.shape == (tokens, 4, 16) and not out.detach().cpu().any()
+        for i in some:
+            assert x[i].grad.shape == x[i].shape and not x[i].grad.cpu().any()
+
+
+def test_no_channels(device):
+    for where in ("cpu", "mojo"):
+        q, k = torch.zeros(5, 4, 0).to(where), torch.zeros(5, 2, 0).to(where).requires_grad_()
+        out = ops.packed_attention(q, k, k, PackedSequences.of_lengths([5], device=where))
+        out.sum().backward()
+        assert out.shape == q.shape and k.grad.shape == k.shape

@@ -268,7 +268,7 @@ def packed_attention(q, k, v, sequences, *, window=0, scale=None):
             raise ValueError(f"{what}: scale {scale} must be finite in 32 bits")
     window = min(window, sequences.tokens)
     if not q.numel():
-        return q * 1.0
+        return packing.nothing_of(q, k, v)
     if not sequences.on_mojo:
         return packing.attention_plain(q, k, v, sequences, window, scale)
     if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or q.shape[2] > 256 or q.shape[2] % 8:

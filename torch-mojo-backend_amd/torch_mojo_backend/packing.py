@@ -83,12 +83,17 @@ class PackedSequences:
         return torch.cat([behind, torch.full_like(tokens[:1], ignore_index)])
 
 
+def nothing_of(q, k, v):
+    """The result of empty q, k and v, whose gradients are there all the same."""
+    return q + (k.sum() + v.sum())
+
+
 def attention_plain(q, k, v, sequences, window, scale):
     """The plain formula of `ops.packed_attention`, in 32 bits at least."""
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
     wide = torch.promote_types(q.dtype, torch.float32)
     at, group = sequences._offsets, q.shape[1] // k.shape[1]
-    parts = [q[:0], torch.zeros_like(q[:at[0]])]
+    parts = [nothing_of(q[:0], k[:0], v[:0]), torch.zeros_like(q[:at[0]])]
     for a, b in itertools.pairwise(at):
         if a == b:
             continue
