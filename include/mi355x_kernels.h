@@ -755,9 +755,13 @@ int mi355x_packed_attn_fwd(void* o, const int64_t* o_th, void* o_low, float* lse
                            int dtype, mi355x_stream_t stream);
 /* dQ, dK, dV (written, zero in padding); those of a K/V head are the sums over
  * its query heads, in head order.  The workspace holds two floats a query row
- * and, where a group's heads are shared out, f32 partials of dK and dV. */
+ * and, where a group's heads are shared out, f32 partials of dK and dV: in f32
+ * always, in 16 bits where there are few blocks without.  The first is enough
+ * for any type, the second is what one needs. */
 int64_t mi355x_packed_attn_bwd_workspace_bytes(int64_t sequences, int64_t tokens, int64_t heads,
                                                int64_t kv_heads, int64_t d);
+int64_t mi355x_packed_attn_bwd_workspace_bytes_for(int64_t sequences, int64_t tokens, int64_t heads,
+                                                   int64_t kv_heads, int64_t d, int dtype);
 int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, const int64_t* dk_th, void* dv,
                            const int64_t* dv_th, const void* dout, const int64_t* do_th, const void* q,
                            const int64_t* q_th, const void* k, const int64_t* k_th, const void* v,

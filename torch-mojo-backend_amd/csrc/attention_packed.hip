@@ -963,18 +963,24 @@ extern "C" int mi355x_packed_attn_fwd(void* o, const int64_t* o_th, void* o_low,
 }
 
 // Whether a K/V head's query heads go to blocks of their own, whose partials are
-// added after them: below two blocks a CU, where one for all of a group would
-// leave CUs idle (bf16 forward and backward, one block a group against one a
-// head: 16384 rows in 16 sequences, 32 over 2 heads of 64 684 and 584 us; 8192 rows
-// in 4, 32 over 8 of 128 747 and 844; 16384 in 4, 16 over 4 of 256 3533 and 3740).
-static bool splits_group(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d) {
-  return heads > kv_heads && (tokens / kPackedRows[d > 192] + 1) * kv_heads < 512;
+// added after them.  In f32 always; in 16 bits below two blocks a CU, where one for
+// all of a group would leave CUs idle (bf16 forward and backward, one block a group
+// against one a head: 16384 rows in 16 sequences, 32 over 2 heads of 64 684 and 584
+// us; 8192 rows in 4, 32 over 8 of 128 747 and 844; 16384 in 4, 16 over 4 of 256
+// 3533 and 3740).
+static bool splits_group(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int dtype) {
+  return heads > kv_heads && (dtype == MI355X_F32 || (tokens / kPackedRows[d > 192] + 1) * kv_heads < 512);
+}
+
+extern "C" int64_t mi355x_packed_attn_bwd_workspace_bytes_for(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                              int64_t d, int dtype) {
+  const int64_t terms = 2 * heads * tokens * (int64_t)sizeof(float) + 512;
+  return splits_group(tokens, heads, kv_heads, d, dtype) ? terms + 2 * heads * tokens * layout_of(d) * (int64_t)sizeof(float) : terms;
 }
 
 extern "C" int64_t mi355x_packed_attn_bwd_workspace_bytes(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                           int64_t d) {
-  const int64_t terms = 2 * heads * tokens * (int64_t)sizeof(float) + 512;
-  return heads > kv_heads ? terms + 2 * heads * tokens * layout_of(d) * (int64_t)sizeof(float) : terms;
+  return mi355x_packed_attn_bwd_workspace_bytes_for(sequences, tokens, heads, kv_heads, d, MI355X_F32);
 }
 
 extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, const int64_t* dk_th, void* dv,
@@ -993,7 +999,7 @@ extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, 
   MI_REQUIRE(wide(o, o_th, es) && wide(q, q_th, es) && wide(k, k_th, es) && wide(v, v_th, es) && wide(dout, do_th, es) &&
                  wide(dq, dq_th, es) && wide(dk, dk_th, es) && wide(dv, dv_th, es) && (uintptr_t)o_low % 16 == 0,
              "%s: rows must be 16-byte aligned, less than 64 MB apart", what);
-  const int64_t need = mi355x_packed_attn_bwd_workspace_bytes(sequences, tokens, heads, kv_heads, d);
+  const int64_t need = mi355x_packed_attn_bwd_workspace_bytes_for(sequences, tokens, heads, kv_heads, d, dtype);
   if (!workspace || ws_bytes < need)
     return fail(MI355X_EWORKSPACE, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
   PackedArgs a{};
@@ -1006,7 +1012,7 @@ extern "C" int mi355x_packed_attn_bwd(void* dq, const int64_t* dq_th, void* dk, 
   set_scale(a, scale);
   a.ndelta = (float*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);
   a.nlse2 = a.ndelta + heads * tokens;
-  if (dtype == MI355X_F32 ? heads > kv_heads : splits_group(tokens, heads, kv_heads, d))
+  if (splits_group(tokens, heads, kv_heads, d, dtype))
     a.kv_part = (float*)(((uintptr_t)(a.nlse2 + heads * tokens) + 255) & ~(uintptr_t)255);
   const Launch l{sequences, tokens, (hipStream_t)stream};
   if (dtype == MI355X_F32) {

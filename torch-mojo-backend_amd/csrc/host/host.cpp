@@ -188,7 +188,8 @@ struct Call<R (*)(A...), Tag> {
   X(mi355x_attn_fwd_sink) X(mi355x_attn_bwd_sink_workspace_bytes) X(mi355x_attn_bwd_sink)                \
   X(mi355x_paged_append) X(mi355x_paged_gather) X(mi355x_paged_attn_workspace_bytes) X(mi355x_paged_attn) \
   X(mi355x_packed_plan_bytes) X(mi355x_packed_plan) X(mi355x_packed_attn_fwd)                            \
-  X(mi355x_packed_attn_bwd_workspace_bytes) X(mi355x_packed_attn_bwd) X(mi355x_rope_at)                  \
+  X(mi355x_packed_attn_bwd_workspace_bytes) X(mi355x_packed_attn_bwd_workspace_bytes_for)                \
+  X(mi355x_packed_attn_bwd) X(mi355x_rope_at)                                                            \
   X(mi355x_token_logprobs_workspace_bytes) X(mi355x_token_logprobs_fwd) X(mi355x_token_logprobs_bwd)
 
 #define TAG(f)                                         \

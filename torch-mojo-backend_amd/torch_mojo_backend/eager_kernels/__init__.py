@@ -355,6 +355,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ],
     ),
     "mi355x_packed_attn_bwd_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "mi355x_packed_attn_bwd_workspace_bytes_for": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_int]),
     "mi355x_packed_attn_bwd": (
         c_int,
         [

@@ -113,7 +113,10 @@ def attention_backward(grad: MT, q: MT, k: MT, v: MT, out: MT, lse: MT, low, seq
         _mark_cat_ready(rows)
     else:
         dq, dk, dv = (_alloc(x._shape, q._dtype, q._device) for x in (q, k, v))
-    ws = library.mi355x_packed_attn_bwd_workspace_bytes(sequences.count, t, h, hk, d)
+    if hk < h and q._dtype is not torch.float32:
+        ws = library.mi355x_packed_attn_bwd_workspace_bytes_for(sequences.count, t, h, hk, d, code)
+    else:  # (the most of any type)
+        ws = library.mi355x_packed_attn_bwd_workspace_bytes(sequences.count, t, h, hk, d)
     hold, wptr = _workspace(ws, q._device)
     check(
         "mi355x_packed_attn_bwd",
