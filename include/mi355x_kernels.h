@@ -786,7 +786,7 @@ int mi355x_rope_at(void* q_out, const int64_t* qo_bht, const void* q, const int6
                    int interleaved, double scale, int inverse, int dtype, mi355x_stream_t stream);
 
 /* ---- log-probabilities of given tokens ----------------------------------
- * Of each row of logits [n][c] (rows at logits + i * ld): logprobs[i] =
+ * Of each row of logits [n][c] (rows at logits + i * ld, c < 2^31 - 2^14): logprobs[i] =
  * log_softmax(row)[tokens[i]] (0 where tokens[i] is ignore_index; a token outside
  * [0, c) sets *error, which may be null, and gives 0), entropy[i] = -sum p log p,
  * and the `top` (up to 64) largest entries, NaN first and equal ones by index:

@@ -4,7 +4,7 @@ take sizes of their own: made on the host, before any launch (no GPU)."""
 import pytest
 
 from test_library import raw  # noqa: F401  (the fixture)
-from test_packed_abi import BF16, EWORKSPACE, F16, F32, backward, lib, th  # noqa: F401
+from test_packed_abi import BF16, EINVAL, EWORKSPACE, F16, F32, backward, gradient, lib, logprobs, th  # noqa: F401
 
 TERMS = 2 * 4  # bytes a row and query head: two floats
 
@@ -26,3 +26,13 @@ def test_backward_workspace(lib, dtype, tokens, h, hk, d, split):  # noqa: F811
     s = th(h * d, d)
     over = dict(tokens=tokens, heads=h, kv_heads=hk, d=d, dtype=dtype, **dict.fromkeys(("dqt", "dkt", "dvt", "dot", "qt", "kt", "vt", "ot"), s))
     assert backward(lib, wsb=need - 1, **over) == EWORKSPACE
+
+
+def test_logprobs_of_the_largest_vocabularies(lib):  # noqa: F811
+    """A row's walk counts elements in 32 bits, up to a batch past its end."""
+    most = 2 ** 31 - 2 ** 14
+    for c in (most, 2 ** 31 - 1):
+        assert logprobs(lib, n=600, c=c, ld=0, top=0, tt=None, tlp=None) == EINVAL
+        assert gradient(lib, n=600, c=c, ld=0, ld_dx=c, top=0) == EINVAL
+        assert lib.mi355x_token_logprobs_workspace_bytes(600, c, 0, BF16) == -1
+    assert lib.mi355x_token_logprobs_workspace_bytes(600, most - 1, 0, BF16) == 0

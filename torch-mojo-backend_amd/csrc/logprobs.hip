@@ -666,7 +666,8 @@ int lp_bwd_launch(LpBwd a, hipStream_t s) {
 }
 
 int lp_check(const char* what, int64_t n, int64_t c, int64_t ld, int top, int dtype) {
-  MI_REQUIRE(n >= 0 && c > 0 && c < (1ll << 31), "%s: %lld rows of %lld columns", what, (long long)n, (long long)c);
+  // (a walk's 32-bit places go a batch past a row's end: lp_stream's 1024 chunks of 8)
+  MI_REQUIRE(n >= 0 && c > 0 && c < (1ll << 31) - (1 << 14), "%s: %lld rows of %lld columns", what, (long long)n, (long long)c);
   MI_REQUIRE(n < (1ll << 23), "%s: %lld rows", what, (long long)n);
   MI_REQUIRE(ld >= 0 && top >= 0 && top <= c, "%s: stride %lld, %d top entries", what, (long long)ld, top);
   if (top > kMostTop) return fail(MI355X_EUNSUPPORTED, "%s: %d top entries (up to %d)", what, top, kMostTop);
