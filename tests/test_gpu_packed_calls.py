@@ -5,8 +5,10 @@ import pytest
 import torch
 
 import logprob_cases
+import packed_cases
 from paged_cases import check
 from torch_mojo_backend import ops
+from torch_mojo_backend.packing import PackedSequences
 from torch_mojo_backend.rotary import rotary_frequencies
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +65,20 @@ def test_logprobs_of_tokens_apart(dtype):
     check(got.logprobs, *want["logprobs"])
     got.logprobs.backward(d.to("mojo"))
     check(leaf.grad, *want["dx"])
+
+
+# ---------------------------------------------------------------------------
+# sequences and windows of up to 64 rows, whose backward has bodies of its own
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,d,h,hk", [(BF, 128, 4, 2), (HF, 128, 2, 2), (HF, 120, 2, 1), (HF, 96, 2, 1), (BF, 80, 2, 2), (HF, 64, 2, 1)])
+@pytest.mark.parametrize("lengths,window", [([5, 0, 40], 0), ([1], 0), ([300, 64, 1, 65], 64), ([300, 64, 1, 65], 65), ([2] * 20 + [200], 0),
+                                            ([64, 65, 63], 0)])
+def test_short_and_long_tiles(dtype, d, h, hk, lengths, window):
+    """All tiles of one kind or of both, with rows of no sequence around them."""
+    at, x = packed_cases.inputs(lengths, h, hk, d, dtype, before=3, behind=9, junk=float("nan"))
+    q, k, v = (y.to("mojo").requires_grad_() for y in x[:3])
+    out = ops.packed_attention(q, k, v, PackedSequences(torch.tensor(at, dtype=torch.int32).to("mojo"), x[0].shape[0]), window=window)
+    out.backward(x[3].to("mojo"))
+    want = packed_cases.expected(at, *x, window)
+    for name, y in (("out", out), ("dq", q.grad), ("dk", k.grad), ("dv", v.grad)):
+        check(y, *want[name], name)

@@ -57,6 +57,7 @@ struct PackedArgs {
   const PackedTile* tiles[2];  // of 128 and of 64 rows
   int tokens, heads, kv_heads, d;
   int window;          // 0: none
+  bool all_fine;       // whether the call can have no other tiles than fine ones (the backward, below)
   float c, sign, scale;  // |scale| log2(e), scale's sign
   float *ndelta, *nlse2;  // [heads][tokens]: -D, -LSE log2(e)
   float* kv_part;      // dK and then dV of each query head [group][kv_heads][tokens][D] (f32), or null
@@ -409,7 +410,12 @@ constexpr int kQueryTiles = 2;
 // in sequences of 2 to 9 rows.  In longer ones it is 1.45 times, and the product a
 // quarter of the queries' pass.  In a body of its own, and at 128 channels the keys
 // in a launch of their own: in one kernel their loop took 1.09 times as long (1397
-// us where it takes 1280), in one body 1.15.
+// us where it takes 1280), in one body 1.15.  Where both bodies share a kernel of two
+// waves a SIMD (96 channels, and the queries at 128) the fine one's halves of a step
+// are a loop: unrolled they spilled 6 to 11 registers of f16 (and 8 of bf16 at 72 to
+// 88 channels); 300 sequences of 55 rows, 32 over 8 heads of 128, f16: queries 147 us,
+// unrolled 163 (the keys, which have the registers, 154 and as a loop 163).  A
+// launch of the fine queries with the fine keys, one wave a SIMD, took 398 us for both.
 constexpr int kFine = 64;
 __device__ __forceinline__ bool is_fine(const PackedArgs& p, const PackedTile& t) {
   return t.len <= kFine || (p.window > 0 && p.window <= kFine);
@@ -498,7 +504,7 @@ __device__ __forceinline__ void dkv_body(const PackedArgs& p, const PackedTile& 
         lo[u] = max(0, kq + kr);
         span[u] = kw + kr < len ? max(0, min(len - qb0, min(64, kq + kr + window)) - lo[u]) : 0;
       }
-#pragma unroll
+#pragma unroll (FINE && W == 96 ? 1 : 2)
     for (int qs = 0; qs < 2; ++qs) {
       if (MASK && (qs * 32 + 31 < kq || qs * 32 >= kq + KW - 1 + window || qb0 + qs * 32 >= len)) continue;
       frag pb[RT], sb[RT], sl[FINE ? RT : 1];
@@ -652,7 +658,7 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
       lim[u] = qw + qr < len ? qk + qr + 1 : 0;
       lo[u] = qk + qr - window + 1;
     }
-#pragma unroll
+#pragma unroll (FINE && (W == 96 || W == 128) ? 1 : 2)
     for (int ks2 = 0; ks2 < 2; ++ks2) {
       if (MASK && (ks2 * 32 > qk + QW - 1 || ks2 * 32 + 31 < qk - window + 1)) continue;
       frag sb[RT], sl[FINE ? RT : 1];
@@ -726,8 +732,9 @@ __device__ __forceinline__ void dq_body(const PackedArgs& p, const PackedTile& t
 // KIND 0, both in one launch: the first nkv blocks take keys, one of a K/V
 // head's or, where their gradients go through partials, one of a query head's;
 // the rest take queries.  1: keys alone, but for FINE tiles, which 3 takes (4.8 us
-// where there are none), 2: queries alone.  At head_dim 128 the keys' blocks need 380 registers, a wave a SIMD, and the queries' 248, two; in
-// one launch both run at the first ([16384 rows, 32 over 8, 128] in 4 sequences:
+// where there are none; 1 is left out where the call can have no others), 2: queries
+// alone.  At head_dim 128 the keys' blocks need 381 registers, a wave a SIMD, and
+// the queries' 251, two; in one launch both run at the first ([16384 rows, 32 over 8, 128] in 4 sequences:
 // 2370 us, 1335 + 774 in two).  Four tiles of keys a wave, two waves a block,
 // spill (4.9 ms, 39 registers of 512 short with the sums pinned in AGPRs); four of
 // queries take 960.  At 64 and 96 both run at two in one launch (96 channels
@@ -739,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, W <= 96 || (W == 128 && KIND == 2) ?
   const int group = p.heads / p.kv_heads;
   if (KIND % 2 || (KIND == 0 && blockIdx.x < nkv)) {
     const PackedAt at = packed_at(p.tiles[kKeyList<W>], p.head->count[kKeyList<W>], blockIdx.x, p.kv_part ? p.heads : p.kv_heads, p.kv_heads);
-    if (!at.live || (KIND == 3 && at.t.tile < 0)) return;
+    if (!at.live || (KIND == 3 && at.t.tile < 0 && !p.all_fine)) return;
     const int g = p.kv_part ? at.h - at.hk * group : 0;
     if (at.t.tile < 0) {
       if (g == 0) zero_rows<T>(p.dk, at.t, at.hk, p.d), zero_rows<T>(p.dv, at.t, at.hk, p.d);
@@ -849,7 +856,7 @@ template <int D>
 constexpr int kBwdLds = 2 * (2 * KvLayout<D>::TILE + 512);
 
 template <typename T, int W, bool RAG>
-int bwd_launch(const PackedArgs& a, const Launch& l) {
+int bwd_launch(PackedArgs a, const Launch& l) {
   constexpr int D = kLayout<W>;
   constexpr bool SPLIT = W == 128;
   auto k0 = packed_bwd<T, W, RAG, SPLIT ? 1 : 0>, k1 = packed_bwd<T, W, RAG, SPLIT ? 2 : 0>, k2 = packed_bwd<T, W, RAG, SPLIT ? 3 : 0>;
@@ -862,9 +869,10 @@ int bwd_launch(const PackedArgs& a, const Launch& l) {
   const int64_t rows = (int64_t)a.heads * a.tokens;
   MI_REQUIRE((nkv + nq) * kThreads < kMostThreads && rows * (D / 4) < kMostThreads - kThreads,
              "mi355x_packed_attn_bwd: too many rows and heads");
+  a.all_fine = a.tokens <= kFine || (a.window > 0 && a.window <= kFine);
   packed_delta<T, D><<<ceil_div(rows, kThreads / (D / 8)), kThreads, 0, l.s>>>(a);
   if (SPLIT) {
-    k0<<<(unsigned)nkv, kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
+    if (!a.all_fine) k0<<<(unsigned)nkv, kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
     k2<<<(unsigned)nkv, kThreads, kBwdLds<D>, l.s>>>(a, (uint32_t)nkv);
     k1<<<(unsigned)nq, kThreads, kBwdLds<D>, l.s>>>(a, 0);
   } else {
