@@ -19,7 +19,9 @@
 // 192 and 256 channels, with rows of D = 64, 128 or 256 in LDS; a head_dim between
 // two runs those of the next (RAG), with zeros in the channels past it.
 // P and dS are rounded to the type for their products, half a step each; what
-// rounding takes from a 16-bit O is kept (o_low) and D taken from both.
+// rounding takes from a 16-bit O is kept (o_low) and D taken from both.  LSE is that
+// of the rounded P, by whose sum O is divided, so that the backward's P carries its
+// rounding and its own.
 //
 // What bounds them: at 128 channels the matrix units, at the rate of a large matrix
 // product (16384 rows in 4 sequences, 32 over 8 heads, bf16: forward 622 us, 1015

@@ -321,7 +321,7 @@ __global__ void __launch_bounds__((LpShape<T, NW, CPT>::kThreads)) lp_rows(LpArg
 // the end; that holds for the finite x below kNear, and -inf makes 2^f f a NaN.  A
 // wave that meets anything else takes its batch again, and those that follow,
 // with f as it is defined, an exponent of -200 for all below it (8192 x 50257
-// bf16, 0.82 GB, 160 us with that for all, 149 so, 5.5 TB/s).
+// bf16, 0.82 GB, 192 us with that for all, 176 so, 4.7 TB/s).
 constexpr int kStreamThreads = 256;
 constexpr float kNear = 32768.f;
 // What fills a row's last chunk: 2^f of it is 0 for every m below kNear.
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kBwdThreads) lp_bwd(LpBwd p) {
 // not, where there are enough rows to fill the 256 CUs; else into segments of 8 KB
 // and more for 512 blocks in all, of which the join takes kJoinList keys (one
 // bf16 row of 262144, 20 top entries: 9.8 us and 5.8 to join 64 segments, 11.4 and
-// 4.8 of 32, 8.5 and 8.3 of 128).  Rows of 8192 x 50257 bf16 stream in 149 us; held
+// 4.8 of 32, 8.5 and 8.3 of 128).  Rows of 8192 x 50257 bf16 stream in 176 us; held
 // in registers they took 239, in blocks of 16 waves 346.
 struct LpPlan {
   int waves;      // of a segment: 1, 4 or 8; 0: lp_stream's block
