@@ -82,3 +82,64 @@ def test_short_and_long_tiles(dtype, d, h, hk, lengths, window):
     want = packed_cases.expected(at, *x, window)
     for name, y in (("out", out), ("dq", q.grad), ("dk", k.grad), ("dv", v.grad)):
         check(y, *want[name], name)
+
+
+# ---------------------------------------------------------------------------
+# what autograd sees
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [HF, F32])
+def test_saved_tensors_through_a_hook(dtype):
+    """From copies on the host, given back dense or every second element of a wider tensor."""
+    at, x = packed_cases.inputs([70, 0, 9], 4, 2, 64, dtype, behind=2)
+    want = packed_cases.expected(at, *x)
+    logits, tokens = logprob_cases.logits(6, 400, dtype)
+    ones = [torch.ones(6), torch.ones(6), torch.ones(6, 3)]
+    dx = logprob_cases.expected(logits, tokens, 3, ones)["dx"]
+    seqs = PackedSequences(torch.tensor(at, dtype=torch.int32).to("mojo"), x[0].shape[0])
+    for give in (lambda t: t.to("mojo"), lambda t: torch.stack([t, t], dim=-1).to("mojo")[..., 0]):
+        q, k, v = (y.to("mojo").requires_grad_() for y in x[:3])
+        leaf = logits.to("mojo").requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), give):
+            out = ops.packed_attention(q, k, v, seqs)
+            got = ops.token_logprobs(leaf, tokens.to("mojo"), top=3, entropy=True)
+        out.backward(x[3].to("mojo"))
+        for name, y in (("out", out), ("dq", q.grad), ("dk", k.grad), ("dv", v.grad)):
+            check(y, *want[name], name)
+        torch.autograd.backward(got[:3], [y.to("mojo") for y in ones])
+        check(leaf.grad, *dx, "dx")
+
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad as fwd
+
+    f = rotary_frequencies(64, device="cpu").frequencies.to("mojo")
+    x = torch.randn(9, 2, 64).to("mojo")
+    seqs = PackedSequences.of_lengths([5, 4])
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, x.clone())
+        for call in (lambda: ops.packed_attention(x, dual, x, seqs), lambda: ops.rotary_at(dual, None, seqs.positions, f),
+                     lambda: ops.token_logprobs(dual, entropy=True)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+def test_gradients_of_no_rows():
+    seqs = PackedSequences.of_lengths([0, 0])
+    q, k, v = (torch.zeros(0, h, 64).to("mojo").requires_grad_() for h in (4, 2, 2))
+    ops.packed_attention(q, k, v, seqs).sum().backward()
+    assert [tuple(y.grad.shape) for y in (q, k, v)] == [(0, 4, 64), (0, 2, 64), (0, 2, 64)]
+
+
+def test_workspace_of_an_unsplit_backward():
+    """A grouped backward without partials takes no more memory than its results and row terms."""
+    t, h, hk, d = 8192, 32, 8, 128
+    x = [torch.zeros(t, n, d, dtype=BF).to("mojo").requires_grad_() for n in (h, hk, hk)]
+    dy = torch.zeros(t, h, d, dtype=BF).to("mojo")
+    out = ops.packed_attention(*x, PackedSequences.of_lengths([t]))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out.backward(dy)
+    torch.cuda.synchronize()
+    results, terms = 2 * t * (h + 2 * hk) * d, 2 * 4 * t * h
+    assert results <= torch.cuda.max_memory_allocated() - before <= results + terms + (4 << 20)  # (blocks of 2 MB)
