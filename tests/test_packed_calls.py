@@ -75,6 +75,15 @@ def test_logprobs_of_tokens_apart(device, monkeypatch, entropy):
         check(leaf.grad, *want["dx"])
 
 
+def test_cross_entropy_of_targets_apart(device):
+    x, tokens = logprob_cases.logits(300, 50, F32)
+    pair = torch.stack([tokens, tokens.flip(0)], dim=1)
+    want, leaf = (y.requires_grad_() for y in (x.clone(), x.to("mojo")))
+    for y, t in ((want, pair), (leaf, pair.to("mojo"))):
+        torch.nn.functional.cross_entropy(y, t[:, 0], reduction="none").sum().backward()
+    assert torch.allclose(leaf.grad.cpu(), want.grad, rtol=0, atol=1e-6)  # (both f32, of values up to 1)
+
+
 # ---------------------------------------------------------------------------
 # what a backward keeps is autograd's
 # ---------------------------------------------------------------------------

@@ -2896,10 +2896,11 @@ def fused_cross_entropy_backward(grad, x: MT, t: MT, lse: MT, total: MT, reducti
         if rc != 3:  # anything but MI355X_EUNSUPPORTED (a shape it does not take) is an error
             check("mi355x_cross_entropy_fwd_bwd", rc)
     materialize(lse)
+    tgt = _contig(t)
     check(
         "mi355x_cross_entropy_bwd",
         lib().mi355x_cross_entropy_bwd(dx._ptr, _code(x._dtype), ld_dx, x._ptr, _code(x._dtype), ld,
-                                       lse._ptr, _contig(t)._ptr, g._ptr, int(reduction), total._ptr,
+                                       lse._ptr, tgt._ptr, g._ptr, int(reduction), total._ptr,
                                        n, c, int(ignore_index), _STREAM),
     )
     return dx
